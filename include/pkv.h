@@ -369,6 +369,131 @@ int pkv_arena_fork(void *stream, void *state, int32_t capacity_pages, int32_t pa
                    int32_t *slot_table, int32_t num_slots, int32_t max_pages, int32_t *slot_lens,
                    const int32_t *src_slots, const int32_t *dst_slots, int32_t count);
 
+/*
+ * ---- which cached state lives on --------------------------------------------------
+ *
+ * No counterpart in the reference: its caches grow until they are trimmed by
+ * length, and it decodes one sequence per request.
+ */
+
+/*
+ * The attention weight that the queries put on each cached token, summed over the
+ * query rows of a KV head and added to the sums so far:
+ *   out[row][kh][t] = old + sum over heads h of kh, queries q of softmax_t(scale * q_h . k_t)
+ * for t < seq_lens[b]; t is visible to query q as in pkv_paged_attention.  `old`
+ * is mass[row][kh][t], or 0 where mass is NULL or t >= counted[b] (tokens that
+ * have no sum yet: what a rolled-back step left behind is not read).  A query
+ * that sees no token (queries q >= widths[b] see none) adds nothing; a token on
+ * an unmapped page draws nothing; entries t >= seq_lens[b], and rows of no
+ * sequence of the call, are left as they are.  Tokens past the block table or
+ * past mass_width do not exist.  Sums, and the softmax over them, in float32.
+ *
+ *  queries    : [batch][num_heads][num_queries][head_dim], float_kind
+ *  block_table, seq_lens, q_pos, widths: as pkv_paged_attention
+ *  scale      : softmax scale (finite)
+ *  mass, out  : [mass_rows][num_kv_heads][mass_width] f32 (may be the same)
+ *  counted    : [batch] tokens that have a sum in mass, or NULL for all
+ *  rows       : [batch] row of mass and out per sequence (distinct; others are
+ *               skipped), or NULL for row b
+ *  workspace  : pkv_attention_mass_workspace_bytes(...) bytes of device scratch
+ *               (calls that may overlap need one each)
+ */
+int pkv_attention_mass(void *stream, const pkv_layout *layout, const void *pool, int64_t num_pages,
+                       const void *queries, int32_t batch, int32_t num_heads, int32_t num_queries,
+                       const int32_t *block_table, int32_t max_pages, const int32_t *seq_lens,
+                       const int32_t *q_pos, const int32_t *widths, float scale, const float *mass,
+                       const int32_t *counted, const int32_t *rows, int32_t mass_rows,
+                       int64_t mass_width, void *workspace, int64_t workspace_bytes, float *out);
+int64_t pkv_attention_mass_workspace_bytes(const pkv_layout *layout, int32_t num_heads,
+                                           int32_t num_queries, int32_t batch, int32_t max_pages);
+
+/*
+ * Which tokens stay when a sequence of L = seq_lens[b] tokens is cut down to
+ * n = min(L, keep[b], max_keep): per layer and KV head the last r = min(recent, n),
+ * the first s = min(sinks, n - r), and of the others the n - r - s of largest
+ * mass (ties: the lowest index; a NaN counts as larger than any number).
+ *
+ *  mass     : [layers][mass_rows][kv_heads][mass_width] f32
+ *  rows     : [batch] row of mass per sequence, or NULL for row b (a sequence
+ *             whose row does not exist keeps nothing)
+ *  keep     : [batch] int32, or NULL for max_keep
+ *  kept     : [layers][batch][kv_heads][max_keep] int32 out, ascending, -1 from n on
+ *  new_lens : [batch] int32 out, n
+ *  new_mass : [layers][mass_rows][kv_heads][new_width] f32 out or NULL: the kept
+ *             tokens' sums, in the same order, 0 from n to max_keep, in the rows of
+ *             the call's sequences (others are left as they are).  May be mass
+ *             (new_width = mass_width): the sums then move in place.
+ */
+int pkv_evict_select(void *stream, const float *mass, int32_t layers, int32_t mass_rows,
+                     int32_t kv_heads, int64_t mass_width, const int32_t *rows,
+                     const int32_t *seq_lens, int32_t batch, const int32_t *keep, int32_t max_keep,
+                     int32_t sinks, int32_t recent, int32_t *kept, int32_t *new_lens,
+                     float *new_mass, int64_t new_width);
+
+/*
+ * The kept tokens' K and V (of every layer's pool, codes and metadata bit for bit)
+ * to positions 0..new_lens[b]-1 of the pages of dst_table, which must not be
+ * pages of src_table.  Nothing else in the destination pages changes; a kept
+ * index without a mapped source page leaves its position as it is, positions
+ * past the destination table are dropped.  Keys move as they were stored, with
+ * the rotation of their original positions.
+ *
+ *  pools     : host array of num_pools (<= 128) device pools of num_pages pages
+ *  kept      : [num_pools][batch][num_kv_heads][max_keep] int32, as pkv_evict_select
+ *  src_table : [batch][src_pages], dst_table: [batch][dst_pages] int32
+ */
+int pkv_evict_pages(void *stream, const pkv_layout *layout, void *const *pools, int32_t num_pools,
+                    int64_t num_pages, const int32_t *kept, const int32_t *new_lens, int32_t batch,
+                    int32_t max_keep, const int32_t *src_table, int32_t src_pages,
+                    const int32_t *dst_table, int32_t dst_pages);
+
+/*
+ * A beam step's selection.  Candidates of a group are the pairs of a beam w and a
+ * token v, c = scores[w] + logits[w][v] - log(sum_v exp(logits[w][v])); the `count`
+ * largest come out in order, ties to the lowest w * vocab + v.  A beam that is
+ * done has one candidate, (w, pad_token) at its score.  A beam whose score is not
+ * finite, or whose logits hold +inf, NaN or nothing but -inf, has none, and a
+ * logit of -inf is none.  Where there are too few, the rest is -inf, at the lowest
+ * pairs that are no candidates.  Candidates are compared in 64 bits.
+ *
+ *  logits     : [groups][beams][vocab], kind 0 = bf16, 1 = f16, 2 = f32; strides in
+ *               elements, each row's tokens adjacent
+ *  scores     : [groups][beams] f32;  done: [groups][beams] bytes, or NULL
+ *  count      : 1..64 (and at most beams * vocab); beams at most 64
+ *  out_scores : [groups][count] f32;  parents, tokens: [groups][count] int32
+ *  workspace  : pkv_beam_workspace_bytes(...) bytes of device scratch
+ */
+int pkv_beam_select(void *stream, const void *logits, int32_t kind, int32_t groups, int32_t beams,
+                    int32_t vocab, int64_t group_stride, int64_t beam_stride, const float *scores,
+                    const uint8_t *done, int32_t pad_token, int32_t count, void *workspace,
+                    int64_t workspace_bytes, float *out_scores, int32_t *parents, int32_t *tokens);
+int64_t pkv_beam_workspace_bytes(int32_t groups, int32_t beams, int32_t vocab, int32_t count);
+
+/*
+ * Rows of state [outer][num_rows][row_bytes] become others' copies, all at once:
+ * row targets[i] gets what row sources[i] held before the call.  Targets must be
+ * distinct (sources need not be); a pair with a row that does not exist is
+ * skipped.  At most 8192 pairs.
+ */
+int pkv_reorder_rows(void *stream, void *state, int64_t outer, int32_t num_rows, int64_t row_bytes,
+                     const int32_t *targets, const int32_t *sources, int32_t count);
+
+/*
+ * The same for sequence slots of the device arena: slot slots[i] (distinct)
+ * becomes a copy of what slot sources[i] held before the call, sharing its pages
+ * (a shared, partly filled tail is copied when it is next written); pages that
+ * no slot holds any more go back on the free stack.  A slot that is out of range
+ * sets PKV_ARENA_BAD_ARGUMENT and its pair is skipped.  At most 8192 pairs.
+ *
+ *  workspace : pkv_arena_reorder_workspace_bytes(count, max_pages) bytes of device
+ *              scratch
+ */
+int pkv_arena_reorder(void *stream, void *state, int32_t capacity_pages, int32_t page_tokens,
+                      int32_t *slot_table, int32_t num_slots, int32_t max_pages, int32_t *slot_lens,
+                      const int32_t *slots, const int32_t *sources, int32_t count, void *workspace,
+                      int64_t workspace_bytes);
+int64_t pkv_arena_reorder_workspace_bytes(int32_t count, int32_t max_pages);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,11 +16,16 @@
 
 #include "pkv.h"
 
+#include "pkv_error.h"
 #include "pkv_launch.h"
 
 namespace {
 
 thread_local std::string g_error = "ok";
+
+}  // namespace
+
+namespace pkv {
 
 int fail(int code, const std::string &message) {
   g_error = message;
@@ -44,6 +49,14 @@ int geometry(const pkv_layout *layout, pkv_geometry *g) {
                                  "float_kind 0/1, num_kv_heads >= 1)");
   return PKV_OK;
 }
+
+}  // namespace pkv
+
+namespace {
+
+using pkv::check_launch;
+using pkv::fail;
+using pkv::geometry;
 
 // Query rows per KV head (queries x heads per KV head) one call may carry.
 constexpr int64_t kMaxRows = 1 << 24;

@@ -1,0 +1,224 @@
+// pkv_evict.hip -- eviction from the paged cache by accumulated attention weight.
+//
+// select: of a sequence's L tokens the n = min(L, budget) that stay are, per
+// (layer, KV head), the last r = min(recent, n), the first s = min(sinks, n - r)
+// and the n - r - s of largest sum among the rest (ties: the lowest index), in
+// ascending order.
+//
+// pages: the kept tokens' K and V, codes and metadata bit for bit, to positions
+// 0..n-1 of other pages.
+#include "pkv_cache_ops.h"
+
+namespace pkv {
+
+namespace {
+
+// ---- select ------------------------------------------------------------------------
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+
+// Unsigned key of the order: NaN above everything, -0 equal to +0.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0xFFFFFFFFu;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ int block_sum(int v, int *s_wave) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  int sum = 0;
+  for (int k = 0; k < kWaves; ++k) sum += s_wave[k];
+  return sum;
+}
+
+// Exclusive prefix sum over the workgroup; *total the sum.
+__device__ __forceinline__ int block_scan(int v, int *s_wave, int *total) {
+  const int incl = wave_scan_incl(v, 0), wave = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) s_wave[wave] = incl;
+  __syncthreads();
+  int before = 0, sum = 0;
+  for (int k = 0; k < kWaves; ++k) {
+    before += k < wave ? s_wave[k] : 0;
+    sum += s_wave[k];
+  }
+  *total = sum;
+  return before + incl - v;
+}
+
+__global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictSelectArgs a) {
+  __shared__ int s_wave[kWaves];
+  const int kh = blockIdx.x % a.hk, b = blockIdx.x / a.hk % a.batch, layer = blockIdx.x / a.hk / a.batch;
+  const int row = a.rows ? a.rows[b] : b;
+  const int L = (int)max((int64_t)0, min((int64_t)a.seq_lens[b], a.width));
+  int n = min(L, a.max_keep);
+  if (a.keep) n = max(0, min(n, a.keep[b]));
+  const bool there = row >= 0 && row < a.mass_rows;
+  if (!there) n = 0;  // no such row: nothing is kept of it
+  if (layer == 0 && kh == 0 && threadIdx.x == 0) a.new_lens[b] = n;
+  int32_t *kept = a.kept + (int64_t)blockIdx.x * a.max_keep;
+  const int64_t base = ((int64_t)layer * a.mass_rows + row) * a.hk + kh;
+  const float *mass = a.mass + base * a.width;
+  float *new_mass = a.new_mass && there ? a.new_mass + base * a.new_width : nullptr;
+  const int r = min(a.recent, n), s = min(a.sinks, n - r);
+  const int lo = s, hi = n > 0 ? L - r : s, need = n - r - s;  // `need` of the tokens lo..hi-1
+  // the need-th largest key, bit by bit from the top: the largest key that at
+  // least `need` tokens reach
+  uint32_t least = 0;
+  if (need > 0 && need < hi - lo)
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t at = least | (1u << bit);
+      int count = 0;
+      for (int t = lo + threadIdx.x; t < hi; t += kThreads) count += order_key(mass[t]) >= at;
+      if (block_sum(count, s_wave) >= need) least = at;
+    }
+  int above = 0;
+  for (int t = lo + threadIdx.x; t < hi; t += kThreads) above += order_key(mass[t]) > least;
+  int room = need - block_sum(above, s_wave);  // tokens of that key itself
+  int done = 0;
+  for (int t0 = 0; t0 < L && n > 0; t0 += kThreads) {
+    const int t = t0 + threadIdx.x;
+    const float m = t < L ? mass[t] : 0.0f;
+    const uint32_t key = order_key(m);
+    const bool middle = t >= lo && t < hi && need > 0;
+    int ties, taken;
+    const int tie = block_scan(middle && key == least, s_wave, &ties);
+    const bool stays = t < L && (t < s || t >= L - r || (middle && (key > least || (key == least && tie < room))));
+    const int at = done + block_scan(stays, s_wave, &taken);  // (its barriers: the chunk is read before it is written)
+    if (stays && at < a.max_keep) {
+      kept[at] = t;
+      if (new_mass) new_mass[at] = m;
+    }
+    room -= min(room, ties);
+    done += taken;
+  }
+  __syncthreads();
+  for (int i = n + threadIdx.x; i < a.max_keep; i += kThreads) {
+    kept[i] = -1;
+    if (new_mass) new_mass[i] = 0.0f;
+  }
+}
+
+// ---- pages -------------------------------------------------------------------------
+
+// One wave per 16-token tile of the new pages.  A K lane's bytes belong to one
+// token, so they move as they are; a V lane holds four tokens of a column, so it
+// gathers four source lanes and takes one token's bytes of each.
+template <int BITS, int DP>
+__global__ __launch_bounds__(256) void evict_pages_kernel(const EvictPagesArgs a) {
+  constexpr int LB = DP * BITS / 32, CS = LB < 16 ? LB : 16, NCH = LB / CS, W = CS / 4;
+  const Geo &g = a.g;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int t0 = (blockIdx.x * 4 + wave) * PKV_TILE;
+  const int kh = blockIdx.y % g.hk, b = blockIdx.y / g.hk;
+  const int n = min(a.new_lens[b], a.max_keep);
+  if (t0 >= n || t0 / g.page >= a.dst_pages) return;
+  const int dst_id = a.dst_table[(int64_t)b * a.dst_pages + t0 / g.page];
+  if (dst_id < 0 || dst_id >= a.num_pages) return;
+  uint8_t *pool = a.pools[blockIdx.z];
+  uint8_t *dst_head = pool + (int64_t)dst_id * g.page_bytes + (int64_t)kh * g.head_bytes;
+  const int dst_slot = t0 % g.page;
+  const int64_t dst_tile = (int64_t)(dst_slot / PKV_TILE) * g.tile_bytes;
+
+  // this lane's token: lane % 16 of the tile
+  const int i = t0 + lane % 16;
+  int slot = -1, id = -1;
+  if (i < n) {
+    const int t = a.kept[(((int64_t)blockIdx.z * a.batch + b) * g.hk + kh) * a.max_keep + i];
+    if (t >= 0 && t / g.page < a.src_pages) {
+      id = a.src_table[(int64_t)b * a.src_pages + t / g.page];
+      slot = t % g.page;
+      if (id < 0 || id >= a.num_pages) id = -1;
+    }
+  }
+  auto head_of = [&](int page) { return pool + (int64_t)page * g.page_bytes + (int64_t)kh * g.head_bytes; };
+  if (id >= 0) {
+    const uint8_t *src = head_of(id) + (int64_t)(slot / PKV_TILE) * g.tile_bytes;
+    const int from = slot % PKV_TILE + (lane & 48);
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      if constexpr (CS == 16)
+        *(u4 *)(dst_head + dst_tile + c * 1024 + lane * 16) = *(const u4 *)(src + c * 1024 + from * 16);
+      else
+        *(u2 *)(dst_head + dst_tile + lane * 8) = *(const u2 *)(src + from * 8);
+    }
+    // its metadata words, groups lane / 16, lane / 16 + 4, ...
+    if (BITS != 16)
+      for (int gi = lane / 16; gi < g.ng; gi += 4) {
+        const int64_t from_w = ((int64_t)slot * g.ng + gi) * 4, to_w = ((int64_t)(dst_slot + lane % 16) * g.ng + gi) * 4;
+        *(uint32_t *)(dst_head + g.kmeta_offset + to_w) = *(const uint32_t *)(head_of(id) + g.kmeta_offset + from_w);
+        *(uint32_t *)(dst_head + g.vmeta_offset + to_w) = *(const uint32_t *)(head_of(id) + g.vmeta_offset + from_w);
+      }
+  }
+  int id4[4], slot4[4];
+  bool all = true, any = false;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    id4[r] = __shfl(id, (lane >> 4) * 4 + r, 64);
+    slot4[r] = __shfl(slot, (lane >> 4) * 4 + r, 64);
+    all = all && id4[r] >= 0;
+    any = any || id4[r] >= 0;
+  }
+  if (!any) return;
+  uint8_t *dst = dst_head + g.v_offset + dst_tile;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    uint32_t out[W] = {};
+    const int64_t at = (int64_t)c * 64 * CS;
+    if (!all)  // positions without a kept token stay as they are
+#pragma unroll
+      for (int w = 0; w < W; ++w) out[w] = *(const uint32_t *)(dst + at + lane * CS + 4 * w);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (id4[r] < 0) continue;
+      const int t = slot4[r] % PKV_TILE;
+      const uint8_t *src = head_of(id4[r]) + g.v_offset + (int64_t)(slot4[r] / PKV_TILE) * g.tile_bytes + at +
+                           (lane % 16 + 16 * (t / 4)) * CS;
+      const int q = t % 4;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if constexpr (BITS == 16) {
+          // dwords (2n, 2n+1) hold tokens (0, 1) and (2, 3) of block n
+          if ((w & 1) != r / 2) continue;
+          const uint32_t x = *(const uint32_t *)(src + 4 * ((w & ~1) + q / 2));
+          const uint32_t h = q & 1 ? x >> 16 : x & 0xFFFFu;
+          out[w] = r & 1 ? (out[w] & 0xFFFFu) | h << 16 : (out[w] & 0xFFFF0000u) | h;
+        } else {
+          const int bq = BITS == 4 ? v4_byte(q) : q, br = BITS == 4 ? v4_byte(r) : r;
+          const uint32_t x = *(const uint32_t *)(src + 4 * w);
+          out[w] = (out[w] & ~(0xFFu << (8 * br))) | ((x >> (8 * bq)) & 0xFFu) << (8 * br);
+        }
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) *(uint32_t *)(dst + at + lane * CS + 4 * w) = out[w];
+  }
+}
+
+template <int BITS>
+void start_pages(hipStream_t stream, const EvictPagesArgs &a, dim3 grid) {
+  if (a.g.dp == 64) hipLaunchKernelGGL((evict_pages_kernel<BITS, 64>), grid, dim3(256), 0, stream, a);
+  else if (a.g.dp == 128) hipLaunchKernelGGL((evict_pages_kernel<BITS, 128>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((evict_pages_kernel<BITS, 256>), grid, dim3(256), 0, stream, a);
+}
+
+}  // namespace
+
+hipError_t launch_evict_select(hipStream_t stream, const EvictSelectArgs &a) {
+  hipLaunchKernelGGL(evict_select_kernel, dim3(a.layers * a.batch * a.hk), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_evict_pages(hipStream_t stream, const EvictPagesArgs &a) {
+  const dim3 grid((a.max_keep + 4 * PKV_TILE - 1) / (4 * PKV_TILE), a.batch * a.g.hk, a.num_pools);
+  if (a.g.bits == 4) start_pages<4>(stream, a, grid);
+  else if (a.g.bits == 8) start_pages<8>(stream, a, grid);
+  else start_pages<16>(stream, a, grid);
+  return hipGetLastError();
+}
+
+}  // namespace pkv

@@ -66,6 +66,21 @@ SIGNATURES = {
                            ctypes.c_int),
     "pkv_arena_fork": ([_c_p, _c_p, _i32, _i32, _c_p, _i32, _i32, _c_p, _c_p, _c_p, _i32],
                        ctypes.c_int),
+    "pkv_attention_mass": ([_c_p, _LP, _c_p, _i64, _c_p, _i32, _i32, _i32, _c_p, _i32, _c_p, _c_p,
+                            _c_p, _f32, _c_p, _c_p, _c_p, _i32, _i64, _c_p, _i64, _c_p],
+                           ctypes.c_int),
+    "pkv_attention_mass_workspace_bytes": ([_LP, _i32, _i32, _i32, _i32], _i64),
+    "pkv_evict_select": ([_c_p, _c_p, _i32, _i32, _i32, _i64, _c_p, _c_p, _i32, _c_p, _i32, _i32,
+                          _i32, _c_p, _c_p, _c_p, _i64], ctypes.c_int),
+    "pkv_evict_pages": ([_c_p, _LP, _c_p, _i32, _i64, _c_p, _c_p, _i32, _i32, _c_p, _i32, _c_p,
+                         _i32], ctypes.c_int),
+    "pkv_beam_select": ([_c_p, _c_p, _i32, _i32, _i32, _i32, _i64, _i64, _c_p, _c_p, _i32, _i32,
+                         _c_p, _i64, _c_p, _c_p, _c_p], ctypes.c_int),
+    "pkv_beam_workspace_bytes": ([_i32, _i32, _i32, _i32], _i64),
+    "pkv_reorder_rows": ([_c_p, _c_p, _i64, _i32, _i64, _c_p, _c_p, _i32], ctypes.c_int),
+    "pkv_arena_reorder": ([_c_p, _c_p, _i32, _i32, _c_p, _i32, _i32, _c_p, _c_p, _c_p, _i32,
+                           _c_p, _i64], ctypes.c_int),
+    "pkv_arena_reorder_workspace_bytes": ([_i32, _i32], _i64),
 }
 
 

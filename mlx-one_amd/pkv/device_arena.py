@@ -76,6 +76,9 @@ class DevicePageArena:
         self._pool_ptrs = (ctypes.c_void_p * num_layers)(*[p.data_ptr() for p in self.pools])
         self._free_slots = list(range(self.max_slots - 1, -1, -1))
         self.lengths = [0] * self.max_slots     # host mirror (exact: growth is by request)
+        # the attention weight each cached token has drawn, and the tokens evicted
+        # from each slot (one more entry than slots): kept once track_mass() asks
+        self.mass = self.evicted = None
         nat.check(lib.pkv_arena_init(nat.stream_handle(self.device), nat.ptr(self.state),
                                      self.capacity), "arena init")
 
@@ -152,6 +155,9 @@ class DevicePageArena:
                                              *self._common(), nat.ptr(slots_d), nat.ptr(keep_d),
                                              count)
         nat.check(code, "arena truncate")
+        if self.evicted is not None:
+            at = self._places(slots_d)
+            self.evicted[at] = self.evicted[at] * (keep_d > 0)   # an emptied slot starts anew
         if host_slots is not None and host_keep is not None:
             for s, k in zip(host_slots, host_keep):
                 self.lengths[s] = k
@@ -177,9 +183,143 @@ class DevicePageArena:
                                          *self._common(), nat.ptr(src_d), nat.ptr(dst_d),
                                          int(src_d.numel()))
         nat.check(code, "arena fork")
+        self._move_mass(dst_d, src_d)
         if host_src is not None and host_dst is not None:
             for s, d in zip(host_src, host_dst):
                 self.lengths[d] = self.lengths[s]
+
+    def reorder(self, slots, sources):
+        """Each slot becomes a copy of what its source held before the call, all at
+        once, sharing its pages; pages that no slot holds any more are freed.  A
+        beam step's bookkeeping: sources are the parents' slots, and may repeat
+        (``fork`` into slots that need not be empty)."""
+        slots_d, host_slots = self._slots(slots)
+        count = int(slots_d.numel())
+        sources_d, host_sources = self._ints(sources, count)
+        if host_sources is not None and any(s < 0 or s >= self.max_slots for s in host_sources):
+            raise ValueError("reorder sources must be valid slot ids")
+        if sources_d.numel() != count:
+            raise ValueError("one source per slot")
+        self._reorder_pages(slots_d, sources_d)
+        self._move_mass(slots_d, sources_d)
+        if host_slots is not None and host_sources is not None:
+            held = [self.lengths[s] for s in host_sources]
+            for s, n in zip(host_slots, held):
+                self.lengths[s] = n
+
+    def _reorder_pages(self, slots_d, sources_d):
+        count = int(slots_d.numel())
+        lib = nat.load()
+        workspace = ops._scratch(lib.pkv_arena_reorder_workspace_bytes(count, self.max_pages),
+                                 self.device, "arena reorder")
+        code = lib.pkv_arena_reorder(nat.stream_handle(self.device), nat.ptr(self.state),
+                                     *self._common(), nat.ptr(slots_d), nat.ptr(sources_d), count,
+                                     nat.ptr(workspace), workspace.numel())
+        nat.check(code, "arena reorder")
+
+    # -- eviction by attention weight -----------------------------------------------------
+    def track_mass(self):
+        """Keep, from now on, the attention weight that every cached token draws
+        (``mass [layers, slots, HK, tokens]`` float32, added to by each step's
+        ``attend``): what ``evict`` goes by.  Call it before steps are captured.
+        The weight of a step that is rolled back stays counted."""
+        if self.mass is None:
+            self.mass = torch.zeros((len(self.pools), self.max_slots, self.fmt.num_kv_heads,
+                                     self.max_pages * self.page_tokens), device=self.device)
+            self.evicted = torch.zeros(self.max_slots + 1, dtype=torch.int32, device=self.device)
+
+    def _places(self, slots_d):
+        """Slot ids as indices of ``evicted`` (ids out of range: its last entry)."""
+        ids = slots_d.long()
+        return torch.where((ids >= 0) & (ids < self.max_slots), ids, self.max_slots)
+
+    def _move_mass(self, to, source):
+        if self.mass is not None:
+            ops.reorder_rows(self.mass, to, source, dim=1)
+            ops.reorder_rows(self.evicted[:self.max_slots], to, source)
+
+    def positions(self, reservation):
+        """``[B]`` positions of the first new tokens in their texts: the cached
+        length, and the tokens evicted before it."""
+        if self.evicted is None:
+            return reservation.starts
+        return reservation.starts + self.evicted[self._places(reservation.slots)]
+
+    def evict(self, slots, keep, *, sinks=4, recent=64, max_keep=None, spare=None):
+        """Cut each slot longer than ``keep`` tokens down to ``keep``: in every layer
+        and KV head its first ``sinks`` and last ``recent`` tokens and the ones that
+        have drawn most attention weight (``ops.evict_select``).  They move to new
+        pages (shared ones stay as they are for the others) and keep their sums;
+        later tokens' positions go on as if none were evicted.
+
+        ``keep`` an int or one per slot (on the device: with ``max_keep``).  The
+        new pages are taken before the old ones go; slots without room for them stay
+        as they are and the arena records ``OUT_OF_PAGES``, which host lists of
+        slots raise.  ``spare``: empty slots to work in, one at least (default:
+        free ones); the slots are cut as many at a time as there are."""
+        if self.mass is None:
+            raise ValueError("eviction goes by the attention weight: call track_mass() first")
+        slots_d, host_slots = self._slots(slots)
+        count = int(slots_d.numel())
+        if isinstance(keep, int):
+            max_keep = keep if max_keep is None else max_keep
+            keep = [keep] * count if host_slots is not None else \
+                torch.full((count,), keep, dtype=torch.int32, device=self.device)
+        keep_d, host_keep = self._ints(keep, count)
+        if host_keep is not None:
+            if any(k < 0 for k in host_keep):
+                raise ValueError("negative budget")
+            max_keep = max(host_keep, default=0) if max_keep is None else max_keep
+            host_keep = [min(k, max_keep) for k in host_keep]
+        if max_keep is None or max_keep < 0:
+            raise ValueError("budgets on the device need max_keep, their bound")
+        if keep_d.numel() != count:
+            raise ValueError("one budget per slot")
+        if count == 0:
+            return
+        opened = []
+        if spare is None:
+            if not self._free_slots:
+                raise CacheCapacityError("eviction needs a free sequence slot", retryable=True)
+            spare = opened = [self.open_slot() for _ in range(min(count, len(self._free_slots)))]
+        try:
+            spare_d, host_spare = self._slots(spare)
+            step = int(spare_d.numel())
+            if step < 1:
+                raise ValueError("eviction needs a spare slot")
+            if host_spare is not None and (any(self.lengths[s] for s in host_spare)
+                                           or set(host_spare) & set(host_slots or ())):
+                raise ValueError("spare slots must be empty")
+            for i in range(0, count, step):      # as many slots at a time as there are spare ones
+                part = slots_d[i:i + step]
+                self._evict(part, keep_d[i:i + step], spare_d[:part.numel()], int(sinks),
+                            int(recent), int(max_keep))
+        finally:
+            self._free_slots.extend(reversed(opened))
+        if host_slots is not None and host_keep is not None:
+            err = self.probe_failed(self.error_probe())
+            if err:
+                self.sync_lengths()
+                self._raise(err)
+            for s, k in zip(host_slots, host_keep):
+                self.lengths[s] = min(self.lengths[s], k)
+
+    def _evict(self, slots_d, keep_d, spare_d, sinks, recent, max_keep):
+        valid = (slots_d >= 0) & (slots_d < self.max_slots)
+        at = slots_d.long().clamp(0, self.max_slots - 1)
+        lens = self.lens[at]
+        kept_lens = keep_d.clamp(0, max_keep)
+        cut = valid & (lens > kept_lens)
+        res = self.reserve(spare_d, torch.where(cut, kept_lens, 0))
+        cut = cut & (res.lens == kept_lens)       # a slot without its new pages stays as it is
+        kept, n, _ = ops.evict_select(self.mass, lens, keep_d, max_keep=max_keep, sinks=sinks,
+                                      recent=recent, rows=torch.where(cut, slots_d, -1),
+                                      new_mass=self.mass)
+        ops.evict_pages(self.fmt, self.pools, kept, n, self.table[at], res.table)
+        places = self._places(slots_d)
+        self.evicted[places] = self.evicted[places] + torch.where(cut, lens - kept_lens, 0)
+        self._reorder_pages(slots_d, torch.where(cut, spare_d, slots_d))  # the sums have moved
+        self.truncate(spare_d, torch.zeros_like(spare_d))
 
     # -- inspection (these synchronise) ---------------------------------------------------
     def sync_lengths(self):
@@ -260,20 +400,27 @@ class DeviceBatchCache:
         dtype = fmt.dtype
         batch, heads, width, _ = queries.shape
         waves = self.waves or ops.split_waves(fmt, heads, width, batch, queries.device)
+        out = self._attend(fmt, pool, dtype, queries, keys, values, width, waves, scale)
+        if self.arena.mass is not None:
+            mass = self.arena.mass[self.layer]
+            ops.attention_mass(fmt, pool, queries.to(dtype), self.res.table, self.res.lens,
+                               scale=scale, widths=self.res.widths, mass=mass,
+                               counted=self.res.starts, rows=self.res.slots)
+        return out.to(queries.dtype)
+
+    def _attend(self, fmt, pool, dtype, queries, keys, values, width, waves, scale):
         if width == 1:
             # a decode step (every width 1): the new token at lens - 1, its
             # query there too -- one fused append + attention call
-            out = ops.append_paged_attention(fmt, pool, keys.to(dtype), values.to(dtype),
-                                             queries.to(dtype), self.res.table, self.res.lens,
-                                             scale=scale, waves=waves,
-                                             workspace=self.workspace)
-            return out.to(queries.dtype)
+            return ops.append_paged_attention(fmt, pool, keys.to(dtype), values.to(dtype),
+                                              queries.to(dtype), self.res.table, self.res.lens,
+                                              scale=scale, waves=waves,
+                                              workspace=self.workspace)
         ops.append_quantize(fmt, pool, keys.to(dtype).contiguous(), values.to(dtype).contiguous(),
                             self.res.table, self.res.starts, self.res.widths)
-        out = ops.paged_attention(fmt, pool, queries.to(dtype).contiguous(), self.res.table,
-                                  self.res.lens, scale=scale, widths=self.res.widths,
-                                  waves=waves, workspace=self.workspace)
-        return out.to(queries.dtype)
+        return ops.paged_attention(fmt, pool, queries.to(dtype).contiguous(), self.res.table,
+                                   self.res.lens, scale=scale, widths=self.res.widths,
+                                   waves=waves, workspace=self.workspace)
 
 
 class DeviceRunner:
@@ -289,7 +436,7 @@ class DeviceRunner:
 
     def _forward(self, hidden, res, workspace=None, waves=0):
         batch, width, _ = hidden.shape
-        positions = res.starts.view(batch, 1)
+        positions = self.arena.positions(res).view(batch, 1)
         if width > 1:
             positions = positions + torch.arange(width, dtype=torch.int32, device=hidden.device)
         caches = tuple(DeviceBatchCache(self.arena, layer, res, workspace=workspace, waves=waves)

@@ -442,3 +442,278 @@ def rope_qkv(qkv, positions, inv_freq, heads, kv_heads):
     nat.check(code, "rope")
     return q, k, v
 
+
+
+# ---- which cached state lives on ---------------------------------------------------
+
+
+class _OnDevice:
+    """Makes ``device`` the current one for a launch, where it is not."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.previous = torch._C._cuda_getDevice()
+        if self.previous != self.index:
+            torch._C._cuda_setDevice(self.index)
+
+    def __exit__(self, *_):
+        if self.previous != self.index:
+            torch._C._cuda_setDevice(self.previous)
+
+
+def _check_dense(t, dtype, device, name, dims):
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != dims or \
+            t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dims}-dimensional {dtype} tensor on {device}")
+
+
+def _per_row(x, device, count, name):
+    """An int32 operand of ``count`` values on the device (None: None)."""
+    t = _i32(x, device)
+    if t is not None and t.numel() != count:
+        raise ValueError(f"{name} must hold {count} values")
+    return t
+
+
+def _scratch(nbytes, device, what, given=None):
+    """The caller's workspace, or the stream's own memory of that size."""
+    if nbytes < 0:
+        nat.check(nat.PKV_INVALID_ARGUMENT, what)
+    if given is None:
+        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    if given.device != device or given.dtype is not torch.uint8 or not given.is_contiguous():
+        raise ValueError(f"{what} workspace must be a contiguous uint8 tensor on {device}")
+    return given
+
+
+def attention_mass(fmt: PageFormat, pool, queries, block_table, seq_lens, *, scale, q_pos=None,
+                   widths=None, mass=None, counted=None, rows=None, workspace=None, out=None):
+    """Attention weight of ``queries [B, H, Q, D]`` on every cached token, summed over
+    the query rows of each KV head and added to the sums so far.
+
+    ``mass [R, HK, N]`` (float32) holds the sums so far (None: zeros) in rows
+    ``rows [B]`` (default: row b; distinct), of which the first ``counted[b]``
+    tokens of sequence b are read (default: all).  The new sums go to ``out``
+    (default: ``mass`` in place, or new zeros ``[B, HK, pages * page_tokens]``),
+    which is returned; its entries from ``seq_lens[b]`` on, and rows that no
+    sequence of the call has, are left as they are.  The other operands are
+    ``paged_attention``'s; a query that sees no token adds nothing.
+    """
+    if queries.dim() != 4:
+        raise ValueError("queries must be [B, H, Q, D]")
+    batch, heads, nq, dim = queries.shape
+    if dim != fmt.head_dim:
+        raise ValueError("query head dimension differs from the page layout")
+    _check_float(queries, fmt, "queries")
+    device = queries.device
+    _check_dense(pool, torch.uint8, device, "pool", 2)
+    if pool.shape[1] != fmt.page_bytes:
+        raise ValueError("the pool's pages are not of this format")
+    table = _i32(block_table, device)
+    if table.dim() != 2 or table.shape[0] != batch:
+        raise ValueError("block table must be [batch, max_pages]")
+    lens = _per_row(seq_lens, device, batch, "seq_lens")
+    if mass is not None:
+        _check_dense(mass, torch.float32, device, "mass", 3)
+    if out is None:
+        out = mass if mass is not None else torch.zeros(
+            (batch, fmt.num_kv_heads, table.shape[1] * fmt.page_tokens), device=device)
+    else:
+        _check_dense(out, torch.float32, device, "out", 3)
+        if mass is not None and mass.shape != out.shape:
+            raise ValueError("mass and out must have one shape")
+    if out.shape[1] != fmt.num_kv_heads or (rows is None and out.shape[0] < batch):
+        raise ValueError("attention mass must be [rows, HK, tokens] with a row per sequence")
+    positions = _per_row(q_pos, device, batch * nq, "q_pos")
+    width = _per_row(widths, device, batch, "widths")
+    known = _per_row(counted, device, batch, "counted")
+    row = _per_row(rows, device, batch, "rows")
+    queries = queries.contiguous()
+    lib = nat.load()
+    workspace = _scratch(lib.pkv_attention_mass_workspace_bytes(fmt.c_layout, heads, nq, batch,
+                                                                table.shape[1]),
+                         device, "attention mass", workspace)
+    with _OnDevice(device):
+        code = lib.pkv_attention_mass(
+            nat.stream_handle(device), fmt.c_layout, pool.data_ptr(), pool.shape[0],
+            queries.data_ptr(), batch, heads, nq, table.data_ptr(), table.shape[1],
+            lens.data_ptr(), nat.ptr(positions), nat.ptr(width), float(scale), nat.ptr(mass),
+            nat.ptr(known), nat.ptr(row), out.shape[0], out.shape[2], workspace.data_ptr(),
+            workspace.numel(), out.data_ptr())
+    nat.check(code, "attention mass")
+    return out
+
+
+def evict_select(mass, seq_lens, keep, *, max_keep=None, sinks=0, recent=0, rows=None,
+                 with_mass=False, new_mass=None):
+    """Which tokens of each sequence stay when it is cut down to ``n = min(seq_lens[b],
+    keep)``: per layer and KV head the last ``min(recent, n)``, the first ``sinks`` as
+    far as there is room, and the heaviest of the others (ties: the lowest index).
+
+    ``mass [R, HK, N]`` or ``[layers, R, HK, N]`` (float32, row ``rows[b]`` or b for
+    sequence b); ``keep`` an int, or one per sequence (on the device: with
+    ``max_keep``, its bound).  Returns ``(kept [(layers,) B, HK, max_keep] int32``
+    ascending, -1 from n on, ``n [B] int32)``; with ``with_mass`` also the kept
+    tokens' sums ``[(layers,) R, HK, max_keep]``, in the same order, 0 from n on.
+    ``new_mass`` takes them instead (at least ``max_keep`` wide; ``mass`` itself: they
+    move in place).
+    """
+    if mass.dim() not in (3, 4):
+        raise ValueError("mass must be [rows, HK, tokens] or [layers, rows, HK, tokens]")
+    device = mass.device
+    if not mass.is_cuda:
+        raise ValueError("mass must be a device tensor")
+    _check_dense(mass, torch.float32, device, "mass", mass.dim())
+    layers = mass.shape[0] if mass.dim() == 4 else 1
+    mass_rows, heads, tokens = mass.shape[-3:]
+    lens = _i32(seq_lens, device)
+    batch = lens.numel()
+    row = _per_row(rows, device, batch, "rows")
+    if row is None and mass_rows < batch:
+        raise ValueError("mass needs a row per sequence")
+    if isinstance(keep, int):
+        if max_keep is None:
+            max_keep, budget = keep, None
+        else:
+            budget = torch.full((batch,), keep, dtype=torch.int32, device=device)
+    else:
+        if max_keep is None:
+            if isinstance(keep, torch.Tensor):
+                raise ValueError("budgets on the device need max_keep, their bound")
+            max_keep = max([int(k) for k in keep], default=0)
+        budget = _per_row(keep, device, batch, "keep")
+    if max_keep < 0:
+        raise ValueError("negative budget")
+    lead = (layers,) if mass.dim() == 4 else ()
+    if new_mass is not None:
+        _check_dense(new_mass, torch.float32, device, "new_mass", mass.dim())
+        if new_mass.shape[:-1] != mass.shape[:-1] or new_mass.shape[-1] < max_keep:
+            raise ValueError("new_mass must be mass's rows of at least max_keep tokens")
+    elif with_mass:
+        make = torch.empty if row is None and mass_rows == batch else torch.zeros
+        new_mass = make(lead + (mass_rows, heads, max_keep), dtype=torch.float32, device=device)
+    kept = torch.empty(lead + (batch, heads, max_keep), dtype=torch.int32, device=device)
+    new_lens = torch.empty(batch, dtype=torch.int32, device=device)
+    with _OnDevice(device):
+        code = nat.load().pkv_evict_select(
+            nat.stream_handle(device), mass.data_ptr(), layers, mass_rows, heads, tokens,
+            nat.ptr(row), lens.data_ptr(), batch, nat.ptr(budget), max_keep, int(sinks),
+            int(recent), kept.data_ptr(), new_lens.data_ptr(), nat.ptr(new_mass),
+            0 if new_mass is None else new_mass.shape[-1])
+    nat.check(code, "eviction select")
+    return (kept, new_lens) if new_mass is None else (kept, new_lens, new_mass)
+
+
+def evict_pages(fmt: PageFormat, pools, kept, new_lens, src_table, dst_table):
+    """Move the ``kept`` tokens of ``evict_select`` from the pages of ``src_table`` to
+    positions ``0 .. new_lens[b] - 1`` of those of ``dst_table`` (other pages), K and V,
+    bit for bit.
+
+    ``pools``: one pool with ``kept [B, HK, K]``, or a ``[layers, pages, page bytes]``
+    tensor or a list of pools with ``kept [layers, B, HK, K]``; one page id addresses
+    the same page in every pool.
+    """
+    device = kept.device
+    single = isinstance(pools, torch.Tensor) and pools.dim() == 2
+    if isinstance(pools, torch.Tensor):
+        _check_dense(pools, torch.uint8, device, "pools", 2 if single else 3)
+        layers, shape = (1 if single else pools.shape[0]), pools.shape[-2:]
+        step = shape[0] * shape[1]
+        addresses = [pools.data_ptr() + i * step for i in range(layers)]
+    else:
+        for p in pools:
+            _check_dense(p, torch.uint8, device, "pools", 2)
+        if not pools or any(p.shape != pools[0].shape for p in pools):
+            raise ValueError("pools of one call must be of one size")
+        layers, shape = len(pools), pools[0].shape
+        addresses = [p.data_ptr() for p in pools]
+    if shape[1] != fmt.page_bytes:
+        raise ValueError("the pools' pages are not of this format")
+    _check_dense(kept, torch.int32, device, "kept", 3 if single else 4)
+    batch, heads, most = kept.shape[-3:]
+    if heads != fmt.num_kv_heads or (not single and kept.shape[0] != layers):
+        raise ValueError("kept must be [(layers,) batch, HK, tokens]")
+    lens = _per_row(new_lens, device, batch, "new_lens")
+    src, dst = _i32(src_table, device), _i32(dst_table, device)
+    if src.dim() != 2 or dst.dim() != 2 or src.shape[0] != batch or dst.shape[0] != batch:
+        raise ValueError("block tables must be [batch, max_pages]")
+    with _OnDevice(device):
+        code = nat.load().pkv_evict_pages(
+            nat.stream_handle(device), fmt.c_layout, (nat._c_p * layers)(*addresses), layers,
+            shape[0], kept.data_ptr(), lens.data_ptr(), batch, most, src.data_ptr(), src.shape[1],
+            dst.data_ptr(), dst.shape[1])
+    nat.check(code, "eviction pages")
+
+
+_LOGIT_KINDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def beam_select(logits, scores, count, *, done=None, pad_token=0, workspace=None):
+    """The ``count`` best (beam, next token) pairs of every group of beams, by
+    ``scores[g, w] + log_softmax(logits[g, w])[v]``, ties to the lowest ``w * V + v``.
+
+    ``logits [G, W, V]`` (float32, bfloat16 or float16; rows may be strided),
+    ``scores [G, W]`` float32, ``done [G, W]`` bool: a beam that is done has the one
+    candidate ``pad_token`` at its score.  A beam without a finite score and
+    log-sum-exp has none; what there are too few of is -inf at the lowest other
+    pairs.  Returns ``(scores [G, count] f32, parents int32, tokens int32)`` in
+    order, ``parents`` as beam numbers 0..W-1 of the group.
+    """
+    if logits.dim() != 3 or logits.dtype not in _LOGIT_KINDS or not logits.is_cuda:
+        raise ValueError("logits must be a [groups, beams, vocab] f32/f16/bf16 device tensor")
+    device = logits.device
+    groups, beams, vocab = logits.shape
+    if logits.stride(2) != 1 and vocab > 1 or logits.stride(0) < 0 or logits.stride(1) < 0:
+        logits = logits.contiguous()
+    if tuple(scores.shape) != (groups, beams) or scores.device != device:
+        raise ValueError("scores must be [groups, beams] on the logits' device")
+    scores = scores.to(torch.float32).contiguous()
+    if done is not None:
+        if tuple(done.shape) != (groups, beams) or done.dtype is not torch.bool or \
+                done.device != device:
+            raise ValueError("done must be a [groups, beams] bool tensor on the logits' device")
+        done = done.contiguous()
+    lib = nat.load()
+    best = torch.empty((groups, count), dtype=torch.float32, device=device)
+    parents = torch.empty((groups, count), dtype=torch.int32, device=device)
+    tokens = torch.empty((groups, count), dtype=torch.int32, device=device)
+    if groups == 0:
+        return best, parents, tokens
+    workspace = _scratch(lib.pkv_beam_workspace_bytes(groups, beams, vocab, count), device,
+                         "beam select", workspace)
+    with _OnDevice(device):
+        code = lib.pkv_beam_select(
+            nat.stream_handle(device), logits.data_ptr(), _LOGIT_KINDS[logits.dtype], groups, beams,
+            vocab, logits.stride(0), logits.stride(1), scores.data_ptr(), nat.ptr(done),
+            int(pad_token), int(count), workspace.data_ptr(), workspace.numel(), best.data_ptr(),
+            parents.data_ptr(), tokens.data_ptr())
+    nat.check(code, "beam select")
+    return best, parents, tokens
+
+
+def reorder_rows(state, targets, sources, *, dim=0):
+    """Rows of ``state`` along ``dim`` become others' copies, in place and all at once:
+    row ``targets[i]`` (distinct) gets what row ``sources[i]`` held before the call.
+    Any type; pairs with a row that does not exist are skipped."""
+    if not state.is_cuda or not state.is_contiguous():
+        raise ValueError("state must be a contiguous device tensor")
+    if not 0 <= dim < state.dim():
+        raise ValueError("no such dimension")
+    device = state.device
+    to, source = _i32(targets, device), _i32(sources, device)
+    count = to.numel()
+    if source.numel() != count:
+        raise ValueError("reordering needs a source per target")
+    shape = state.shape
+    outer, num_rows = math.prod(shape[:dim]), shape[dim]
+    row_bytes = math.prod(shape[dim + 1:]) * state.element_size()
+    with _OnDevice(device):
+        code = nat.load().pkv_reorder_rows(nat.stream_handle(device), state.data_ptr(), outer,
+                                           num_rows, row_bytes, to.data_ptr(), source.data_ptr(),
+                                           count)
+    nat.check(code, "reorder")
+    return state
