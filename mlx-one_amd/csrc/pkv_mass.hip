@@ -3,45 +3,37 @@
 //   out[h, t] = old[h, t] + sum over query rows r of KV head h of softmax_t(scale * q_r . k_t)
 //
 // over the tokens t that row r sees (t <= its position, t < the sequence's
-// length).  Two passes: the log-sum-exp of each row, then the weights summed
-// over the rows of a token, in row order.
+// length).  A row's weights need its log-sum-exp over all its tokens first, so K
+// is gone through twice, or once and its scores kept:
+//
+//  * few rows (at most 8 per KV head: decode and short verify steps): one pass
+//    over K writes every score (float32) and the (max, sum) of each row and
+//    256-token part; a second launch reads the scores back.  16 bytes per token
+//    written and read at up to 4 rows, where K itself is 136 (8-bit, head_dim 128).
+//  * more rows: a pass over K for the log-sum-exps, a launch that joins their
+//    parts, and a second pass over K that sums the weights.
+//
+// Scores come from the matrix cores.  Quantized K enters as its exact codes (f16),
+// queries as f16 with each row scaled by a power of two, so that its largest
+// element lies in [2^14, 2^15): bfloat16 queries are exact then down to 2^-28 of
+// that, and the rest is smaller than the float32 accumulator's own rounding.  A
+// group's scale is applied to its accumulator in float32 and its bias to the sum of
+// the row's elements in the group, so a score is a float32 sum of exact products.
+#include <algorithm>
+
 #include "pkv_cache_ops.h"
+#include "pkv_mfma.h"
 
 namespace pkv {
 
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kFewRows = 8;
+constexpr float kLog2e = 1.4426950408889634f;
 
-// Element d (< dp) of token `slot` of a head block's K side, dequantized.
-__device__ __forceinline__ float k_element(const Geo &g, const uint8_t *head, int slot, int d) {
-  const uint8_t *tile = head + (int64_t)(slot / PKV_TILE) * g.tile_bytes;
-  const int lane = slot % PKV_TILE + 16 * ((d % 32) / 8), kb = d / 32, e = d % 8;
-  if (g.bits == 16)
-    return bits_to_float(*(const uint16_t *)(tile + payload_offset(lane, 2 * (8 * kb + e), g.chunk)), g.float_kind);
-  int code;
-  if (g.bits == 8) {
-    code = tile[payload_offset(lane, 8 * kb + e, g.chunk)];
-  } else {
-    const int nib = k4_nibble(e);
-    code = (tile[payload_offset(lane, 4 * kb + nib / 2, g.chunk)] >> (4 * (nib & 1))) & 15;
-  }
-  const uint32_t w = *(const uint32_t *)(head + g.kmeta_offset + ((int64_t)slot * g.ng + d / g.group) * 4);
-  return (float)code * f16_bits_to_f32(w) + f16_bits_to_f32(w >> 16);
-}
-
-__device__ __forceinline__ const uint8_t *token_head(const MassArgs &a, int b, int kh, int t) {
-  const int p = t / a.g.page;
-  const int id = p < a.max_pages ? a.table[(int64_t)b * a.max_pages + p] : -1;
-  if (id < 0 || id >= a.num_pages) return nullptr;
-  return a.pool + (int64_t)id * a.g.page_bytes + (int64_t)kh * a.g.head_bytes;
-}
-
-__device__ __forceinline__ float score(const MassArgs &a, const uint8_t *head, int t, const float *q) {
-  float s = 0.0f;
-  for (int d = 0; d < a.g.dim; ++d) s += q[d] * k_element(a.g, head, t % a.g.page, d);
-  return s * a.scale;
-}
+// ---- sequences, rows, units ---------------------------------------------------------
 
 // The tokens of sequence b that count, and the tokens its row qi sees.
 __device__ __forceinline__ int mass_len(const MassArgs &a, int b) {
@@ -52,77 +44,711 @@ __device__ __forceinline__ int row_sees(const MassArgs &a, int b, int qi, int L)
   const int w = a.widths ? a.widths[b] : a.nq;
   if (qi >= w) return 0;
   const int pos = a.q_pos ? a.q_pos[(int64_t)b * a.nq + qi] : a.seq_lens[b] - w + qi;
-  return pos >= L ? L : pos + 1;
+  return max(0, pos >= L ? L : pos + 1);
 }
 
-__device__ __forceinline__ void load_query(const MassArgs &a, int b, int kh, int row, float *q) {
-  const int qi = row / a.gqa, h = kh * a.gqa + row % a.gqa;
+// The units of a launch: parts of `size` tokens of every sequence, for each KV
+// head; a workgroup walks unit blockIdx.x, + gridDim.x, ...  Lane l of every wave
+// keeps the running count of parts of sequence base + l.
+struct Units {
+  int base, carry, incl, len;
+  int b, kh, part, L;
+
+  __device__ __forceinline__ void load(const MassArgs &a, int size, int lane) {
+    len = base + lane < a.batch ? max(0, mass_len(a, base + lane)) : 0;
+    incl = carry + wave_scan_incl((len + size - 1) / size, lane);
+  }
+  __device__ __forceinline__ void start(const MassArgs &a, int size, int lane) {
+    base = carry = 0;
+    load(a, size, lane);
+  }
+  // The whole wave calls, with rising units.  False past the last one.
+  __device__ __forceinline__ bool find(const MassArgs &a, int size, int64_t unit, int lane) {
+    const int64_t u = unit / a.g.hk;
+    kh = (int)(unit % a.g.hk);
+    for (;;) {
+      const unsigned long long hit = __ballot(incl > u);
+      if (hit) {
+        const int f = __ffsll((long long)hit) - 1;
+        L = __builtin_amdgcn_readlane(len, f);
+        b = base + f;
+        part = (int)u - (__builtin_amdgcn_readlane(incl, f) - (L + size - 1) / size);
+        return true;
+      }
+      if (base + 64 >= a.batch) return false;
+      carry = __builtin_amdgcn_readlane(incl, 63);
+      base += 64;
+      load(a, size, lane);
+    }
+  }
+};
+
+// ---- tiles and query rows -------------------------------------------------------------
+
+template <int BITS, int DP, int G, int FK>
+struct MassCfg : Cfg<BITS, DP, G, 1, FK, 1> {
+  using Base = Cfg<BITS, DP, G, 1, FK, 1>;
+  static constexpr int PAGE_BITS = BITS;
+  static constexpr int OPS = BITS == 16 ? FK : 1;  // operand type: f16 for codes
+  using KT = typename FloatOps<OPS>::KT;
+  static constexpr int GB = Base::QUANT ? G / 32 : Base::KB;  // 32-element blocks per accumulator
+};
+
+// A zero accumulator in registers: an inline constant 0 as an MFMA's accumulator has
+// given wrong results where its destination partly overlaps an operand.
+__device__ __forceinline__ f4 register_zero() {
+  f4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+  asm volatile("" : "+v"(z));
+  return z;
+}
+
+// Page ids of the N tiles from token t0 of sequence b: lane l's for tile l % N.
+template <int N>
+__device__ __forceinline__ int tile_page(const MassArgs &a, int b, int t0, int L, int lane) {
+  const int t = t0 + (lane % N) * PKV_TILE;
+  if (t >= L) return -1;
+  const int id = a.table[(int64_t)b * a.max_pages + t / a.g.page];
+  return id >= 0 && id < a.num_pages ? id : -1;
+}
+
+// A lane's K operands of a tile: codes as exact f16, or the float elements.
+template <typename C>
+__device__ __forceinline__ typename C::KT k_operand(const uint32_t (&w)[C::LW], int kb) {
+  if constexpr (C::QUANT) {
+    const h8 biased = Conv<C::PAGE_BITS>::kop(w, kb);  // 1024 + code
+    return biased - (h8)(_Float16)1024.0f;
+  } else {
+    return __builtin_bit_cast(typename C::KT, u4{w[4 * kb], w[4 * kb + 1], w[4 * kb + 2], w[4 * kb + 3]});
+  }
+}
+
+// One query row's elements d = 32 kb + 8 jj + e as operands (zeros without a row or
+// past the head dim), its multiplier (of a raw score, to log2 units) and its sums
+// per group.  The whole wave calls: lanes l, l ^ 16, l ^ 32 share a row.
+template <typename C>
+__device__ __forceinline__ void query_operands(const MassArgs &a, int b, int kh, int row, int jj,
+                                               typename C::KT (&op)[C::KB], float &mult, float (&qs)[C::NG]) {
+  const bool there = row < a.rows;
+  const int qi = there ? row / a.gqa : 0, h = kh * a.gqa + (there ? row % a.gqa : 0);
   const uint16_t *src = a.q + (((int64_t)b * a.heads + h) * a.nq + qi) * a.g.dim;
-  for (int d = threadIdx.x; d < a.g.dim; d += kThreads) q[d] = bits_to_float(src[d], a.g.float_kind);
+  uint16_t raw[C::KB][8];
+#pragma unroll
+  for (int kb = 0; kb < C::KB; ++kb) {
+    const int d0 = 32 * kb + 8 * jj;
+    if ((a.g.dim & 7) == 0 && ((uintptr_t)a.q & 15) == 0) {
+      u4 x = {0, 0, 0, 0};
+      if (there && d0 < a.g.dim) x = *(const u4 *)(src + d0);
+      __builtin_memcpy(raw[kb], &x, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) raw[kb][e] = there && d0 + e < a.g.dim ? src[d0 + e] : (uint16_t)0;
+    }
+  }
+  mult = a.scale * kLog2e;
+  if constexpr (!C::QUANT) {
+#pragma unroll
+    for (int kb = 0; kb < C::KB; ++kb) __builtin_memcpy(&op[kb], raw[kb], 16);
+    qs[0] = 0.0f;
+  } else {
+    const int fk = a.g.float_kind;
+    float most = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < C::KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(bits_to_float(raw[kb][e], fk)));
+    most = xor32_max(xor16_max(most));
+    const int shift = most > 0.0f && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+    mult = ldexpf(mult, -shift);
+#pragma unroll
+    for (int g = 0; g < C::NG; ++g) qs[g] = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < C::KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const _Float16 x = (_Float16)ldexpf(bits_to_float(raw[kb][e], fk), shift);
+        op[kb][e] = x;
+        qs[kb / C::GB] += (float)x;
+      }
+#pragma unroll
+    for (int g = 0; g < C::NG; ++g) qs[g] = xor32_add(xor16_add(qs[g]));
+  }
 }
 
-__global__ __launch_bounds__(kThreads) void mass_lse_kernel(const MassArgs a) {
-  __shared__ float q[256], part[2][kThreads];
-  const int row = blockIdx.x % a.rows, seg = blockIdx.x / a.rows;
-  const int b = seg / a.g.hk, kh = seg % a.g.hk;
-  const int L = mass_len(a, b), see = row_sees(a, b, row / a.gqa, L);
-  load_query(a, b, kh, row, q);
-  __syncthreads();
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// (m, l) with another pair of the same row; an empty one is (-inf, 0).
+__device__ __forceinline__ void join(float &m, float &l, float m2, float l2) {
+  const float n = fmaxf(m, m2), z = n == -INFINITY ? 0.0f : n;
+  l = l * exp2_fast(m - z) + l2 * exp2_fast(m2 - z);
+  m = n;
+}
+
+// ---- few rows: scores kept --------------------------------------------------------------
+
+constexpr int kPart = 256;  // tokens per unit: four tiles per wave
+constexpr int kTiles = kPart / PKV_TILE / kWaves;
+
+__host__ __device__ inline int quads(int rows) { return rows > 4 ? (rows + 3) / 4 : 1; }
+
+// Workspace: [scores: segment][R / 4][tokens][4] f32, [parts: segment][parts][8] (m, l).
+struct FewParts {
+  int64_t tokens, parts, scores, total;
+  __host__ __device__ FewParts(int64_t segs, int rows, int64_t cap) {
+    tokens = (cap + kPart - 1) / kPart * kPart;
+    parts = tokens / kPart;
+    scores = segs * quads(rows) * tokens * 16;
+    total = scores + segs * parts * kFewRows * 8;
+  }
+};
+
+// S = Q K^T with query row 4 r + jj in row 4 jj + r of the 16x16 tile: its four
+// rows per lane are then the lane's registers r, and a call of at most 4 rows has
+// one score per lane and tile, a call of 8 two.
+template <typename C, int NR>
+__global__ __launch_bounds__(kThreads) void mass_scores_kernel(const MassArgs a, const FewParts w) {
+  __shared__ float s_ml[kWaves][NR * 4][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
+  const Geo &g = a.g;
+  const f4 zero = register_zero();
+  Units u;
+  u.start(a, kPart, lane);
+  for (int64_t unit = blockIdx.x; u.find(a, kPart, unit, lane); unit += gridDim.x) {
+    const int t0 = u.part * kPart + wave * (kTiles * PKV_TILE);
+    const int ids = tile_page<kTiles>(a, u.b, t0, u.L, lane);
+    uint32_t kw[kTiles][C::LW], mw[kTiles][C::NG];
+    bool there[kTiles];
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const int id = __builtin_amdgcn_readlane(ids, i);
+      there[i] = id >= 0;
+      const int slot = (t0 + i * PKV_TILE) % g.page;
+      const uint8_t *head = a.pool + (int64_t)max(id, 0) * g.page_bytes + (int64_t)u.kh * g.head_bytes;
+#pragma unroll
+      for (int k = 0; k < C::LW; ++k) kw[i][k] = 0;
+#pragma unroll
+      for (int k = 0; k < C::NG; ++k) mw[i][k] = 0;
+      if (there[i]) {
+        load_payload<C, true>(kw[i], head + (slot / PKV_TILE) * g.tile_bytes, lane);
+        if constexpr (C::QUANT) {
+          const uint32_t *meta = (const uint32_t *)(head + g.kmeta_offset) + (slot + col) * C::NG;
+#pragma unroll
+          for (int k = 0; k < C::NG; ++k) mw[i][k] = meta[k];
+        }
+      }
+    }
+    typename C::KT q[C::KB];
+    float qs_row[C::NG], mult_row;
+    query_operands<C>(a, u.b, u.kh, 4 * (col & 3) + (col >> 2), jj, q, mult_row, qs_row);
+    float qs[NR][C::NG], mult[NR], m[NR], l[NR], s[NR][kTiles];
+    int sees[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int row = 4 * r + jj;
+      sees[r] = row < a.rows ? row_sees(a, u.b, row / a.gqa, u.L) : 0;
+      mult[r] = __shfl(mult_row, 4 * jj + r, 64);
+#pragma unroll
+      for (int k = 0; k < C::NG; ++k) qs[r][k] = __shfl(qs_row[k], 4 * jj + r, 64);
+    }
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      f4 acc[C::NG];
+#pragma unroll
+      for (int k = 0; k < C::NG; ++k) acc[k] = zero;
+#pragma unroll
+      for (int kb = 0; kb < C::KB; ++kb)
+        acc[kb / C::GB] = FloatOps<C::OPS>::qk(q[kb], k_operand<C>(kw[i], kb), acc[kb / C::GB]);
+      const int t = t0 + i * PKV_TILE + col;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float x = 0.0f;
+        if constexpr (C::QUANT) {
+#pragma unroll
+          for (int k = 0; k < C::NG; ++k) x = fmaf(f16_bits_to_f32(mw[i][k] >> 16), qs[r][k], x);
+#pragma unroll
+          for (int k = 0; k < C::NG; ++k) x = fmaf(f16_bits_to_f32(mw[i][k]), acc[k][r], x);
+        } else {
+          x = acc[0][r];
+        }
+        s[r][i] = there[i] && t < sees[r] ? x * mult[r] : -INFINITY;
+      }
+    }
+    const int64_t seg = (int64_t)u.b * g.hk + u.kh;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float *to = (float *)a.workspace + ((seg * quads(a.rows) + r) * w.tokens + t0 + col) * 4 + jj;
+      m[r] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        m[r] = fmaxf(m[r], s[r][i]);
+        to[i * PKV_TILE * 4] = s[r][i];  // (the row of parts is whole: nothing past it is written)
+      }
+      const float z = m[r] == -INFINITY ? 0.0f : m[r];
+      l[r] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) l[r] += exp2_fast(s[r][i] - z);
+      // the row's 16 lanes
+      float mm = m[r];
+      mm = fmaxf(mm, row_xchg<0xB1>(mm));
+      mm = fmaxf(mm, row_xchg<0x4E>(mm));
+      mm = fmaxf(mm, row_xchg<0x141>(mm));
+      mm = fmaxf(mm, row_xchg<0x140>(mm));
+      float ll = l[r] * exp2_fast(z - (mm == -INFINITY ? 0.0f : mm));
+      if (m[r] == -INFINITY) ll = l[r];  // 0, or NaN
+      ll += row_xchg<0xB1>(ll);
+      ll += row_xchg<0x4E>(ll);
+      ll += row_xchg<0x141>(ll);
+      ll += row_xchg<0x140>(ll);
+      if (col == 0) {
+        s_ml[wave][4 * r + jj][0] = mm;
+        s_ml[wave][4 * r + jj][1] = ll;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x < NR * 4) {
+      float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) join(mm, ll, s_ml[k][threadIdx.x][0], s_ml[k][threadIdx.x][1]);
+      float *to = (float *)((char *)a.workspace + w.scores) +
+                  ((seg * w.parts + u.part) * kFewRows + threadIdx.x) * 2;
+      to[0] = mm;
+      to[1] = ll;
+    }
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ void store_mass(const MassArgs &a, int b, int kh, int row, int t, float sum) {
+  const int64_t at = ((int64_t)row * a.g.hk + kh) * a.width + t;
+  const bool old = a.mass && (!a.counted || t < a.counted[b]);
+  a.out[at] = (old ? a.mass[at] : 0.0f) + sum;
+}
+__device__ __forceinline__ int mass_row(const MassArgs &a, int b) {
+  const int row = a.out_rows ? a.out_rows[b] : b;
+  return row >= 0 && row < a.mass_rows ? row : -1;
+}
+
+constexpr int kSumPart = 1024;  // tokens per unit of the second launch
+
+template <int NR>
+__global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a, const FewParts w) {
+  __shared__ float s_lse[kFewRows];
+  const int lane = threadIdx.x & 63;
+  Units u;
+  u.start(a, kSumPart, lane);
+  for (int64_t unit = blockIdx.x; u.find(a, kSumPart, unit, lane); unit += gridDim.x) {
+    const int row = mass_row(a, u.b);
+    if (row < 0) continue;
+    const int64_t seg = (int64_t)u.b * a.g.hk + u.kh;
+    // the rows' log-sum-exps: 32 lanes per row
+    {
+      const int r = threadIdx.x / 32, parts = (u.L + kPart - 1) / kPart;
+      const float2 *ml = (const float2 *)((const char *)a.workspace + w.scores) + seg * w.parts * kFewRows + r;
+      float m = -INFINITY, l = 0.0f;
+      if (r < NR * 4)
+        for (int p = threadIdx.x % 32; p < parts; p += 32) {
+          const float2 x = ml[(int64_t)p * kFewRows];
+          join(m, l, x.x, x.y);
+        }
+#pragma unroll
+      for (int k = 16; k > 0; k /= 2) join(m, l, __shfl_xor(m, k, 64), __shfl_xor(l, k, 64));
+      __syncthreads();
+      // a row that sees nothing weighs nothing
+      if (threadIdx.x % 32 == 0 && r < kFewRows) s_lse[r] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
+      __syncthreads();
+    }
+    const float *scores = (const float *)a.workspace + seg * quads(a.rows) * w.tokens * 4;
+    float4 s[NR][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = u.part * kSumPart + i * kThreads + threadIdx.x;
+      if (t < u.L)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r][i] = *(const float4 *)(scores + ((int64_t)r * w.tokens + t) * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = u.part * kSumPart + i * kThreads + threadIdx.x;
+      if (t >= u.L) continue;
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float x[4] = {s[r][i].x, s[r][i].y, s[r][i].z, s[r][i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // a token that the row does not see adds 0 also where the row's sum is NaN
+          sum += x[k] == -INFINITY ? 0.0f : exp2_fast(x[k] - s_lse[4 * r + k]);
+      }
+      store_mass(a, u.b, u.kh, row, t, sum);
+    }
+  }
+}
+
+// ---- many rows: K twice -----------------------------------------------------------------
+
+// Rows in blocks of 16.  Workspace: query operands [segment][block][KB][64 lanes]
+// 16 bytes; per row [segment][block][16]: multiplier, tokens seen (as int), group
+// sums [NG], log-sum-exp; per block the most that any of its rows sees; parts
+// [segment][parts][rows] (m, l).
+struct ManyParts {
+  int64_t blocks, parts, ops, mult, sees, qs, lse, most, ml, total;
+  int part;  // tokens per unit
+  __host__ __device__ ManyParts(int64_t segs, int rows, int64_t cap, int dp, int ng) {
+    part = 16 * kWaves * (dp > 128 ? 2 : 4);
+    blocks = (rows + 15) / 16;
+    parts = (cap + part - 1) / part;
+    const int64_t n = segs * blocks;
+    ops = 0;
+    mult = ops + n * 16 * dp * 2;
+    sees = mult + n * 16 * 4;
+    qs = sees + n * 16 * 4;
+    lse = qs + n * 16 * ng * 4;
+    most = lse + n * 16 * 4;
+    ml = (most + n * 4 + 15) / 16 * 16;
+    total = ml + segs * parts * blocks * 16 * 8;
+  }
+};
+
+template <typename C>
+__global__ __launch_bounds__(kThreads) void mass_prepare_kernel(const MassArgs a, const ManyParts w) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
+  const int64_t n = (int64_t)blockIdx.x * kWaves + wave;  // (segment, block)
+  if (n >= w.blocks * a.batch * a.g.hk) return;
+  const int64_t seg = n / w.blocks;
+  const int block = (int)(n % w.blocks), b = (int)(seg / a.g.hk), kh = (int)(seg % a.g.hk);
+  const int row = block * 16 + col, L = max(0, mass_len(a, b));
+  typename C::KT q[C::KB];
+  float qs[C::NG], mult;
+  query_operands<C>(a, b, kh, row, jj, q, mult, qs);
+  const int sees = row < a.rows ? row_sees(a, b, row / a.gqa, L) : 0;
+  if (sees == 0) {  // a row that is not live may hold anything
+#pragma unroll
+    for (int kb = 0; kb < C::KB; ++kb) q[kb] = typename C::KT{};
+#pragma unroll
+    for (int k = 0; k < C::NG; ++k) qs[k] = 0.0f;
+    mult = 0.0f;
+  }
+  char *base = (char *)a.workspace;
+#pragma unroll
+  for (int kb = 0; kb < C::KB; ++kb)
+    *(u4 *)(base + w.ops + ((n * C::KB + kb) * 64 + lane) * 16) = __builtin_bit_cast(u4, q[kb]);
+  int most = sees;
+  most = max(most, __shfl_xor(most, 1, 64));
+  most = max(most, __shfl_xor(most, 2, 64));
+  most = max(most, __shfl_xor(most, 4, 64));
+  most = max(most, __shfl_xor(most, 8, 64));
+  if (lane == 0) ((int *)(base + w.most))[n] = most;
+  if (jj == 0) {
+    ((float *)(base + w.mult))[n * 16 + col] = mult;
+    ((int *)(base + w.sees))[n * 16 + col] = sees;
+    if (C::QUANT)
+#pragma unroll
+      for (int k = 0; k < C::NG; ++k) ((float *)(base + w.qs))[(n * C::NG + k) * 16 + col] = qs[k];
+  }
+}
+
+// A wave's tiles as operands.
+template <typename C, int N>
+struct KTiles {
+  typename C::KT k[N][C::KB];
+  bool there[N];
+
+  // The head block of each tile, for its metadata.
+  __device__ __forceinline__ void load(const MassArgs &a, const Units &u, int t0, int lane,
+                                       const uint8_t *(&meta)[N]) {
+    const Geo &g = a.g;
+    const int ids = tile_page<N>(a, u.b, t0, u.L, lane);
+    uint32_t w[N][C::LW];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = __builtin_amdgcn_readlane(ids, i);
+      there[i] = id >= 0;
+      const int slot = (t0 + i * PKV_TILE) % g.page;
+      const uint8_t *head = a.pool + (int64_t)max(id, 0) * g.page_bytes + (int64_t)u.kh * g.head_bytes;
+      meta[i] = head + g.kmeta_offset + (int64_t)slot * C::NG * 4;
+#pragma unroll
+      for (int j = 0; j < C::LW; ++j) w[i][j] = 0;
+      if (there[i]) load_payload<C>(w[i], head + (slot / PKV_TILE) * g.tile_bytes, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int kb = 0; kb < C::KB; ++kb) k[i][kb] = k_operand<C>(w[i], kb);
+  }
+};
+
+template <typename C>
+__device__ __forceinline__ void load_block(const char *base, const ManyParts &w, int64_t n, int lane,
+                                           typename C::KT (&q)[C::KB]) {
+#pragma unroll
+  for (int kb = 0; kb < C::KB; ++kb)
+    q[kb] = __builtin_bit_cast(typename C::KT, *(const u4 *)(base + w.ops + ((n * C::KB + kb) * 64 + lane) * 16));
+}
+
+// The (max, sum) of each row over the unit's tokens: S^T = K Q^T, a lane has one
+// query row (its column) and four tokens of each tile.
+template <typename C, int N>
+__global__ __launch_bounds__(kThreads) void mass_parts_kernel(const MassArgs a, const ManyParts w) {
+  constexpr int kBatch = 32;  // row blocks between two joins of the waves
+  __shared__ float2 s_ml[kWaves][kBatch * 16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
+  char *base = (char *)a.workspace;
+  const f4 zero = register_zero();
+  Units u;
+  u.start(a, w.part, lane);
+  for (int64_t unit = blockIdx.x; u.find(a, w.part, unit, lane); unit += gridDim.x) {
+    const int t0 = u.part * w.part + wave * (N * PKV_TILE);
+    const int64_t seg = (int64_t)u.b * a.g.hk + u.kh;
+    const uint8_t *meta[N];
+    KTiles<C, N> tiles;
+    tiles.load(a, u, t0, lane, meta);
+    uint32_t mw[N][4 * C::NG];
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      all = all && tiles.there[i];
+#pragma unroll
+      for (int k = 0; k < 4 * C::NG; ++k) mw[i][k] = 0;
+      if (C::QUANT && tiles.there[i])
+#pragma unroll
+        for (int k = 0; k < C::NG; ++k) {
+          const u4 x = ((const u4 *)meta[i])[jj * C::NG + k];
+          mw[i][4 * k] = x.x; mw[i][4 * k + 1] = x.y; mw[i][4 * k + 2] = x.z; mw[i][4 * k + 3] = x.w;
+        }
+    }
+    for (int64_t b0 = 0; b0 < w.blocks; b0 += kBatch) {
+      const int nb = (int)min((int64_t)kBatch, w.blocks - b0);
+      for (int k = 0; k < nb; ++k) {
+        const int64_t n = seg * w.blocks + b0 + k;
+        float m = -INFINITY, l = 0.0f;
+        if (((const int *)(base + w.most))[n] > t0) {
+          typename C::KT q[C::KB];
+          load_block<C>(base, w, n, lane, q);
+          const float mult = ((const float *)(base + w.mult))[n * 16 + col];
+          const int sees = ((const int *)(base + w.sees))[n * 16 + col];
+          float qs[C::NG];
+          if (C::QUANT)
+#pragma unroll
+            for (int j = 0; j < C::NG; ++j) qs[j] = ((const float *)(base + w.qs))[(n * C::NG + j) * 16 + col];
+          float s[N][4];
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            f4 acc[C::NG];
+#pragma unroll
+            for (int j = 0; j < C::NG; ++j) acc[j] = zero;
+#pragma unroll
+            for (int kb = 0; kb < C::KB; ++kb)
+              acc[kb / C::GB] = FloatOps<C::OPS>::qk(tiles.k[i][kb], q[kb], acc[kb / C::GB]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              float x = 0.0f;
+              if constexpr (C::QUANT) {
+#pragma unroll
+                for (int j = 0; j < C::NG; ++j) x = fmaf(f16_bits_to_f32(mw[i][r * C::NG + j] >> 16), qs[j], x);
+#pragma unroll
+                for (int j = 0; j < C::NG; ++j) x = fmaf(f16_bits_to_f32(mw[i][r * C::NG + j]), acc[j][r], x);
+              } else {
+                x = acc[0][r];
+              }
+              x *= mult;
+              s[i][r] = tiles.there[i] && t0 + i * PKV_TILE + 4 * jj + r < sees ? x : -INFINITY;
+              m = fmaxf(m, s[i][r]);
+            }
+          }
+          const float mm = xor32_max(xor16_max(m)), z = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l += exp2_fast(s[i][r] - z);
+          l = xor32_add(xor16_add(l));
+          m = mm;
+        }
+        if (jj == 0) s_ml[wave][k * 16 + col] = float2{m, l};
+      }
+      __syncthreads();
+      float2 *to = (float2 *)(base + w.ml) + ((seg * w.parts + u.part) * w.blocks + b0) * 16;
+      for (int r = threadIdx.x; r < nb * 16; r += kThreads) {
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) join(m, l, s_ml[k][r].x, s_ml[k][r].y);
+        to[r] = float2{m, l};
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Each row's log-sum-exp from its parts: 16 rows of 16 lanes per workgroup.
+__global__ __launch_bounds__(kThreads) void mass_join_kernel(const MassArgs a, const ManyParts w) {
+  const int64_t rows = w.blocks * 16;
+  const int64_t seg = blockIdx.x / w.blocks, row = blockIdx.x % w.blocks * 16 + threadIdx.x % 16;
+  __shared__ float s_ml[2][16][17];
+  const int parts = (max(0, mass_len(a, (int)(seg / a.g.hk))) + w.part - 1) / w.part, slice = threadIdx.x / 16;
+  const float2 *ml = (const float2 *)((const char *)a.workspace + w.ml) + seg * w.parts * rows + row;
   float m = -INFINITY, l = 0.0f;
-  for (int t = threadIdx.x; t < see; t += kThreads) {
-    const uint8_t *head = token_head(a, b, kh, t);
-    if (!head) continue;
-    const float s = score(a, head, t, q);
-    const float n = fmaxf(m, s);
-    l = l * expf(m - n) + expf(s - n);
-    m = n;
+  for (int p = slice; p < parts; p += 16) {
+    const float2 x = ml[p * rows];
+    join(m, l, x.x, x.y);
   }
-  part[0][threadIdx.x] = m;
-  part[1][threadIdx.x] = l;
+  s_ml[0][slice][threadIdx.x % 16] = m;
+  s_ml[1][slice][threadIdx.x % 16] = l;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float mm = -INFINITY, ll = 0.0f;
-    for (int i = 0; i < kThreads; ++i) mm = fmaxf(mm, part[0][i]);
-    for (int i = 0; i < kThreads; ++i)
-      if (part[1][i] != 0.0f) ll += part[1][i] * expf(part[0][i] - mm);
-    ((float *)a.workspace)[blockIdx.x] = ll == 0.0f ? INFINITY : mm + logf(ll);  // a row that sees nothing weighs nothing
+  if (slice == 0) {
+    for (int k = 1; k < 16; ++k) join(m, l, s_ml[0][k][threadIdx.x], s_ml[1][k][threadIdx.x]);
+    ((float *)((char *)a.workspace + w.lse))[seg * rows + row] =
+        l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);  // a row that sees nothing weighs nothing
   }
 }
 
-__global__ __launch_bounds__(kThreads) void mass_sum_kernel(const MassArgs a) {
-  __shared__ float q[256];
-  const int seg = blockIdx.y, b = seg / a.g.hk, kh = seg % a.g.hk;
-  const int L = mass_len(a, b);
-  const int t0 = blockIdx.x * kThreads, t = t0 + threadIdx.x;
-  const int out_row = a.out_rows ? a.out_rows[b] : b;
-  if (t0 >= L || out_row < 0 || out_row >= a.mass_rows) return;
-  const uint8_t *head = t < L ? token_head(a, b, kh, t) : nullptr;
-  float sum = 0.0f;
-  for (int row = 0; row < a.rows; ++row) {
-    const int see = row_sees(a, b, row / a.gqa, L);
-    __syncthreads();
-    load_query(a, b, kh, row, q);
-    __syncthreads();
-    if (head && t < see) sum += expf(score(a, head, t, q) - ((const float *)a.workspace)[seg * a.rows + row]);
+// The weights summed over the rows: S = Q K^T, a lane has one token of each tile
+// and four query rows.
+template <typename C, int N>
+__global__ __launch_bounds__(kThreads) void mass_sum_kernel(const MassArgs a, const ManyParts w) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
+  const char *base = (const char *)a.workspace;
+  const f4 zero = register_zero();
+  Units u;
+  u.start(a, w.part, lane);
+  for (int64_t unit = blockIdx.x; u.find(a, w.part, unit, lane); unit += gridDim.x) {
+    const int t0 = u.part * w.part + wave * (N * PKV_TILE);
+    const int row = mass_row(a, u.b);
+    if (t0 >= u.L || row < 0) continue;
+    const int64_t seg = (int64_t)u.b * a.g.hk + u.kh;
+    const uint8_t *meta[N];
+    KTiles<C, N> tiles;
+    tiles.load(a, u, t0, lane, meta);
+    float scale[N][C::NG], bias[N][C::NG], sum[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      sum[i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < C::NG; ++j) {
+        uint32_t x = 0;
+        if (C::QUANT && tiles.there[i]) x = ((const uint32_t *)meta[i])[col * C::NG + j];
+        scale[i][j] = f16_bits_to_f32(x);
+        bias[i][j] = f16_bits_to_f32(x >> 16);
+      }
+    }
+    for (int64_t k = 0; k < w.blocks; ++k) {
+      const int64_t n = seg * w.blocks + k;
+      if (((const int *)(base + w.most))[n] <= t0) continue;
+      typename C::KT q[C::KB];
+      load_block<C>(base, w, n, lane, q);
+      const f4 mult = *(const f4 *)(base + w.mult + (n * 16 + 4 * jj) * 4);
+      const f4 lse = *(const f4 *)(base + w.lse + (n * 16 + 4 * jj) * 4);
+      const int4 sees = *(const int4 *)(base + w.sees + (n * 16 + 4 * jj) * 4);
+      const int see[4] = {sees.x, sees.y, sees.z, sees.w};
+      f4 qs[C::NG];
+      if (C::QUANT)
+#pragma unroll
+        for (int j = 0; j < C::NG; ++j) qs[j] = *(const f4 *)(base + w.qs + ((n * C::NG + j) * 16 + 4 * jj) * 4);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        f4 acc[C::NG];
+#pragma unroll
+        for (int j = 0; j < C::NG; ++j) acc[j] = zero;
+#pragma unroll
+        for (int kb = 0; kb < C::KB; ++kb)
+          acc[kb / C::GB] = FloatOps<C::OPS>::qk(q[kb], tiles.k[i][kb], acc[kb / C::GB]);
+        const int t = t0 + i * PKV_TILE + col;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = 0.0f;
+          if constexpr (C::QUANT) {
+#pragma unroll
+            for (int j = 0; j < C::NG; ++j) x = fmaf(bias[i][j], qs[j][r], x);
+#pragma unroll
+            for (int j = 0; j < C::NG; ++j) x = fmaf(scale[i][j], acc[j][r], x);
+          } else {
+            x = acc[0][r];
+          }
+          const float p = exp2_fast(fmaf(x, mult[r], -lse[r]));
+          sum[i] += tiles.there[i] && t < see[r] ? p : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float all = xor32_add(xor16_add(sum[i]));
+      const int t = t0 + i * PKV_TILE + col;
+      if (jj == 0 && t < u.L) store_mass(a, u.b, u.kh, row, t, all);
+    }
   }
-  if (t < L) {
-    const int64_t at = ((int64_t)out_row * a.g.hk + kh) * a.width + t;
-    const bool old = a.mass && (!a.counted || t < a.counted[b]);
-    a.out[at] = (old ? a.mass[at] : 0.0f) + sum;
+}
+
+// ---- launches -----------------------------------------------------------------------------
+
+// Scores are kept where they cost less than reading K again and take no more
+// than this.
+constexpr int64_t kMostScores = (int64_t)2 << 30;
+
+bool keeps_scores(const Geo &g, int64_t segs, int rows, int64_t cap) {
+  return rows <= kFewRows && FewParts(segs, rows, cap).scores <= kMostScores;
+}
+
+// Workgroups of a walk over `units` units: no more than stay resident.
+int walkers(int64_t units) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(units, 8 * (int64_t)std::max(1, device_cus())));
+}
+
+template <typename C>
+void launch(hipStream_t stream, const MassArgs &a, int64_t cap) {
+  const int64_t segs = (int64_t)a.batch * a.g.hk;
+  if (keeps_scores(a.g, segs, a.rows, cap)) {
+    const FewParts w(segs, a.rows, cap);
+    const dim3 grid(walkers(segs * w.parts)), second(walkers(segs * ((cap + kSumPart - 1) / kSumPart)));
+    if (a.rows <= 4) {
+      hipLaunchKernelGGL((mass_scores_kernel<C, 1>), grid, dim3(kThreads), 0, stream, a, w);
+      hipLaunchKernelGGL((mass_weights_kernel<1>), second, dim3(kThreads), 0, stream, a, w);
+    } else {
+      hipLaunchKernelGGL((mass_scores_kernel<C, 2>), grid, dim3(kThreads), 0, stream, a, w);
+      hipLaunchKernelGGL((mass_weights_kernel<2>), second, dim3(kThreads), 0, stream, a, w);
+    }
+    return;
   }
+  constexpr int N = C::KB > 4 ? 2 : 4;
+  const ManyParts w(segs, a.rows, cap, a.g.dp, C::QUANT ? C::NG : 0);
+  const dim3 grid(walkers(segs * w.parts));
+  const unsigned blocks = (unsigned)(segs * w.blocks);
+  hipLaunchKernelGGL((mass_prepare_kernel<C>), dim3((blocks + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a, w);
+  hipLaunchKernelGGL((mass_parts_kernel<C, N>), grid, dim3(kThreads), 0, stream, a, w);
+  hipLaunchKernelGGL(mass_join_kernel, dim3(blocks), dim3(kThreads), 0, stream, a, w);
+  hipLaunchKernelGGL((mass_sum_kernel<C, N>), grid, dim3(kThreads), 0, stream, a, w);
+}
+
+template <int BITS, int DP>
+void launch_group(hipStream_t stream, const MassArgs &a, int64_t cap) {
+  if (a.g.group == 32) return launch<MassCfg<BITS, DP, 32, 1>>(stream, a, cap);
+  if (a.g.group == 64) return launch<MassCfg<BITS, DP, 64, 1>>(stream, a, cap);
+  if constexpr (DP >= 128) launch<MassCfg<BITS, DP, 128, 1>>(stream, a, cap);
+}
+
+template <int BITS>
+void launch_dim(hipStream_t stream, const MassArgs &a, int64_t cap) {
+  if (a.g.dp == 64) launch_group<BITS, 64>(stream, a, cap);
+  else if (a.g.dp == 128) launch_group<BITS, 128>(stream, a, cap);
+  else launch_group<BITS, 256>(stream, a, cap);
+}
+
+template <int FK>
+void launch_float(hipStream_t stream, const MassArgs &a, int64_t cap) {
+  if (a.g.dp == 64) launch<MassCfg<16, 64, 32, FK>>(stream, a, cap);
+  else if (a.g.dp == 128) launch<MassCfg<16, 128, 32, FK>>(stream, a, cap);
+  else launch<MassCfg<16, 256, 32, FK>>(stream, a, cap);
 }
 
 }  // namespace
 
-int64_t mass_workspace(const Geo &g, int batch, int rows, int /*max_pages*/) {
-  return (int64_t)batch * g.hk * rows * 4;
+int64_t mass_workspace(const Geo &g, int batch, int rows, int max_pages) {
+  const int64_t segs = (int64_t)batch * g.hk, cap = (int64_t)max_pages * g.page;
+  if (keeps_scores(g, segs, rows, cap)) return FewParts(segs, rows, cap).total;
+  return ManyParts(segs, rows, cap, g.dp, g.ng).total;
 }
 
 hipError_t launch_mass(hipStream_t stream, const MassArgs &a) {
-  const int segs = a.batch * a.g.hk;
-  const int64_t tokens = min((int64_t)a.max_pages * a.g.page, a.width);
-  hipLaunchKernelGGL(mass_lse_kernel, dim3(segs * a.rows), dim3(kThreads), 0, stream, a);
-  hipLaunchKernelGGL(mass_sum_kernel, dim3((tokens + kThreads - 1) / kThreads, segs), dim3(kThreads), 0, stream, a);
+  const int64_t cap = (int64_t)a.max_pages * a.g.page;  // as the workspace is sized, whatever the mass's width
+  if (a.g.bits == 8) launch_dim<8>(stream, a, cap);
+  else if (a.g.bits == 4) launch_dim<4>(stream, a, cap);
+  else if (a.g.float_kind == 0) launch_float<0>(stream, a, cap);
+  else launch_float<1>(stream, a, cap);
   return hipGetLastError();
 }
 
