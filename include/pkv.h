@@ -454,7 +454,8 @@ int pkv_evict_pages(void *stream, const pkv_layout *layout, void *const *pools, 
  * done has one candidate, (w, pad_token) at its score.  A beam whose score is not
  * finite, or whose logits hold +inf, NaN or nothing but -inf, has none, and a
  * logit of -inf is none.  Where there are too few, the rest is -inf, at the lowest
- * pairs that are no candidates.  Candidates are compared in 64 bits.
+ * pairs that are no candidates.  Candidates of different beams are compared in 64
+ * bits, those of one beam by their logits.
  *
  *  logits     : [groups][beams][vocab], kind 0 = bf16, 1 = f16, 2 = f32; strides in
  *               elements, each row's tokens adjacent

@@ -10,6 +10,14 @@
 // Which of two beams' tokens comes first hangs on the last digits of their
 // log-sum-exps, so those, and the comparison, are in 64 bits; within a beam the
 // logits themselves give the order.
+//
+// One launch reads the logits, in chunks of a row held in registers: the chunk's
+// maximum and sum of exponentials, and its `count` best tokens.  Each wave finds
+// the count-th largest of its lanes' maxima, by bisection on the bits of the order;
+// what reaches the largest of the waves' bounds, a few times `count`, goes to LDS
+// and is ranked there.  A second launch joins the chunks' sums and does the same
+// with the lists' entries.  Memory-bound: one read of the
+// logits.
 #include "pkv_cache_ops.h"
 
 namespace pkv {
@@ -17,42 +25,11 @@ namespace pkv {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kHeld = 16;  // candidates per thread of the second launch in registers
+constexpr int kList = 1024;  // candidates in LDS
 
-struct RowBest {
-  double log_sum;  // of exp(x - most); not finite: the row has no candidates
-  float most;      // apart from the sum, which it would swallow where it is large
-  int32_t n;       // its best tokens, in order
-};
-
-struct BeamParts {
-  RowBest *row;
-  float *value;
-  int32_t *token;
-  __device__ BeamParts(const BeamArgs &a) {
-    const int64_t rows = (int64_t)a.groups * a.beams;
-    row = (RowBest *)a.workspace;
-    value = (float *)(row + rows);
-    token = (int32_t *)(value + rows * a.count);
-  }
-};
-
-__device__ __forceinline__ float logit(const BeamArgs &a, int64_t base, int v) {
-  if (a.kind == 2) return ((const float *)a.logits)[base + v];
-  return bits_to_float(((const uint16_t *)a.logits)[base + v], a.kind);
-}
-
-template <typename T, typename F>
-__device__ __forceinline__ T block_reduce(T v, T *s, F f) {
-  __syncthreads();
-  s[threadIdx.x] = v;
-  for (int k = kThreads / 2; k > 0; k /= 2) {
-    __syncthreads();
-    if ((int)threadIdx.x < k) s[threadIdx.x] = f(s[threadIdx.x], s[threadIdx.x + k]);
-  }
-  __syncthreads();
-  return s[0];
-}
-
+// Order of float32 as unsigned numbers; -inf and below (nothing) as 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -61,111 +38,456 @@ __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// One workgroup per row: its log-sum-exp, then its best tokens one after another.
-__global__ __launch_bounds__(kThreads) void beam_row_kernel(const BeamArgs a) {
-  __shared__ double s_sum[kThreads];
-  __shared__ float s_max[kThreads];
-  __shared__ uint64_t s_key[kThreads];
-  const BeamParts p(a);
-  const int64_t row = blockIdx.x;
-  const int64_t base = row / a.beams * a.group_stride + row % a.beams * a.beam_stride;
-  float m = -INFINITY;
-  bool nan = false;
-  for (int v = threadIdx.x; v < a.vocab; v += kThreads) {
-    const float x = logit(a, base, v);
-    nan = nan || x != x;
-    m = fmaxf(m, x);
+// Of a chunk: its sum of exp(x - most) and its maximum (NaN where there is a NaN).
+struct Chunk {
+  double sum;
+  float most;
+};
+
+// Workspace: [groups][beams][chunks] Chunk, then as many lists [count] of (order, token).
+struct BeamParts {
+  int chunks;
+  int64_t lists, total;
+  __host__ __device__ BeamParts(int groups, int beams, int vocab, int count, int chunk) {
+    chunks = (vocab + chunk - 1) / chunk;
+    const int64_t n = (int64_t)groups * beams * chunks;
+    lists = n * (int64_t)sizeof(Chunk);
+    total = lists + n * count * 8;
   }
-  m = block_reduce(nan ? INFINITY : m, s_max, [](float x, float y) { return fmaxf(x, y); });
-  double sum = 0.0;
-  const bool dead = !(fabsf(m) < INFINITY);
-  if (!dead)
-    for (int v = threadIdx.x; v < a.vocab; v += kThreads) sum += exp((double)logit(a, base, v) - (double)m);
-  sum = block_reduce(sum, s_sum, [](double x, double y) { return x + y; });
-  // order: the logit, then the lowest token; 0 is no token
-  uint64_t last = ~0ull;
-  int n = 0;
-  for (; n < a.count && !dead; ++n) {
-    uint64_t best = 0;
-    for (int v = threadIdx.x; v < a.vocab; v += kThreads) {
-      const float x = logit(a, base, v);
-      const uint64_t key = (uint64_t)order_key(x) << 32 | (uint32_t)(~v);
-      if (x > -INFINITY && key < last && key > best) best = key;
+};
+
+// Eight logits from v on (-inf from the end of the row on), wherever they lie: as
+// they are in memory.
+template <int KIND>
+struct Eight {
+  uint32_t w[KIND == 2 ? 8 : 4];
+
+  __device__ __forceinline__ void load(const BeamArgs &a, int64_t base, int v) {
+    if (v + 8 <= a.vocab) {
+      if constexpr (KIND == 2) __builtin_memcpy(w, (const float *)a.logits + base + v, 32);
+      else __builtin_memcpy(w, (const uint16_t *)a.logits + base + v, 16);
+      return;
     }
-    best = block_reduce(best, s_key, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
-    if (best == 0) break;
-    last = best;
-    if (threadIdx.x == 0) {
-      p.value[row * a.count + n] = key_value((uint32_t)(best >> 32));
-      p.token[row * a.count + n] = (int32_t)~(uint32_t)best;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = v + e < a.vocab;
+      if constexpr (KIND == 2) {
+        w[e] = in ? ((const uint32_t *)a.logits)[base + v + e] : 0xFF800000u;
+      } else {
+        const uint32_t x = in ? ((const uint16_t *)a.logits)[base + v + e] : KIND == 0 ? 0xFF80u : 0xFC00u;
+        w[e / 2] = e % 2 ? w[e / 2] | x << 16 : x;
+      }
     }
   }
-  if (threadIdx.x == 0) p.row[row] = RowBest{dead ? (double)INFINITY : log(sum), m, n};
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (KIND == 2) return __uint_as_float(w[e]);
+    else if constexpr (KIND == 0) return __uint_as_float(e % 2 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
+    else return f16_bits_to_f32(e % 2 ? w[e / 2] >> 16 : w[e / 2]);
+  }
+};
+
+// The largest bound that `count` of the wave's N x 64 keys reach, to BITS bits from
+// the top (the rest 0); 0 where fewer than `count` are above 0.
+template <int BITS, int N>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t (&key)[N], int count) {
+  uint32_t at = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 32 - BITS; --bit) {
+    const uint32_t next = at | 1u << bit;
+    int reach = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) reach += __popcll(__ballot(key[j] >= next));
+    if (reach >= count) at = next;
+  }
+  return at;
 }
 
-// One thread per group: the rows' lists are in order, so the best of their heads
-// is the next of all.
-__global__ void beam_merge_kernel(const BeamArgs a) {
-  const int group = blockIdx.x * blockDim.x + threadIdx.x;
-  if (group >= a.groups) return;
-  const BeamParts p(a);
-  int at[kMaxBeams];
-  for (int w = 0; w < a.beams; ++w) at[w] = 0;
-  const int64_t out = (int64_t)group * a.count;
-  int n = 0;
-  for (; n < a.count; ++n) {
-    double best = -INFINITY;
-    int bw = -1, bt = 0;
-    for (int w = 0; w < a.beams; ++w) {
-      const int64_t row = (int64_t)group * a.beams + w;
-      const float score = a.scores[row];
-      if (!(fabsf(score) < INFINITY)) continue;
-      double c;
-      int t;
-      if (a.done && a.done[row]) {
-        if (at[w] > 0) continue;
-        c = score;
-        t = a.pad_token;
-      } else {
-        const RowBest best_of = p.row[row];
-        if (!(fabs(best_of.log_sum) < INFINITY) || at[w] >= best_of.n) continue;
-        c = (double)score - best_of.log_sum + ((double)p.value[row * a.count + at[w]] - (double)best_of.most);
-        t = p.token[row * a.count + at[w]];
-      }
-      if (c > best) {
-        best = c;
-        bw = w;
-        bt = t;
-      }
+// Lane exchanges of a 64-bit value, as two halves, without LDS.
+template <int CTRL>
+__device__ __forceinline__ double row_xchg64(double v) {
+  const u2 h = __builtin_bit_cast(u2, v);
+  return __builtin_bit_cast(double, u2{(uint32_t)__builtin_amdgcn_mov_dpp((int)h.x, CTRL, 0xF, 0xF, false),
+                                       (uint32_t)__builtin_amdgcn_mov_dpp((int)h.y, CTRL, 0xF, 0xF, false)});
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += row_xchg64<0xB1>(v);
+  v += row_xchg64<0x4E>(v);
+  v += row_xchg64<0x141>(v);
+  v += row_xchg64<0x140>(v);
+  const u2 h = __builtin_bit_cast(u2, v);
+  const auto x = __builtin_amdgcn_permlane16_swap(h.x, h.x, false, false), y = __builtin_amdgcn_permlane16_swap(h.y, h.y, false, false);
+  v = __builtin_bit_cast(double, u2{x[0], y[0]}) + __builtin_bit_cast(double, u2{x[1], y[1]});
+  const u2 g = __builtin_bit_cast(u2, v);
+  const auto z = __builtin_amdgcn_permlane32_swap(g.x, g.x, false, false), t = __builtin_amdgcn_permlane32_swap(g.y, g.y, false, false);
+  return __builtin_bit_cast(double, u2{z[0], t[0]}) + __builtin_bit_cast(double, u2{z[1], t[1]});
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, row_xchg<0xB1>(v));
+  v = fmaxf(v, row_xchg<0x4E>(v));
+  v = fmaxf(v, row_xchg<0x141>(v));
+  v = fmaxf(v, row_xchg<0x140>(v));
+  return xor32_max(xor16_max(v));
+}
+
+// The list in LDS, in order: entry i's rank is the number of larger ones (they
+// differ in the token), counted by four lanes.  Keys are (order << 32 | ~token).
+template <typename F>
+__device__ __forceinline__ void ranked(const uint64_t *s_list, int n, int count, F store) {
+  for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
+    const int i = min(i0 + (int)threadIdx.x / 4, n - 1);
+    const uint64_t mine = s_list[i];
+    int rank = 0;
+#pragma unroll 8
+    for (int k = threadIdx.x % 4; k < n; k += 4) rank += s_list[k] > mine;
+    rank += __builtin_amdgcn_mov_dpp(rank, 0xB1, 0xF, 0xF, false);
+    rank += __builtin_amdgcn_mov_dpp(rank, 0x4E, 0xF, 0xF, false);
+    if (threadIdx.x % 4 == 0 && rank < count && i == i0 + (int)threadIdx.x / 4) store(rank, mine);
+  }
+}
+
+template <int KIND, int E>
+__global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, const BeamParts w) {
+  constexpr int V = E / 8;  // vectors of 8 per thread
+  __shared__ uint64_t s_list[kList];
+  __shared__ double s_sum[kWaves];
+  __shared__ float s_most[kWaves];
+  __shared__ uint32_t s_bound[kWaves];
+  __shared__ int s_n, s_nan;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x / w.chunks;
+  if (a.done && a.done[row]) return;  // its logits are not asked for
+  const int64_t base = row / a.beams * a.group_stride + row % a.beams * a.beam_stride;
+  const int v0 = (int)(blockIdx.x % w.chunks) * (E * kThreads) + threadIdx.x * 8;
+  Eight<KIND> x[V];
+  float vm[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) x[j].load(a, base, v0 + j * 8 * kThreads);
+  if (threadIdx.x == 0) s_n = s_nan = 0;
+  bool nan = false;
+  float m = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    vm[j] = x[j][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) vm[j] = __builtin_elementwise_maximum(vm[j], x[j][e]);  // NaN stays
+    m = __builtin_elementwise_maximum(m, vm[j]);
+  }
+  nan = m != m;
+  // A bound from the lanes' maxima; for many tokens from those of their vectors,
+  // which also do where masks leave lanes without a token.  bfloat16's order has 16
+  // bits, float16's 19, of float32's 24 are enough.
+  constexpr int kBits = KIND == 0 ? 16 : KIND == 1 ? 19 : 24;
+  auto key_of = [](float v) { return v == -INFINITY ? 0u : order_key(v); };
+  uint32_t bound;
+  if (V == 1 || a.count <= 16) {
+    const uint32_t key[1] = {key_of(m)};
+    bound = wave_bound<kBits>(key, a.count);
+  } else {
+    uint32_t key[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) key[j] = key_of(vm[j]);
+    bound = wave_bound<kBits>(key, a.count);
+  }
+  const float most = wave_max(m);
+  // exp(x - most) as 2^(x L - R), L = log2(e) in float32 and R the integer next to
+  // most L: the product is not rounded, R is exact, and 2^(R - most L) makes up for it
+  constexpr float kL = 1.4426950408889634f;
+  const float from = fabsf(most) < 8e6f ? rintf(most * kL) : most * kL;
+  const bool flat = !(fabsf(from) < INFINITY);  // rows that have no sum, or all at the type's end
+  float sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      sum += __builtin_amdgcn_exp2f(flat ? (x[j][e] - most) * kL : fmaf(x[j][e], kL, -from));
+  const double total = wave_sum64((double)sum) * (flat ? 1.0 : exp2((double)from - (double)most * (double)kL));
+  if (lane == 0) {
+    s_sum[wave] = total;
+    s_most[wave] = most;
+    s_bound[wave] = bound;
+  }
+  __syncthreads();
+  if (nan) s_nan = 1;
+  // what reaches the highest bound: `count` tokens at least, if there are as many
+  uint32_t least = 1;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) least = max(least, s_bound[k]);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (vm[j] == -INFINITY || order_key(vm[j]) < least) continue;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t k = order_key(x[j][e]);
+      if (k < least || x[j][e] == -INFINITY) continue;
+      const int at = atomicAdd(&s_n, 1);
+      if (at < kList) s_list[at] = (uint64_t)k << 32 | (uint32_t)~(v0 + j * 8 * kThreads + e);
     }
-    if (bw < 0) break;
-    ++at[bw];
-    a.out_scores[out + n] = (float)best;
-    a.parents[out + n] = bw;
-    a.tokens[out + n] = bt;
   }
-  const int found = n;
-  for (int64_t f = 0; n < a.count; ++f) {  // the lowest pairs that were not taken
-    const int w = (int)(f / a.vocab), t = (int)(f % a.vocab);
-    bool taken = false;
-    for (int k = 0; k < found; ++k) taken = taken || (a.parents[out + k] == w && a.tokens[out + k] == t);
-    if (taken) continue;
-    a.out_scores[out + n] = -INFINITY;
-    a.parents[out + n] = w;
-    a.tokens[out + n] = t;
-    ++n;
+  __syncthreads();
+  uint2 *list = (uint2 *)((char *)a.workspace + w.lists) + (int64_t)blockIdx.x * a.count;
+  int n = s_n;
+  if (n > kList) {
+    // more equal (or adjacent) tokens than the list holds: one after another
+    uint64_t last = ~0ull;
+    __shared__ uint64_t s_best[kWaves];
+    for (n = 0; n < a.count; ++n) {
+      uint64_t best = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint64_t k = (uint64_t)order_key(x[j][e]) << 32 | (uint32_t)~(v0 + j * 8 * kThreads + e);
+          if (x[j][e] > -INFINITY && k < last && k > best) best = k;
+        }
+#pragma unroll
+      for (int k = 1; k < 64; k *= 2) {
+        const uint64_t other = __shfl_xor((unsigned long long)best, k, 64);
+        best = other > best ? other : best;
+      }
+      __syncthreads();
+      if (lane == 0) s_best[wave] = best;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < kWaves; ++k) best = s_best[k] > best ? s_best[k] : best;
+      if (best == 0) break;
+      last = best;
+      if (threadIdx.x == 0) list[n] = uint2{(uint32_t)(best >> 32), ~(uint32_t)best};
+    }
+  } else {
+    ranked(s_list, n, a.count, [&](int rank, uint64_t k) { list[rank] = uint2{(uint32_t)(k >> 32), ~(uint32_t)k}; });
+    n = min(n, a.count);
   }
+  for (int k = n + (int)threadIdx.x; k < a.count; k += kThreads) list[k] = uint2{0u, 0u};  // 0: none
+  if (threadIdx.x < kWaves) {  // (four lanes of one row)
+    const float part = s_most[threadIdx.x];
+    float all = fmaxf(part, row_xchg<0xB1>(part));
+    all = fmaxf(all, row_xchg<0x4E>(all));
+    double sums = part > -INFINITY ? s_sum[threadIdx.x] * exp((double)part - (double)all) : 0.0;
+    sums += row_xchg64<0xB1>(sums);
+    sums += row_xchg64<0x4E>(sums);
+    if (threadIdx.x == 0) ((Chunk *)a.workspace)[blockIdx.x] = Chunk{sums, s_nan ? NAN : all};
+  }
+}
+
+// One workgroup per group of beams.
+__global__ __launch_bounds__(kThreads) void beam_merge_kernel(const BeamArgs a, const BeamParts w) {
+  struct Pair {
+    double c;
+    uint32_t key;  // the logit's: the order within a beam
+    int32_t beam, token;
+  };
+  __shared__ Pair s_list[kList], s_best[kWaves];
+  __shared__ double s_c[kList];
+  __shared__ double s_offset[kMaxBeams];  // score - log of the sum; -inf: no candidates
+  __shared__ float s_most[kMaxBeams];
+  __shared__ int s_n, s_reach[2][kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr double kNone = -(double)INFINITY;
+  const int64_t row0 = (int64_t)blockIdx.x * a.beams, out = (int64_t)blockIdx.x * a.count;
+  const Chunk *chunk = (const Chunk *)a.workspace + row0 * w.chunks;
+  const uint2 *lists = (const uint2 *)((const char *)a.workspace + w.lists) + row0 * w.chunks * a.count;
+  auto done = [&](int beam) { return a.done && a.done[row0 + beam]; };
+  // entry e of the beams' lists, requested before what it needs of their rows
+  const int entries = a.beams * w.chunks * a.count;  // (less than 2^31 pairs per group: so are these)
+  uint2 raw[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int e = threadIdx.x + k * kThreads;
+    raw[k] = uint2{0u, 0u};
+    if (k * kThreads < entries && e < entries) raw[k] = lists[e];
+  }
+  // a row's sum: lanes beside each other take its chunks
+  int width = 1;
+  while (width < 64 && width < w.chunks && width * 2 * a.beams <= kThreads) width *= 2;
+  const int beam = threadIdx.x / width, slice = threadIdx.x % width;
+  if (threadIdx.x == 0) s_n = 0;
+  if (beam < a.beams) {
+    const float score = a.scores[row0 + beam];
+    bool dead = !(fabsf(score) < INFINITY);
+    float most = -INFINITY;
+    double sum = 0.0;
+    if (!done(beam)) {
+      for (int k = slice; k < w.chunks; k += width) {
+        const float x = chunk[beam * w.chunks + k].most;
+        dead = dead || x != x;
+        most = fmaxf(most, x);
+      }
+      for (int k = 1; k < width; k *= 2) {
+        most = fmaxf(most, __shfl_xor(most, k, 64));
+        dead = __shfl_xor((int)dead, k, 64) || dead;
+      }
+      dead = dead || !(fabsf(most) < INFINITY);
+      for (int k = slice; k < w.chunks && !dead; k += width) {
+        const Chunk c = chunk[beam * w.chunks + k];
+        if (c.most > -INFINITY) sum += c.sum * exp((double)c.most - (double)most);
+      }
+      for (int k = 1; k < width; k *= 2) sum += __shfl_xor(sum, k, 64);
+    }
+    if (slice == 0) {
+      s_most[beam] = most;
+      s_offset[beam] = dead ? kNone : done(beam) ? (double)score : (double)score - log(sum);
+    }
+  }
+  __syncthreads();
+  // entry e, as loaded, as a candidate: false past its list's end
+  auto candidate = [&](int e, uint2 x, Pair &p) {
+    const int list = e / a.count, b = list / w.chunks;
+    p = Pair{s_offset[b], x.x, b, (int)x.y};
+    if (p.c == kNone) return false;
+    if (done(b)) {
+      p.key = 0u;
+      p.token = a.pad_token;
+      return e == b * w.chunks * a.count;  // (lists of rows that are done hold anything)
+    }
+    if (x.x == 0) return false;
+    p.c += (double)key_value(x.x) - (double)s_most[b];
+    return p.c > kNone;
+  };
+  // A bound that `count` candidates reach and few others: bisection on the bits of
+  // the candidates' order in float32 (rounding keeps it), until the rest fits easily.
+  constexpr int kIn = kHeld * kThreads;  // entries from there on are read again each time
+  Pair p;
+  uint32_t keys[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int e = threadIdx.x + k * kThreads;
+    keys[k] = 0u;
+    if (k * kThreads < entries && e < entries && candidate(e, raw[k], p)) keys[k] = order_key((float)p.c);
+  }
+  uint32_t least = 0;
+  for (int bit = 31, step = 0; bit >= 0; --bit, ++step) {
+    const uint32_t next = least | 1u << bit;
+    int reach = 0;
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (k * kThreads < entries) reach += __popcll(__ballot(keys[k] >= next));
+    if (entries > kIn) {
+      int more = 0;
+      for (int e = threadIdx.x + kIn; e < entries; e += kThreads)
+        more += candidate(e, lists[e], p) && order_key((float)p.c) >= next;
+      reach += wave_sum(more);
+    }
+    if (lane == 0) s_reach[step & 1][wave] = reach;
+    __syncthreads();
+    reach = 0;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) reach += s_reach[step & 1][k];
+    if (reach < a.count) continue;
+    least = next;
+    if (reach <= a.count + 16) break;
+  }
+  least = max(least, 1u);
+  auto take = [&](int e, uint2 x) {
+    candidate(e, x, p);
+    const int at = atomicAdd(&s_n, 1);
+    if (at < kList) {
+      s_list[at] = p;
+      s_c[at] = p.c;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (keys[k] >= least) take(threadIdx.x + k * kThreads, raw[k]);
+  for (int e = threadIdx.x + kIn; e < entries; e += kThreads)
+    if (candidate(e, lists[e], p) && order_key((float)p.c) >= least) take(e, lists[e]);
+  __syncthreads();
+  auto before = [](const Pair &x, const Pair &y) {
+    if (x.c != y.c) return x.c > y.c;
+    if (x.beam != y.beam) return x.beam < y.beam;
+    return x.key != y.key ? x.key > y.key : x.token < y.token;
+  };
+  auto put = [&](int rank, const Pair &p) {
+    a.out_scores[out + rank] = (float)p.c;
+    a.parents[out + rank] = p.beam;
+    a.tokens[out + rank] = p.token;
+  };
+  const int n = s_n;
+  if (n > kList) {
+    // more than LDS holds (then there are `count` of them): one after another
+    Pair last{(double)INFINITY, 0u, 0, 0};
+    for (int rank = 0; rank < a.count; ++rank) {
+      Pair best{kNone, 0u, INT32_MAX, 0};
+      for (int e = threadIdx.x; e < entries; e += kThreads)
+        if (candidate(e, lists[e], p) && before(last, p) && before(p, best)) best = p;
+      for (int k = 1; k < 64; k *= 2) {
+        Pair other;
+        other.c = __shfl_xor(best.c, k, 64);
+        other.key = __shfl_xor(best.key, k, 64);
+        other.beam = __shfl_xor(best.beam, k, 64);
+        other.token = __shfl_xor(best.token, k, 64);
+        if (before(other, best)) best = other;
+      }
+      __syncthreads();
+      if (lane == 0) s_best[wave] = best;
+      __syncthreads();
+      for (int k = 0; k < kWaves; ++k)
+        if (before(s_best[k], best)) best = s_best[k];
+      last = best;
+      if (threadIdx.x == 0) put(rank, best);
+    }
+    return;
+  }
+  // ranks, four lanes a candidate; candidates of one value (rare) in full
+  for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
+    const int i = min(i0 + (int)threadIdx.x / 4, n - 1);
+    const double c = s_c[i];
+    int rank = 0, level = 0;
+#pragma unroll 8
+    for (int k = threadIdx.x % 4; k < n; k += 4) {
+      const double x = s_c[k];
+      rank += x > c;
+      level += x == c;
+    }
+    rank += __builtin_amdgcn_mov_dpp(rank, 0xB1, 0xF, 0xF, false);
+    rank += __builtin_amdgcn_mov_dpp(rank, 0x4E, 0xF, 0xF, false);
+    level += __builtin_amdgcn_mov_dpp(level, 0xB1, 0xF, 0xF, false);
+    level += __builtin_amdgcn_mov_dpp(level, 0x4E, 0xF, 0xF, false);
+    if (threadIdx.x % 4 != 0 || i != i0 + (int)threadIdx.x / 4) continue;
+    const Pair mine = s_list[i];
+    if (level > 1) {
+      rank = 0;
+      for (int k = 0; k < n; ++k) rank += before(s_list[k], mine);
+    }
+    if (rank < a.count) put(rank, mine);
+  }
+  if (threadIdx.x == 0 && n < a.count) {
+    // the lowest pairs that are no candidates
+    int at = n;
+    for (int64_t f = 0; at < a.count; ++f) {
+      const int b = (int)(f / a.vocab), t = (int)(f % a.vocab);
+      bool taken = false;
+      for (int k = 0; k < n; ++k) taken = taken || (s_list[k].beam == b && s_list[k].token == t);
+      if (!taken) put(at++, Pair{kNone, 0u, b, t});
+    }
+  }
+}
+
+// Elements per thread: 32, or 8 where the chunks of 8192 would not fill the CUs.
+int chunk_elements(int64_t rows, int vocab) {
+  return rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) < 256 ? 8 : 32;
+}
+
+template <int E>
+void start_chunks(hipStream_t stream, const BeamArgs &a, const BeamParts &w) {
+  const dim3 grid((unsigned)((int64_t)a.groups * a.beams * w.chunks));
+  if (a.kind == 0) hipLaunchKernelGGL((beam_chunk_kernel<0, E>), grid, dim3(kThreads), 0, stream, a, w);
+  else if (a.kind == 1) hipLaunchKernelGGL((beam_chunk_kernel<1, E>), grid, dim3(kThreads), 0, stream, a, w);
+  else hipLaunchKernelGGL((beam_chunk_kernel<2, E>), grid, dim3(kThreads), 0, stream, a, w);
 }
 
 }  // namespace
 
-int64_t beam_workspace(int groups, int beams, int /*vocab*/, int count) {
-  return (int64_t)groups * beams * ((int64_t)sizeof(RowBest) + (int64_t)count * 8);
+int64_t beam_workspace(int groups, int beams, int vocab, int count) {
+  const int e = chunk_elements((int64_t)groups * beams, vocab);
+  return BeamParts(groups, beams, vocab, count, e * kThreads).total;
 }
 
 hipError_t launch_beam(hipStream_t stream, const BeamArgs &a) {
-  hipLaunchKernelGGL(beam_row_kernel, dim3(a.groups * a.beams), dim3(kThreads), 0, stream, a);
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((a.groups + 63) / 64), dim3(64), 0, stream, a);
+  const int e = chunk_elements((int64_t)a.groups * a.beams, a.vocab);
+  const BeamParts w(a.groups, a.beams, a.vocab, a.count, e * kThreads);
+  if (e == 8) start_chunks<8>(stream, a, w);
+  else start_chunks<32>(stream, a, w);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3(a.groups), dim3(kThreads), 0, stream, a, w);
   return hipGetLastError();
 }
 
