@@ -14,35 +14,35 @@ namespace pkv {
 namespace {
 
 // ---- select ------------------------------------------------------------------------
+//
+// One workgroup per (layer, sequence, KV head).  The need-th largest key is found by
+// its digits from the top, 11, 11 and 10 bits, each by a histogram in LDS of the keys
+// that agree so far; as a rule the second digit's bin is to be taken whole and the
+// third is not needed.  The row stays in registers up to 32 values per thread and
+// is read again for each step beyond that.  Latency-bound: a few round trips of LDS
+// and barriers (8192 sums in a row, 256 rows: see launch_evict_select).
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
+constexpr int kVectors = 8;  // of four values, per thread
+constexpr int kBins = 2048;
 
 // Unsigned key of the order: NaN above everything, -0 equal to +0.
-__device__ __forceinline__ uint32_t order_key(float x) {
+__device__ __forceinline__ uint32_t order_key(uint32_t bits) {
+  const float x = __uint_as_float(bits);
   if (x != x) return 0xFFFFFFFFu;
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ int block_sum(int v, int *s_wave) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
-  __syncthreads();
-  int sum = 0;
-  for (int k = 0; k < kWaves; ++k) sum += s_wave[k];
-  return sum;
-}
-
 // Exclusive prefix sum over the workgroup; *total the sum.
+template <int NT>
 __device__ __forceinline__ int block_scan(int v, int *s_wave, int *total) {
   const int incl = wave_scan_incl(v, 0), wave = threadIdx.x >> 6;
   __syncthreads();
   if ((threadIdx.x & 63) == 63) s_wave[wave] = incl;
   __syncthreads();
   int before = 0, sum = 0;
-  for (int k = 0; k < kWaves; ++k) {
+#pragma unroll
+  for (int k = 0; k < NT / 64; ++k) {
     before += k < wave ? s_wave[k] : 0;
     sum += s_wave[k];
   }
@@ -50,8 +50,10 @@ __device__ __forceinline__ int block_scan(int v, int *s_wave, int *total) {
   return before + incl - v;
 }
 
-__global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictSelectArgs a) {
-  __shared__ int s_wave[kWaves];
+template <int NT>
+__global__ __launch_bounds__(NT) void evict_select_kernel(const EvictSelectArgs a) {
+  constexpr int kWaves = NT / 64, kChunk = NT * kVectors * 4;
+  __shared__ int s_wave[kWaves], s_bins[kBins], s_found[3], s_sums[kVectors][kWaves];
   const int kh = blockIdx.x % a.hk, b = blockIdx.x / a.hk % a.batch, layer = blockIdx.x / a.hk / a.batch;
   const int row = a.rows ? a.rows[b] : b;
   const int L = (int)max((int64_t)0, min((int64_t)a.seq_lens[b], a.width));
@@ -66,38 +68,173 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const EvictSelec
   float *new_mass = a.new_mass && there ? a.new_mass + base * a.new_width : nullptr;
   const int r = min(a.recent, n), s = min(a.sinks, n - r);
   const int lo = s, hi = n > 0 ? L - r : s, need = n - r - s;  // `need` of the tokens lo..hi-1
-  // the need-th largest key, bit by bit from the top: the largest key that at
-  // least `need` tokens reach
-  uint32_t least = 0;
-  if (need > 0 && need < hi - lo)
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t at = least | (1u << bit);
-      int count = 0;
-      for (int t = lo + threadIdx.x; t < hi; t += kThreads) count += order_key(mass[t]) >= at;
-      if (block_sum(count, s_wave) >= need) least = at;
+  const int chunks = n > 0 ? (L + kChunk - 1) / kChunk : 0;
+
+  // chunk c: this thread's vectors, four tokens from c * kChunk + (j * NT + thread) * 4 on
+  uint32_t bits[kVectors][4];
+  auto first = [&](int c, int j) { return c * kChunk + (j * NT + (int)threadIdx.x) * 4; };
+  auto load = [&](int c) {
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) {
+      const int t = first(c, j);
+      if (t + 4 <= L) {
+        __builtin_memcpy(bits[j], mass + t, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bits[j][e] = t + e < L ? __float_as_uint(mass[t + e]) : 0u;
+      }
     }
-  int above = 0;
-  for (int t = lo + threadIdx.x; t < hi; t += kThreads) above += order_key(mass[t]) > least;
-  int room = need - block_sum(above, s_wave);  // tokens of that key itself
-  int done = 0;
-  for (int t0 = 0; t0 < L && n > 0; t0 += kThreads) {
-    const int t = t0 + threadIdx.x;
-    const float m = t < L ? mass[t] : 0.0f;
-    const uint32_t key = order_key(m);
-    const bool middle = t >= lo && t < hi && need > 0;
-    int ties, taken;
-    const int tie = block_scan(middle && key == least, s_wave, &ties);
-    const bool stays = t < L && (t < s || t >= L - r || (middle && (key > least || (key == least && tie < room))));
-    const int at = done + block_scan(stays, s_wave, &taken);  // (its barriers: the chunk is read before it is written)
-    if (stays && at < a.max_keep) {
-      kept[at] = t;
-      if (new_mass) new_mass[at] = m;
+  };
+  if (chunks > 0) load(0);
+
+  uint32_t least = 0;  // keys above it stay, and `room` of those that are equal to it
+  int room = INT32_MAX;
+  if (need > 0 && need < hi - lo) {
+    int left = need, shift = 21;
+    for (;;) {
+      for (int k = threadIdx.x; k < kBins; k += NT) s_bins[k] = 0;
+      __syncthreads();
+      const uint32_t digits = shift > 0 ? kBins - 1 : 1023;  // the last digit has 10 bits
+      for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) load(c);
+#pragma unroll
+        for (int j = 0; j < kVectors; ++j) {
+          if (c * kChunk + j * NT * 4 >= hi) break;
+          const int t = first(c, j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t key = order_key(bits[j][e]);
+            const bool same = shift == 21 || key >> (shift == 10 ? 21 : 10) == least >> (shift == 10 ? 21 : 10);
+            if (t + e >= lo && t + e < hi && same) atomicAdd(&s_bins[key >> shift & digits], 1);
+          }
+        }
+      }
+      __syncthreads();
+      // the bin of the left-th from the top: thread i has the bins below those of i - 1
+      int mine = 0;
+#pragma unroll
+      for (int k = 0; k < kBins / NT; ++k) mine += s_bins[kBins - 1 - (int)threadIdx.x * (kBins / NT) - k];
+      int total;
+      int above = block_scan<NT>(mine, s_wave, &total);
+      if (above < left && above + mine >= left)
+#pragma unroll
+        for (int k = 0; k < kBins / NT; ++k) {
+          const int bin = kBins - 1 - (int)threadIdx.x * (kBins / NT) - k;
+          if (above < left && above + s_bins[bin] >= left) {
+            s_found[0] = bin;
+            s_found[1] = left - above;
+            s_found[2] = s_bins[bin];
+          }
+          above += s_bins[bin];
+        }
+      __syncthreads();
+      least |= (uint32_t)s_found[0] << shift;
+      left = s_found[1];
+      if (left == s_found[2]) break;  // the whole bin stays: everything from its lowest key on
+      room = left;
+      if (shift == 0) break;
+      room = INT32_MAX;
+      shift = shift == 21 ? 10 : 0;
+      __syncthreads();
     }
-    room -= min(room, ties);
-    done += taken;
+    if (room == INT32_MAX && least > 0) --least;  // "above it" is then all that stays
   }
-  __syncthreads();
-  for (int i = n + threadIdx.x; i < a.max_keep; i += kThreads) {
+  int done = 0;
+  for (int c = 0; c < chunks; ++c) {
+    if (chunks > 1) load(c);
+    // which of its tokens each thread keeps: a bit each, and how many its wave's
+    // lanes before it keep of the vector
+    uint32_t keep[kVectors];
+    auto live = [&](int j) { return c * kChunk + j * NT * 4 < L; };
+    // s_sums, as the waves' counts of each vector, becomes what comes before them
+    auto prefix = [&]() {
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        constexpr int kPer = (kVectors * kWaves + 63) / 64;
+        int *sums = &s_sums[0][0], v[kPer], all = 0;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int i = (int)threadIdx.x * kPer + k;
+          v[k] = i < kVectors * kWaves ? sums[i] : 0;
+          all += v[k];
+        }
+        const int incl = wave_scan_incl(all, 0);
+        int at = incl - all;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int i = (int)threadIdx.x * kPer + k;
+          if (i < kVectors * kWaves) sums[i] = at;
+          at += v[k];
+        }
+        if (threadIdx.x == 63) s_found[0] = incl;
+      }
+      __syncthreads();
+    };
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) keep[j] = 0;
+    if (room != INT32_MAX) {
+      // ties: the lowest indices
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) {
+        uint32_t tie = 0;
+        if (live(j)) {
+          const int t = first(c, j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            tie |= (uint32_t)(t + e >= lo && t + e < hi && order_key(bits[j][e]) == least) << e;
+        }
+        const int incl = wave_scan_incl(__popc(tie), 0);
+        if ((threadIdx.x & 63) == 63) s_sums[j][wave] = incl;
+        keep[j] = tie | (uint32_t)(incl - __popc(tie)) << 8;
+      }
+      prefix();
+      const int ties = s_found[0];
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j) {
+        int at = s_sums[j][wave] + (int)(keep[j] >> 8);
+        uint32_t taken = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (keep[j] >> e & 1) taken |= (uint32_t)(at++ < room) << e;
+        keep[j] = taken;
+      }
+      room -= min(room, ties);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) {
+      if (live(j)) {
+        const int t = first(c, j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool stays = t + e < L && (t + e < lo || t + e >= hi || (need > 0 && order_key(bits[j][e]) > least));
+          keep[j] |= (uint32_t)stays << e;
+        }
+      }
+      const int incl = wave_scan_incl(__popc(keep[j]), 0);
+      if ((threadIdx.x & 63) == 63) s_sums[j][wave] = incl;
+      keep[j] |= (uint32_t)(incl - __popc(keep[j])) << 8;
+    }
+    prefix();  // (the chunk's sums are all read: they may be written over)
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) {
+      if (!live(j)) break;
+      int at = done + s_sums[j][wave] + (int)(keep[j] >> 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (keep[j] >> e & 1) {
+          if (at < a.max_keep) {
+            kept[at] = first(c, j) + e;
+            if (new_mass) new_mass[at] = __uint_as_float(bits[j][e]);
+          }
+          ++at;
+        }
+    }
+    done += s_found[0];
+    __syncthreads();
+  }
+  for (int i = n + threadIdx.x; i < a.max_keep; i += NT) {
     kept[i] = -1;
     if (new_mass) new_mass[i] = 0.0f;
   }
@@ -209,7 +346,9 @@ void start_pages(hipStream_t stream, const EvictPagesArgs &a, dim3 grid) {
 }  // namespace
 
 hipError_t launch_evict_select(hipStream_t stream, const EvictSelectArgs &a) {
-  hipLaunchKernelGGL(evict_select_kernel, dim3(a.layers * a.batch * a.hk), dim3(kThreads), 0, stream, a);
+  const dim3 grid(a.layers * a.batch * a.hk);
+  if (a.width <= 2048) hipLaunchKernelGGL(evict_select_kernel<256>, grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL(evict_select_kernel<1024>, grid, dim3(1024), 0, stream, a);
   return hipGetLastError();
 }
 
