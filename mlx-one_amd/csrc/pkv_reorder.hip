@@ -13,27 +13,85 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ bool pair_moves(const ReorderArgs &a, int i, int &to, int &from) {
-  to = a.targets[i];
-  from = a.sources[i];
-  return to >= 0 && to < a.num_rows && from >= 0 && from < a.num_rows && to != from;
-}
+// ---- rows of a tensor ------------------------------------------------------------------
+//
+// A workgroup holds its columns of all the rows in registers: PER units of 16 bytes
+// per thread, 2^log_columns units beside each other of every row, read before the
+// barrier and written after it.  Where a row ends inside a unit (TAIL), the threads
+// of its last whole unit also move its last 16 bytes, which overlap that one.
+// Memory-bound, one read and one write of the rows that move; rows at odd addresses
+// are read and written unaligned.
 
-// One byte column per thread and step, through LDS: [count][columns].
-__global__ __launch_bounds__(kThreads) void reorder_rows_kernel(const ReorderArgs a, int columns) {
-  extern __shared__ uint8_t s_bytes[];
+typedef u4 __attribute__((aligned(1))) Unit;  // 16 bytes anywhere
+
+template <int PER, int NT, bool TAIL>
+__global__ __launch_bounds__(NT) void reorder_rows_kernel(const ReorderArgs a, int log_columns) {
   uint8_t *state = a.state + (int64_t)blockIdx.y * a.num_rows * a.row_bytes;
-  const int64_t c0 = (int64_t)blockIdx.x * columns;
-  for (int e = threadIdx.x; e < a.count * columns; e += kThreads) {
-    int to, from;
-    const int64_t c = c0 + e % columns;
-    if (c < a.row_bytes && pair_moves(a, e / columns, to, from)) s_bytes[e] = state[from * a.row_bytes + c];
+  const int columns = 1 << log_columns, step = NT >> log_columns;
+  const int64_t units = a.row_bytes / 16;
+  const int64_t c = (int64_t)blockIdx.x * columns + (threadIdx.x & (columns - 1));  // this thread's column
+  const int64_t at = min(c, units - 1) * 16, end = a.row_bytes - 16;
+  const bool tail = TAIL && c == units - 1;
+  int to[PER], from[PER];
+  u4 v[PER], w[TAIL ? PER : 1];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = min((int)(threadIdx.x >> log_columns) + k * step, a.count - 1);
+    to[k] = a.targets[i];
+    from[k] = a.sources[i];
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const bool moves = to[k] >= 0 && to[k] < a.num_rows && from[k] >= 0 && from[k] < a.num_rows && to[k] != from[k] &&
+                       (int)(threadIdx.x >> log_columns) + k * step < a.count && c < units;
+    if (!moves) to[k] = -1;
+    const uint8_t *row = state + (moves ? from[k] : 0) * a.row_bytes;  // (a load without a branch)
+    v[k] = *(const Unit *)(row + at);
+    if constexpr (TAIL) w[k] = *(const Unit *)(row + (tail ? end : at));
+  }
+  // the loads have returned, not only been issued, before any wave stores
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    asm volatile("" : "+v"(v[k]));
+    if constexpr (TAIL) asm volatile("" : "+v"(w[k]));
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.count * columns; e += kThreads) {
-    int to, from;
-    const int64_t c = c0 + e % columns;
-    if (c < a.row_bytes && pair_moves(a, e / columns, to, from)) state[to * a.row_bytes + c] = s_bytes[e];
+#pragma unroll
+  for (int k = 0; k < PER; ++k)
+    if (to[k] >= 0) {
+      uint8_t *row = state + to[k] * a.row_bytes;
+      *(Unit *)(row + at) = v[k];
+      if (tail) *(Unit *)(row + end) = w[TAIL ? k : 0];
+    }
+}
+
+// Rows of fewer than 16 bytes, one thread a row.
+__global__ __launch_bounds__(1024) void reorder_short_kernel(const ReorderArgs a) {
+  uint8_t *state = a.state + (int64_t)blockIdx.x * a.num_rows * a.row_bytes;
+  const int bytes = (int)a.row_bytes;
+  uint32_t v[kMaxReorder / 1024][4];
+#pragma unroll
+  for (int k = 0; k < kMaxReorder / 1024; ++k) {
+    const int i = threadIdx.x + k * 1024;
+    const int s = i < a.count ? a.sources[i] : -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[k][e] = 0;
+    if (s >= 0 && s < a.num_rows)
+#pragma unroll
+      for (int e = 0; e < 15; ++e)
+        if (e < bytes) v[k][e / 4] |= (uint32_t)state[s * a.row_bytes + e] << (e % 4 * 8);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(v[k][e]));  // returned before any wave stores
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kMaxReorder / 1024; ++k) {
+    const int i = threadIdx.x + k * 1024;
+    const int t = i < a.count ? a.targets[i] : -1, s = i < a.count ? a.sources[i] : -1;
+    if (t >= 0 && t < a.num_rows && s >= 0 && s < a.num_rows)
+#pragma unroll
+      for (int e = 0; e < 15; ++e)
+        if (e < bytes) state[t * a.row_bytes + e] = (uint8_t)(v[k][e / 4] >> (e % 4 * 8));
   }
 }
 
@@ -166,11 +224,29 @@ int arena_blocks(int count, int max_pages) {
 
 }  // namespace
 
+template <int PER, int NT>
+void start_rows(hipStream_t stream, const ReorderArgs &a, int log_columns) {
+  const int64_t units = a.row_bytes / 16;
+  const dim3 grid((unsigned)((units + (1 << log_columns) - 1) >> log_columns), (unsigned)a.outer);
+  if (a.row_bytes % 16)
+    hipLaunchKernelGGL((reorder_rows_kernel<PER, NT, true>), grid, dim3(NT), 0, stream, a, log_columns);
+  else
+    hipLaunchKernelGGL((reorder_rows_kernel<PER, NT, false>), grid, dim3(NT), 0, stream, a, log_columns);
+}
+
 hipError_t launch_reorder_rows(hipStream_t stream, const ReorderArgs &a) {
-  int columns = 256;
-  while (columns > 1 && a.count * columns > 65536) columns /= 2;
-  const dim3 grid((unsigned)((a.row_bytes + columns - 1) / columns), (unsigned)a.outer);
-  hipLaunchKernelGGL(reorder_rows_kernel, grid, dim3(kThreads), a.count * columns, stream, a, columns);
+  if (a.row_bytes < 16) {
+    hipLaunchKernelGGL(reorder_short_kernel, dim3((unsigned)a.outer), dim3(1024), 0, stream, a);
+  } else if (a.count <= 128) {
+    // 16 columns (256 bytes of a row) or more beside each other
+    int log_columns = 4;
+    while (log_columns < 8 && (a.count << (log_columns + 1)) <= 8 * kThreads) ++log_columns;
+    start_rows<8, kThreads>(stream, a, log_columns);
+  } else {
+    int log_columns = 0;
+    while (log_columns < 6 && (a.count << (log_columns + 1)) <= 8 * 1024) ++log_columns;
+    start_rows<8, 1024>(stream, a, log_columns);
+  }
   return hipGetLastError();
 }
 
