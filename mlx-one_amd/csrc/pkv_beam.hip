@@ -18,6 +18,8 @@
 // and is ranked there.  A second launch joins the chunks' sums and does the same
 // with the lists' entries.  Memory-bound: one read of the
 // logits.
+#include <cfloat>
+
 #include "pkv_cache_ops.h"
 
 namespace pkv {
@@ -26,8 +28,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kHeld = 16;  // candidates per thread of the second launch in registers
-constexpr int kList = 1024;  // candidates in LDS
+constexpr int kMergeThreads = 1024;
+constexpr int kMergeWaves = kMergeThreads / 64;
+constexpr int kMergeList = 512;  // candidates of a group in LDS
+constexpr int kHeld = 4096;  // candidates of a group whose order is kept in LDS
+constexpr int kList = 256;  // candidates in LDS, per wave
 
 // Order of float32 as unsigned numbers; -inf and below (nothing) as 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -47,10 +52,13 @@ struct Chunk {
 // Workspace: [groups][beams][chunks] Chunk, then as many lists [count] of (order, token).
 struct BeamParts {
   int chunks;
+  uint32_t by_count, by_chunks;  // floor(2^32 / d) + 1: __umulhi(e, it) = e / d for e < 2^32 / d
   int64_t lists, total;
   __host__ __device__ BeamParts(int groups, int beams, int vocab, int count, int chunk) {
     chunks = (vocab + chunk - 1) / chunk;
     const int64_t n = (int64_t)groups * beams * chunks;
+    by_count = (uint32_t)(((uint64_t)1 << 32) / count) + 1;
+    by_chunks = (uint32_t)(((uint64_t)1 << 32) / chunks) + 1;
     lists = n * (int64_t)sizeof(Chunk);
     total = lists + n * count * 8;
   }
@@ -129,30 +137,25 @@ __device__ __forceinline__ float wave_max(float v) {
   return xor32_max(xor16_max(v));
 }
 
-// The list in LDS, in order: entry i's rank is the number of larger ones (they
-// differ in the token), counted by four lanes.  Keys are (order << 32 | ~token).
-template <typename F>
-__device__ __forceinline__ void ranked(const uint64_t *s_list, int n, int count, F store) {
-  for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
-    const int i = min(i0 + (int)threadIdx.x / 4, n - 1);
-    const uint64_t mine = s_list[i];
-    int rank = 0;
-#pragma unroll 8
-    for (int k = threadIdx.x % 4; k < n; k += 4) rank += s_list[k] > mine;
-    rank += __builtin_amdgcn_mov_dpp(rank, 0xB1, 0xF, 0xF, false);
-    rank += __builtin_amdgcn_mov_dpp(rank, 0x4E, 0xF, 0xF, false);
-    if (threadIdx.x % 4 == 0 && rank < count && i == i0 + (int)threadIdx.x / 4) store(rank, mine);
-  }
+// Lanes of the wave before this one that are in `mask`.
+__device__ __forceinline__ int lanes_before(unsigned long long mask) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// Sum over four neighbouring lanes.
+__device__ __forceinline__ int sum4(int v) {
+  v += __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, false);
+  return v + __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);
 }
 
 template <int KIND, int E>
 __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, const BeamParts w) {
   constexpr int V = E / 8;  // vectors of 8 per thread
-  __shared__ uint64_t s_list[kList];
+  __shared__ uint64_t s_list[kWaves][kList];  // (order << 32 | ~token), what each wave found
   __shared__ double s_sum[kWaves];
   __shared__ float s_most[kWaves];
   __shared__ uint32_t s_bound[kWaves];
-  __shared__ int s_n, s_nan;
+  __shared__ int s_n[kWaves], s_nan;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x / w.chunks;
   if (a.done && a.done[row]) return;  // its logits are not asked for
@@ -162,7 +165,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, 
   float vm[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) x[j].load(a, base, v0 + j * 8 * kThreads);
-  if (threadIdx.x == 0) s_n = s_nan = 0;
+  if (threadIdx.x == 0) s_nan = 0;
   bool nan = false;
   float m = -INFINITY;
 #pragma unroll
@@ -193,13 +196,20 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, 
   // most L: the product is not rounded, R is exact, and 2^(R - most L) makes up for it
   constexpr float kL = 1.4426950408889634f;
   const float from = fabsf(most) < 8e6f ? rintf(most * kL) : most * kL;
-  const bool flat = !(fabsf(from) < INFINITY);  // rows that have no sum, or all at the type's end
+  // (not for rows that have no sum, or only logits at their type's end)
+  const bool flat = __builtin_amdgcn_readfirstlane(!(fabsf(from) < INFINITY));
   float sum = 0.0f;
+  if (flat) {
 #pragma unroll
-  for (int j = 0; j < V; ++j)
+    for (int j = 0; j < V; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      sum += __builtin_amdgcn_exp2f(flat ? (x[j][e] - most) * kL : fmaf(x[j][e], kL, -from));
+      for (int e = 0; e < 8; ++e) sum += __builtin_amdgcn_exp2f((x[j][e] - most) * kL);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += __builtin_amdgcn_exp2f(fmaf(x[j][e], kL, -from));
+  }
   const double total = wave_sum64((double)sum) * (flat ? 1.0 : exp2((double)from - (double)most * (double)kL));
   if (lane == 0) {
     s_sum[wave] = total;
@@ -212,21 +222,32 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, 
   uint32_t least = 1;
 #pragma unroll
   for (int k = 0; k < kWaves; ++k) least = max(least, s_bound[k]);
+  const float reach = fmaxf(key_value(least), -FLT_MAX);
+  int found = 0;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    if (vm[j] == -INFINITY || order_key(vm[j]) < least) continue;
+    if (__ballot(vm[j] >= reach) == 0) continue;  // (in a row with a NaN nothing matters)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t k = order_key(x[j][e]);
-      if (k < least || x[j][e] == -INFINITY) continue;
-      const int at = atomicAdd(&s_n, 1);
-      if (at < kList) s_list[at] = (uint64_t)k << 32 | (uint32_t)~(v0 + j * 8 * kThreads + e);
+      const bool in = x[j][e] >= reach;
+      const unsigned long long mask = __ballot(in);
+      if (mask == 0) continue;
+      const int at = found + lanes_before(mask);
+      if (in && at < kList)
+        s_list[wave][at] = (uint64_t)order_key(x[j][e]) << 32 | (uint32_t)~(v0 + j * 8 * kThreads + e);
+      found += __popcll(mask);
     }
   }
+  if (lane == 0) s_n[wave] = found;
   __syncthreads();
   uint2 *list = (uint2 *)((char *)a.workspace + w.lists) + (int64_t)blockIdx.x * a.count;
-  int n = s_n;
-  if (n > kList) {
+  int n = 0, longest = 0;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    n += s_n[k];
+    longest = max(longest, s_n[k]);
+  }
+  if (longest > kList) {
     // more equal (or adjacent) tokens than the list holds: one after another
     uint64_t last = ~0ull;
     __shared__ uint64_t s_best[kWaves];
@@ -254,53 +275,63 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, 
       if (threadIdx.x == 0) list[n] = uint2{(uint32_t)(best >> 32), ~(uint32_t)best};
     }
   } else {
-    ranked(s_list, n, a.count, [&](int rank, uint64_t k) { list[rank] = uint2{(uint32_t)(k >> 32), ~(uint32_t)k}; });
+    // a rank is the number of larger ones (no two are equal), counted by four lanes,
+    // one of the waves' finds each
+    for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
+      int i = i0 + (int)threadIdx.x / 4, from = 0;
+      const bool mine = i < n;
+#pragma unroll
+      for (int k = 0; k < kWaves - 1; ++k)
+        if (mine && from == k && i >= s_n[k]) {
+          i -= s_n[k];
+          ++from;
+        }
+      const uint64_t key = mine ? s_list[from][i] : 0;
+      const int other = threadIdx.x % 4, most = s_n[other];
+      int rank = 0;
+#pragma unroll 8
+      for (int k = 0; k < most; ++k) rank += s_list[other][k] > key;
+      rank = sum4(rank);
+      if (mine && other == 0 && rank < a.count) list[rank] = uint2{(uint32_t)(key >> 32), ~(uint32_t)key};
+    }
     n = min(n, a.count);
   }
   for (int k = n + (int)threadIdx.x; k < a.count; k += kThreads) list[k] = uint2{0u, 0u};  // 0: none
-  if (threadIdx.x < kWaves) {  // (four lanes of one row)
-    const float part = s_most[threadIdx.x];
+  if (wave == kWaves - 1 && lane < kWaves) {  // four lanes of the last wave, which has the least to rank
+    const float part = s_most[lane];
     float all = fmaxf(part, row_xchg<0xB1>(part));
     all = fmaxf(all, row_xchg<0x4E>(all));
-    double sums = part > -INFINITY ? s_sum[threadIdx.x] * exp((double)part - (double)all) : 0.0;
+    double sums = part > -INFINITY ? s_sum[lane] * exp((double)part - (double)all) : 0.0;
     sums += row_xchg64<0xB1>(sums);
     sums += row_xchg64<0x4E>(sums);
-    if (threadIdx.x == 0) ((Chunk *)a.workspace)[blockIdx.x] = Chunk{sums, s_nan ? NAN : all};
+    if (lane == 0) ((Chunk *)a.workspace)[blockIdx.x] = Chunk{sums, s_nan ? NAN : all};
   }
 }
 
 // One workgroup per group of beams.
-__global__ __launch_bounds__(kThreads) void beam_merge_kernel(const BeamArgs a, const BeamParts w) {
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArgs a, const BeamParts w) {
   struct Pair {
     double c;
     uint32_t key;  // the logit's: the order within a beam
     int32_t beam, token;
   };
-  __shared__ Pair s_list[kList], s_best[kWaves];
-  __shared__ double s_c[kList];
+  __shared__ Pair s_list[kMergeList], s_best[kMergeWaves];
+  __shared__ double s_c[kMergeList];
+  __shared__ uint32_t s_order[kHeld];
   __shared__ double s_offset[kMaxBeams];  // score - log of the sum; -inf: no candidates
   __shared__ float s_most[kMaxBeams];
-  __shared__ int s_n, s_reach[2][kWaves];
+  __shared__ int s_reach[2][3][kMergeWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   constexpr double kNone = -(double)INFINITY;
   const int64_t row0 = (int64_t)blockIdx.x * a.beams, out = (int64_t)blockIdx.x * a.count;
   const Chunk *chunk = (const Chunk *)a.workspace + row0 * w.chunks;
   const uint2 *lists = (const uint2 *)((const char *)a.workspace + w.lists) + row0 * w.chunks * a.count;
   auto done = [&](int beam) { return a.done && a.done[row0 + beam]; };
-  // entry e of the beams' lists, requested before what it needs of their rows
   const int entries = a.beams * w.chunks * a.count;  // (less than 2^31 pairs per group: so are these)
-  uint2 raw[kHeld];
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k) {
-    const int e = threadIdx.x + k * kThreads;
-    raw[k] = uint2{0u, 0u};
-    if (k * kThreads < entries && e < entries) raw[k] = lists[e];
-  }
   // a row's sum: lanes beside each other take its chunks
   int width = 1;
-  while (width < 64 && width < w.chunks && width * 2 * a.beams <= kThreads) width *= 2;
+  while (width < 64 && width < w.chunks && width * 2 * a.beams <= kMergeThreads) width *= 2;
   const int beam = threadIdx.x / width, slice = threadIdx.x % width;
-  if (threadIdx.x == 0) s_n = 0;
   if (beam < a.beams) {
     const float score = a.scores[row0 + beam];
     bool dead = !(fabsf(score) < INFINITY);
@@ -331,7 +362,10 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(const BeamArgs a, 
   __syncthreads();
   // entry e, as loaded, as a candidate: false past its list's end
   auto candidate = [&](int e, uint2 x, Pair &p) {
-    const int list = e / a.count, b = list / w.chunks;
+    // (quotients by 1 are no multiples of 2^32 / 1)
+    const bool near = e < kHeld && w.chunks < 1 << 16;
+    const int list = a.count == 1 ? e : near ? (int)__umulhi(e, w.by_count) : e / a.count;
+    const int b = w.chunks == 1 ? list : near ? (int)__umulhi(list, w.by_chunks) : list / w.chunks;
     p = Pair{s_offset[b], x.x, b, (int)x.y};
     if (p.c == kNone) return false;
     if (done(b)) {
@@ -345,51 +379,76 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(const BeamArgs a, 
   };
   // A bound that `count` candidates reach and few others: bisection on the bits of
   // the candidates' order in float32 (rounding keeps it), until the rest fits easily.
-  constexpr int kIn = kHeld * kThreads;  // entries from there on are read again each time
+  // (Loops, not unrolled code: with one workgroup per group, instruction fetch counts.)
   Pair p;
-  uint32_t keys[kHeld];
+  auto order_of = [&](int e) { return candidate(e, lists[e], p) ? order_key((float)p.c) : 0u; };
+  // candidates that reach the bound: in the waves before this one, and in all
+  uint32_t least = 1;
+  int first = 0, n = 0;
+  auto counted = [&](const int (&reach)[kMergeWaves], int &before) {
+    int sum = 0;
+    before = 0;
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k) {
-    const int e = threadIdx.x + k * kThreads;
-    keys[k] = 0u;
-    if (k * kThreads < entries && e < entries && candidate(e, raw[k], p)) keys[k] = order_key((float)p.c);
-  }
-  uint32_t least = 0;
-  for (int bit = 31, step = 0; bit >= 0; --bit, ++step) {
-    const uint32_t next = least | 1u << bit;
-    int reach = 0;
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k)
-      if (k * kThreads < entries) reach += __popcll(__ballot(keys[k] >= next));
-    if (entries > kIn) {
-      int more = 0;
-      for (int e = threadIdx.x + kIn; e < entries; e += kThreads)
-        more += candidate(e, lists[e], p) && order_key((float)p.c) >= next;
-      reach += wave_sum(more);
+    for (int k = 0; k < kMergeWaves; ++k) {
+      before += k < wave ? reach[k] : 0;
+      sum += reach[k];
     }
-    if (lane == 0) s_reach[step & 1][wave] = reach;
-    __syncthreads();
-    reach = 0;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) reach += s_reach[step & 1][k];
-    if (reach < a.count) continue;
-    least = next;
-    if (reach <= a.count + 16) break;
-  }
-  least = max(least, 1u);
-  auto take = [&](int e, uint2 x) {
-    candidate(e, x, p);
-    const int at = atomicAdd(&s_n, 1);
-    if (at < kList) {
-      s_list[at] = p;
-      s_c[at] = p.c;
-    }
+    return sum;
   };
+  {
+    int reach = 0;
+#pragma unroll 1
+    for (int e0 = 0; e0 < entries; e0 += kMergeThreads) {
+      const int e = e0 + threadIdx.x;
+      const uint32_t key = e < entries ? order_of(e) : 0u;
+      if (e < min(entries, kHeld)) s_order[e] = key;
+      reach += __popcll(__ballot(key > 0));
+    }
+    if (lane == 0) s_reach[1][0][wave] = reach;
+    __syncthreads();
+    n = counted(s_reach[1][0], first);
+  }
+  uint32_t at = 0;
+#pragma unroll 1
+  for (int shift = 30, step = 0; shift >= 0 && n > a.count + 48; shift -= 2, ++step) {  // two bits at a time
+    int reach[3] = {0, 0, 0};
+#pragma unroll 1
+    for (int e0 = 0; e0 < entries; e0 += kMergeThreads) {
+      const int e = e0 + threadIdx.x;
+      const uint32_t key = e >= entries ? 0u : e < kHeld ? s_order[e] : order_of(e);
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (keys[k] >= least) take(threadIdx.x + k * kThreads, raw[k]);
-  for (int e = threadIdx.x + kIn; e < entries; e += kThreads)
-    if (candidate(e, lists[e], p) && order_key((float)p.c) >= least) take(e, lists[e]);
+      for (int d = 0; d < 3; ++d) reach[d] += __popcll(__ballot(key >= (at | (d + 1u) << shift)));
+    }
+    if (lane == 0)
+#pragma unroll
+      for (int d = 0; d < 3; ++d) s_reach[step & 1][d][wave] = reach[d];
+    __syncthreads();
+#pragma unroll
+    for (int d = 2; d >= 0; --d) {
+      int before;
+      const int sum = counted(s_reach[step & 1][d], before);
+      if (sum < a.count) continue;
+      at |= (d + 1u) << shift;
+      least = at;
+      first = before;
+      n = sum;
+      break;
+    }
+  }
+#pragma unroll 1
+  for (int e0 = 0; e0 < entries && n <= kMergeList; e0 += kMergeThreads) {
+    const int e = e0 + threadIdx.x;
+    const bool in = e < entries && (e < kHeld ? s_order[e] : order_of(e)) >= least;
+    const unsigned long long mask = __ballot(in);
+    if (mask == 0) continue;
+    if (in) {
+      candidate(e, lists[e], p);
+      const int to = first + lanes_before(mask);
+      s_list[to] = p;
+      s_c[to] = p.c;
+    }
+    first += __popcll(mask);
+  }
   __syncthreads();
   auto before = [](const Pair &x, const Pair &y) {
     if (x.c != y.c) return x.c > y.c;
@@ -401,13 +460,12 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(const BeamArgs a, 
     a.parents[out + rank] = p.beam;
     a.tokens[out + rank] = p.token;
   };
-  const int n = s_n;
-  if (n > kList) {
+  if (n > kMergeList) {
     // more than LDS holds (then there are `count` of them): one after another
     Pair last{(double)INFINITY, 0u, 0, 0};
     for (int rank = 0; rank < a.count; ++rank) {
       Pair best{kNone, 0u, INT32_MAX, 0};
-      for (int e = threadIdx.x; e < entries; e += kThreads)
+      for (int e = threadIdx.x; e < entries; e += kMergeThreads)
         if (candidate(e, lists[e], p) && before(last, p) && before(p, best)) best = p;
       for (int k = 1; k < 64; k *= 2) {
         Pair other;
@@ -420,35 +478,36 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(const BeamArgs a, 
       __syncthreads();
       if (lane == 0) s_best[wave] = best;
       __syncthreads();
-      for (int k = 0; k < kWaves; ++k)
+      for (int k = 0; k < kMergeWaves; ++k)
         if (before(s_best[k], best)) best = s_best[k];
       last = best;
       if (threadIdx.x == 0) put(rank, best);
     }
     return;
   }
-  // ranks, four lanes a candidate; candidates of one value (rare) in full
-  for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
-    const int i = min(i0 + (int)threadIdx.x / 4, n - 1);
-    const double c = s_c[i];
+  // ranks, by four lanes a candidate; candidates of one value (rare) in full
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kMergeThreads / 4) {
+    const int i = i0 + (int)threadIdx.x / 4;
+    const bool mine = i < n;
+    const double c = mine ? s_c[i] : kNone;
     int rank = 0, level = 0;
-#pragma unroll 8
+#pragma unroll 4
     for (int k = threadIdx.x % 4; k < n; k += 4) {
       const double x = s_c[k];
       rank += x > c;
       level += x == c;
     }
-    rank += __builtin_amdgcn_mov_dpp(rank, 0xB1, 0xF, 0xF, false);
-    rank += __builtin_amdgcn_mov_dpp(rank, 0x4E, 0xF, 0xF, false);
-    level += __builtin_amdgcn_mov_dpp(level, 0xB1, 0xF, 0xF, false);
-    level += __builtin_amdgcn_mov_dpp(level, 0x4E, 0xF, 0xF, false);
-    if (threadIdx.x % 4 != 0 || i != i0 + (int)threadIdx.x / 4) continue;
-    const Pair mine = s_list[i];
+    rank = sum4(rank);
+    level = sum4(level);
+    if (!mine || threadIdx.x % 4 != 0) continue;
+    const Pair pair = s_list[i];
     if (level > 1) {
       rank = 0;
-      for (int k = 0; k < n; ++k) rank += before(s_list[k], mine);
+#pragma unroll 1
+      for (int k = 0; k < n; ++k) rank += before(s_list[k], pair);
     }
-    if (rank < a.count) put(rank, mine);
+    if (rank < a.count) put(rank, pair);
   }
   if (threadIdx.x == 0 && n < a.count) {
     // the lowest pairs that are no candidates
@@ -487,7 +546,7 @@ hipError_t launch_beam(hipStream_t stream, const BeamArgs &a) {
   const BeamParts w(a.groups, a.beams, a.vocab, a.count, e * kThreads);
   if (e == 8) start_chunks<8>(stream, a, w);
   else start_chunks<32>(stream, a, w);
-  hipLaunchKernelGGL(beam_merge_kernel, dim3(a.groups), dim3(kThreads), 0, stream, a, w);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3(a.groups), dim3(kMergeThreads), 0, stream, a, w);
   return hipGetLastError();
 }
 
