@@ -28,8 +28,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMergeThreads = 1024;
-constexpr int kMergeWaves = kMergeThreads / 64;
 constexpr int kMergeList = 512;  // candidates of a group in LDS
 constexpr int kHeld = 4096;  // candidates of a group whose order is kept in LDS
 constexpr int kList = 256;  // candidates in LDS, per wave
@@ -309,7 +307,9 @@ __global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, 
 }
 
 // One workgroup per group of beams.
+template <int kMergeThreads>
 __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArgs a, const BeamParts w) {
+  constexpr int kMergeWaves = kMergeThreads / 64;
   struct Pair {
     double c;
     uint32_t key;  // the logit's: the order within a beam
@@ -317,11 +317,12 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArg
   };
   __shared__ Pair s_list[kMergeList], s_best[kMergeWaves];
   __shared__ double s_c[kMergeList];
+  __shared__ uint64_t s_tie[kMergeList];  // order of equal ones but for the token: (beam, the logit's falling)
   __shared__ uint32_t s_order[kHeld];
   __shared__ double s_offset[kMaxBeams];  // score - log of the sum; -inf: no candidates
   __shared__ float s_most[kMaxBeams];
   __shared__ int s_reach[2][3][kMergeWaves];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr double kNone = -(double)INFINITY;
   const int64_t row0 = (int64_t)blockIdx.x * a.beams, out = (int64_t)blockIdx.x * a.count;
   const Chunk *chunk = (const Chunk *)a.workspace + row0 * w.chunks;
@@ -386,14 +387,16 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArg
   uint32_t least = 1;
   int first = 0, n = 0;
   auto counted = [&](const int (&reach)[kMergeWaves], int &before) {
-    int sum = 0;
-    before = 0;
-#pragma unroll
-    for (int k = 0; k < kMergeWaves; ++k) {
-      before += k < wave ? reach[k] : 0;
-      sum += reach[k];
+    // lanes 0..15 of a row hold the waves' counts
+    int v = lane < kMergeWaves ? reach[lane] : 0;
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    if (kMergeWaves > 4) {
+      v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+      v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
     }
-    return sum;
+    before = wave > 0 ? __builtin_amdgcn_readlane(v, wave - 1) : 0;
+    return __builtin_amdgcn_readlane(v, kMergeWaves - 1);
   };
   {
     int reach = 0;
@@ -446,6 +449,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArg
       const int to = first + lanes_before(mask);
       s_list[to] = p;
       s_c[to] = p.c;
+      s_tie[to] = (uint64_t)p.beam << 32 | ~p.key;
     }
     first += __popcll(mask);
   }
@@ -485,29 +489,22 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArg
     }
     return;
   }
-  // ranks, by four lanes a candidate; candidates of one value (rare) in full
+  // ranks, by four lanes a candidate
 #pragma unroll 1
   for (int i0 = 0; i0 < n; i0 += kMergeThreads / 4) {
     const int i = i0 + (int)threadIdx.x / 4;
-    const bool mine = i < n;
-    const double c = mine ? s_c[i] : kNone;
-    int rank = 0, level = 0;
+    const Pair pair = s_list[min(i, n - 1)];
+    const uint64_t tie = (uint64_t)pair.beam << 32 | ~pair.key;
+    int rank = 0;
 #pragma unroll 4
     for (int k = threadIdx.x % 4; k < n; k += 4) {
-      const double x = s_c[k];
-      rank += x > c;
-      level += x == c;
+      const double c = s_c[k];
+      const uint64_t t = s_tie[k];
+      const int token = s_list[k].token;
+      rank += c > pair.c || (c == pair.c && (t < tie || (t == tie && token < pair.token)));
     }
     rank = sum4(rank);
-    level = sum4(level);
-    if (!mine || threadIdx.x % 4 != 0) continue;
-    const Pair pair = s_list[i];
-    if (level > 1) {
-      rank = 0;
-#pragma unroll 1
-      for (int k = 0; k < n; ++k) rank += before(s_list[k], pair);
-    }
-    if (rank < a.count) put(rank, pair);
+    if (i < n && threadIdx.x % 4 == 0 && rank < a.count) put(rank, pair);
   }
   if (threadIdx.x == 0 && n < a.count) {
     // the lowest pairs that are no candidates
@@ -546,7 +543,10 @@ hipError_t launch_beam(hipStream_t stream, const BeamArgs &a) {
   const BeamParts w(a.groups, a.beams, a.vocab, a.count, e * kThreads);
   if (e == 8) start_chunks<8>(stream, a, w);
   else start_chunks<32>(stream, a, w);
-  hipLaunchKernelGGL(beam_merge_kernel, dim3(a.groups), dim3(kMergeThreads), 0, stream, a, w);
+  if (a.beams * w.chunks * a.count <= 1024)
+    hipLaunchKernelGGL(beam_merge_kernel<256>, dim3(a.groups), dim3(256), 0, stream, a, w);
+  else
+    hipLaunchKernelGGL(beam_merge_kernel<1024>, dim3(a.groups), dim3(1024), 0, stream, a, w);
   return hipGetLastError();
 }
 
