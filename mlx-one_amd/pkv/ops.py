@@ -447,36 +447,45 @@ def rope_qkv(qkv, positions, inv_freq, heads, kv_heads):
 # ---- which cached state lives on ---------------------------------------------------
 
 
-class _OnDevice:
-    """Makes ``device`` the current one for a launch, where it is not."""
+def _launch(device, what, entry, *args):
+    """Call a C entry point on the current stream of ``device``, as its current device."""
+    index, current = device.index, torch._C._cuda_getDevice()
+    if current == index:
+        code = entry(torch._C._cuda_getCurrentRawStream(index), *args)
+    else:
+        torch._C._cuda_setDevice(index)
+        try:
+            code = entry(torch._C._cuda_getCurrentRawStream(index), *args)
+        finally:
+            torch._C._cuda_setDevice(current)
+    if code:
+        nat.check(code, what)
 
-    __slots__ = ("index", "previous")
 
-    def __init__(self, device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.previous = torch._C._cuda_getDevice()
-        if self.previous != self.index:
-            torch._C._cuda_setDevice(self.index)
-
-    def __exit__(self, *_):
-        if self.previous != self.index:
-            torch._C._cuda_setDevice(self.previous)
+def _dense(t, dtype, device, dims):
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device
+            and t.dim() == dims and t.is_contiguous())
 
 
 def _check_dense(t, dtype, device, name, dims):
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != dims or \
-            t.device != device or not t.is_contiguous():
+    if not _dense(t, dtype, device, dims):
         raise ValueError(f"{name} must be a contiguous {dims}-dimensional {dtype} tensor on {device}")
 
 
 def _per_row(x, device, count, name):
-    """An int32 operand of ``count`` values on the device (None: None)."""
+    """An int32 operand of ``count`` values on the device."""
     t = _i32(x, device)
-    if t is not None and t.numel() != count:
+    if t.numel() != count:
         raise ValueError(f"{name} must hold {count} values")
     return t
+
+
+def _address(x, device, count, name):
+    """``(tensor, its address)`` of an int32 operand of ``count`` values; None: NULL."""
+    if x is None:
+        return None, None
+    t = _per_row(x, device, count, name)
+    return t, t.data_ptr()
 
 
 def _scratch(nbytes, device, what, given=None):
@@ -484,7 +493,7 @@ def _scratch(nbytes, device, what, given=None):
     if nbytes < 0:
         nat.check(nat.PKV_INVALID_ARGUMENT, what)
     if given is None:
-        return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+        return torch.empty(nbytes or 16, dtype=torch.uint8, device=device)
     if given.device != device or given.dtype is not torch.uint8 or not given.is_contiguous():
         raise ValueError(f"{what} workspace must be a contiguous uint8 tensor on {device}")
     return given
@@ -511,40 +520,38 @@ def attention_mass(fmt: PageFormat, pool, queries, block_table, seq_lens, *, sca
     _check_float(queries, fmt, "queries")
     device = queries.device
     _check_dense(pool, torch.uint8, device, "pool", 2)
-    if pool.shape[1] != fmt.page_bytes:
+    pages, page_bytes = pool.shape
+    if page_bytes != fmt.page_bytes:
         raise ValueError("the pool's pages are not of this format")
     table = _i32(block_table, device)
     if table.dim() != 2 or table.shape[0] != batch:
         raise ValueError("block table must be [batch, max_pages]")
-    lens = _per_row(seq_lens, device, batch, "seq_lens")
-    if mass is not None:
-        _check_dense(mass, torch.float32, device, "mass", 3)
+    width = table.shape[1]
     if out is None:
         out = mass if mass is not None else torch.zeros(
-            (batch, fmt.num_kv_heads, table.shape[1] * fmt.page_tokens), device=device)
-    else:
-        _check_dense(out, torch.float32, device, "out", 3)
-        if mass is not None and mass.shape != out.shape:
+            (batch, fmt.num_kv_heads, width * fmt.page_tokens), device=device)
+    _check_dense(out, torch.float32, device, "out", 3)
+    if mass is not None and mass is not out:
+        _check_dense(mass, torch.float32, device, "mass", 3)
+        if mass.shape != out.shape:
             raise ValueError("mass and out must have one shape")
-    if out.shape[1] != fmt.num_kv_heads or (rows is None and out.shape[0] < batch):
+    mass_rows, kv_heads, tokens = out.shape
+    if kv_heads != fmt.num_kv_heads or (rows is None and mass_rows < batch):
         raise ValueError("attention mass must be [rows, HK, tokens] with a row per sequence")
-    positions = _per_row(q_pos, device, batch * nq, "q_pos")
-    width = _per_row(widths, device, batch, "widths")
-    known = _per_row(counted, device, batch, "counted")
-    row = _per_row(rows, device, batch, "rows")
+    lens = _per_row(seq_lens, device, batch, "seq_lens")
+    # (the tensors are named so that they live until the launch)
+    positions, positions_at = _address(q_pos, device, batch * nq, "q_pos")
+    live, live_at = _address(widths, device, batch, "widths")
+    known, known_at = _address(counted, device, batch, "counted")
+    row, row_at = _address(rows, device, batch, "rows")
     queries = queries.contiguous()
-    lib = nat.load()
-    workspace = _scratch(lib.pkv_attention_mass_workspace_bytes(fmt.c_layout, heads, nq, batch,
-                                                                table.shape[1]),
+    lib, layout = nat.load(), fmt.c_layout
+    workspace = _scratch(lib.pkv_attention_mass_workspace_bytes(layout, heads, nq, batch, width),
                          device, "attention mass", workspace)
-    with _OnDevice(device):
-        code = lib.pkv_attention_mass(
-            nat.stream_handle(device), fmt.c_layout, pool.data_ptr(), pool.shape[0],
-            queries.data_ptr(), batch, heads, nq, table.data_ptr(), table.shape[1],
-            lens.data_ptr(), nat.ptr(positions), nat.ptr(width), float(scale), nat.ptr(mass),
-            nat.ptr(known), nat.ptr(row), out.shape[0], out.shape[2], workspace.data_ptr(),
-            workspace.numel(), out.data_ptr())
-    nat.check(code, "attention mass")
+    _launch(device, "attention mass", lib.pkv_attention_mass, layout, pool.data_ptr(), pages,
+            queries.data_ptr(), batch, heads, nq, table.data_ptr(), width, lens.data_ptr(),
+            positions_at, live_at, scale, None if mass is None else mass.data_ptr(), known_at,
+            row_at, mass_rows, tokens, workspace.data_ptr(), workspace.numel(), out.data_ptr())
     return out
 
 
@@ -572,20 +579,22 @@ def evict_select(mass, seq_lens, keep, *, max_keep=None, sinks=0, recent=0, rows
     mass_rows, heads, tokens = mass.shape[-3:]
     lens = _i32(seq_lens, device)
     batch = lens.numel()
-    row = _per_row(rows, device, batch, "rows")
+    row, row_at = _address(rows, device, batch, "rows")
     if row is None and mass_rows < batch:
         raise ValueError("mass needs a row per sequence")
     if isinstance(keep, int):
+        budget_at = None
         if max_keep is None:
-            max_keep, budget = keep, None
+            max_keep = keep
         else:
             budget = torch.full((batch,), keep, dtype=torch.int32, device=device)
+            budget_at = budget.data_ptr()
     else:
         if max_keep is None:
             if isinstance(keep, torch.Tensor):
                 raise ValueError("budgets on the device need max_keep, their bound")
             max_keep = max([int(k) for k in keep], default=0)
-        budget = _per_row(keep, device, batch, "keep")
+        budget, budget_at = _address(keep, device, batch, "keep")
     if max_keep < 0:
         raise ValueError("negative budget")
     lead = (layers,) if mass.dim() == 4 else ()
@@ -598,13 +607,11 @@ def evict_select(mass, seq_lens, keep, *, max_keep=None, sinks=0, recent=0, rows
         new_mass = make(lead + (mass_rows, heads, max_keep), dtype=torch.float32, device=device)
     kept = torch.empty(lead + (batch, heads, max_keep), dtype=torch.int32, device=device)
     new_lens = torch.empty(batch, dtype=torch.int32, device=device)
-    with _OnDevice(device):
-        code = nat.load().pkv_evict_select(
-            nat.stream_handle(device), mass.data_ptr(), layers, mass_rows, heads, tokens,
-            nat.ptr(row), lens.data_ptr(), batch, nat.ptr(budget), max_keep, int(sinks),
-            int(recent), kept.data_ptr(), new_lens.data_ptr(), nat.ptr(new_mass),
-            0 if new_mass is None else new_mass.shape[-1])
-    nat.check(code, "eviction select")
+    sums_at, sums_width = (None, 0) if new_mass is None else (new_mass.data_ptr(),
+                                                              new_mass.shape[-1])
+    _launch(device, "eviction select", nat.load().pkv_evict_select, mass.data_ptr(), layers,
+            mass_rows, heads, tokens, row_at, lens.data_ptr(), batch, budget_at, max_keep, sinks,
+            recent, kept.data_ptr(), new_lens.data_ptr(), sums_at, sums_width)
     return (kept, new_lens) if new_mass is None else (kept, new_lens, new_mass)
 
 
@@ -641,12 +648,9 @@ def evict_pages(fmt: PageFormat, pools, kept, new_lens, src_table, dst_table):
     src, dst = _i32(src_table, device), _i32(dst_table, device)
     if src.dim() != 2 or dst.dim() != 2 or src.shape[0] != batch or dst.shape[0] != batch:
         raise ValueError("block tables must be [batch, max_pages]")
-    with _OnDevice(device):
-        code = nat.load().pkv_evict_pages(
-            nat.stream_handle(device), fmt.c_layout, (nat._c_p * layers)(*addresses), layers,
-            shape[0], kept.data_ptr(), lens.data_ptr(), batch, most, src.data_ptr(), src.shape[1],
-            dst.data_ptr(), dst.shape[1])
-    nat.check(code, "eviction pages")
+    _launch(device, "eviction pages", nat.load().pkv_evict_pages, fmt.c_layout,
+            (nat._c_p * layers)(*addresses), layers, shape[0], kept.data_ptr(), lens.data_ptr(),
+            batch, most, src.data_ptr(), src.shape[1], dst.data_ptr(), dst.shape[1])
 
 
 _LOGIT_KINDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -666,32 +670,32 @@ def beam_select(logits, scores, count, *, done=None, pad_token=0, workspace=None
     if logits.dim() != 3 or logits.dtype not in _LOGIT_KINDS or not logits.is_cuda:
         raise ValueError("logits must be a [groups, beams, vocab] f32/f16/bf16 device tensor")
     device = logits.device
-    groups, beams, vocab = logits.shape
-    if logits.stride(2) != 1 and vocab > 1 or logits.stride(0) < 0 or logits.stride(1) < 0:
+    groups, beams, vocab = shape = logits.shape
+    group_stride, beam_stride, token_stride = logits.stride()
+    if (token_stride != 1 and vocab > 1) or group_stride < 0 or beam_stride < 0:
         logits = logits.contiguous()
-    if tuple(scores.shape) != (groups, beams) or scores.device != device:
+        group_stride, beam_stride, _ = logits.stride()
+    if scores.shape != shape[:2] or scores.device != device:
         raise ValueError("scores must be [groups, beams] on the logits' device")
-    scores = scores.to(torch.float32).contiguous()
+    if scores.dtype is not torch.float32 or not scores.is_contiguous():
+        scores = scores.to(torch.float32).contiguous()
+    done_at = None
     if done is not None:
-        if tuple(done.shape) != (groups, beams) or done.dtype is not torch.bool or \
-                done.device != device:
+        if done.shape != shape[:2] or done.dtype is not torch.bool or done.device != device:
             raise ValueError("done must be a [groups, beams] bool tensor on the logits' device")
         done = done.contiguous()
-    lib = nat.load()
+        done_at = done.data_ptr()
     best = torch.empty((groups, count), dtype=torch.float32, device=device)
-    parents = torch.empty((groups, count), dtype=torch.int32, device=device)
-    tokens = torch.empty((groups, count), dtype=torch.int32, device=device)
+    parents, tokens = torch.empty((2, groups, count), dtype=torch.int32, device=device).unbind(0)
     if groups == 0:
         return best, parents, tokens
+    lib = nat.load()
     workspace = _scratch(lib.pkv_beam_workspace_bytes(groups, beams, vocab, count), device,
                          "beam select", workspace)
-    with _OnDevice(device):
-        code = lib.pkv_beam_select(
-            nat.stream_handle(device), logits.data_ptr(), _LOGIT_KINDS[logits.dtype], groups, beams,
-            vocab, logits.stride(0), logits.stride(1), scores.data_ptr(), nat.ptr(done),
-            int(pad_token), int(count), workspace.data_ptr(), workspace.numel(), best.data_ptr(),
-            parents.data_ptr(), tokens.data_ptr())
-    nat.check(code, "beam select")
+    _launch(device, "beam select", lib.pkv_beam_select, logits.data_ptr(),
+            _LOGIT_KINDS[logits.dtype], groups, beams, vocab, group_stride, beam_stride,
+            scores.data_ptr(), done_at, pad_token, count, workspace.data_ptr(), workspace.numel(),
+            best.data_ptr(), parents.data_ptr(), tokens.data_ptr())
     return best, parents, tokens
 
 
@@ -711,9 +715,6 @@ def reorder_rows(state, targets, sources, *, dim=0):
     shape = state.shape
     outer, num_rows = math.prod(shape[:dim]), shape[dim]
     row_bytes = math.prod(shape[dim + 1:]) * state.element_size()
-    with _OnDevice(device):
-        code = nat.load().pkv_reorder_rows(nat.stream_handle(device), state.data_ptr(), outer,
-                                           num_rows, row_bytes, to.data_ptr(), source.data_ptr(),
-                                           count)
-    nat.check(code, "reorder")
+    _launch(device, "reorder", nat.load().pkv_reorder_rows, state.data_ptr(), outer, num_rows,
+            row_bytes, to.data_ptr(), source.data_ptr(), count)
     return state
