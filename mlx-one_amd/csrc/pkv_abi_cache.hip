@@ -40,6 +40,8 @@ int mass_shape(const pkv_layout *layout, int32_t num_heads, int32_t num_queries,
     return fail(PKV_UNSUPPORTED, "at most 2^24 query rows per KV head");
   if ((int64_t)max_pages * g->page > INT32_MAX) return fail(PKV_INVALID_ARGUMENT, "block table too wide");
   if ((int64_t)batch * g->hk > 65535) return fail(PKV_UNSUPPORTED, "at most 65535 (sequence, KV head) pairs");
+  if ((int64_t)batch * g->hk * max_pages > (1 << 30))
+    return fail(PKV_UNSUPPORTED, "at most 2^30 pages of (sequence, KV head) pairs");
   return PKV_OK;
 }
 

@@ -83,6 +83,72 @@ struct Units {
   }
 };
 
+// The same units in the order (sequence, KV head, part), shared out as equal runs of
+// consecutive ones over the workgroups: a run's units of one (sequence, KV head) share
+// their query operands and their running (max, sum).
+struct Runs {
+  int total;             // units of the launch (fewer than 2^31)
+  int each, more;        // units per run, and one more in the first `more` runs
+  int b, kh, part, L;    // where the run stands
+  int parts;             // of sequence b
+
+  // The units of the sequences before b, in parts of one KV head.
+  static __device__ __forceinline__ int parts_before(const MassArgs &a, int size, int lane, int b) {
+    int sum = 0;
+    for (int base = 0; base < b; base += 64) {
+      const int n = base + lane < b ? (max(0, mass_len(a, base + lane)) + size - 1) / size : 0;
+      sum += wave_sum(n);
+    }
+    return sum;
+  }
+  __device__ __forceinline__ void share(int units, int grid) {
+    total = units;
+    each = total / grid;
+    more = total - each * grid;
+  }
+  // First unit of workgroup w, and the workgroup of unit u.
+  __device__ __forceinline__ int first(int w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ int owner(int u) const {
+    const int longer = more * (each + 1);
+    return u < longer ? u / (each + 1) : more + (u - longer) / each;
+  }
+  __device__ __forceinline__ void set(const MassArgs &a, int size, int to) {
+    b = to;
+    L = mass_len(a, b);
+    parts = (max(0, L) + size - 1) / size;
+  }
+  // Stands at unit u < total.
+  __device__ __forceinline__ void seek(const MassArgs &a, int size, int lane, int u) {
+    int carry = 0;
+    for (int base = 0;; base += 64) {
+      const int n = base + lane < a.batch ? (max(0, mass_len(a, base + lane)) + size - 1) / size : 0;
+      const int incl = wave_scan_incl(n, lane);
+      const unsigned long long hit = __ballot((carry + incl) * a.g.hk > u);
+      if (hit || base + 64 >= a.batch) {
+        const int f = hit ? __ffsll((long long)hit) - 1 : 0;
+        parts = __builtin_amdgcn_readlane(n, f);
+        const int r = u - (carry + __builtin_amdgcn_readlane(incl, f) - parts) * a.g.hk;
+        b = base + f;
+        L = mass_len(a, b);
+        kh = r / max(parts, 1);
+        part = r - kh * parts;
+        return;
+      }
+      carry += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  // The next unit (there is one); true where it is of another (sequence, KV head).
+  __device__ __forceinline__ bool next(const MassArgs &a, int size) {
+    if (++part < parts) return false;
+    part = 0;
+    if (++kh < a.g.hk) return true;
+    kh = 0;
+    do set(a, size, b + 1);
+    while (parts == 0);
+    return true;
+  }
+};
+
 // ---- tiles and query rows -------------------------------------------------------------
 
 template <int BITS, int DP, int G, int FK>
@@ -190,14 +256,17 @@ constexpr int kTiles = kPart / PKV_TILE / kWaves;
 
 __host__ __device__ inline int quads(int rows) { return rows > 4 ? (rows + 3) / 4 : 1; }
 
-// Workspace: [scores: segment][R / 4][tokens][4] f32, [parts: segment][parts][8] (m, l).
+// Workspace: [scores: segment][R / 4][tokens][4] f32, [segment][k][8] (m, l) of the
+// k-th workgroup that had units of the segment (k < its parts).
 struct FewParts {
   int64_t tokens, parts, scores, total;
+  int grid;  // workgroups of the first launch
   __host__ __device__ FewParts(int64_t segs, int rows, int64_t cap) {
     tokens = (cap + kPart - 1) / kPart * kPart;
     parts = tokens / kPart;
     scores = segs * quads(rows) * tokens * 16;
     total = scores + segs * parts * kFewRows * 8;
+    grid = 0;
   }
 };
 
@@ -205,16 +274,27 @@ struct FewParts {
 // rows per lane are then the lane's registers r, and a call of at most 4 rows has
 // one score per lane and tile, a call of 8 two.
 template <typename C, int NR>
-__global__ __launch_bounds__(kThreads) void mass_scores_kernel(const MassArgs a, const FewParts w) {
+__global__ __launch_bounds__(kThreads, C::KB > 4 ? 2 : 4) void mass_scores_kernel(const MassArgs a, const FewParts w) {
   __shared__ float s_ml[kWaves][NR * 4][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
   const Geo &g = a.g;
   const f4 zero = register_zero();
-  Units u;
-  u.start(a, kPart, lane);
-  for (int64_t unit = blockIdx.x; u.find(a, kPart, unit, lane); unit += gridDim.x) {
-    const int t0 = u.part * kPart + wave * (kTiles * PKV_TILE);
-    const int ids = tile_page<kTiles>(a, u.b, t0, u.L, lane);
+  Runs run;
+  run.share(Runs::parts_before(a, kPart, lane, a.batch) * g.hk, gridDim.x);
+  int unit = run.first(blockIdx.x);
+  const int end = run.first(blockIdx.x + 1);
+  if (unit >= end) return;
+  run.seek(a, kPart, lane, unit);
+  auto pages = [&]() { return tile_page<kTiles>(a, run.b, run.part * kPart + wave * (kTiles * PKV_TILE), run.L, lane); };
+  int ids = pages();
+  bool fresh = true;
+  typename C::KT q[C::KB];
+  float qs[NR][C::NG], mult[NR], m[NR], l[NR];
+  int sees[NR];
+  for (; unit < end; ++unit) {
+    const int b = run.b, kh = run.kh, part = run.part;
+    const int t0 = part * kPart + wave * (kTiles * PKV_TILE);
+    const int64_t seg = (int64_t)b * g.hk + kh;
     uint32_t kw[kTiles][C::LW], mw[kTiles][C::NG];
     bool there[kTiles];
 #pragma unroll
@@ -222,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void mass_scores_kernel(const MassArgs a,
       const int id = __builtin_amdgcn_readlane(ids, i);
       there[i] = id >= 0;
       const int slot = (t0 + i * PKV_TILE) % g.page;
-      const uint8_t *head = a.pool + (int64_t)max(id, 0) * g.page_bytes + (int64_t)u.kh * g.head_bytes;
+      const uint8_t *head = a.pool + (int64_t)max(id, 0) * g.page_bytes + (int64_t)kh * g.head_bytes;
 #pragma unroll
       for (int k = 0; k < C::LW; ++k) kw[i][k] = 0;
 #pragma unroll
@@ -236,19 +316,25 @@ __global__ __launch_bounds__(kThreads) void mass_scores_kernel(const MassArgs a,
         }
       }
     }
-    typename C::KT q[C::KB];
-    float qs_row[C::NG], mult_row;
-    query_operands<C>(a, u.b, u.kh, 4 * (col & 3) + (col >> 2), jj, q, mult_row, qs_row);
-    float qs[NR][C::NG], mult[NR], m[NR], l[NR], s[NR][kTiles];
-    int sees[NR];
+    if (fresh) {
+      float qs_row[C::NG], mult_row;
+      query_operands<C>(a, b, kh, 4 * (col & 3) + (col >> 2), jj, q, mult_row, qs_row);
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      const int row = 4 * r + jj;
-      sees[r] = row < a.rows ? row_sees(a, u.b, row / a.gqa, u.L) : 0;
-      mult[r] = __shfl(mult_row, 4 * jj + r, 64);
+      for (int r = 0; r < NR; ++r) {
+        const int row = 4 * r + jj;
+        sees[r] = row < a.rows ? row_sees(a, b, row / a.gqa, run.L) : 0;
+        mult[r] = __shfl(mult_row, 4 * jj + r, 64);
 #pragma unroll
-      for (int k = 0; k < C::NG; ++k) qs[r][k] = __shfl(qs_row[k], 4 * jj + r, 64);
+        for (int k = 0; k < C::NG; ++k) qs[r][k] = __shfl(qs_row[k], 4 * jj + r, 64);
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+      }
     }
+    // the next unit's page ids are under way while this one's tiles are used
+    const bool last = unit + 1 >= end;
+    fresh = last || run.next(a, kPart);
+    if (!last) ids = pages();
+    float s[NR][kTiles];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       f4 acc[C::NG];
@@ -272,28 +358,31 @@ __global__ __launch_bounds__(kThreads) void mass_scores_kernel(const MassArgs a,
         s[r][i] = there[i] && t < sees[r] ? x * mult[r] : -INFINITY;
       }
     }
-    const int64_t seg = (int64_t)u.b * g.hk + u.kh;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       float *to = (float *)a.workspace + ((seg * quads(a.rows) + r) * w.tokens + t0 + col) * 4 + jj;
-      m[r] = -INFINITY;
+      float n = m[r];
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
-        m[r] = fmaxf(m[r], s[r][i]);
+        n = fmaxf(n, s[r][i]);
         to[i * PKV_TILE * 4] = s[r][i];  // (the row of parts is whole: nothing past it is written)
       }
-      const float z = m[r] == -INFINITY ? 0.0f : m[r];
-      l[r] = 0.0f;
+      const float z = n == -INFINITY ? 0.0f : n;
+      l[r] = m[r] == -INFINITY ? l[r] : l[r] * exp2_fast(m[r] - z);  // (0, or NaN, stays)
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) l[r] += exp2_fast(s[r][i] - z);
-      // the row's 16 lanes
+      m[r] = n;
+    }
+    if (!fresh) continue;
+    // the end of the segment's units here: its rows' (m, l) over the lanes and waves
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
       float mm = m[r];
       mm = fmaxf(mm, row_xchg<0xB1>(mm));
       mm = fmaxf(mm, row_xchg<0x4E>(mm));
       mm = fmaxf(mm, row_xchg<0x141>(mm));
       mm = fmaxf(mm, row_xchg<0x140>(mm));
-      float ll = l[r] * exp2_fast(z - (mm == -INFINITY ? 0.0f : mm));
-      if (m[r] == -INFINITY) ll = l[r];  // 0, or NaN
+      float ll = m[r] == -INFINITY ? l[r] : l[r] * exp2_fast(m[r] - mm);
       ll += row_xchg<0xB1>(ll);
       ll += row_xchg<0x4E>(ll);
       ll += row_xchg<0x141>(ll);
@@ -308,8 +397,10 @@ __global__ __launch_bounds__(kThreads) void mass_scores_kernel(const MassArgs a,
       float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
       for (int k = 0; k < kWaves; ++k) join(mm, ll, s_ml[k][threadIdx.x][0], s_ml[k][threadIdx.x][1]);
+      // of the segment's workgroups, this is the one after those before its first unit here
+      const int owner = run.owner(unit - part);
       float *to = (float *)((char *)a.workspace + w.scores) +
-                  ((seg * w.parts + u.part) * kFewRows + threadIdx.x) * 2;
+                  ((seg * w.parts + (blockIdx.x - owner)) * kFewRows + threadIdx.x) * 2;
       to[0] = mm;
       to[1] = ll;
     }
@@ -331,53 +422,68 @@ constexpr int kSumPart = 1024;  // tokens per unit of the second launch
 
 template <int NR>
 __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a, const FewParts w) {
-  __shared__ float s_lse[kFewRows];
   const int lane = threadIdx.x & 63;
+  auto parts_of = [](int len) { return (len + kPart - 1) / kPart; };
   Units u;
   u.start(a, kSumPart, lane);
-  for (int64_t unit = blockIdx.x; u.find(a, kSumPart, unit, lane); unit += gridDim.x) {
+  // the first launch's units: of the sequences before u.base, and of all
+  int before = 0, total = wave_sum(parts_of(u.len));
+  if (a.batch > 64) total = Runs::parts_before(a, kPart, lane, a.batch);
+  Runs run;
+  run.share(total * a.g.hk, w.grid);
+  for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
+    const int base = u.base;
+    if (!u.find(a, kSumPart, unit, lane)) return;
     const int row = mass_row(a, u.b);
     if (row < 0) continue;
     const int64_t seg = (int64_t)u.b * a.g.hk + u.kh;
-    // the rows' log-sum-exps: 32 lanes per row
+    // everything is requested before any of it is used
+    const float *scores = (const float *)a.workspace + seg * quads(a.rows) * w.tokens * 4;
+    float4 s[NR][4];
+    float old[4];
+    const int counted = !a.mass ? 0 : a.counted ? a.counted[u.b] : u.L;
+    const int64_t to = ((int64_t)row * a.g.hk + u.kh) * a.width;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = u.part * kSumPart + i * kThreads + threadIdx.x;
+      const int at = min(t, u.L - 1);
+#pragma unroll
+      for (int r = 0; r < NR; ++r) s[r][i] = *(const float4 *)(scores + ((int64_t)r * w.tokens + at) * 4);
+      old[i] = t < min(counted, u.L) ? a.mass[to + t] : 0.0f;
+    }
+    // the rows' log-sum-exps from the workgroups' (m, l): lane 8 k + r the k-th's of row r
+    float lse;
     {
-      const int r = threadIdx.x / 32, parts = (u.L + kPart - 1) / kPart;
-      const float2 *ml = (const float2 *)((const char *)a.workspace + w.scores) + seg * w.parts * kFewRows + r;
+      if (u.base != base) before = Runs::parts_before(a, kPart, lane, u.base);
+      const int n1 = parts_of(u.len), f = u.b - u.base, parts = __builtin_amdgcn_readlane(n1, f);
+      const int upto = __builtin_amdgcn_readlane(wave_scan_incl(n1, lane), f);
+      const int first = (before + upto - parts) * a.g.hk + u.kh * parts;
+      const int n = run.owner(first + parts - 1) - run.owner(first) + 1;
+      const float2 *ml = (const float2 *)((const char *)a.workspace + w.scores) + seg * w.parts * kFewRows;
       float m = -INFINITY, l = 0.0f;
-      if (r < NR * 4)
-        for (int p = threadIdx.x % 32; p < parts; p += 32) {
-          const float2 x = ml[(int64_t)p * kFewRows];
+      for (int k = lane / 8; k < n; k += 8)
+        if (lane % 8 < NR * 4) {
+          const float2 x = ml[k * kFewRows + lane % 8];
           join(m, l, x.x, x.y);
         }
 #pragma unroll
-      for (int k = 16; k > 0; k /= 2) join(m, l, __shfl_xor(m, k, 64), __shfl_xor(l, k, 64));
-      __syncthreads();
-      // a row that sees nothing weighs nothing
-      if (threadIdx.x % 32 == 0 && r < kFewRows) s_lse[r] = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);
-      __syncthreads();
-    }
-    const float *scores = (const float *)a.workspace + seg * quads(a.rows) * w.tokens * 4;
-    float4 s[NR][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = u.part * kSumPart + i * kThreads + threadIdx.x;
-      if (t < u.L)
-#pragma unroll
-        for (int r = 0; r < NR; ++r) s[r][i] = *(const float4 *)(scores + ((int64_t)r * w.tokens + t) * 4);
+      for (int k = 8; k < 64; k *= 2) join(m, l, __shfl_xor(m, k, 64), __shfl_xor(l, k, 64));
+      lse = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);  // a row that sees nothing weighs nothing
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = u.part * kSumPart + i * kThreads + threadIdx.x;
-      if (t >= u.L) continue;
       float sum = 0.0f;
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const float x[4] = {s[r][i].x, s[r][i].y, s[r][i].z, s[r][i].w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k)  // a token that the row does not see adds 0 also where the row's sum is NaN
-          sum += x[k] == -INFINITY ? 0.0f : exp2_fast(x[k] - s_lse[4 * r + k]);
+        for (int k = 0; k < 4; ++k) {  // a token that the row does not see adds 0 also where the row's sum is NaN
+          const float of_row = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lse), 4 * r + k));
+          sum += x[k] == -INFINITY ? 0.0f : exp2_fast(x[k] - of_row);
+        }
       }
-      store_mass(a, u.b, u.kh, row, t, sum);
+      if (t < u.L) a.out[to + t] = old[i] + sum;
     }
   }
 }
@@ -689,12 +795,19 @@ int walkers(int64_t units) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(units, 8 * (int64_t)std::max(1, device_cus())));
 }
 
+// Workgroups that share out at most `units` units: as many as stay resident at the
+// registers that the kernel needs (four of four waves per CU).
+int runs(int64_t units) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(units, 4 * (int64_t)std::max(1, device_cus())));
+}
+
 template <typename C>
 void launch(hipStream_t stream, const MassArgs &a, int64_t cap) {
   const int64_t segs = (int64_t)a.batch * a.g.hk;
   if (keeps_scores(a.g, segs, a.rows, cap)) {
-    const FewParts w(segs, a.rows, cap);
-    const dim3 grid(walkers(segs * w.parts)), second(walkers(segs * ((cap + kSumPart - 1) / kSumPart)));
+    FewParts w(segs, a.rows, cap);
+    w.grid = runs(segs * w.parts);
+    const dim3 grid(w.grid), second(walkers(segs * ((cap + kSumPart - 1) / kSumPart)));
     if (a.rows <= 4) {
       hipLaunchKernelGGL((mass_scores_kernel<C, 1>), grid, dim3(kThreads), 0, stream, a, w);
       hipLaunchKernelGGL((mass_weights_kernel<1>), second, dim3(kThreads), 0, stream, a, w);
