@@ -155,6 +155,7 @@ template <int BITS, int DP, int G, int FK>
 struct MassCfg : Cfg<BITS, DP, G, 1, FK, 1> {
   using Base = Cfg<BITS, DP, G, 1, FK, 1>;
   static constexpr int PAGE_BITS = BITS;
+  static constexpr int BM = (Base::NG + 3) / 4;  // float32 products per score tile of the group biases
   static constexpr int OPS = BITS == 16 ? FK : 1;  // operand type: f16 for codes
   using KT = typename FloatOps<OPS>::KT;
   static constexpr int GB = Base::QUANT ? G / 32 : Base::KB;  // 32-element blocks per accumulator
@@ -210,7 +211,13 @@ __device__ __forceinline__ void query_operands(const MassArgs &a, int b, int kh,
       for (int e = 0; e < 8; ++e) raw[kb][e] = there && d0 + e < a.g.dim ? src[d0 + e] : (uint16_t)0;
     }
   }
-  mult = a.scale * kLog2e;
+  // a multiplier of at least 0: the scale's sign goes to the elements
+  const uint16_t sign = a.scale < 0.0f ? 0x8000u : 0u;
+  mult = fabsf(a.scale) * kLog2e;
+#pragma unroll
+  for (int kb = 0; kb < C::KB; ++kb)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) raw[kb][e] ^= sign;
   if constexpr (!C::QUANT) {
 #pragma unroll
     for (int kb = 0; kb < C::KB; ++kb) __builtin_memcpy(&op[kb], raw[kb], 16);
@@ -489,32 +496,41 @@ __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a
 }
 
 // ---- many rows: K twice -----------------------------------------------------------------
+//
+// Rows in blocks of 16.  A workgroup of eight waves holds a unit's K tiles in
+// registers, two per wave, and goes through the row blocks, which it stages in LDS a
+// few at a time, the next ones under way while these are used.  Bound by the vector
+// ALU (the group scales and the exponentials, quarter rate) beside the matrix cores.
 
-// Rows in blocks of 16.  Workspace: query operands [segment][block][KB][64 lanes]
-// 16 bytes; per row [segment][block][16]: multiplier, tokens seen (as int), group
-// sums [NG], log-sum-exp; per block the most that any of its rows sees; parts
-// [segment][parts][rows] (m, l).
+constexpr int kManyWaves = 8, kManyThreads = 64 * kManyWaves;
+constexpr int kManyTiles = 2;  // per wave
+constexpr int kManyPart = kManyWaves * kManyTiles * PKV_TILE;
+
+// A block's record: query operands [KB][64 lanes] 16 bytes; then [16 rows] f32 each:
+// multiplier, log-sum-exp, tokens seen (int), the group sums [NG], and a last one: the
+// most and the least that its rows see.
+template <typename C>
+struct Record {
+  static constexpr int MULT = C::KB * 1024, LSE = MULT + 64, SEES = LSE + 64, QS = SEES + 64, RANGE = QS + C::NG * 64,
+                       BYTES = RANGE + 64;
+  static constexpr int STAGE = C::KB > 4 ? 2 : 4;  // records per stage
+};
+
+// Workspace: records [segment][block], parts [segment][part][rows] (m, l).
 struct ManyParts {
-  int64_t blocks, parts, ops, mult, sees, qs, lse, most, ml, total;
-  int part;  // tokens per unit
+  int64_t blocks, parts, record, ml, total;
   __host__ __device__ ManyParts(int64_t segs, int rows, int64_t cap, int dp, int ng) {
-    part = 16 * kWaves * (dp > 128 ? 2 : 4);
     blocks = (rows + 15) / 16;
-    parts = (cap + part - 1) / part;
-    const int64_t n = segs * blocks;
-    ops = 0;
-    mult = ops + n * 16 * dp * 2;
-    sees = mult + n * 16 * 4;
-    qs = sees + n * 16 * 4;
-    lse = qs + n * 16 * ng * 4;
-    most = lse + n * 16 * 4;
-    ml = (most + n * 4 + 15) / 16 * 16;
+    parts = (cap + kManyPart - 1) / kManyPart;
+    record = dp * 32 + 64 * (4 + (ng > 0 ? ng : 1));
+    ml = segs * blocks * record + 4 * record;  // (a stage's last copy reads past the last record)
     total = ml + segs * parts * blocks * 16 * 8;
   }
 };
 
 template <typename C>
 __global__ __launch_bounds__(kThreads) void mass_prepare_kernel(const MassArgs a, const ManyParts w) {
+  using R = Record<C>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
   const int64_t n = (int64_t)blockIdx.x * kWaves + wave;  // (segment, block)
   if (n >= w.blocks * a.batch * a.g.hk) return;
@@ -532,162 +548,250 @@ __global__ __launch_bounds__(kThreads) void mass_prepare_kernel(const MassArgs a
     for (int k = 0; k < C::NG; ++k) qs[k] = 0.0f;
     mult = 0.0f;
   }
-  char *base = (char *)a.workspace;
+  char *record = (char *)a.workspace + n * R::BYTES;
 #pragma unroll
-  for (int kb = 0; kb < C::KB; ++kb)
-    *(u4 *)(base + w.ops + ((n * C::KB + kb) * 64 + lane) * 16) = __builtin_bit_cast(u4, q[kb]);
-  int most = sees;
-  most = max(most, __shfl_xor(most, 1, 64));
-  most = max(most, __shfl_xor(most, 2, 64));
-  most = max(most, __shfl_xor(most, 4, 64));
-  most = max(most, __shfl_xor(most, 8, 64));
-  if (lane == 0) ((int *)(base + w.most))[n] = most;
+  for (int kb = 0; kb < C::KB; ++kb) *(u4 *)(record + (kb * 64 + lane) * 16) = __builtin_bit_cast(u4, q[kb]);
+  int most = sees, least = sees > 0 ? sees : INT32_MAX;  // (rows that see nothing weigh nothing in any case)
+#pragma unroll
+  for (int k = 1; k < 16; k *= 2) {
+    most = max(most, __shfl_xor(most, k, 64));
+    least = min(least, __shfl_xor(least, k, 64));
+  }
   if (jj == 0) {
-    ((float *)(base + w.mult))[n * 16 + col] = mult;
-    ((int *)(base + w.sees))[n * 16 + col] = sees;
-    if (C::QUANT)
+    ((float *)(record + R::MULT))[col] = mult;
+    ((float *)(record + R::LSE))[col] = 0.0f;
+    ((int *)(record + R::SEES))[col] = sees;
 #pragma unroll
-      for (int k = 0; k < C::NG; ++k) ((float *)(base + w.qs))[(n * C::NG + k) * 16 + col] = qs[k];
+    for (int k = 0; k < C::NG; ++k) ((float *)(record + R::QS))[k * 16 + col] = qs[k];
+    ((int *)(record + R::RANGE))[col] = col == 0 ? most : col == 1 ? least : 0;
   }
 }
 
-// A wave's tiles as operands.
-template <typename C, int N>
-struct KTiles {
-  typename C::KT k[N][C::KB];
-  bool there[N];
+// The group biases' part of 16x16 scores, in float32: rows a (of 16) and columns b,
+// lane l's a and b of its group l / 16 (and + 4).  For float pages a zero.
+template <typename C>
+__device__ __forceinline__ f4 bias_scores(const float (&a)[C::BM], const float (&b)[C::BM], f4 zero) {
+  f4 acc = zero;
+  if constexpr (C::QUANT)
+#pragma unroll
+    for (int k = 0; k < C::BM; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], acc, 0, 0, 0);
+  return acc;
+}
 
-  // The head block of each tile, for its metadata.
-  __device__ __forceinline__ void load(const MassArgs &a, const Units &u, int t0, int lane,
-                                       const uint8_t *(&meta)[N]) {
-    const Geo &g = a.g;
+// The pass over a launch's units.  SUM false: the (max, sum) of each row over the
+// unit's tokens, from S^T = K Q^T (a lane has one query row, its column, and four
+// tokens of each tile).  SUM true: the weights summed over the rows, from S = Q K^T
+// (a lane has one token of each tile and four rows).
+template <typename C, bool SUM>
+__global__ __launch_bounds__(kManyThreads, C::KB > 4 ? 2 : 4) void mass_pass_kernel(const MassArgs a, const ManyParts w) {
+  using R = Record<C>;
+  constexpr int N = kManyTiles, S = R::STAGE, kUnits = (S * R::BYTES + 15) / 16;
+  constexpr int kCopies = (kUnits + kManyThreads - 1) / kManyThreads;
+  __shared__ __align__(16) char s_rec[2][S * R::BYTES];
+  __shared__ float2 s_ml[SUM ? 1 : 2][SUM ? 1 : kManyWaves][SUM ? 1 : S * 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jj = lane >> 4,
+            col = lane & 15;
+  const Geo &g = a.g;
+  const f4 zero = register_zero();
+  Units u;
+  u.start(a, kManyPart, lane);
+  for (int64_t unit = blockIdx.x; u.find(a, kManyPart, unit, lane); unit += gridDim.x) {
+    const int first = u.part * kManyPart, t0 = first + wave * (N * PKV_TILE);
+    const int out_row = SUM ? mass_row(a, u.b) : 0;
+    if (SUM && out_row < 0) continue;
+    const int64_t seg = (int64_t)u.b * g.hk + u.kh;
+    const char *records = (const char *)a.workspace + seg * w.blocks * R::BYTES;
+    // the records of S blocks from b0 on straight to LDS, 16 bytes per lane (what lies
+    // past the last block is in the workspace and not used)
+    auto fetch = [&](int64_t b0, int buffer) {
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k) {
+        const int unit0 = (wave + k * kManyWaves) * 64;
+        if (unit0 < kUnits) {
+          const char *from = records + b0 * R::BYTES + (int64_t)(unit0 + lane) * 16;
+          if (unit0 + lane < kUnits)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)from,
+                                             (__attribute__((address_space(3))) uint32_t *)(s_rec[buffer] + unit0 * 16),
+                                             16, 0, 0);
+        }
+      }
+    };
+    fetch(0, 0);
+
+    // the wave's tiles
+    typename C::KT kt[N][C::KB];
+    bool there[N], all = true;
+    float scale[N][SUM ? 1 : 4][C::NG], bias[N][C::BM];  // of the lane's token, or its four
     const int ids = tile_page<N>(a, u.b, t0, u.L, lane);
-    uint32_t w[N][C::LW];
+    uint32_t kw[N][C::LW];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int id = __builtin_amdgcn_readlane(ids, i);
       there[i] = id >= 0;
+      all = all && there[i];
       const int slot = (t0 + i * PKV_TILE) % g.page;
       const uint8_t *head = a.pool + (int64_t)max(id, 0) * g.page_bytes + (int64_t)u.kh * g.head_bytes;
-      meta[i] = head + g.kmeta_offset + (int64_t)slot * C::NG * 4;
+      const uint8_t *meta = head + g.kmeta_offset + (int64_t)slot * C::NG * 4;
 #pragma unroll
-      for (int j = 0; j < C::LW; ++j) w[i][j] = 0;
-      if (there[i]) load_payload<C>(w[i], head + (slot / PKV_TILE) * g.tile_bytes, lane);
+      for (int j = 0; j < C::LW; ++j) kw[i][j] = 0;
+      if (there[i]) load_payload<C>(kw[i], head + (slot / PKV_TILE) * g.tile_bytes, lane);
+      if constexpr (C::QUANT) {
+#pragma unroll
+        for (int k = 0; k < C::BM; ++k) {
+          const int gi = jj + 4 * k;
+          uint32_t x = 0;
+          if (there[i] && gi < C::NG) x = ((const uint32_t *)meta)[col * C::NG + gi];
+          bias[i][k] = f16_bits_to_f32(x >> 16);
+        }
+        if constexpr (SUM) {
+#pragma unroll
+          for (int j = 0; j < C::NG; ++j)
+            scale[i][0][j] = there[i] ? f16_bits_to_f32(((const uint32_t *)meta)[col * C::NG + j]) : 0.0f;
+        } else {
+          uint32_t mw[4 * C::NG];
+#pragma unroll
+          for (int k = 0; k < C::NG; ++k) {
+            u4 x = {0, 0, 0, 0};
+            if (there[i]) x = ((const u4 *)meta)[jj * C::NG + k];
+            mw[4 * k] = x.x; mw[4 * k + 1] = x.y; mw[4 * k + 2] = x.z; mw[4 * k + 3] = x.w;
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < C::NG; ++j) scale[i][SUM ? 0 : r][j] = f16_bits_to_f32(mw[r * C::NG + j]);
+        }
+      }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int kb = 0; kb < C::KB; ++kb) k[i][kb] = k_operand<C>(w[i], kb);
-  }
-};
+      for (int kb = 0; kb < C::KB; ++kb) kt[i][kb] = k_operand<C>(kw[i], kb);
+    float sum[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the records have arrived
+    __syncthreads();
 
-template <typename C>
-__device__ __forceinline__ void load_block(const char *base, const ManyParts &w, int64_t n, int lane,
-                                           typename C::KT (&q)[C::KB]) {
-#pragma unroll
-  for (int kb = 0; kb < C::KB; ++kb)
-    q[kb] = __builtin_bit_cast(typename C::KT, *(const u4 *)(base + w.ops + ((n * C::KB + kb) * 64 + lane) * 16));
-}
-
-// The (max, sum) of each row over the unit's tokens: S^T = K Q^T, a lane has one
-// query row (its column) and four tokens of each tile.
-template <typename C, int N>
-__global__ __launch_bounds__(kThreads) void mass_parts_kernel(const MassArgs a, const ManyParts w) {
-  constexpr int kBatch = 32;  // row blocks between two joins of the waves
-  __shared__ float2 s_ml[kWaves][kBatch * 16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
-  char *base = (char *)a.workspace;
-  const f4 zero = register_zero();
-  Units u;
-  u.start(a, w.part, lane);
-  for (int64_t unit = blockIdx.x; u.find(a, w.part, unit, lane); unit += gridDim.x) {
-    const int t0 = u.part * w.part + wave * (N * PKV_TILE);
-    const int64_t seg = (int64_t)u.b * a.g.hk + u.kh;
-    const uint8_t *meta[N];
-    KTiles<C, N> tiles;
-    tiles.load(a, u, t0, lane, meta);
-    uint32_t mw[N][4 * C::NG];
-    bool all = true;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      all = all && tiles.there[i];
-#pragma unroll
-      for (int k = 0; k < 4 * C::NG; ++k) mw[i][k] = 0;
-      if (C::QUANT && tiles.there[i])
-#pragma unroll
-        for (int k = 0; k < C::NG; ++k) {
-          const u4 x = ((const u4 *)meta[i])[jj * C::NG + k];
-          mw[i][4 * k] = x.x; mw[i][4 * k + 1] = x.y; mw[i][4 * k + 2] = x.z; mw[i][4 * k + 3] = x.w;
-        }
-    }
-    for (int64_t b0 = 0; b0 < w.blocks; b0 += kBatch) {
-      const int nb = (int)min((int64_t)kBatch, w.blocks - b0);
+    int buffer = 0;
+    for (int64_t b0 = 0; b0 < w.blocks; b0 += S, buffer ^= 1) {
+      const bool more = b0 + S < w.blocks;
+      if (more) fetch(b0 + S, buffer ^ 1);
+      const int nb = (int)min((int64_t)S, w.blocks - b0);
       for (int k = 0; k < nb; ++k) {
-        const int64_t n = seg * w.blocks + b0 + k;
-        float m = -INFINITY, l = 0.0f;
-        if (((const int *)(base + w.most))[n] > t0) {
-          typename C::KT q[C::KB];
-          load_block<C>(base, w, n, lane, q);
-          const float mult = ((const float *)(base + w.mult))[n * 16 + col];
-          const int sees = ((const int *)(base + w.sees))[n * 16 + col];
-          float qs[C::NG];
-          if (C::QUANT)
+        const char *rec = s_rec[buffer] + k * R::BYTES;
+        const int most = __builtin_amdgcn_readfirstlane(((const int *)(rec + R::RANGE))[0]);
+        const int least = __builtin_amdgcn_readfirstlane(((const int *)(rec + R::RANGE))[1]);
+        if (most <= t0) {  // no row sees any of the wave's tokens
+          if (!SUM && jj == 0) s_ml[buffer & (SUM ? 0 : 1)][SUM ? 0 : wave][SUM ? 0 : k * 16 + col] = float2{-INFINITY, 0.0f};
+          continue;
+        }
+        typename C::KT q[C::KB];
 #pragma unroll
-            for (int j = 0; j < C::NG; ++j) qs[j] = ((const float *)(base + w.qs))[(n * C::NG + j) * 16 + col];
-          float s[N][4];
+        for (int kb = 0; kb < C::KB; ++kb) q[kb] = __builtin_bit_cast(typename C::KT, *(const u4 *)(rec + (kb * 64 + lane) * 16));
+        float qs[C::BM];
+        // (group sums past the last are met by biases of 0: read the last one's)
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            f4 acc[C::NG];
+        for (int j = 0; j < C::BM; ++j)
+          qs[j] = C::QUANT ? ((const float *)(rec + R::QS))[min(jj + 4 * j, C::NG - 1) * 16 + col] : 0.0f;
+        float x[N][4];
 #pragma unroll
-            for (int j = 0; j < C::NG; ++j) acc[j] = zero;
+        for (int i = 0; i < N; ++i) {
+          f4 acc[C::NG];
+          const f4 base = SUM ? bias_scores<C>(qs, bias[i], zero) : bias_scores<C>(bias[i], qs, zero);
 #pragma unroll
-            for (int kb = 0; kb < C::KB; ++kb)
-              acc[kb / C::GB] = FloatOps<C::OPS>::qk(tiles.k[i][kb], q[kb], acc[kb / C::GB]);
+          for (int j = 0; j < C::NG; ++j) acc[j] = zero;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              float x = 0.0f;
-              if constexpr (C::QUANT) {
+          for (int kb = 0; kb < C::KB; ++kb)
+            acc[kb / C::GB] = SUM ? FloatOps<C::OPS>::qk(q[kb], kt[i][kb], acc[kb / C::GB])
+                                  : FloatOps<C::OPS>::qk(kt[i][kb], q[kb], acc[kb / C::GB]);
 #pragma unroll
-                for (int j = 0; j < C::NG; ++j) x = fmaf(f16_bits_to_f32(mw[i][r * C::NG + j] >> 16), qs[j], x);
+          for (int r = 0; r < 4; ++r) {
+            x[i][r] = C::QUANT ? base[r] : acc[0][r];
+            if constexpr (C::QUANT)
 #pragma unroll
-                for (int j = 0; j < C::NG; ++j) x = fmaf(f16_bits_to_f32(mw[i][r * C::NG + j]), acc[j][r], x);
-              } else {
-                x = acc[0][r];
-              }
-              x *= mult;
-              s[i][r] = tiles.there[i] && t0 + i * PKV_TILE + 4 * jj + r < sees ? x : -INFINITY;
-              m = fmaxf(m, s[i][r]);
-            }
+              for (int j = 0; j < C::NG; ++j)
+                x[i][r] = fmaf(scale[i][SUM ? 0 : r][j], acc[j][r], x[i][r]);
           }
-          const float mm = xor32_max(xor16_max(m)), z = mm == -INFINITY ? 0.0f : mm;
+        }
+        const bool masked = !all || least < t0 + N * PKV_TILE;  // not every row sees every token
+        if constexpr (SUM) {
+          const f4 mult = *(const f4 *)(rec + R::MULT + jj * 16), lse = *(const f4 *)(rec + R::LSE + jj * 16);
+          f4 p[N];
 #pragma unroll
           for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) l += exp2_fast(s[i][r] - z);
+            for (int r = 0; r < 4; ++r) p[i][r] = exp2_fast(fmaf(x[i][r], mult[r], -lse[r]));
+          if (masked) {
+            const int4 sees = *(const int4 *)(rec + R::SEES + jj * 16);
+            const int see[4] = {sees.x, sees.y, sees.z, sees.w};
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (!there[i] || t0 + i * PKV_TILE + col >= see[r]) p[i][r] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[i] += (p[i][0] + p[i][1]) + (p[i][2] + p[i][3]);
+        } else {
+          const float mult = ((const float *)(rec + R::MULT))[col];
+          int sees = INT32_MAX;
+          if (masked) {
+            sees = ((const int *)(rec + R::SEES))[col];
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (!there[i] || t0 + i * PKV_TILE + 4 * jj + r >= sees) x[i][r] = -INFINITY;
+          }
+          // raw scores, one multiplier (not negative) for the row
+          float m = -INFINITY, l = 0.0f;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) m = fmaxf(m, x[i][r]);
+          m = xor32_max(xor16_max(m));
+          const float z = m == -INFINITY ? 0.0f : m * mult;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) l += exp2_fast(fmaf(x[i][r], mult, -z));
           l = xor32_add(xor16_add(l));
-          m = mm;
+          if (sees == 0) l = 0.0f;  // (its multiplier is 0, and -inf times that is no number)
+          if (jj == 0) s_ml[SUM ? 0 : buffer][SUM ? 0 : wave][SUM ? 0 : k * 16 + col] = float2{m == -INFINITY ? m : z, l};
         }
-        if (jj == 0) s_ml[wave][k * 16 + col] = float2{m, l};
       }
+      // the next records have arrived
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
-      float2 *to = (float2 *)(base + w.ml) + ((seg * w.parts + u.part) * w.blocks + b0) * 16;
-      for (int r = threadIdx.x; r < nb * 16; r += kThreads) {
+      if (!SUM && (int)threadIdx.x < nb * 16) {
+        // (these are written again two stages on, behind another barrier)
         float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) join(m, l, s_ml[k][r].x, s_ml[k][r].y);
-        to[r] = float2{m, l};
+        for (int k = 0; k < kManyWaves; ++k) {
+          const float2 y = s_ml[SUM ? 0 : buffer][SUM ? 0 : k][SUM ? 0 : threadIdx.x];
+          join(m, l, y.x, y.y);
+        }
+        ((float2 *)((char *)a.workspace + w.ml))[((seg * w.parts + u.part) * w.blocks + b0) * 16 + threadIdx.x] = float2{m, l};
       }
-      __syncthreads();
     }
+    if constexpr (SUM) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float total = xor32_add(xor16_add(sum[i]));
+        const int t = t0 + i * PKV_TILE + col;
+        if (jj == 0 && t < u.L) store_mass(a, u.b, u.kh, out_row, t, total);
+      }
+    }
+    __syncthreads();  // the buffers and sums are used again
   }
 }
 
 // Each row's log-sum-exp from its parts: 16 rows of 16 lanes per workgroup.
-__global__ __launch_bounds__(kThreads) void mass_join_kernel(const MassArgs a, const ManyParts w) {
+__global__ __launch_bounds__(kThreads) void mass_join_kernel(const MassArgs a, const ManyParts w, int at_lse, int at_sees) {
   const int64_t rows = w.blocks * 16;
-  const int64_t seg = blockIdx.x / w.blocks, row = blockIdx.x % w.blocks * 16 + threadIdx.x % 16;
+  const int64_t seg = blockIdx.x / w.blocks, block = blockIdx.x % w.blocks, row = block * 16 + threadIdx.x % 16;
   __shared__ float s_ml[2][16][17];
-  const int parts = (max(0, mass_len(a, (int)(seg / a.g.hk))) + w.part - 1) / w.part, slice = threadIdx.x / 16;
+  const int parts = (max(0, mass_len(a, (int)(seg / a.g.hk))) + kManyPart - 1) / kManyPart, slice = threadIdx.x / 16;
   const float2 *ml = (const float2 *)((const char *)a.workspace + w.ml) + seg * w.parts * rows + row;
   float m = -INFINITY, l = 0.0f;
   for (int p = slice; p < parts; p += 16) {
@@ -699,84 +803,10 @@ __global__ __launch_bounds__(kThreads) void mass_join_kernel(const MassArgs a, c
   __syncthreads();
   if (slice == 0) {
     for (int k = 1; k < 16; ++k) join(m, l, s_ml[0][k][threadIdx.x], s_ml[1][k][threadIdx.x]);
-    ((float *)((char *)a.workspace + w.lse))[seg * rows + row] =
-        l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);  // a row that sees nothing weighs nothing
-  }
-}
-
-// The weights summed over the rows: S = Q K^T, a lane has one token of each tile
-// and four query rows.
-template <typename C, int N>
-__global__ __launch_bounds__(kThreads) void mass_sum_kernel(const MassArgs a, const ManyParts w) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
-  const char *base = (const char *)a.workspace;
-  const f4 zero = register_zero();
-  Units u;
-  u.start(a, w.part, lane);
-  for (int64_t unit = blockIdx.x; u.find(a, w.part, unit, lane); unit += gridDim.x) {
-    const int t0 = u.part * w.part + wave * (N * PKV_TILE);
-    const int row = mass_row(a, u.b);
-    if (t0 >= u.L || row < 0) continue;
-    const int64_t seg = (int64_t)u.b * a.g.hk + u.kh;
-    const uint8_t *meta[N];
-    KTiles<C, N> tiles;
-    tiles.load(a, u, t0, lane, meta);
-    float scale[N][C::NG], bias[N][C::NG], sum[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      sum[i] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < C::NG; ++j) {
-        uint32_t x = 0;
-        if (C::QUANT && tiles.there[i]) x = ((const uint32_t *)meta[i])[col * C::NG + j];
-        scale[i][j] = f16_bits_to_f32(x);
-        bias[i][j] = f16_bits_to_f32(x >> 16);
-      }
-    }
-    for (int64_t k = 0; k < w.blocks; ++k) {
-      const int64_t n = seg * w.blocks + k;
-      if (((const int *)(base + w.most))[n] <= t0) continue;
-      typename C::KT q[C::KB];
-      load_block<C>(base, w, n, lane, q);
-      const f4 mult = *(const f4 *)(base + w.mult + (n * 16 + 4 * jj) * 4);
-      const f4 lse = *(const f4 *)(base + w.lse + (n * 16 + 4 * jj) * 4);
-      const int4 sees = *(const int4 *)(base + w.sees + (n * 16 + 4 * jj) * 4);
-      const int see[4] = {sees.x, sees.y, sees.z, sees.w};
-      f4 qs[C::NG];
-      if (C::QUANT)
-#pragma unroll
-        for (int j = 0; j < C::NG; ++j) qs[j] = *(const f4 *)(base + w.qs + ((n * C::NG + j) * 16 + 4 * jj) * 4);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        f4 acc[C::NG];
-#pragma unroll
-        for (int j = 0; j < C::NG; ++j) acc[j] = zero;
-#pragma unroll
-        for (int kb = 0; kb < C::KB; ++kb)
-          acc[kb / C::GB] = FloatOps<C::OPS>::qk(q[kb], tiles.k[i][kb], acc[kb / C::GB]);
-        const int t = t0 + i * PKV_TILE + col;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = 0.0f;
-          if constexpr (C::QUANT) {
-#pragma unroll
-            for (int j = 0; j < C::NG; ++j) x = fmaf(bias[i][j], qs[j][r], x);
-#pragma unroll
-            for (int j = 0; j < C::NG; ++j) x = fmaf(scale[i][j], acc[j][r], x);
-          } else {
-            x = acc[0][r];
-          }
-          const float p = exp2_fast(fmaf(x, mult[r], -lse[r]));
-          sum[i] += tiles.there[i] && t < see[r] ? p : 0.0f;
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float all = xor32_add(xor16_add(sum[i]));
-      const int t = t0 + i * PKV_TILE + col;
-      if (jj == 0 && t < u.L) store_mass(a, u.b, u.kh, row, t, all);
-    }
+    char *record = (char *)a.workspace + (seg * w.blocks + block) * w.record;
+    // a row that sees nothing weighs nothing
+    const bool none = ((const int *)(record + at_sees))[threadIdx.x] == 0 || l == 0.0f;
+    ((float *)(record + at_lse))[threadIdx.x] = none ? INFINITY : m + __builtin_amdgcn_logf(l);
   }
 }
 
@@ -817,14 +847,15 @@ void launch(hipStream_t stream, const MassArgs &a, int64_t cap) {
     }
     return;
   }
-  constexpr int N = C::KB > 4 ? 2 : 4;
-  const ManyParts w(segs, a.rows, cap, a.g.dp, C::QUANT ? C::NG : 0);
+  using R = Record<C>;
+  const ManyParts w(segs, a.rows, cap, a.g.dp, a.g.ng);
+  static_assert(R::BYTES == C::KB * 1024 + 64 * (4 + C::NG), "as ManyParts has it");
   const dim3 grid(walkers(segs * w.parts));
   const unsigned blocks = (unsigned)(segs * w.blocks);
   hipLaunchKernelGGL((mass_prepare_kernel<C>), dim3((blocks + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a, w);
-  hipLaunchKernelGGL((mass_parts_kernel<C, N>), grid, dim3(kThreads), 0, stream, a, w);
-  hipLaunchKernelGGL(mass_join_kernel, dim3(blocks), dim3(kThreads), 0, stream, a, w);
-  hipLaunchKernelGGL((mass_sum_kernel<C, N>), grid, dim3(kThreads), 0, stream, a, w);
+  hipLaunchKernelGGL((mass_pass_kernel<C, false>), grid, dim3(kManyThreads), 0, stream, a, w);
+  hipLaunchKernelGGL(mass_join_kernel, dim3(blocks), dim3(kThreads), 0, stream, a, w, R::LSE, R::SEES);
+  hipLaunchKernelGGL((mass_pass_kernel<C, true>), grid, dim3(kManyThreads), 0, stream, a, w);
 }
 
 template <int BITS, int DP>
