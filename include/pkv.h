@@ -373,7 +373,9 @@ int pkv_arena_fork(void *stream, void *state, int32_t capacity_pages, int32_t pa
  * ---- which cached state lives on --------------------------------------------------
  *
  * No counterpart in the reference: its caches grow until they are trimmed by
- * length, and it decodes one sequence per request.
+ * length, and it decodes one sequence per request.  The sizes that these
+ * operators' workspace queries return are negative for shapes that the operator
+ * refuses, by its status (-PKV_INVALID_ARGUMENT, -PKV_UNSUPPORTED).
  */
 
 /*
@@ -415,7 +417,8 @@ int64_t pkv_attention_mass_workspace_bytes(const pkv_layout *layout, int32_t num
  *
  *  mass     : [layers][mass_rows][kv_heads][mass_width] f32
  *  rows     : [batch] row of mass per sequence, or NULL for row b (a sequence
- *             whose row does not exist keeps nothing)
+ *             whose row does not exist keeps nothing); distinct where new_mass is
+ *             given
  *  keep     : [batch] int32, or NULL for max_keep
  *  kept     : [layers][batch][kv_heads][max_keep] int32 out, ascending, -1 from n on
  *  new_lens : [batch] int32 out, n
@@ -432,8 +435,8 @@ int pkv_evict_select(void *stream, const float *mass, int32_t layers, int32_t ma
 
 /*
  * The kept tokens' K and V (of every layer's pool, codes and metadata bit for bit)
- * to positions 0..new_lens[b]-1 of the pages of dst_table, which must not be
- * pages of src_table.  Nothing else in the destination pages changes; a kept
+ * to positions 0..new_lens[b]-1 of the pages of dst_table, which must be distinct
+ * and no pages of src_table.  Nothing else in the destination pages changes; a kept
  * index without a mapped source page leaves its position as it is, positions
  * past the destination table are dropped.  Keys move as they were stored, with
  * the rotation of their original positions.
@@ -484,7 +487,7 @@ int pkv_reorder_rows(void *stream, void *state, int64_t outer, int32_t num_rows,
  * becomes a copy of what slot sources[i] held before the call, sharing its pages
  * (a shared, partly filled tail is copied when it is next written); pages that
  * no slot holds any more go back on the free stack.  A slot that is out of range
- * sets PKV_ARENA_BAD_ARGUMENT and its pair is skipped.  At most 8192 pairs.
+ * sets PKV_ARENA_BAD_ARGUMENT and its pair is skipped.  At most 4096 pairs.
  *
  *  workspace : pkv_arena_reorder_workspace_bytes(count, max_pages) bytes of device
  *              scratch

@@ -42,6 +42,25 @@ int mass_shape(const pkv_layout *layout, int32_t num_heads, int32_t num_queries,
   if ((int64_t)batch * g->hk > 65535) return fail(PKV_UNSUPPORTED, "at most 65535 (sequence, KV head) pairs");
   if ((int64_t)batch * g->hk * max_pages > (1 << 30))
     return fail(PKV_UNSUPPORTED, "at most 2^30 pages of (sequence, KV head) pairs");
+  if ((int64_t)batch * g->hk * num_queries * (num_heads / g->hk) > (1 << 30))
+    return fail(PKV_UNSUPPORTED, "at most 2^30 query rows");
+  return PKV_OK;
+}
+
+int beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count) {
+  if (groups < 0 || beams < 1 || vocab < 1 || count < 1) return fail(PKV_INVALID_ARGUMENT, "invalid beam shape");
+  if (beams > pkv::kMaxBeams || count > pkv::kMaxBeamCount)
+    return fail(PKV_UNSUPPORTED, "at most 64 beams and 64 selected pairs per group");
+  if ((int64_t)beams * vocab > INT32_MAX || (int64_t)groups * beams > (1 << 24) ||
+      (int64_t)groups * beams * vocab > ((int64_t)1 << 40))
+    return fail(PKV_UNSUPPORTED, "at most 2^31 - 1 (beam, token) pairs per group, 2^24 beams and 2^40 pairs");
+  if (count > (int64_t)beams * vocab) return fail(PKV_INVALID_ARGUMENT, "fewer (beam, token) pairs than the count");
+  return PKV_OK;
+}
+
+int reorder_shape(int32_t count, int32_t max_pages) {
+  if (count < 0 || max_pages < 1) return fail(PKV_INVALID_ARGUMENT, "invalid reorder shape");
+  if (count > pkv::kMaxArenaReorder) return fail(PKV_UNSUPPORTED, "at most 4096 slots are reordered in a call");
   return PKV_OK;
 }
 
@@ -53,7 +72,7 @@ int64_t pkv_attention_mass_workspace_bytes(const pkv_layout *layout, int32_t num
                                            int32_t batch, int32_t max_pages) {
   return guarded([&]() -> int64_t {
     pkv_geometry g;
-    if (mass_shape(layout, num_heads, num_queries, batch, max_pages, &g)) return -1;
+    if (int rc = mass_shape(layout, num_heads, num_queries, batch, max_pages, &g)) return -rc;
     return pkv::mass_workspace(pkv::to_geo(g), batch, num_queries * (num_heads / g.hk), max_pages);
   });
 }
@@ -175,10 +194,7 @@ int pkv_evict_pages(void *stream, const pkv_layout *layout, void *const *pools, 
 
 int64_t pkv_beam_workspace_bytes(int32_t groups, int32_t beams, int32_t vocab, int32_t count) {
   return guarded([&]() -> int64_t {
-    if (groups < 0 || beams < 1 || beams > pkv::kMaxBeams || vocab < 1 || count < 1 || count > pkv::kMaxBeamCount) {
-      fail(PKV_INVALID_ARGUMENT, "invalid beam shape");
-      return -1;
-    }
+    if (int rc = beam_shape(groups, beams, vocab, count)) return -rc;
     return pkv::beam_workspace(groups, beams, vocab, count);
   });
 }
@@ -189,12 +205,7 @@ int pkv_beam_select(void *stream, const void *logits, int32_t kind, int32_t grou
                     int32_t *parents, int32_t *tokens) {
   return guarded([&]() -> int {
     if (kind < 0 || kind > 2) return fail(PKV_INVALID_ARGUMENT, "logits must be bf16 (0), f16 (1) or f32 (2)");
-    if (groups < 0 || beams < 1 || vocab < 1 || count < 1) return fail(PKV_INVALID_ARGUMENT, "invalid beam shape");
-    if (beams > pkv::kMaxBeams || count > pkv::kMaxBeamCount)
-      return fail(PKV_UNSUPPORTED, "at most 64 beams and 64 selected pairs per group");
-    if ((int64_t)beams * vocab > INT32_MAX || (int64_t)groups * beams > (1 << 24))
-      return fail(PKV_UNSUPPORTED, "at most 2^31 - 1 (beam, token) pairs per group and 2^24 beams");
-    if (count > (int64_t)beams * vocab) return fail(PKV_INVALID_ARGUMENT, "fewer (beam, token) pairs than the count");
+    if (int rc = beam_shape(groups, beams, vocab, count)) return rc;
     if (group_stride < 0 || beam_stride < 0) return fail(PKV_INVALID_ARGUMENT, "negative logits stride");
     if (done && (pad_token < 0 || pad_token >= vocab))
       return fail(PKV_INVALID_ARGUMENT, "the pad token must lie in the vocabulary");
@@ -247,10 +258,7 @@ int pkv_reorder_rows(void *stream, void *state, int64_t outer, int32_t num_rows,
 
 int64_t pkv_arena_reorder_workspace_bytes(int32_t count, int32_t max_pages) {
   return guarded([&]() -> int64_t {
-    if (count < 0 || count > pkv::kMaxReorder || max_pages < 1) {
-      fail(PKV_INVALID_ARGUMENT, "invalid reorder shape");
-      return -1;
-    }
+    if (int rc = reorder_shape(count, max_pages)) return -rc;
     return count == 0 ? 0 : pkv::arena_reorder_workspace(count, max_pages);
   });
 }
@@ -265,8 +273,7 @@ int pkv_arena_reorder(void *stream, void *state, int32_t capacity_pages, int32_t
       return fail(PKV_INVALID_ARGUMENT, "page_tokens must be 16, 32, 64 or 128");
     if (num_slots < 1 || max_pages < 1 || (int64_t)max_pages * page_tokens > INT32_MAX)
       return fail(PKV_INVALID_ARGUMENT, "invalid slot table shape");
-    if (count < 0) return fail(PKV_INVALID_ARGUMENT, "negative count");
-    if (count > pkv::kMaxReorder) return fail(PKV_UNSUPPORTED, "at most 8192 slots are reordered in a call");
+    if (int rc = reorder_shape(count, max_pages)) return rc;
     if (!state || !slot_table || !slot_lens || (count > 0 && (!slots || !sources)))
       return fail(PKV_INVALID_ARGUMENT, "NULL arena tensor");
     if (count == 0) return PKV_OK;

@@ -80,7 +80,7 @@ struct ReorderArgs {
   int count;
 };
 
-constexpr int kMaxReorder = 8192;
+constexpr int kMaxReorder = 8192, kMaxArenaReorder = 4096;
 hipError_t launch_reorder_rows(hipStream_t stream, const ReorderArgs &a);
 
 struct ArenaReorderArgs {

@@ -734,9 +734,8 @@ __global__ __launch_bounds__(kManyThreads, C::KB > 4 ? 2 : 4) void mass_pass_ker
           for (int i = 0; i < N; ++i) sum[i] += (p[i][0] + p[i][1]) + (p[i][2] + p[i][3]);
         } else {
           const float mult = ((const float *)(rec + R::MULT))[col];
-          int sees = INT32_MAX;
           if (masked) {
-            sees = ((const int *)(rec + R::SEES))[col];
+            const int sees = ((const int *)(rec + R::SEES))[col];
 #pragma unroll
             for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -751,12 +750,18 @@ __global__ __launch_bounds__(kManyThreads, C::KB > 4 ? 2 : 4) void mass_pass_ker
             for (int r = 0; r < 4; ++r) m = fmaxf(m, x[i][r]);
           m = xor32_max(xor16_max(m));
           const float z = m == -INFINITY ? 0.0f : m * mult;
+          if (!masked) {
 #pragma unroll
-          for (int i = 0; i < N; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) l += exp2_fast(fmaf(x[i][r], mult, -z));
+              for (int r = 0; r < 4; ++r) l += exp2_fast(fmaf(x[i][r], mult, -z));
+          } else {  // (-inf times a multiplier of 0 is no number)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) l += x[i][r] == -INFINITY ? 0.0f : exp2_fast(fmaf(x[i][r], mult, -z));
+          }
           l = xor32_add(xor16_add(l));
-          if (sees == 0) l = 0.0f;  // (its multiplier is 0, and -inf times that is no number)
           if (jj == 0) s_ml[SUM ? 0 : buffer][SUM ? 0 : wave][SUM ? 0 : k * 16 + col] = float2{m == -INFINITY ? m : z, l};
         }
       }

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void arena_reorder_kernel(const ArenaReor
 // One workgroup: the lists onto the free stack, in the workgroups' order, and the
 // slots' lengths.
 __global__ __launch_bounds__(1024) void arena_reorder_finish_kernel(const ArenaReorderArgs a, int columns, int blocks) {
-  __shared__ int s_len[kMaxReorder];
+  __shared__ int s_len[kMaxArenaReorder];
   int32_t *stack = a.state + kArenaHeaderWords;
   for (int i = threadIdx.x; i < a.count; i += 1024) {
     const int from = a.sources[i];

@@ -250,10 +250,11 @@ class DevicePageArena:
         and KV head its first ``sinks`` and last ``recent`` tokens and the ones that
         have drawn most attention weight (``ops.evict_select``).  They move to new
         pages (shared ones stay as they are for the others) and keep their sums;
-        later tokens' positions go on as if none were evicted.
+        later tokens' positions go on as if none were evicted, and ``truncate``
+        takes back tokens that came after.
 
-        ``keep`` an int or one per slot (on the device: with ``max_keep``).  The
-        new pages are taken before the old ones go; slots without room for them stay
+        ``keep`` an int or one per slot (on the device: with ``max_keep``).  The new
+        pages are taken before the old ones go; slots without room for them stay
         as they are and the arena records ``OUT_OF_PAGES``, which host lists of
         slots raise.  ``spare``: empty slots to work in, one at least (default:
         free ones); the slots are cut as many at a time as there are."""

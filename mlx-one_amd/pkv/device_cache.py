@@ -117,6 +117,8 @@ class DevicePrefixIndex:
         pages = min(len(tokens), self.arena.lengths[slot]) // self.arena.page_tokens
         if pages == 0 or pages > self.capacity_pages:
             return False
+        if self.arena.evicted is not None and int(self.arena.evicted[slot]) > 0:
+            return False     # tokens were evicted: its pages are no prefix of the text
         keys = self._keys(fingerprint, tokens, pages)
         for entry in self._entries:
             if entry.fingerprint == fingerprint.digest and entry.keys[:pages] == keys:

@@ -491,7 +491,7 @@ def _address(x, device, count, name):
 def _scratch(nbytes, device, what, given=None):
     """The caller's workspace, or the stream's own memory of that size."""
     if nbytes < 0:
-        nat.check(nat.PKV_INVALID_ARGUMENT, what)
+        nat.check(-nbytes, what)
     if given is None:
         return torch.empty(nbytes or 16, dtype=torch.uint8, device=device)
     if given.device != device or given.dtype is not torch.uint8 or not given.is_contiguous():
@@ -685,13 +685,11 @@ def beam_select(logits, scores, count, *, done=None, pad_token=0, workspace=None
             raise ValueError("done must be a [groups, beams] bool tensor on the logits' device")
         done = done.contiguous()
         done_at = done.data_ptr()
-    best = torch.empty((groups, count), dtype=torch.float32, device=device)
-    parents, tokens = torch.empty((2, groups, count), dtype=torch.int32, device=device).unbind(0)
-    if groups == 0:
-        return best, parents, tokens
     lib = nat.load()
     workspace = _scratch(lib.pkv_beam_workspace_bytes(groups, beams, vocab, count), device,
                          "beam select", workspace)
+    best = torch.empty((groups, count), dtype=torch.float32, device=device)
+    parents, tokens = torch.empty((2, groups, count), dtype=torch.int32, device=device).unbind(0)
     _launch(device, "beam select", lib.pkv_beam_select, logits.data_ptr(),
             _LOGIT_KINDS[logits.dtype], groups, beams, vocab, group_stride, beam_stride,
             scores.data_ptr(), done_at, pad_token, count, workspace.data_ptr(), workspace.numel(),

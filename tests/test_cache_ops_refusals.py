@@ -35,7 +35,7 @@ def _mass(**kw):
     (dict(scale=float("inf")), 1), (dict(mass_rows=1), 1), (dict(width=-1), 1), (dict(out=None), 1),
     (dict(pool=None), 1), (dict(queries=None), 1), (dict(table=None), 1), (dict(lens=None), 1),
     (dict(nq=1 << 23), 2), (dict(max_pages=1 << 28), 1), (dict(batch=10000, mass_rows=10000), 2),
-    (dict(ws=None), 3), (dict(ws_bytes=0), 3)])
+    (dict(ws=None), 3), (dict(ws_bytes=0), 3), (dict(nq=1 << 20, batch=1000, mass_rows=1000), 2)])
 def test_attention_mass(kw, code):
     assert _mass(**kw) == code and nat.last_error()
 
@@ -89,7 +89,8 @@ def _beam(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(kind=3), 1), (dict(beams=0), 1), (dict(beams=65), 2), (dict(vocab=0), 1), (dict(count=0), 1),
-    (dict(count=65, vocab=100), 2), (dict(count=21), 1), (dict(vocab=1 << 30, beams=64), 2), (dict(gs=-1), 1),
+    (dict(count=65, vocab=100), 2), (dict(count=21), 1), (dict(vocab=1 << 30, beams=64), 2),
+    (dict(groups=1 << 20, vocab=1 << 24), 2), (dict(groups=1 << 24), 2), (dict(gs=-1), 1),
     (dict(done=FAKE, pad=10), 1), (dict(done=FAKE, pad=-1), 1), (dict(scores=None), 1), (dict(tokens=None), 1),
     (dict(ws=None), 3), (dict(ws_bytes=8), 3)])
 def test_beam_select(kw, code):
@@ -118,7 +119,7 @@ def _arena(**kw):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(capacity=0), 1), (dict(page=24), 1), (dict(num_slots=0), 1), (dict(max_pages=0), 1), (dict(count=-1), 1),
-    (dict(count=8193), 2), (dict(state=None), 1), (dict(sources=None), 1), (dict(ws=None), 3), (dict(ws_bytes=4), 3)])
+    (dict(count=4097), 2), (dict(state=None), 1), (dict(sources=None), 1), (dict(ws=None), 3), (dict(ws_bytes=4), 3)])
 def test_arena_reorder(kw, code):
     assert _arena(**kw) == code
 
@@ -128,9 +129,11 @@ def test_workspace_sizes():
     assert lib.pkv_attention_mass_workspace_bytes(_layout(), 32, 1, 2, 4) > 0
     assert lib.pkv_attention_mass_workspace_bytes(_layout(), 30, 1, 2, 4) == -1
     assert lib.pkv_beam_workspace_bytes(1, 2, 10, 4) > 0
-    assert lib.pkv_beam_workspace_bytes(1, 2, 10, 65) == -1
+    assert lib.pkv_beam_workspace_bytes(1, 2, 100, 65) == -2
+    assert lib.pkv_beam_workspace_bytes(1, 2, 10, 0) == -1
     assert lib.pkv_arena_reorder_workspace_bytes(2, 8) > 0
-    assert lib.pkv_arena_reorder_workspace_bytes(8193, 8) == -1
+    assert lib.pkv_arena_reorder_workspace_bytes(4097, 8) == -2
+    assert lib.pkv_arena_reorder_workspace_bytes(-1, 8) == -1
 
 
 def test_python_checks():

@@ -193,3 +193,94 @@ def test_another_stream():
             got.append(ops.attention_mass(fmt, pool, q, table, lens, scale=0.1))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_few_rows_under_a_table_too_wide_to_keep_scores():
+    """The scores of 8 sequences under a table of 2^23 tokens each would take 4 GiB: K is
+    read twice instead, with the same sums."""
+    from pkv import ops
+
+    fmt = _format(8, 128, 64, 128, 4)
+    lens = [300, 17, 0, 1, 1000, 129, 256, 40]
+    pool, table, _ = filled(fmt, lens)
+    q = _queries(fmt, 8, 2, 1)
+    wide = torch.full((8, 1 << 16), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    out = [torch.zeros((8, 4, 1024), device="cuda") for _ in range(2)]
+    want, bound = mass64(fmt, pool, table, lens, q, scale_of(fmt))
+    for t, o in zip((table, wide), out):
+        ops.attention_mass(fmt, pool, q, t, lens, scale=scale_of(fmt), out=o)
+        got = o.double().cpu().numpy()
+        for b, n in enumerate(lens):
+            assert np.all(np.abs(got[b, :, :n] - want[b]) <= bound[b])
+
+
+@pytest.mark.parametrize("nq", [1, 12])
+def test_many_sequences(nq):
+    """More sequences than a wave has lanes, many of them empty, behind and between the others."""
+    fmt = _format(4, 64, 32, 16, 2)
+    rng = np.random.default_rng(nq)
+    lens = [int(n) if rng.random() < 0.6 else 0 for n in rng.integers(1, 700, 150)]
+    lens[70:130] = [0] * 60
+    lens[-3:] = [0] * 3
+    _check(fmt, lens, 2, nq)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30])
+@pytest.mark.parametrize("nq,gqa", [(1, 2), (9, 2)])
+def test_scales(scale, nq, gqa):
+    from pkv import ops
+
+    for bits in (8, 16):
+        fmt = _format(bits, 64, 32)
+        pool, table, _ = filled(fmt, [90, 33])
+        q = _queries(fmt, 2, gqa, nq)
+        want, bound = mass64(fmt, pool, table, [90, 33], q, scale)
+        got = ops.attention_mass(fmt, pool, q, table, [90, 33], scale=scale).double().cpu().numpy()
+        for b, n in enumerate((90, 33)):
+            assert np.all(np.abs(got[b, :, :n] - want[b]) <= bound[b])
+    with pytest.raises(ValueError):
+        ops.attention_mass(fmt, pool, q, table, [90, 33], scale=float("nan"))
+
+
+def test_python_refusals():
+    from pkv import ops
+    from pkv.cache_errors import CacheCapacityError
+    from pkv.modes import ModelCapabilityUnsupported
+
+    fmt = _format(8, 64, 32)
+    pool, table, _ = filled(fmt, [40, 9])
+    q = _queries(fmt, 2, 2, 1)
+    out = torch.zeros((2, 2, 64), device="cuda")
+    good = dict(scale=0.1, out=out)
+    bad = [dict(out=out.double()), dict(out=out[:1]), dict(out=out[:, :1]), dict(out=out.transpose(1, 2)),
+           dict(out=out, mass=torch.zeros((2, 2, 63), device="cuda")), dict(rows=[0]), dict(counted=[1, 2, 3]),
+           dict(widths=[1]), dict(q_pos=[1]), dict(out=out.cpu()),
+           dict(workspace=torch.zeros(1 << 20, device="cuda"))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            ops.attention_mass(fmt, pool, q, table, [40, 9], **{**good, **kw})
+    with pytest.raises(ValueError):
+        ops.attention_mass(fmt, pool[:, :100].contiguous(), q, table, [40, 9], **good)
+    with pytest.raises(ValueError):
+        ops.attention_mass(fmt, pool, q.half(), table, [40, 9], **good)
+    with pytest.raises(CacheCapacityError):
+        ops.attention_mass(fmt, pool, q, table, [40, 9], workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"),
+                           **good)
+    logits, scores = torch.zeros((1, 2, 100), device="cuda"), torch.zeros((1, 2), device="cuda")
+    for kw in (dict(count=0), dict(count=201), dict(count=4, done=scores), dict(count=4, done=scores > 0, pad_token=100)):
+        with pytest.raises((ValueError, ModelCapabilityUnsupported)):
+            ops.beam_select(logits, scores, **kw)
+    with pytest.raises(ModelCapabilityUnsupported):
+        ops.beam_select(logits, scores, 65)
+    with pytest.raises(ValueError):
+        ops.beam_select(logits, scores[:, :1], 4)
+    with pytest.raises(ValueError):
+        ops.reorder_rows(torch.zeros((4, 6), device="cuda")[:, :3], [0], [1])
+    with pytest.raises(ModelCapabilityUnsupported):
+        ops.reorder_rows(torch.zeros((4, 6), device="cuda"), [0] * 8193, [1] * 8193)
+    kept = torch.zeros((2, 2, 4), dtype=torch.int32, device="cuda")
+    for kw in (dict(kept=kept[:, :1].contiguous()), dict(kept=kept.float()), dict(new_lens=[1]), dict(dst=table[:1])):
+        a = dict(dict(kept=kept, new_lens=[4, 4], dst=table), **kw)
+        with pytest.raises(ValueError):
+            ops.evict_pages(fmt, pool, a["kept"], a["new_lens"], table, a["dst"])

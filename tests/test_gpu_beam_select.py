@@ -171,3 +171,26 @@ def test_replay():
         want = ops.beam_select(logits, scores, 8)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_masks_that_leave_lanes_without_tokens():
+    """Many tokens from rows where most lanes of a wave hold none, and scattered ones."""
+    gen = torch.Generator().manual_seed(3)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn((2, 3, 30000), generator=gen).cuda().to(dtype)
+        scores = torch.rand((2, 3), generator=gen).cuda()
+        for share in (0.001, 0.03, 0.5):
+            y = x.clone()
+            y[(torch.rand(x.shape, generator=gen) > share).cuda()] = -math.inf
+            _check(y, scores, 64)
+        z = torch.full_like(x, -math.inf)
+        z[..., 4000:4100] = x[..., 4000:4100]
+        _check(z, scores, 50)
+
+
+def test_groups_with_more_candidates_than_lds_holds():
+    """Equal values across many beams: more reach the bound than are ranked at once."""
+    logits = torch.zeros((1, 64, 20000), device="cuda", dtype=torch.bfloat16)
+    _check(logits, torch.zeros((1, 64), device="cuda"), 64)
+    logits[0, 5, 19999] = 1
+    _check(logits, torch.zeros((1, 64), device="cuda"), 64)

@@ -293,3 +293,57 @@ def test_attention_over_what_is_kept():
     want = (s @ vd.contiguous()).view(4, 64)
     assert (out[0, :, 0].double() - want).abs().max() < 2e-2      # the attention's own bound against its oracle
     assert math.isfinite(float(out.float().sum()))
+
+
+def test_captured_eviction():
+    """Growth and eviction as one graph over device operands, replayed between eager
+    steps of another arena that does the same: the same tables, sums and pages."""
+    arenas = [_arena(capacity=200, slots=8), _arena(capacity=200, slots=8)]
+    slots = torch.arange(4, dtype=torch.int32, device="cuda")
+    spare = torch.arange(4, 8, dtype=torch.int32, device="cuda")
+    keep = torch.tensor([40, 25, 60, 0], dtype=torch.int32, device="cuda")
+    grow = torch.full_like(slots, 9)
+    for a in arenas:
+        gen = torch.Generator().manual_seed(4)
+        _step(a, [0, 1, 2, 3], 70, 2, gen)
+    plain, graphed = arenas
+    res = graphed.reserve(slots, torch.zeros_like(grow))
+    warm = _arena(capacity=200, slots=8)
+    warm.reserve(slots, grow)
+    warm.evict(slots, keep, sinks=2, recent=5, max_keep=64, spare=spare)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        graphed.reserve(slots, grow, out=res)
+        graphed.evict(slots, keep, sinks=2, recent=5, max_keep=64, spare=spare)
+    torch.cuda.current_stream().wait_stream(stream)
+    for k in range(4):
+        graph.replay()
+        plain.reserve(slots, grow)
+        plain.evict(slots, keep, sinks=2, recent=5, max_keep=64, spare=spare)
+        torch.cuda.synchronize()
+        for x, y in ((plain.table, graphed.table), (plain.lens, graphed.lens), (plain.state, graphed.state),
+                     (plain.evicted, graphed.evicted), (plain.pools[1], graphed.pools[1])):
+            assert torch.equal(x, y)
+        n = plain.lens[:4].tolist()
+        assert n == [40, 25, 60, 0]
+        for s in range(4):
+            assert torch.equal(plain.mass[:, s, :, :n[s]], graphed.mass[:, s, :, :n[s]])
+    assert graphed.status()[1] == 0
+
+
+def test_an_evicted_prompt_is_not_published():
+    from pkv.device_cache import DevicePrefixIndex
+
+    class Fingerprint:
+        digest = "text"
+
+    arena = _arena(slots=6)
+    index = DevicePrefixIndex(arena, capacity_pages=20, max_entries=2)
+    a, b = arena.open_slot(), arena.open_slot()
+    gen = torch.Generator().manual_seed(1)
+    _step(arena, [a, b], 100, 2, gen)
+    arena.evict([a], 40)
+    assert not index.publish(a, Fingerprint, list(range(100)))
+    assert index.publish(b, Fingerprint, list(range(100)))

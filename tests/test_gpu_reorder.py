@@ -132,6 +132,20 @@ def test_arena_reorder_by_steps():
             _consistent(arena)
 
 
+def test_arena_reorder_of_many_slots():
+    rng = random.Random(3)
+    arena = _arena(9000, 4096, 64)
+    arena.reserve(list(range(4096)), [rng.randint(0, 33) for _ in range(4096)])
+    table, lens = arena.table.cpu(), arena.lens.cpu()
+    some = rng.sample(range(4096), 4096)
+    sources = [rng.randrange(4096) for _ in some]
+    arena.reorder(some, sources)
+    table[some], lens[some] = table[sources], lens[sources]
+    assert torch.equal(arena.table.cpu(), table) and torch.equal(arena.lens.cpu(), lens)
+    _consistent(arena)
+    arena.reorder([], [])
+
+
 def test_arena_reorder_is_deterministic():
     """Two arenas through the same calls hand out the same pages."""
     stacks = []
