@@ -29,7 +29,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMergeList = 512;  // candidates of a group in LDS
-constexpr int kHeld = 4096;  // candidates of a group whose order is kept in LDS
+constexpr int kHeld = 16384;  // candidates of a group whose order is kept in LDS
 constexpr int kList = 256;  // candidates in LDS, per wave
 
 // Order of float32 as unsigned numbers; -inf and below (nothing) as 0.
@@ -147,7 +147,7 @@ __device__ __forceinline__ int sum4(int v) {
 }
 
 template <int KIND, int E>
-__global__ __launch_bounds__(kThreads) void beam_chunk_kernel(const BeamArgs a, const BeamParts w) {
+__global__ __launch_bounds__(kThreads, 6) void beam_chunk_kernel(const BeamArgs a, const BeamParts w) {
   constexpr int V = E / 8;  // vectors of 8 per thread
   __shared__ uint64_t s_list[kWaves][kList];  // (order << 32 | ~token), what each wave found
   __shared__ double s_sum[kWaves];
