@@ -6,10 +6,10 @@
 // length).  A row's weights need its log-sum-exp over all its tokens first, so K
 // is gone through twice, or once and its scores kept:
 //
-//  * few rows (at most 8 per KV head: decode and short verify steps): one pass
-//    over K writes every score (float32) and the (max, sum) of each row and
-//    256-token part; a second launch reads the scores back.  16 bytes per token
-//    written and read at up to 4 rows, where K itself is 136 (8-bit, head_dim 128).
+//  * few rows (at most 16 per KV head: decode and verify steps): one pass over K
+//    writes every score (float32) and the rows' (max, sum) of each run of tokens; a
+//    second launch reads the scores back.  16 bytes per token written and read at up
+//    to 4 rows, 32 at up to 8, 64 beyond, where K itself is 136 (8-bit, head_dim 128).
 //  * more rows: a pass over K for the log-sum-exps, a launch that joins their
 //    parts, and a second pass over K that sums the weights.
 //
@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kFewRows = 8;
+constexpr int kFewRows = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- sequences, rows, units ---------------------------------------------------------
@@ -261,9 +261,10 @@ __device__ __forceinline__ void join(float &m, float &l, float m2, float l2) {
 constexpr int kPart = 256;  // tokens per unit: four tiles per wave
 constexpr int kTiles = kPart / PKV_TILE / kWaves;
 
-__host__ __device__ inline int quads(int rows) { return rows > 4 ? (rows + 3) / 4 : 1; }
+// Rows by fours, as the kernels are built: 1, 2 or 4.
+__host__ __device__ inline int quads(int rows) { return rows > 8 ? 4 : rows > 4 ? 2 : 1; }
 
-// Workspace: [scores: segment][R / 4][tokens][4] f32, [segment][k][8] (m, l) of the
+// Workspace: [scores: segment][quad][tokens][4] f32, [segment][k][16] (m, l) of the
 // k-th workgroup that had units of the segment (k < its parts).
 struct FewParts {
   int64_t tokens, parts, scores, total;
@@ -279,9 +280,12 @@ struct FewParts {
 
 // S = Q K^T with query row 4 r + jj in row 4 jj + r of the 16x16 tile: its four
 // rows per lane are then the lane's registers r, and a call of at most 4 rows has
-// one score per lane and tile, a call of 8 two.
+// one score per lane and tile, a call of 8 two.  Memory-bound: 32 sequences of 4.6K
+// tokens in the mean, 8 KV heads, 8-bit pages, read 160 MB and write 19 in 38.5 us
+// (4.6 TB/s; 31 us without the stores).  Runs of units against strided ones 42.5 us;
+// four waves per SIMD (128 registers) against three 37.4 and 43.9.
 template <typename C, int NR>
-__global__ __launch_bounds__(kThreads, C::KB > 4 ? 2 : 4) void mass_scores_kernel(const MassArgs a, const FewParts w) {
+__global__ __launch_bounds__(kThreads, C::KB > 4 ? 2 : NR > 2 ? 3 : 4) void mass_scores_kernel(const MassArgs a, const FewParts w) {
   __shared__ float s_ml[kWaves][NR * 4][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, jj = lane >> 4, col = lane & 15;
   const Geo &g = a.g;
@@ -425,7 +429,8 @@ __device__ __forceinline__ int mass_row(const MassArgs &a, int b) {
   return row >= 0 && row < a.mass_rows ? row : -1;
 }
 
-constexpr int kSumPart = 1024;  // tokens per unit of the second launch
+// The second launch: 19 MB of scores and 9 of sums in 7.7 us at the size above.
+constexpr int kSumPart = 1024;  // tokens per unit
 
 template <int NR>
 __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a, const FewParts w) {
@@ -458,7 +463,7 @@ __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a
       for (int r = 0; r < NR; ++r) s[r][i] = *(const float4 *)(scores + ((int64_t)r * w.tokens + at) * 4);
       old[i] = t < min(counted, u.L) ? a.mass[to + t] : 0.0f;
     }
-    // the rows' log-sum-exps from the workgroups' (m, l): lane 8 k + r the k-th's of row r
+    // the rows' log-sum-exps from the workgroups' (m, l): lane 16 k + r the k-th's of row r
     float lse;
     {
       if (u.base != base) before = Runs::parts_before(a, kPart, lane, u.base);
@@ -468,13 +473,13 @@ __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a
       const int n = run.owner(first + parts - 1) - run.owner(first) + 1;
       const float2 *ml = (const float2 *)((const char *)a.workspace + w.scores) + seg * w.parts * kFewRows;
       float m = -INFINITY, l = 0.0f;
-      for (int k = lane / 8; k < n; k += 8)
-        if (lane % 8 < NR * 4) {
-          const float2 x = ml[k * kFewRows + lane % 8];
+      for (int k = lane / 16; k < n; k += 4)
+        if (lane % 16 < NR * 4) {
+          const float2 x = ml[k * kFewRows + lane % 16];
           join(m, l, x.x, x.y);
         }
 #pragma unroll
-      for (int k = 8; k < 64; k *= 2) join(m, l, __shfl_xor(m, k, 64), __shfl_xor(l, k, 64));
+      for (int k = 16; k < 64; k *= 2) join(m, l, __shfl_xor(m, k, 64), __shfl_xor(l, k, 64));
       lse = l == 0.0f ? INFINITY : m + __builtin_amdgcn_logf(l);  // a row that sees nothing weighs nothing
     }
 #pragma unroll
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a
 // ---- many rows: K twice -----------------------------------------------------------------
 //
 // Rows in blocks of 16.  A workgroup of eight waves holds a unit's K tiles in
-// registers, two per wave, and goes through the row blocks, which it stages in LDS a
+// registers, two per wave, and goes through the row blocks, which it stages in LDS
 // few at a time, the next ones under way while these are used.  Bound by the vector
 // ALU (the group scales and the exponentials, quarter rate) beside the matrix cores.
 
@@ -817,8 +822,11 @@ __global__ __launch_bounds__(kThreads) void mass_join_kernel(const MassArgs a, c
 
 // ---- launches -----------------------------------------------------------------------------
 
-// Scores are kept where they cost less than reading K again and take no more
-// than this.
+// Scores are kept for up to 16 rows where they take no more than this (the size goes
+// by the block table's width).  32 sequences of 1K..8K tokens, 8 KV heads, head_dim
+// 128, kept against K read twice, us: 8-bit pages, 4 rows 46 and 134, 8 rows 55 and
+// 133, 16 rows 79 and 134; 4-bit pages, 4 rows 38 and 120, 12 rows 60 and 122; bf16
+// pages, 16 rows 100 and 136.  Past 16 rows the first kernel has no registers for them.
 constexpr int64_t kMostScores = (int64_t)2 << 30;
 
 bool keeps_scores(const Geo &g, int64_t segs, int rows, int64_t cap) {
@@ -843,12 +851,15 @@ void launch(hipStream_t stream, const MassArgs &a, int64_t cap) {
     FewParts w(segs, a.rows, cap);
     w.grid = runs(segs * w.parts);
     const dim3 grid(w.grid), second(walkers(segs * ((cap + kSumPart - 1) / kSumPart)));
-    if (a.rows <= 4) {
+    if (quads(a.rows) == 1) {
       hipLaunchKernelGGL((mass_scores_kernel<C, 1>), grid, dim3(kThreads), 0, stream, a, w);
       hipLaunchKernelGGL((mass_weights_kernel<1>), second, dim3(kThreads), 0, stream, a, w);
-    } else {
+    } else if (quads(a.rows) == 2) {
       hipLaunchKernelGGL((mass_scores_kernel<C, 2>), grid, dim3(kThreads), 0, stream, a, w);
       hipLaunchKernelGGL((mass_weights_kernel<2>), second, dim3(kThreads), 0, stream, a, w);
+    } else {
+      hipLaunchKernelGGL((mass_scores_kernel<C, 4>), grid, dim3(kThreads), 0, stream, a, w);
+      hipLaunchKernelGGL((mass_weights_kernel<4>), second, dim3(kThreads), 0, stream, a, w);
     }
     return;
   }
