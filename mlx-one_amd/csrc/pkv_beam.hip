@@ -16,8 +16,11 @@
 // the count-th largest of its lanes' maxima, by bisection on the bits of the order;
 // what reaches the largest of the waves' bounds, a few times `count`, goes to LDS
 // and is ranked there.  A second launch joins the chunks' sums and does the same
-// with the lists' entries.  Memory-bound: one read of the
-// logits.
+// with the lists' entries.  One read of the logits: 128 rows of 128256 bfloat16 (33
+// MB) take 14 us (2.3 TB/s; about 530 vector instructions, a bisection among them, per
+// wave and 2048 logits, eight chunks to a CU) and the merge 9.9 us, a chain
+// of dependent steps; 768 rows of 104543 float16, 21 selected (161 MB), 57 us (2.8 TB/s)
+// and 18.
 #include <cfloat>
 
 #include "pkv_cache_ops.h"
@@ -28,6 +31,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
+constexpr int kVectors = 4;  // of eight logits, per thread
+// logits of a workgroup; 4 rows of 8000, both launches: 10.1 us, by a quarter of it 12.1,
+// by half 12.4; 8 rows of 128256: 18.9, 27.5 and 21.4
+constexpr int kChunk = 8 * kVectors * kThreads;
 constexpr int kMergeList = 512;  // candidates of a group in LDS
 constexpr int kHeld = 16384;  // candidates of a group whose order is kept in LDS
 constexpr int kList = 256;  // candidates in LDS, per wave
@@ -52,8 +59,8 @@ struct BeamParts {
   int chunks;
   uint32_t by_count, by_chunks;  // floor(2^32 / d) + 1: __umulhi(e, it) = e / d for e < 2^32 / d
   int64_t lists, total;
-  __host__ __device__ BeamParts(int groups, int beams, int vocab, int count, int chunk) {
-    chunks = (vocab + chunk - 1) / chunk;
+  __host__ __device__ BeamParts(int groups, int beams, int vocab, int count) {
+    chunks = (vocab + kChunk - 1) / kChunk;
     const int64_t n = (int64_t)groups * beams * chunks;
     by_count = (uint32_t)(((uint64_t)1 << 32) / count) + 1;
     by_chunks = (uint32_t)(((uint64_t)1 << 32) / chunks) + 1;
@@ -146,9 +153,9 @@ __device__ __forceinline__ int sum4(int v) {
   return v + __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);
 }
 
-template <int KIND, int E>
+template <int KIND>
 __global__ __launch_bounds__(kThreads, 6) void beam_chunk_kernel(const BeamArgs a, const BeamParts w) {
-  constexpr int V = E / 8;  // vectors of 8 per thread
+  constexpr int V = kVectors;
   __shared__ uint64_t s_list[kWaves][kList];  // (order << 32 | ~token), what each wave found
   __shared__ double s_sum[kWaves];
   __shared__ float s_most[kWaves];
@@ -158,7 +165,7 @@ __global__ __launch_bounds__(kThreads, 6) void beam_chunk_kernel(const BeamArgs 
   const int64_t row = blockIdx.x / w.chunks;
   if (a.done && a.done[row]) return;  // its logits are not asked for
   const int64_t base = row / a.beams * a.group_stride + row % a.beams * a.beam_stride;
-  const int v0 = (int)(blockIdx.x % w.chunks) * (E * kThreads) + threadIdx.x * 8;
+  const int v0 = (int)(blockIdx.x % w.chunks) * kChunk + threadIdx.x * 8;
   Eight<KIND> x[V];
   float vm[V];
 #pragma unroll
@@ -180,7 +187,7 @@ __global__ __launch_bounds__(kThreads, 6) void beam_chunk_kernel(const BeamArgs 
   constexpr int kBits = KIND == 0 ? 16 : KIND == 1 ? 19 : 24;
   auto key_of = [](float v) { return v == -INFINITY ? 0u : order_key(v); };
   uint32_t bound;
-  if (V == 1 || a.count <= 16) {
+  if (a.count <= 16) {
     const uint32_t key[1] = {key_of(m)};
     bound = wave_bound<kBits>(key, a.count);
   } else {
@@ -518,31 +525,20 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArg
   }
 }
 
-// Elements per thread: 32, or 8 where the chunks of 8192 would not fill the CUs.
-int chunk_elements(int64_t rows, int vocab) {
-  return rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) < 256 ? 8 : 32;
-}
-
-template <int E>
-void start_chunks(hipStream_t stream, const BeamArgs &a, const BeamParts &w) {
-  const dim3 grid((unsigned)((int64_t)a.groups * a.beams * w.chunks));
-  if (a.kind == 0) hipLaunchKernelGGL((beam_chunk_kernel<0, E>), grid, dim3(kThreads), 0, stream, a, w);
-  else if (a.kind == 1) hipLaunchKernelGGL((beam_chunk_kernel<1, E>), grid, dim3(kThreads), 0, stream, a, w);
-  else hipLaunchKernelGGL((beam_chunk_kernel<2, E>), grid, dim3(kThreads), 0, stream, a, w);
-}
-
 }  // namespace
 
 int64_t beam_workspace(int groups, int beams, int vocab, int count) {
-  const int e = chunk_elements((int64_t)groups * beams, vocab);
-  return BeamParts(groups, beams, vocab, count, e * kThreads).total;
+  return BeamParts(groups, beams, vocab, count).total;
 }
 
 hipError_t launch_beam(hipStream_t stream, const BeamArgs &a) {
-  const int e = chunk_elements((int64_t)a.groups * a.beams, a.vocab);
-  const BeamParts w(a.groups, a.beams, a.vocab, a.count, e * kThreads);
-  if (e == 8) start_chunks<8>(stream, a, w);
-  else start_chunks<32>(stream, a, w);
+  const BeamParts w(a.groups, a.beams, a.vocab, a.count);
+  const dim3 grid((unsigned)((int64_t)a.groups * a.beams * w.chunks));
+  if (a.kind == 0) hipLaunchKernelGGL(beam_chunk_kernel<0>, grid, dim3(kThreads), 0, stream, a, w);
+  else if (a.kind == 1) hipLaunchKernelGGL(beam_chunk_kernel<1>, grid, dim3(kThreads), 0, stream, a, w);
+  else hipLaunchKernelGGL(beam_chunk_kernel<2>, grid, dim3(kThreads), 0, stream, a, w);
+  // us by 256 and by 1024 threads: 128 candidates of a group 7.4 and 8.5, 512 10.1 and
+  // 10.2, 2048 18.9 and 11.4
   if (a.beams * w.chunks * a.count <= 1024)
     hipLaunchKernelGGL(beam_merge_kernel<256>, dim3(a.groups), dim3(256), 0, stream, a, w);
   else

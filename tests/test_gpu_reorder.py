@@ -58,7 +58,7 @@ def test_rows(dtype, size):
     _check((n, size), dtype, [0, 1, 2, 50, 3], [1, 0, -1, 2, 13])              # rows that do not exist
 
 
-@pytest.mark.parametrize("count,size", [(1, 100000), (256, 1000), (1000, 77), (4097, 40), (8192, 5)])
+@pytest.mark.parametrize("count,size", [(1, 100000), (256, 1000), (300, 4099), (512, 2064), (513, 33), (1000, 77), (4097, 40), (8192, 5)])
 def test_many_rows(count, size):
     rng = random.Random(count)
     perm = list(range(count))
