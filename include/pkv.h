@@ -375,7 +375,8 @@ int pkv_arena_fork(void *stream, void *state, int32_t capacity_pages, int32_t pa
  * No counterpart in the reference: its caches grow until they are trimmed by
  * length, and it decodes one sequence per request.  The sizes that these
  * operators' workspace queries return are negative for shapes that the operator
- * refuses, by its status (-PKV_INVALID_ARGUMENT, -PKV_UNSUPPORTED).
+ * refuses, by its status (-PKV_INVALID_ARGUMENT, -PKV_UNSUPPORTED).  Workspaces are
+ * 16-byte aligned.
  */
 
 /*

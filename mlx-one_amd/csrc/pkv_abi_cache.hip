@@ -4,6 +4,7 @@
 // lets an exception out.
 #include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <string>
 
 #include "pkv.h"
@@ -28,7 +29,11 @@ auto guarded(F body) noexcept -> decltype(body()) {
   }
 }
 
+// The bounds below keep every grid under 2^32 threads.
 constexpr int64_t kMaxRows = 1 << 24;  // query rows per KV head of a call
+
+// Kernels read and write their workspace 16 bytes at a time.
+bool aligned(const void *workspace) { return (uintptr_t)workspace % 16 == 0; }
 
 int mass_shape(const pkv_layout *layout, int32_t num_heads, int32_t num_queries, int32_t batch, int32_t max_pages,
                pkv_geometry *g) {
@@ -42,8 +47,8 @@ int mass_shape(const pkv_layout *layout, int32_t num_heads, int32_t num_queries,
   if ((int64_t)batch * g->hk > 65535) return fail(PKV_UNSUPPORTED, "at most 65535 (sequence, KV head) pairs");
   if ((int64_t)batch * g->hk * max_pages > (1 << 30))
     return fail(PKV_UNSUPPORTED, "at most 2^30 pages of (sequence, KV head) pairs");
-  if ((int64_t)batch * g->hk * num_queries * (num_heads / g->hk) > (1 << 30))
-    return fail(PKV_UNSUPPORTED, "at most 2^30 query rows");
+  if ((int64_t)batch * g->hk * num_queries * (num_heads / g->hk) > (1 << 27))
+    return fail(PKV_UNSUPPORTED, "at most 2^27 query rows");
   return PKV_OK;
 }
 
@@ -51,9 +56,9 @@ int beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count) {
   if (groups < 0 || beams < 1 || vocab < 1 || count < 1) return fail(PKV_INVALID_ARGUMENT, "invalid beam shape");
   if (beams > pkv::kMaxBeams || count > pkv::kMaxBeamCount)
     return fail(PKV_UNSUPPORTED, "at most 64 beams and 64 selected pairs per group");
-  if ((int64_t)beams * vocab > INT32_MAX || (int64_t)groups * beams > (1 << 24) ||
-      (int64_t)groups * beams * vocab > ((int64_t)1 << 40))
-    return fail(PKV_UNSUPPORTED, "at most 2^31 - 1 (beam, token) pairs per group, 2^24 beams and 2^40 pairs");
+  if ((int64_t)beams * vocab > INT32_MAX || groups > (1 << 21) || (int64_t)groups * beams > (1 << 22) ||
+      (int64_t)groups * beams * vocab > ((int64_t)1 << 36))
+    return fail(PKV_UNSUPPORTED, "at most 2^31 - 1 (beam, token) pairs per group, 2^21 groups, 2^22 beams and 2^36 pairs");
   if (count > (int64_t)beams * vocab) return fail(PKV_INVALID_ARGUMENT, "fewer (beam, token) pairs than the count");
   return PKV_OK;
 }
@@ -61,6 +66,7 @@ int beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count) {
 int reorder_shape(int32_t count, int32_t max_pages) {
   if (count < 0 || max_pages < 1) return fail(PKV_INVALID_ARGUMENT, "invalid reorder shape");
   if (count > pkv::kMaxArenaReorder) return fail(PKV_UNSUPPORTED, "at most 4096 slots are reordered in a call");
+  if (max_pages > (1 << 23)) return fail(PKV_UNSUPPORTED, "slot tables of at most 2^23 pages");
   return PKV_OK;
 }
 
@@ -99,6 +105,7 @@ int pkv_attention_mass(void *stream, const pkv_layout *layout, const void *pool,
     const int64_t need = pkv::mass_workspace(a.g, batch, a.rows, max_pages);
     if (need > 0 && (!workspace || workspace_bytes < need))
       return fail(PKV_OUT_OF_MEMORY, "attention mass workspace too small: need " + std::to_string(need) + " bytes");
+    if (need > 0 && !aligned(workspace)) return fail(PKV_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
     a.pool = (const uint8_t *)pool;
     a.num_pages = num_pages;
     a.q = (const uint16_t *)queries;
@@ -133,8 +140,8 @@ int pkv_evict_select(void *stream, const float *mass, int32_t layers, int32_t ma
     if (sinks < 0 || recent < 0) return fail(PKV_INVALID_ARGUMENT, "negative count of protected tokens");
     if (new_mass && new_width < max_keep)
       return fail(PKV_INVALID_ARGUMENT, "the kept sums need room for max_keep tokens");
-    if ((int64_t)layers * batch * kv_heads > (1 << 30))
-      return fail(PKV_UNSUPPORTED, "at most 2^30 (layer, sequence, KV head) rows");
+    if ((int64_t)layers * batch * kv_heads > (1 << 21))
+      return fail(PKV_UNSUPPORTED, "at most 2^21 (layer, sequence, KV head) rows");
     if (layers == 0 || batch == 0) return PKV_OK;
     if (!mass || !seq_lens || !new_lens || (!kept && max_keep > 0)) return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
     pkv::EvictSelectArgs a;
@@ -170,6 +177,7 @@ int pkv_evict_pages(void *stream, const pkv_layout *layout, void *const *pools, 
         (int64_t)src_pages * g.page > INT32_MAX || (int64_t)dst_pages * g.page > INT32_MAX)
       return fail(PKV_INVALID_ARGUMENT, "invalid eviction shape");
     if ((int64_t)batch * g.hk > 65535) return fail(PKV_UNSUPPORTED, "at most 65535 (sequence, KV head) pairs");
+    if (max_keep > (1 << 29)) return fail(PKV_UNSUPPORTED, "at most 2^29 kept tokens");
     if (num_pools == 0 || batch == 0 || max_keep == 0 || src_pages == 0 || dst_pages == 0) return PKV_OK;
     if (!pools || !kept || !new_lens || !src_table || !dst_table) return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
     pkv::EvictPagesArgs a;
@@ -214,6 +222,7 @@ int pkv_beam_select(void *stream, const void *logits, int32_t kind, int32_t grou
     const int64_t need = pkv::beam_workspace(groups, beams, vocab, count);
     if (!workspace || workspace_bytes < need)
       return fail(PKV_OUT_OF_MEMORY, "beam workspace too small: need " + std::to_string(need) + " bytes");
+    if (!aligned(workspace)) return fail(PKV_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
     pkv::BeamArgs a;
     a.logits = logits;
     a.kind = kind;
@@ -242,6 +251,7 @@ int pkv_reorder_rows(void *stream, void *state, int64_t outer, int32_t num_rows,
     if (count > pkv::kMaxReorder) return fail(PKV_UNSUPPORTED, "at most 8192 rows are reordered in a call");
     if (outer > 65535) return fail(PKV_UNSUPPORTED, "at most 65535 outer slices");
     if (row_bytes > ((int64_t)1 << 31)) return fail(PKV_UNSUPPORTED, "rows of at most 2^31 bytes");
+    if (row_bytes * count > ((int64_t)1 << 37)) return fail(PKV_UNSUPPORTED, "rows of at most 2^37 bytes in a slice");
     if (outer == 0 || num_rows == 0 || row_bytes == 0 || count == 0) return PKV_OK;
     if (!state || !targets || !sources) return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
     pkv::ReorderArgs a;
@@ -280,6 +290,7 @@ int pkv_arena_reorder(void *stream, void *state, int32_t capacity_pages, int32_t
     const int64_t need = pkv::arena_reorder_workspace(count, max_pages);
     if (!workspace || workspace_bytes < need)
       return fail(PKV_OUT_OF_MEMORY, "reorder workspace too small: need " + std::to_string(need) + " bytes");
+    if (!aligned(workspace)) return fail(PKV_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
     pkv::ArenaReorderArgs a;
     a.state = (int32_t *)state;
     a.capacity = capacity_pages;

@@ -124,6 +124,16 @@ def test_arena_reorder(kw, code):
     assert _arena(**kw) == code
 
 
+def test_grids_that_no_launch_takes_and_misaligned_workspaces():
+    assert _mass(nq=1 << 16, batch=300, mass_rows=300) == 2 and _mass(ws=FAKE + 8) == 1
+    assert _select(layers=1 << 12, hk=1 << 9) == 2
+    assert _pages(max_keep=(1 << 29) + 1) == 2
+    assert _beam(groups=(1 << 21) + 1, beams=1) == 2 and _beam(groups=1 << 21, beams=3) == 2
+    assert _beam(groups=1 << 16, vocab=1 << 20) == 2 and _beam(ws=FAKE + 4) == 1
+    assert _rows(row_bytes=1 << 31, count=65) == 2
+    assert _arena(max_pages=(1 << 23) + 1) == 2 and _arena(ws=FAKE + 4) == 1
+
+
 def test_workspace_sizes():
     lib = nat.load()
     assert lib.pkv_attention_mass_workspace_bytes(_layout(), 32, 1, 2, 4) > 0
