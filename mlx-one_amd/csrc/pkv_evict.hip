@@ -18,18 +18,22 @@ namespace {
 // One workgroup per (layer, sequence, KV head).  The need-th largest key is found by
 // its digits from the top, 11, 11 and 10 bits, each by a histogram in LDS of the keys
 // that agree so far; as a rule the second digit's bin is to be taken whole and the
-// third is not needed.  The row stays in registers up to 32 values per thread and
-// is read again for each step beyond that.  Bound by the steps of one workgroup: 256
-// rows of up to 8192 sums 12.8 us, 32 rows of 32700 26 us.  Four copies of each bin
-// for the atomics: 13.1 and 26.2 us.
+// third is not needed.  The row's keys stay in registers up to 32 per thread (a longer
+// row is read again for each step); protected tokens have a key of their own above
+// all others, so no step looks at positions (32 rows of 32700 sums: 26.4 -> 20.2 us).
+// Bound by the steps of one workgroup, vector instructions first (a quarter LDS
+// atomics): 256 rows of up to 8191 sums 12.4 us.  Four copies of each bin changed
+// nothing.
 
 constexpr int kVectors = 8;  // of four values, per thread
 constexpr int kBins = 2048;
 
-// Unsigned key of the order: NaN above everything, -0 equal to +0.
+// Unsigned key of the order: a NaN above every number, -0 equal to +0.  No key is 0
+// (no token) or kStays (a protected one).
+constexpr uint32_t kStays = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t order_key(uint32_t bits) {
   const float x = __uint_as_float(bits);
-  if (x != x) return 0xFFFFFFFFu;
+  if (x != x) return kStays - 1;
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
@@ -68,21 +72,35 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(const EvictSelectArgs 
   const float *mass = a.mass + base * a.width;
   float *new_mass = a.new_mass && there ? a.new_mass + base * a.new_width : nullptr;
   const int r = min(a.recent, n), s = min(a.sinks, n - r);
-  const int lo = s, hi = n > 0 ? L - r : s, need = n - r - s;  // `need` of the tokens lo..hi-1
+  const int lo = s, hi = L - r;  // the tokens lo..hi-1 are ordered by their sums
   const int chunks = n > 0 ? (L + kChunk - 1) / kChunk : 0;
 
-  // chunk c: this thread's vectors, four tokens from c * kChunk + (j * NT + thread) * 4 on
-  uint32_t bits[kVectors][4];
+  // keys of chunk c: this thread's vectors, four tokens from c * kChunk + (j * NT + thread) * 4 on
+  uint32_t keys[kVectors][4];
   auto first = [&](int c, int j) { return c * kChunk + (j * NT + (int)threadIdx.x) * 4; };
+  auto live = [&](int c, int j) { return c * kChunk + j * NT * 4 < L; };
+  auto read = [&](int c, int j) {
+    const int t = first(c, j);
+    if (t + 4 <= L) {
+      __builtin_memcpy(keys[j], mass + t, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keys[j][e] = t + e < L ? __float_as_uint(mass[t + e]) : 0u;
+    }
+  };
   auto load = [&](int c) {
 #pragma unroll
-    for (int j = 0; j < kVectors; ++j) {
-      const int t = first(c, j);
-      if (t + 4 <= L) {
-        __builtin_memcpy(bits[j], mass + t, 16);
-      } else {
+    for (int j = 0; j < kVectors; ++j)
+      if (live(c, j)) read(c, j);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bits[j][e] = t + e < L ? __float_as_uint(mass[t + e]) : 0u;
+    for (int j = 0; j < kVectors; ++j) {
+      if (!live(c, j)) break;
+      const int t = first(c, j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keys[j][e] = order_key(keys[j][e]);
+      if (t < lo || t + 4 > hi) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) keys[j][e] = t + e >= L ? 0u : t + e < lo || t + e >= hi ? kStays : keys[j][e];
       }
     }
   };
@@ -90,8 +108,8 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(const EvictSelectArgs 
 
   uint32_t least = 0;  // keys above it stay, and `room` of those that are equal to it
   int room = INT32_MAX;
-  if (need > 0 && need < hi - lo) {
-    int left = need, shift = 21;
+  if (n > 0 && n < L) {
+    int left = n, shift = 21;
     for (;;) {
       for (int k = threadIdx.x; k < kBins; k += NT) s_bins[k] = 0;
       __syncthreads();
@@ -100,13 +118,12 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(const EvictSelectArgs 
         if (chunks > 1) load(c);
 #pragma unroll
         for (int j = 0; j < kVectors; ++j) {
-          if (c * kChunk + j * NT * 4 >= hi) break;
-          const int t = first(c, j);
+          if (!live(c, j)) break;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t key = order_key(bits[j][e]);
+            const uint32_t key = keys[j][e];
             const bool same = shift == 21 || key >> (shift == 10 ? 21 : 10) == least >> (shift == 10 ? 21 : 10);
-            if (t + e >= lo && t + e < hi && same) atomicAdd(&s_bins[key >> shift & digits], 1);
+            if (same) atomicAdd(&s_bins[key >> shift & digits], 1);
           }
         }
       }
@@ -146,7 +163,6 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(const EvictSelectArgs 
     // which of its tokens each thread keeps: a bit each, and how many its wave's
     // lanes before it keep of the vector
     uint32_t keep[kVectors];
-    auto live = [&](int j) { return c * kChunk + j * NT * 4 < L; };
     // s_sums, as the waves' counts of each vector, becomes what comes before them
     auto prefix = [&]() {
       __syncthreads();
@@ -179,12 +195,9 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(const EvictSelectArgs 
 #pragma unroll
       for (int j = 0; j < kVectors; ++j) {
         uint32_t tie = 0;
-        if (live(j)) {
-          const int t = first(c, j);
+        if (live(c, j))
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            tie |= (uint32_t)(t + e >= lo && t + e < hi && order_key(bits[j][e]) == least) << e;
-        }
+          for (int e = 0; e < 4; ++e) tie |= (uint32_t)(keys[j][e] == least) << e;
         const int incl = wave_scan_incl(__popc(tie), 0);
         if ((threadIdx.x & 63) == 63) s_sums[j][wave] = incl;
         keep[j] = tie | (uint32_t)(incl - __popc(tie)) << 8;
@@ -205,29 +218,34 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(const EvictSelectArgs 
     }
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      if (live(j)) {
-        const int t = first(c, j);
+      if (live(c, j))
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool stays = t + e < L && (t + e < lo || t + e >= hi || (need > 0 && order_key(bits[j][e]) > least));
-          keep[j] |= (uint32_t)stays << e;
-        }
-      }
+        for (int e = 0; e < 4; ++e) keep[j] |= (uint32_t)(keys[j][e] > least) << e;
       const int incl = wave_scan_incl(__popc(keep[j]), 0);
       if ((threadIdx.x & 63) == 63) s_sums[j][wave] = incl;
       keep[j] |= (uint32_t)(incl - __popc(keep[j])) << 8;
     }
-    prefix();  // (the chunk's sums are all read: they may be written over)
+    // the chunk's sums again, here before any are written: new_mass may be mass
+    if (new_mass) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j)
+        if (live(c, j)) read(c, j);
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(keys[j][e]));
+    }
+    prefix();
 #pragma unroll
     for (int j = 0; j < kVectors; ++j) {
-      if (!live(j)) break;
+      if (!live(c, j)) break;
       int at = done + s_sums[j][wave] + (int)(keep[j] >> 8);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (keep[j] >> e & 1) {
           if (at < a.max_keep) {
             kept[at] = first(c, j) + e;
-            if (new_mass) new_mass[at] = __uint_as_float(bits[j][e]);
+            if (new_mass) new_mass[at] = __uint_as_float(keys[j][e]);
           }
           ++at;
         }
@@ -352,9 +370,11 @@ void start_pages(hipStream_t stream, const EvictPagesArgs &a, dim3 grid) {
 
 hipError_t launch_evict_select(hipStream_t stream, const EvictSelectArgs &a) {
   const dim3 grid(a.layers * a.batch * a.hk);
-  // 64 rows of 500 and 2000 sums, us: 8.0 and 10.0 by 256 threads, 9.0 and 10.2 by
-  // 1024; 512 rows of 2000: 11.6 and 18.1; 64 rows of 4000: 11.9 and 10.3
-  if (a.width <= 2048) hipLaunchKernelGGL(evict_select_kernel<256>, grid, dim3(256), 0, stream, a);
+  // us by 256, 512 and 1024 threads: 64 rows of 1000 sums 7.3, 7.9 and 10.8, of 4000
+  // 9.9, 8.8 and 9.7; 512 rows of 2000 9.9, 9.4 and 19.6; 256 rows of up to 8191 14.3,
+  // 12.4 and 13.2.  Past 16384, 512 threads would read a row again for each digit.
+  if (a.width <= 1024) hipLaunchKernelGGL(evict_select_kernel<256>, grid, dim3(256), 0, stream, a);
+  else if (a.width <= 16384) hipLaunchKernelGGL(evict_select_kernel<512>, grid, dim3(512), 0, stream, a);
   else hipLaunchKernelGGL(evict_select_kernel<1024>, grid, dim3(1024), 0, stream, a);
   return hipGetLastError();
 }

@@ -107,7 +107,7 @@ def test_select_budgets_rows_and_garbage_past_the_length():
     assert after[:, [1, 2, 4]].tobytes() == mass[:, [1, 2, 4]].tobytes()
 
 
-@pytest.mark.parametrize("length,keep", [(40000, 1000), (70001, 69000), (131072, 65536)])
+@pytest.mark.parametrize("length,keep", [(16384, 4000), (16385, 16000), (32768, 9), (40000, 1000), (70001, 69000), (131072, 65536)])
 def test_select_long(length, keep):
     rng = np.random.default_rng(length)
     mass = (rng.exponential(1.0, (1, 1, 2, length)) ** 3).astype(np.float32)
@@ -123,6 +123,23 @@ def test_select_in_place_long():
     kept, _, apart = ops.evict_select(m, [40000, 35000], 30000, recent=10, with_mass=True)
     again, _, _ = ops.evict_select(m, [40000, 35000], 30000, recent=10, new_mass=m)
     assert torch.equal(kept, again) and torch.equal(m[..., :30000], apart)
+
+
+@pytest.mark.parametrize("length", [300, 3000, 16384, 16385, 40000])
+def test_select_protected_tokens_beside_nan(length):
+    """NaN sums come before numbers and after protected tokens, in place as well."""
+    from pkv import ops
+
+    rng = np.random.default_rng(length)
+    mass = rng.random((1, 1, 2, length), dtype=np.float32)
+    mass[0, 0, 0, rng.permutation(length)[:length // 3]] = np.nan
+    mass[0, 0, 1] = np.nan
+    for keep, sinks, recent in ((50, 20, 30), (51, 20, 30), (length // 4, 4, 60), (length - 1, 4, 60)):
+        _check(mass, [length], keep, sinks, recent)
+        m = torch.from_numpy(mass).cuda()
+        _, _, apart = ops.evict_select(m, [length], keep, sinks=sinks, recent=recent, with_mass=True)
+        ops.evict_select(m, [length], keep, sinks=sinks, recent=recent, new_mass=m)
+        assert torch.equal(m[..., :keep].view(torch.int32), apart.view(torch.int32))
 
 
 # ---- pages --------------------------------------------------------------------------------
