@@ -480,6 +480,14 @@ def _per_row(x, device, count, name):
     return t
 
 
+def _distinct(x, name):
+    """Refuse a host list that names a row twice (a tensor is the caller's to know)."""
+    if x is not None and not isinstance(x, torch.Tensor):
+        named = [int(v) for v in x if v >= 0]
+        if len(set(named)) != len(named):
+            raise ValueError(f"{name} must be distinct")
+
+
 def _address(x, device, count, name):
     """``(tensor, its address)`` of an int32 operand of ``count`` values; None: NULL."""
     if x is None:
@@ -543,6 +551,7 @@ def attention_mass(fmt: PageFormat, pool, queries, block_table, seq_lens, *, sca
     positions, positions_at = _address(q_pos, device, batch * nq, "q_pos")
     live, live_at = _address(widths, device, batch, "widths")
     known, known_at = _address(counted, device, batch, "counted")
+    _distinct(rows, "rows")
     row, row_at = _address(rows, device, batch, "rows")
     queries = queries.contiguous()
     lib, layout = nat.load(), fmt.c_layout
@@ -582,6 +591,8 @@ def evict_select(mass, seq_lens, keep, *, max_keep=None, sinks=0, recent=0, rows
     row, row_at = _address(rows, device, batch, "rows")
     if row is None and mass_rows < batch:
         raise ValueError("mass needs a row per sequence")
+    if with_mass or new_mass is not None:
+        _distinct(rows, "rows")
     if isinstance(keep, int):
         budget_at = None
         if max_keep is None:
@@ -706,6 +717,7 @@ def reorder_rows(state, targets, sources, *, dim=0):
     if not 0 <= dim < state.dim():
         raise ValueError("no such dimension")
     device = state.device
+    _distinct(targets, "targets")
     to, source = _i32(targets, device), _i32(sources, device)
     count = to.numel()
     if source.numel() != count:

@@ -278,7 +278,7 @@ def test_python_refusals():
     with pytest.raises(ValueError):
         ops.reorder_rows(torch.zeros((4, 6), device="cuda")[:, :3], [0], [1])
     with pytest.raises(ModelCapabilityUnsupported):
-        ops.reorder_rows(torch.zeros((4, 6), device="cuda"), [0] * 8193, [1] * 8193)
+        ops.reorder_rows(torch.zeros((4, 6), device="cuda"), list(range(8193)), [1] * 8193)
     kept = torch.zeros((2, 2, 4), dtype=torch.int32, device="cuda")
     for kw in (dict(kept=kept[:, :1].contiguous()), dict(kept=kept.float()), dict(new_lens=[1]), dict(dst=table[:1])):
         a = dict(dict(kept=kept, new_lens=[4, 4], dst=table), **kw)

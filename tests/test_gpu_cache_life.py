@@ -347,3 +347,22 @@ def test_an_evicted_prompt_is_not_published():
     arena.evict([a], 40)
     assert not index.publish(a, Fingerprint, list(range(100)))
     assert index.publish(b, Fingerprint, list(range(100)))
+
+
+def test_rows_named_twice_are_refused():
+    from pkv import ops
+
+    state = torch.zeros((4, 8), device="cuda")
+    with pytest.raises(ValueError):
+        ops.reorder_rows(state, [1, 1], [0, 2])
+    ops.reorder_rows(state, [1, -1, -1], [0, 2, 3])          # rows that do not exist are none
+    mass = torch.zeros((4, 1, 16), device="cuda")
+    with pytest.raises(ValueError):
+        ops.evict_select(mass, [16, 16], 4, rows=[2, 2], with_mass=True)
+    kept, _ = ops.evict_select(mass, [16, 16], 4, rows=[2, 2])
+    assert torch.equal(kept[0], kept[1])
+    fmt = ops.PageFormat(1, 64, 16, 8, 32, torch.bfloat16)
+    pool = torch.zeros((2, fmt.page_bytes), dtype=torch.uint8, device="cuda")
+    q = torch.zeros((2, 1, 1, 64), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        ops.attention_mass(fmt, pool, q, [[0], [1]], [5, 5], scale=1.0, mass=mass, rows=[1, 1])
