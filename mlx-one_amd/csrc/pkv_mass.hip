@@ -15,8 +15,8 @@
 //
 // Scores come from the matrix cores.  Quantized K enters as its exact codes (f16),
 // queries as f16 with each row scaled by a power of two, so that its largest
-// element lies in [2^14, 2^15): bfloat16 queries are exact then down to 2^-28 of
-// that, and the rest is smaller than the float32 accumulator's own rounding.  A
+// element lies in [2^7, 2^8): bfloat16 queries are exact then down to 2^-24 of that,
+// and what is lost below is smaller than the float32 accumulator's own rounding.  A
 // group's scale is applied to its accumulator in float32 and its bias to the sum of
 // the row's elements in the group, so a score is a float32 sum of exact products.
 #include <algorithm>
@@ -155,7 +155,6 @@ template <int BITS, int DP, int G, int FK>
 struct MassCfg : Cfg<BITS, DP, G, 1, FK, 1> {
   using Base = Cfg<BITS, DP, G, 1, FK, 1>;
   static constexpr int PAGE_BITS = BITS;
-  static constexpr int BM = (Base::NG + 3) / 4;  // float32 products per score tile of the group biases
   static constexpr int OPS = BITS == 16 ? FK : 1;  // operand type: f16 for codes
   using KT = typename FloatOps<OPS>::KT;
   static constexpr int GB = Base::QUANT ? G / 32 : Base::KB;  // 32-element blocks per accumulator
@@ -230,7 +229,7 @@ __device__ __forceinline__ void query_operands(const MassArgs &a, int b, int kh,
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(bits_to_float(raw[kb][e], fk)));
     most = xor32_max(xor16_max(most));
-    const int shift = most > 0.0f && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+    const int shift = most > 0.0f && most < INFINITY ? 8 - __builtin_amdgcn_frexp_expf(most) : 0;
     mult = ldexpf(mult, -shift);
 #pragma unroll
     for (int g = 0; g < C::NG; ++g) qs[g] = 0.0f;
@@ -504,20 +503,24 @@ __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a
 //
 // Rows in blocks of 16.  A workgroup of eight waves holds a unit's K tiles in
 // registers, two per wave, and goes through the row blocks, which it stages in LDS
-// few at a time, the next ones under way while these are used.  Bound by the vector
-// ALU (the group scales and the exponentials, quarter rate) beside the matrix cores.
+// few at a time, the next ones under way while these are used.  Bound by the issue of
+// vector instructions (group scales, exponentials at quarter rate) and matrix ones (80
+// cycles per 16x16 tile at head_dim 128), which add up.  256 rows per KV head, 4
+// sequences of 28K tokens, 4 KV heads, 4-bit: 75 us for the (max, sum), 63 for the
+// weights (the biases by float32 matrix instructions: 80 and 70).
 
 constexpr int kManyWaves = 8, kManyThreads = 64 * kManyWaves;
 constexpr int kManyTiles = 2;  // per wave
 constexpr int kManyPart = kManyWaves * kManyTiles * PKV_TILE;
 
 // A block's record: query operands [KB][64 lanes] 16 bytes; then [16 rows] f32 each:
-// multiplier, log-sum-exp, tokens seen (int), the group sums [NG], and a last one: the
-// most and the least that its rows see.
+// multiplier, log-sum-exp, tokens seen (int), and a last one: the most and the least
+// that its rows see; then, for quantized pages, the operands [64 lanes] 16 bytes of
+// the groups' sums.
 template <typename C>
 struct Record {
-  static constexpr int MULT = C::KB * 1024, LSE = MULT + 64, SEES = LSE + 64, QS = SEES + 64, RANGE = QS + C::NG * 64,
-                       BYTES = RANGE + 64;
+  static constexpr int MULT = C::KB * 1024, LSE = MULT + 64, SEES = LSE + 64, RANGE = SEES + 64, SUMS = RANGE + 64,
+                       BYTES = SUMS + (C::QUANT ? 1024 : 0);
   static constexpr int STAGE = C::KB > 4 ? 2 : 4;  // records per stage
 };
 
@@ -527,7 +530,7 @@ struct ManyParts {
   __host__ __device__ ManyParts(int64_t segs, int rows, int64_t cap, int dp, int ng) {
     blocks = (rows + 15) / 16;
     parts = (cap + kManyPart - 1) / kManyPart;
-    record = dp * 32 + 64 * (4 + (ng > 0 ? ng : 1));
+    record = dp * 32 + 4 * 64 + (ng > 0 ? 1024 : 0);
     ml = segs * blocks * record + 4 * record;  // (a stage's last copy reads past the last record)
     total = ml + segs * parts * blocks * 16 * 8;
   }
@@ -566,21 +569,25 @@ __global__ __launch_bounds__(kThreads) void mass_prepare_kernel(const MassArgs a
     ((float *)(record + R::MULT))[col] = mult;
     ((float *)(record + R::LSE))[col] = 0.0f;
     ((int *)(record + R::SEES))[col] = sees;
-#pragma unroll
-    for (int k = 0; k < C::NG; ++k) ((float *)(record + R::QS))[k * 16 + col] = qs[k];
     ((int *)(record + R::RANGE))[col] = col == 0 ? most : col == 1 ? least : 0;
   }
-}
-
-// The group biases' part of 16x16 scores, in float32: rows a (of 16) and columns b,
-// lane l's a and b of its group l / 16 (and + 4).  For float pages a zero.
-template <typename C>
-__device__ __forceinline__ f4 bias_scores(const float (&a)[C::BM], const float (&b)[C::BM], f4 zero) {
-  f4 acc = zero;
-  if constexpr (C::QUANT)
+  if constexpr (C::QUANT) {
+    // a group's sum (at most 2^15, float32) as three float16 that add up to it: their
+    // products with the bias are exact, and one matrix instruction takes eight groups
+    h8 sums = {};
 #pragma unroll
-    for (int k = 0; k < C::BM; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], acc, 0, 0, 0);
-  return acc;
+    for (int k = 0; k < C::NG; ++k) {
+      const _Float16 hi = (_Float16)qs[k], mid = (_Float16)(qs[k] - (float)hi);
+      const _Float16 lo = (_Float16)(qs[k] - (float)hi - (float)mid);
+      const bool finite = fabsf(qs[k]) < INFINITY;
+      if (k / 2 == jj) {
+        sums[k % 2 * 3] = hi;
+        sums[k % 2 * 3 + 1] = finite ? mid : (_Float16)0.0f;
+        sums[k % 2 * 3 + 2] = finite ? lo : (_Float16)0.0f;
+      }
+    }
+    *(u4 *)(record + R::SUMS + lane * 16) = __builtin_bit_cast(u4, sums);
+  }
 }
 
 // The pass over a launch's units.  SUM false: the (max, sum) of each row over the
@@ -626,7 +633,8 @@ __global__ __launch_bounds__(kManyThreads, C::KB > 4 ? 2 : 4) void mass_pass_ker
     // the wave's tiles
     typename C::KT kt[N][C::KB];
     bool there[N], all = true;
-    float scale[N][SUM ? 1 : 4][C::NG], bias[N][C::BM];  // of the lane's token, or its four
+    float scale[N][SUM ? 1 : 4][C::NG];  // of the lane's token, or its four
+    h8 bias[N];  // operand: thrice that of groups 2 jj and 2 jj + 1 of token col
     const int ids = tile_page<N>(a, u.b, t0, u.L, lane);
     uint32_t kw[N][C::LW];
 #pragma unroll
@@ -641,13 +649,10 @@ __global__ __launch_bounds__(kManyThreads, C::KB > 4 ? 2 : 4) void mass_pass_ker
       for (int j = 0; j < C::LW; ++j) kw[i][j] = 0;
       if (there[i]) load_payload<C>(kw[i], head + (slot / PKV_TILE) * g.tile_bytes, lane);
       if constexpr (C::QUANT) {
-#pragma unroll
-        for (int k = 0; k < C::BM; ++k) {
-          const int gi = jj + 4 * k;
-          uint32_t x = 0;
-          if (there[i] && gi < C::NG) x = ((const uint32_t *)meta)[col * C::NG + gi];
-          bias[i][k] = f16_bits_to_f32(x >> 16);
-        }
+        uint32_t b0 = 0, b1 = 0;
+        if (there[i] && 2 * jj < C::NG) b0 = ((const uint32_t *)meta)[col * C::NG + 2 * jj] >> 16;
+        if (there[i] && 2 * jj + 1 < C::NG) b1 = ((const uint32_t *)meta)[col * C::NG + 2 * jj + 1] >> 16;
+        bias[i] = __builtin_bit_cast(h8, u4{b0 | b0 << 16, b0 | b1 << 16, b1 | b1 << 16, 0u});
         if constexpr (SUM) {
 #pragma unroll
           for (int j = 0; j < C::NG; ++j)
@@ -693,16 +698,14 @@ __global__ __launch_bounds__(kManyThreads, C::KB > 4 ? 2 : 4) void mass_pass_ker
         typename C::KT q[C::KB];
 #pragma unroll
         for (int kb = 0; kb < C::KB; ++kb) q[kb] = __builtin_bit_cast(typename C::KT, *(const u4 *)(rec + (kb * 64 + lane) * 16));
-        float qs[C::BM];
-        // (group sums past the last are met by biases of 0: read the last one's)
-#pragma unroll
-        for (int j = 0; j < C::BM; ++j)
-          qs[j] = C::QUANT ? ((const float *)(rec + R::QS))[min(jj + 4 * j, C::NG - 1) * 16 + col] : 0.0f;
+        h8 qs = {};
+        if constexpr (C::QUANT) qs = __builtin_bit_cast(h8, *(const u4 *)(rec + R::SUMS + lane * 16));
         float x[N][4];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           f4 acc[C::NG];
-          const f4 base = SUM ? bias_scores<C>(qs, bias[i], zero) : bias_scores<C>(bias[i], qs, zero);
+          f4 base = zero;  // the biases' part
+          if constexpr (C::QUANT) base = SUM ? FloatOps<1>::qk(qs, bias[i], zero) : FloatOps<1>::qk(bias[i], qs, zero);
 #pragma unroll
           for (int j = 0; j < C::NG; ++j) acc[j] = zero;
 #pragma unroll
@@ -773,15 +776,20 @@ __global__ __launch_bounds__(kManyThreads, C::KB > 4 ? 2 : 4) void mass_pass_ker
       // the next records have arrived
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
       __syncthreads();
-      if (!SUM && (int)threadIdx.x < nb * 16) {
+      const int mine = (int)threadIdx.x - (int)(b0 / S % kManyWaves) * 64;  // another wave at each stage
+      if (!SUM && mine >= 0 && mine < nb * 16) {
         // (these are written again two stages on, behind another barrier)
         float m = -INFINITY, l = 0.0f;
+        float2 y[kManyWaves];
 #pragma unroll
         for (int k = 0; k < kManyWaves; ++k) {
-          const float2 y = s_ml[SUM ? 0 : buffer][SUM ? 0 : k][SUM ? 0 : threadIdx.x];
-          join(m, l, y.x, y.y);
+          y[k] = s_ml[SUM ? 0 : buffer][SUM ? 0 : k][SUM ? 0 : mine];
+          m = fmaxf(m, y[k].x);
         }
-        ((float2 *)((char *)a.workspace + w.ml))[((seg * w.parts + u.part) * w.blocks + b0) * 16 + threadIdx.x] = float2{m, l};
+        const float z = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int k = 0; k < kManyWaves; ++k) l += y[k].y * exp2_fast(y[k].x - z);
+        ((float2 *)((char *)a.workspace + w.ml))[((seg * w.parts + u.part) * w.blocks + b0) * 16 + mine] = float2{m, l};
       }
     }
     if constexpr (SUM) {
@@ -865,7 +873,7 @@ void launch(hipStream_t stream, const MassArgs &a, int64_t cap) {
   }
   using R = Record<C>;
   const ManyParts w(segs, a.rows, cap, a.g.dp, a.g.ng);
-  static_assert(R::BYTES == C::KB * 1024 + 64 * (4 + C::NG), "as ManyParts has it");
+  static_assert(R::BYTES == C::KB * 1024 + 4 * 64 + (C::QUANT ? 1024 : 0), "as ManyParts has it");
   const dim3 grid(walkers(segs * w.parts));
   const unsigned blocks = (unsigned)(segs * w.blocks);
   hipLaunchKernelGGL((mass_prepare_kernel<C>), dim3((blocks + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, a, w);
