@@ -17,10 +17,9 @@
 // what reaches the largest of the waves' bounds, a few times `count`, goes to LDS
 // and is ranked there.  A second launch joins the chunks' sums and does the same
 // with the lists' entries.  One read of the logits: 128 rows of 128256 bfloat16 (33
-// MB) take 14 us (2.3 TB/s; about 530 vector instructions, a bisection among them, per
-// wave and 2048 logits, eight chunks to a CU) and the merge 9.9 us, a chain
-// of dependent steps; 768 rows of 104543 float16, 21 selected (161 MB), 57 us (2.8 TB/s)
-// and 18.
+// MB) take 13.8 us (2.4 TB/s: all chunks resident at once, one round of loads, sums,
+// bisection and ranks, half of it the issue of instructions) and the merge 8.6 us, a chain of dependent steps; 768 rows of 104543
+// float16, 21 selected (161 MB), 62 us (2.6 TB/s) and 14.
 #include <cfloat>
 
 #include "pkv_cache_ops.h"
@@ -31,10 +30,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kVectors = 4;  // of eight logits, per thread
-// logits of a workgroup; 4 rows of 8000, both launches: 10.1 us, by a quarter of it 12.1,
-// by half 12.4; 8 rows of 128256: 18.9, 27.5 and 21.4
-constexpr int kChunk = 8 * kVectors * kThreads;
 constexpr int kMergeList = 512;  // candidates of a group in LDS
 constexpr int kHeld = 16384;  // candidates of a group whose order is kept in LDS
 constexpr int kList = 256;  // candidates in LDS, per wave
@@ -59,8 +54,9 @@ struct BeamParts {
   int chunks;
   uint32_t by_count, by_chunks;  // floor(2^32 / d) + 1: __umulhi(e, it) = e / d for e < 2^32 / d
   int64_t lists, total;
-  __host__ __device__ BeamParts(int groups, int beams, int vocab, int count) {
-    chunks = (vocab + kChunk - 1) / kChunk;
+  __host__ __device__ BeamParts(int groups, int beams, int vocab, int count, int vectors) {
+    const int chunk = 8 * vectors * kThreads;
+    chunks = (vocab + chunk - 1) / chunk;
     const int64_t n = (int64_t)groups * beams * chunks;
     by_count = (uint32_t)(((uint64_t)1 << 32) / count) + 1;
     by_chunks = (uint32_t)(((uint64_t)1 << 32) / chunks) + 1;
@@ -153,9 +149,10 @@ __device__ __forceinline__ int sum4(int v) {
   return v + __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, false);
 }
 
-template <int KIND>
-__global__ __launch_bounds__(kThreads, 6) void beam_chunk_kernel(const BeamArgs a, const BeamParts w) {
-  constexpr int V = kVectors;
+// V vectors of eight logits per thread
+template <int KIND, int V>
+__global__ __launch_bounds__(kThreads, V > 4 ? 4 : 6) void beam_chunk_kernel(const BeamArgs a, const BeamParts w) {
+  constexpr int kChunk = 8 * V * kThreads;
   __shared__ uint64_t s_list[kWaves][kList];  // (order << 32 | ~token), what each wave found
   __shared__ double s_sum[kWaves];
   __shared__ float s_most[kWaves];
@@ -525,18 +522,35 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArg
   }
 }
 
+// Vectors per thread: 4 (chunks of 8192 logits), or 8 where the grid is large anyhow
+// and many lists of a group are to be merged.  Both launches, us, by 4 and by 8: 4 rows
+// of 8000 logits 10.7 and 12.3, 256 of 32000 (8 selected) 17.5 and 19.2, 8 of 128256
+// 18.7 and 20.8; 128 of 128256 24.6 and 22.8, 256 of 49999 (32 selected) 35.2 and 32.2,
+// 512 of 32000 (16 selected) 26.6 and 24.3; 768 of 104543 75.0 and 76.2.
+int chunk_vectors(int groups, int beams, int vocab, int count) {
+  const int64_t chunks = (vocab + 8191) / 8192;
+  return groups * beams * chunks >= 1024 && beams * chunks * count >= 512 ? 8 : 4;
+}
+
+template <int V>
+void start_chunks(hipStream_t stream, const BeamArgs &a, const BeamParts &w) {
+  const dim3 grid((unsigned)((int64_t)a.groups * a.beams * w.chunks));
+  if (a.kind == 0) hipLaunchKernelGGL((beam_chunk_kernel<0, V>), grid, dim3(kThreads), 0, stream, a, w);
+  else if (a.kind == 1) hipLaunchKernelGGL((beam_chunk_kernel<1, V>), grid, dim3(kThreads), 0, stream, a, w);
+  else hipLaunchKernelGGL((beam_chunk_kernel<2, V>), grid, dim3(kThreads), 0, stream, a, w);
+}
+
 }  // namespace
 
 int64_t beam_workspace(int groups, int beams, int vocab, int count) {
-  return BeamParts(groups, beams, vocab, count).total;
+  return BeamParts(groups, beams, vocab, count, chunk_vectors(groups, beams, vocab, count)).total;
 }
 
 hipError_t launch_beam(hipStream_t stream, const BeamArgs &a) {
-  const BeamParts w(a.groups, a.beams, a.vocab, a.count);
-  const dim3 grid((unsigned)((int64_t)a.groups * a.beams * w.chunks));
-  if (a.kind == 0) hipLaunchKernelGGL(beam_chunk_kernel<0>, grid, dim3(kThreads), 0, stream, a, w);
-  else if (a.kind == 1) hipLaunchKernelGGL(beam_chunk_kernel<1>, grid, dim3(kThreads), 0, stream, a, w);
-  else hipLaunchKernelGGL(beam_chunk_kernel<2>, grid, dim3(kThreads), 0, stream, a, w);
+  const int vectors = chunk_vectors(a.groups, a.beams, a.vocab, a.count);
+  const BeamParts w(a.groups, a.beams, a.vocab, a.count, vectors);
+  if (vectors == 8) start_chunks<8>(stream, a, w);
+  else start_chunks<4>(stream, a, w);
   // us by 256 and by 1024 threads: 128 candidates of a group 7.4 and 8.5, 512 10.1 and
   // 10.2, 2048 18.9 and 11.4
   if (a.beams * w.chunks * a.count <= 1024)

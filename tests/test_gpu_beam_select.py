@@ -121,6 +121,28 @@ def test_banned_tokens_and_dead_beams(dtype, vocab):
     _check(logits[:, :1].expand(4, 4, vocab), first, 8)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("groups,beams,vocab,count", [(8, 64, 9001, 8), (8, 64, 16384, 20), (22, 16, 16390, 11)])
+def test_large_grids(dtype, groups, beams, vocab, count):
+    """Many rows and long lists: plain rows, ties, masks, NaN, done beams, rising rows."""
+    dtype = getattr(torch, dtype)
+    logits, scores = _inputs(groups, beams, vocab, dtype, vocab)
+    low = torch.finfo(dtype).min
+    logits[1] = 0                                        # more ties than any list holds
+    logits[2, :, :vocab - 3] = -math.inf
+    logits[3, :, :vocab - 3] = low
+    logits[3, 1] = low
+    logits[4, 1, 5], logits[4, 2, vocab - 1], logits[4, 3] = math.nan, math.inf, -math.inf
+    logits[5] = torch.linspace(-20, 20, vocab, device="cuda").to(dtype)
+    logits[6] = torch.linspace(20, -20, vocab, device="cuda").to(dtype)
+    logits[7] = torch.randint(0, 3, (beams, vocab), generator=torch.Generator().manual_seed(7)).cuda().to(dtype)
+    scores[1] = scores[7] = 0
+    scores[4, 0], scores[4, 4] = -math.inf, math.nan
+    _check(logits, scores, count)
+    done = torch.rand((groups, beams), generator=torch.Generator().manual_seed(count)).cuda() < 0.3
+    _check(logits, scores, count, done, 2)
+
+
 @pytest.mark.parametrize("order", ["rising", "falling"])
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_sorted_rows(order, dtype):
