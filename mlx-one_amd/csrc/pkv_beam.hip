@@ -197,9 +197,11 @@ __global__ __launch_bounds__(kThreads, V > 4 ? 4 : 6) void beam_chunk_kernel(con
   // exp(x - most) as 2^(x L - R), L = log2(e) in float32 and R the integer next to
   // most L: the product is not rounded, R is exact, and 2^(R - most L) makes up for it
   constexpr float kL = 1.4426950408889634f;
-  const float from = fabsf(most) < 8e6f ? rintf(most * kL) : most * kL;
-  // (not for rows that have no sum, or only logits at their type's end)
-  const bool flat = __builtin_amdgcn_readfirstlane(!(fabsf(from) < INFINITY));
+  const float from = rintf(most * kL);
+  // From 8e6 on float32 holds no such R (and one that is off by hundreds leaves a sum of
+  // inf or 0).  Logits there lie half a unit apart at least, so x - most is exact where
+  // its exponential is not 0.  Masks of -1e9 to -1e38 come here, and rows without a sum.
+  const bool flat = __builtin_amdgcn_readfirstlane(!(fabsf(most) < 8e6f));
   float sum = 0.0f;
   if (flat) {
 #pragma unroll
