@@ -445,6 +445,7 @@ __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a
   for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
     const int base = u.base;
     if (!u.find(a, kSumPart, unit, lane)) return;
+    if (u.base != base) before = Runs::parts_before(a, kPart, lane, u.base);  // (also where the row is skipped)
     const int row = mass_row(a, u.b);
     if (row < 0) continue;
     const int64_t seg = (int64_t)u.b * a.g.hk + u.kh;
@@ -465,7 +466,6 @@ __global__ __launch_bounds__(kThreads) void mass_weights_kernel(const MassArgs a
     // the rows' log-sum-exps from the workgroups' (m, l): lane 16 k + r the k-th's of row r
     float lse;
     {
-      if (u.base != base) before = Runs::parts_before(a, kPart, lane, u.base);
       const int n1 = parts_of(u.len), f = u.b - u.base, parts = __builtin_amdgcn_readlane(n1, f);
       const int upto = __builtin_amdgcn_readlane(wave_scan_incl(n1, lane), f);
       const int first = (before + upto - parts) * a.g.hk + u.kh * parts;
