@@ -260,12 +260,19 @@ class DevicePageArena:
         free ones); the slots are cut as many at a time as there are."""
         if self.mass is None:
             raise ValueError("eviction goes by the attention weight: call track_mass() first")
+        if sinks < 0 or recent < 0:
+            raise ValueError("negative count of protected tokens")
         slots_d, host_slots = self._slots(slots)
         count = int(slots_d.numel())
+        # a budget past what a slot can hold cuts nothing
+        most = self.max_pages * self.page_tokens
         if isinstance(keep, int):
+            keep = min(keep, most)
             max_keep = keep if max_keep is None else max_keep
             keep = [keep] * count if host_slots is not None else \
                 torch.full((count,), keep, dtype=torch.int32, device=self.device)
+        elif not isinstance(keep, torch.Tensor):
+            keep = [min(int(k), most) for k in keep]
         keep_d, host_keep = self._ints(keep, count)
         if host_keep is not None:
             if any(k < 0 for k in host_keep):
@@ -274,6 +281,7 @@ class DevicePageArena:
             host_keep = [min(k, max_keep) for k in host_keep]
         if max_keep is None or max_keep < 0:
             raise ValueError("budgets on the device need max_keep, their bound")
+        max_keep = min(int(max_keep), most)
         if keep_d.numel() != count:
             raise ValueError("one budget per slot")
         if count == 0:
@@ -294,7 +302,11 @@ class DevicePageArena:
             for i in range(0, count, step):      # as many slots at a time as there are spare ones
                 part = slots_d[i:i + step]
                 self._evict(part, keep_d[i:i + step], spare_d[:part.numel()], int(sinks),
-                            int(recent), int(max_keep))
+                            int(recent), max_keep)
+        except BaseException:
+            if host_slots is not None:           # (slots before this one may have been cut)
+                self.sync_lengths()
+            raise
         finally:
             self._free_slots.extend(reversed(opened))
         if host_slots is not None and host_keep is not None:
@@ -311,16 +323,21 @@ class DevicePageArena:
         lens = self.lens[at]
         kept_lens = keep_d.clamp(0, max_keep)
         cut = valid & (lens > kept_lens)
-        res = self.reserve(spare_d, torch.where(cut, kept_lens, 0))
-        cut = cut & (res.lens == kept_lens)       # a slot without its new pages stays as it is
-        kept, n, _ = ops.evict_select(self.mass, lens, keep_d, max_keep=max_keep, sinks=sinks,
-                                      recent=recent, rows=torch.where(cut, slots_d, -1),
-                                      new_mass=self.mass)
-        ops.evict_pages(self.fmt, self.pools, kept, n, self.table[at], res.table)
-        places = self._places(slots_d)
-        self.evicted[places] = self.evicted[places] + torch.where(cut, lens - kept_lens, 0)
-        self._reorder_pages(slots_d, torch.where(cut, spare_d, slots_d))  # the sums have moved
-        self.truncate(spare_d, torch.zeros_like(spare_d))
+        widths, none = torch.where(cut, kept_lens, 0), torch.zeros_like(spare_d)
+        res = self.reserve(spare_d, widths)
+        try:
+            cut = cut & (res.lens == kept_lens)   # a slot without its new pages stays as it is
+            rows, sources = torch.where(cut, slots_d, -1), torch.where(cut, spare_d, slots_d)
+            table, places = self.table[at], self._places(slots_d)
+            evicted = self.evicted[places] + torch.where(cut, lens - kept_lens, 0)
+            kept, n, _ = ops.evict_select(self.mass, lens, keep_d, max_keep=max_keep, sinks=sinks,
+                                          recent=recent, rows=rows, new_mass=self.mass)
+            ops.evict_pages(self.fmt, self.pools, kept, n, table, res.table)
+            self.evicted[places] = evicted
+            self._reorder_pages(slots_d, sources)     # the sums have moved
+        finally:
+            # (whatever failed on the way: the spare slots are empty again)
+            self.truncate(spare_d, none)
 
     # -- inspection (these synchronise) ---------------------------------------------------
     def sync_lengths(self):
