@@ -179,11 +179,18 @@ class DevicePageArena:
                 raise ValueError("fork sources and destinations must pair up and be disjoint")
             if any(self.lengths[d] for d in host_dst):
                 raise ValueError("fork destinations must be empty")
+        to = dst_d
+        if self.mass is not None:
+            # the pairs that the kernel takes (the sums of the others stay)
+            at, source = self._places(dst_d), self._places(src_d)
+            takes = (at < self.max_slots) & (source < self.max_slots) & (at != source)
+            takes = takes & (self.lens[at.clamp(max=self.max_slots - 1)] == 0)
+            to = torch.where(takes, dst_d, -1)
         code = nat.load().pkv_arena_fork(nat.stream_handle(self.device), nat.ptr(self.state),
                                          *self._common(), nat.ptr(src_d), nat.ptr(dst_d),
                                          int(src_d.numel()))
         nat.check(code, "arena fork")
-        self._move_mass(dst_d, src_d)
+        self._move_mass(to, src_d)
         if host_src is not None and host_dst is not None:
             for s, d in zip(host_src, host_dst):
                 self.lengths[d] = self.lengths[s]
