@@ -157,7 +157,7 @@ class DevicePageArena:
         nat.check(code, "arena truncate")
         if self.evicted is not None:
             at = self._places(slots_d)
-            self.evicted[at] = self.evicted[at] * (keep_d > 0)   # an emptied slot starts anew
+            self.evicted[at] = self.evicted[at] * (keep_d != 0)  # an emptied slot starts anew
         if host_slots is not None and host_keep is not None:
             for s, k in zip(host_slots, host_keep):
                 self.lengths[s] = k

@@ -47,3 +47,13 @@ def test_refused_forks():
     assert torch.equal(arena.table[:4], table[:4])
     with pytest.raises(CacheCorruptionError):
         arena.check()
+
+
+def test_refused_truncations():
+    from pkv.cache_errors import CacheCorruptionError
+
+    arena = _evicted_arena()
+    arena.truncate(_i32(0, 1, 2, 7), _i32(-1, 61, 0, 0))
+    assert arena.evicted[:3].tolist() == [50, 30, 0] and arena.lens[:3].tolist() == [40, 60, 0]
+    with pytest.raises(CacheCorruptionError):
+        arena.check()
