@@ -13,10 +13,11 @@ replayed as a HIP graph.
 
 Semantics follow the reference's paged cache: ``fork`` is ``clone`` (pages
 shared by reference count; a shared, partly filled tail is copied when it is
-first written, not at fork time), ``truncate`` is ``trim``/rollback by length,
-``release`` is ``reset``.  Errors (no free page, a full table) are recorded on
-the device and raised by ``check()`` as ``CacheCapacityError`` /
-``CacheCorruptionError``; a call that hits one leaves its slots unchanged.
+first written, not at fork time), ``truncate`` is ``trim``, ``rollback`` takes a
+step back by length, ``release`` is ``reset``.  Errors (no free page, a full
+table) are recorded on the device and raised by ``check()`` as
+``CacheCapacityError`` / ``CacheCorruptionError``; a call that hits one leaves
+its slots unchanged.
 """
 
 from __future__ import annotations
@@ -143,10 +144,19 @@ class DevicePageArena:
         return Reservation(slots_d, widths_d, table, starts, lens)
 
     def truncate(self, slots, keep_tokens):
-        """Cut each slot back to ``keep_tokens`` (rollback by length / ``trim``)."""
+        """Cut each slot back to ``keep_tokens`` (``trim``); an emptied slot starts
+        anew, with no token evicted from it."""
+        slots_d, keep_d = self.rollback(slots, keep_tokens)
+        if self.evicted is not None:
+            at = self._places(slots_d)
+            self.evicted[at] = self.evicted[at] * (keep_d != 0)
+
+    def rollback(self, slots, lengths):
+        """Cut each slot back to the length it had before a step: as ``truncate``, but a
+        slot that eviction had emptied goes on at its text's position."""
         slots_d, host_slots = self._slots(slots)
         count = int(slots_d.numel())
-        keep_d, host_keep = self._ints(keep_tokens, count)
+        keep_d, host_keep = self._ints(lengths, count)
         if host_slots is not None and host_keep is not None:
             for s, k in zip(host_slots, host_keep):
                 if k < 0 or k > self.lengths[s]:
@@ -155,12 +165,10 @@ class DevicePageArena:
                                              *self._common(), nat.ptr(slots_d), nat.ptr(keep_d),
                                              count)
         nat.check(code, "arena truncate")
-        if self.evicted is not None:
-            at = self._places(slots_d)
-            self.evicted[at] = self.evicted[at] * (keep_d != 0)  # an emptied slot starts anew
         if host_slots is not None and host_keep is not None:
             for s, k in zip(host_slots, host_keep):
                 self.lengths[s] = k
+        return slots_d, keep_d
 
     def release(self, slots):
         """Drop every page of the slots and return them to the free slot list."""
@@ -344,7 +352,7 @@ class DevicePageArena:
             self._reorder_pages(slots_d, sources)     # the sums have moved
         finally:
             # (whatever failed on the way: the spare slots are empty again)
-            self.truncate(spare_d, none)
+            self.rollback(spare_d, none)
 
     # -- inspection (these synchronise) ---------------------------------------------------
     def sync_lengths(self):
@@ -452,7 +460,7 @@ class DeviceRunner:
     """Batch steps of a model over device-arena slots: ``PagedRunner.execute``
     (``engine/paged.py:308-417``) with the page bookkeeping on the device.  One
     reservation covers every layer; a step that raises is rolled back by
-    length (``truncate`` to the lengths before it)."""
+    length (``rollback`` to the lengths before it)."""
 
     def __init__(self, model, arena):
         if len(arena.pools) != model.spec.num_layers:
@@ -484,7 +492,7 @@ class DeviceRunner:
         try:
             out = self._forward(hidden, res)
         except BaseException:
-            self.arena.truncate(slots, before)
+            self.arena.rollback(slots, before)
             raise
         err = self.arena.probe_failed(probe)
         if err:

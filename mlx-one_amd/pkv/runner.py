@@ -298,7 +298,7 @@ class PagedRunner:
             # cancelled (or late) requests keep their length before the step
             dropped = [(s, n) for r, s, n in zip(requests, slots, history) if request_cancelled(r)]
             if dropped:
-                arena.truncate([s for s, _ in dropped], [n for _, n in dropped])
+                arena.rollback([s for s, _ in dropped], [n for _, n in dropped])
         if uniform and not any(r.return_all_logits for r in requests):
             outputs = y[:, width - 1:width].split(1)            # one call for every view
         else:
