@@ -297,8 +297,11 @@ class PagedRunner:
                 y = runner.execute(slots, self._inputs(model, requests, widths), widths)
             # cancelled (or late) requests keep their length before the step
             dropped = [(s, n) for r, s, n in zip(requests, slots, history) if request_cancelled(r)]
-            if dropped:
-                arena.rollback([s for s, _ in dropped], [n for _, n in dropped])
+            held = [(s, n) for s, n in dropped if n]
+            if held:
+                arena.truncate([s for s, _ in held], [n for _, n in held])
+            if len(held) < len(dropped):      # (truncated to 0 a slot would start anew)
+                arena.rollback([s for s, n in dropped if not n], [0] * (len(dropped) - len(held)))
         if uniform and not any(r.return_all_logits for r in requests):
             outputs = y[:, width - 1:width].split(1)            # one call for every view
         else:

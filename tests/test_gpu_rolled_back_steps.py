@@ -46,3 +46,40 @@ def test_positions_go_on_after_a_failed_step():
     # emptied by truncation, a slot starts anew
     arena.truncate([a, b], [0, 0])
     assert arena.positions(arena.reserve([a, b], [0, 0])).tolist() == [0, 0]
+
+
+def test_positions_go_on_after_a_cancelled_step():
+    import threading
+
+    from pkv.runner import ForwardRequest, PagedRunner
+    from test_gpu_device_cache import _setup
+
+    model, cm = _setup("device")
+    handles = [cm.create_handle(f"r{i}", key_type="q8_0", value_type="q8_0") for i in range(3)]
+    arena = handles[0].bundle.entries[0].arena
+    arena.track_mass()
+    runner = PagedRunner(model)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+
+    def run(widths, cancel):
+        return runner.execute([
+            ForwardRequest(None, (), h.bundle.entries, phase="prefill", runtime=cm, handle=h, request_id=h.request_id,
+                           hidden=torch.randn((n, 256), generator=gen, device="cuda").half(), cancel=c)
+            for h, n, c in zip(handles, widths, cancel)])
+
+    run([50, 60, 70], [None] * 3)
+    slots = [h.bundle.entries[0].slot for h in handles]
+    arena.evict(slots, [0, 20, 0])
+    stop = threading.Event()
+    forward = model.forward
+
+    def forward_and_cancel(*args, **kw):
+        stop.set()
+        return forward(*args, **kw)
+
+    model.forward = forward_and_cancel
+    run([1, 1, 1], [stop, stop, None])
+    model.forward = forward
+    assert arena.lens[slots].tolist() == [0, 20, 1] and [arena.lengths[s] for s in slots] == [0, 20, 1]
+    assert [h.token_count for h in handles] == [0, 20, 1]
+    assert arena.positions(arena.reserve(slots, [0, 0, 0])).tolist() == [50, 60, 71]
