@@ -324,12 +324,13 @@ class DevicePageArena:
             raise
         finally:
             self._free_slots.extend(reversed(opened))
-        if host_slots is not None and host_keep is not None:
+        if host_slots is not None:
             err = self.probe_failed(self.error_probe())
-            if err:
+            if err or host_keep is None:
                 self.sync_lengths()
+            if err:
                 self._raise(err)
-            for s, k in zip(host_slots, host_keep):
+            for s, k in zip(host_slots, host_keep or ()):
                 self.lengths[s] = min(self.lengths[s], k)
 
     def _evict(self, slots_d, keep_d, spare_d, sinks, recent, max_keep):
