@@ -32,6 +32,11 @@ auto guarded(F body) noexcept -> decltype(body()) {
 // The bounds below keep every grid under 2^32 threads.
 constexpr int64_t kMaxRows = 1 << 24;  // query rows per KV head of a call
 
+// Kernels count tokens in 32 bits up to the end of a row's last part: of 1024 tokens
+// (attention mass), 16384 logits (beams), 32768 sums (select).
+constexpr int64_t kMaxMassTokens = (int64_t)INT32_MAX - 1023;
+constexpr int64_t kMaxVocab = (int64_t)INT32_MAX - ((1 << 15) - 1), kMaxSelectTokens = (int64_t)INT32_MAX - ((1 << 16) - 1);
+
 // Kernels read and write their workspace 16 bytes at a time.
 bool aligned(const void *workspace) { return (uintptr_t)workspace % 16 == 0; }
 
@@ -44,6 +49,7 @@ int mass_shape(const pkv_layout *layout, int32_t num_heads, int32_t num_queries,
   if ((int64_t)num_queries * (num_heads / g->hk) > kMaxRows)
     return fail(PKV_UNSUPPORTED, "at most 2^24 query rows per KV head");
   if ((int64_t)max_pages * g->page > INT32_MAX) return fail(PKV_INVALID_ARGUMENT, "block table too wide");
+  if ((int64_t)max_pages * g->page > kMaxMassTokens) return fail(PKV_UNSUPPORTED, "block tables of at most 2^31 - 1024 tokens");
   if ((int64_t)batch * g->hk > 65535) return fail(PKV_UNSUPPORTED, "at most 65535 (sequence, KV head) pairs");
   if ((int64_t)batch * g->hk * max_pages > (1 << 30))
     return fail(PKV_UNSUPPORTED, "at most 2^30 pages of (sequence, KV head) pairs");
@@ -56,9 +62,9 @@ int beam_shape(int32_t groups, int32_t beams, int32_t vocab, int32_t count) {
   if (groups < 0 || beams < 1 || vocab < 1 || count < 1) return fail(PKV_INVALID_ARGUMENT, "invalid beam shape");
   if (beams > pkv::kMaxBeams || count > pkv::kMaxBeamCount)
     return fail(PKV_UNSUPPORTED, "at most 64 beams and 64 selected pairs per group");
-  if ((int64_t)beams * vocab > INT32_MAX || groups > (1 << 21) || (int64_t)groups * beams > (1 << 22) ||
+  if (vocab > kMaxVocab || (int64_t)beams * vocab > INT32_MAX || groups > (1 << 21) || (int64_t)groups * beams > (1 << 22) ||
       (int64_t)groups * beams * vocab > ((int64_t)1 << 36))
-    return fail(PKV_UNSUPPORTED, "at most 2^31 - 1 (beam, token) pairs per group, 2^21 groups, 2^22 beams and 2^36 pairs");
+    return fail(PKV_UNSUPPORTED, "at most 2^31 - 2^15 tokens, 2^31 - 1 (beam, token) pairs per group, 2^21 groups, 2^22 beams and 2^36 pairs");
   if (count > (int64_t)beams * vocab) return fail(PKV_INVALID_ARGUMENT, "fewer (beam, token) pairs than the count");
   return PKV_OK;
 }
@@ -140,6 +146,8 @@ int pkv_evict_select(void *stream, const float *mass, int32_t layers, int32_t ma
     if (sinks < 0 || recent < 0) return fail(PKV_INVALID_ARGUMENT, "negative count of protected tokens");
     if (new_mass && new_width < max_keep)
       return fail(PKV_INVALID_ARGUMENT, "the kept sums need room for max_keep tokens");
+    if (mass_width > kMaxSelectTokens || max_keep > kMaxSelectTokens)
+      return fail(PKV_UNSUPPORTED, "at most 2^31 - 2^16 tokens");
     if ((int64_t)layers * batch * kv_heads > (1 << 21))
       return fail(PKV_UNSUPPORTED, "at most 2^21 (layer, sequence, KV head) rows");
     if (layers == 0 || batch == 0) return PKV_OK;
