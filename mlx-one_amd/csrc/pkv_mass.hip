@@ -528,7 +528,7 @@ struct Record {
 struct ManyParts {
   int64_t blocks, parts, record, ml, total;
   __host__ __device__ ManyParts(int64_t segs, int rows, int64_t cap, int dp, int ng) {
-    blocks = (rows + 15) / 16;
+    blocks = rows > 0 ? (rows + 15) / 16 : 1;  // (no rows: one block that sees nothing)
     parts = (cap + kManyPart - 1) / kManyPart;
     record = dp * 32 + 4 * 64 + (ng > 0 ? 1024 : 0);
     ml = segs * blocks * record + 4 * record;  // (a stage's last copy reads past the last record)
