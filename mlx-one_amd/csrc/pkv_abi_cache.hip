@@ -151,7 +151,9 @@ int pkv_evict_select(void *stream, const float *mass, int32_t layers, int32_t ma
     if ((int64_t)layers * batch * kv_heads > (1 << 21))
       return fail(PKV_UNSUPPORTED, "at most 2^21 (layer, sequence, KV head) rows");
     if (layers == 0 || batch == 0) return PKV_OK;
-    if (!mass || !seq_lens || !new_lens || (!kept && max_keep > 0)) return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
+    const bool sums = mass_rows > 0 && mass_width > 0;  // (else no row has a token)
+    if ((!mass && sums) || !seq_lens || !new_lens || (!kept && max_keep > 0))
+      return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
     pkv::EvictSelectArgs a;
     a.mass = mass;
     a.layers = layers;
