@@ -314,7 +314,10 @@ class DevicePageArena:
             if host_spare is not None and (any(self.lengths[s] for s in host_spare)
                                            or set(host_spare) & set(host_slots or ())):
                 raise ValueError("spare slots must be empty")
-            for i in range(0, count, step):      # as many slots at a time as there are spare ones
+            # as many slots at a time as there are spare ones and the kernels take
+            heads = self.fmt.num_kv_heads
+            step = max(1, min(step, 4096, 65535 // heads, (1 << 21) // (heads * len(self.pools))))
+            for i in range(0, count, step):
                 part = slots_d[i:i + step]
                 self._evict(part, keep_d[i:i + step], spare_d[:part.numel()], int(sinks),
                             int(recent), max_keep)
