@@ -198,7 +198,8 @@ class DevicePageArena:
                                          *self._common(), nat.ptr(src_d), nat.ptr(dst_d),
                                          int(src_d.numel()))
         nat.check(code, "arena fork")
-        self._move_mass(to, src_d)
+        for i in range(0, to.numel(), 8192):       # (what one reordering takes)
+            self._move_mass(to[i:i + 8192], src_d[i:i + 8192])
         if host_src is not None and host_dst is not None:
             for s, d in zip(host_src, host_dst):
                 self.lengths[d] = self.lengths[s]

@@ -48,3 +48,14 @@ def test_eviction():
             assert np.array_equal(x[:, :10], y[:, kept])
     arena.release(slots)
     assert arena.status() == (13000, 0)
+
+
+def test_fork():
+    arena = _arena(16500, 13000)
+    slots = [arena.open_slot() for _ in range(16400)]
+    heads, others = slots[:8200], slots[8200:]
+    arena.reserve(heads, [5] * len(heads))
+    mass = arena.mass.clone()
+    arena.fork(heads, others)
+    assert arena.status()[1] == 0 and set(arena.lens[others].tolist()) == {5}
+    assert torch.equal(arena.mass[:, others], mass[:, heads]) and torch.equal(arena.mass[:, heads], mass[:, heads])
