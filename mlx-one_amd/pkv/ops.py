@@ -496,6 +496,13 @@ def _address(x, device, count, name):
     return t, t.data_ptr()
 
 
+def _int32(value, name):
+    """A number for a 32-bit argument (ctypes would drop what lies above)."""
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"{name} does not fit 32 bits")
+    return value
+
+
 def _scratch(nbytes, device, what, given=None):
     """The caller's workspace, or the stream's own memory of that size."""
     if nbytes < 0:
@@ -606,8 +613,11 @@ def evict_select(mass, seq_lens, keep, *, max_keep=None, sinks=0, recent=0, rows
                 raise ValueError("budgets on the device need max_keep, their bound")
             max_keep = max([int(k) for k in keep], default=0)
         budget, budget_at = _address(keep, device, batch, "keep")
-    if max_keep < 0:
+    if _int32(max_keep, "max_keep") < 0:
         raise ValueError("negative budget")
+    if sinks < 0 or recent < 0:
+        raise ValueError("negative count of protected tokens")
+    sinks, recent = min(sinks, max_keep), min(recent, max_keep)
     lead = (layers,) if mass.dim() == 4 else ()
     if new_mass is not None:
         _check_dense(new_mass, torch.float32, device, "new_mass", mass.dim())
@@ -696,6 +706,8 @@ def beam_select(logits, scores, count, *, done=None, pad_token=0, workspace=None
             raise ValueError("done must be a [groups, beams] bool tensor on the logits' device")
         done = done.contiguous()
         done_at = done.data_ptr()
+    _int32(count, "count")
+    _int32(pad_token, "pad_token")
     lib = nat.load()
     workspace = _scratch(lib.pkv_beam_workspace_bytes(groups, beams, vocab, count), device,
                          "beam select", workspace)
@@ -723,7 +735,7 @@ def reorder_rows(state, targets, sources, *, dim=0):
     if source.numel() != count:
         raise ValueError("reordering needs a source per target")
     shape = state.shape
-    outer, num_rows = math.prod(shape[:dim]), shape[dim]
+    outer, num_rows = math.prod(shape[:dim]), _int32(shape[dim], "the number of rows")
     row_bytes = math.prod(shape[dim + 1:]) * state.element_size()
     _launch(device, "reorder", nat.load().pkv_reorder_rows, state.data_ptr(), outer, num_rows,
             row_bytes, to.data_ptr(), source.data_ptr(), count)
