@@ -525,13 +525,17 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(const BeamArg
 }
 
 // Vectors per thread: 4 (chunks of 8192 logits), or 8 where the grid is large anyhow
-// and many lists of a group are to be merged.  Both launches, us, by 4 and by 8: 4 rows
-// of 8000 logits 10.7 and 12.3, 256 of 32000 (8 selected) 17.5 and 19.2, 8 of 128256
-// 18.7 and 20.8; 128 of 128256 24.6 and 22.8, 256 of 49999 (32 selected) 35.2 and 32.2,
-// 512 of 32000 (16 selected) 26.6 and 24.3; 768 of 104543 75.0 and 76.2.
-int chunk_vectors(int groups, int beams, int vocab, int count) {
+// and many lists of a group are to be merged: fewer lists against fewer waves that hide
+// loads, which float32's 32 bytes a vector need more.  Both launches by 8 over by 4, 16,384
+// to 152,064 logits, 64 to 1,024 rows, 1 to 32 selected, grids of 1,024 chunks or more
+// (median, a tenth below and above):
+//   candidates of a group   up to 511           512 to 8191         from 8192 on
+//   bfloat16                1.02 (0.93, 1.08)   0.97 (0.90, 1.06)   0.84 (0.60, 0.91)
+//   float32                 1.05 (0.95, 1.23)   1.04 (0.94, 1.23)   0.96 (0.67, 1.11)
+// and 1.02, 1.01 for smaller grids.
+int chunk_vectors(int kind, int groups, int beams, int vocab, int count) {
   const int64_t chunks = (vocab + 8191) / 8192;
-  return groups * beams * chunks >= 1024 && beams * chunks * count >= 512 ? 8 : 4;
+  return groups * beams * chunks >= 1024 && beams * chunks * count >= (kind == 2 ? 8192 : 512) ? 8 : 4;
 }
 
 template <int V>
@@ -545,11 +549,11 @@ void start_chunks(hipStream_t stream, const BeamArgs &a, const BeamParts &w) {
 }  // namespace
 
 int64_t beam_workspace(int groups, int beams, int vocab, int count) {
-  return BeamParts(groups, beams, vocab, count, chunk_vectors(groups, beams, vocab, count)).total;
+  return BeamParts(groups, beams, vocab, count, 4).total;  // (chunks of 16384 need less)
 }
 
 hipError_t launch_beam(hipStream_t stream, const BeamArgs &a) {
-  const int vectors = chunk_vectors(a.groups, a.beams, a.vocab, a.count);
+  const int vectors = chunk_vectors(a.kind, a.groups, a.beams, a.vocab, a.count);
   const BeamParts w(a.groups, a.beams, a.vocab, a.count, vectors);
   if (vectors == 8) start_chunks<8>(stream, a, w);
   else start_chunks<4>(stream, a, w);
