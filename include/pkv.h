@@ -376,7 +376,8 @@ int pkv_arena_fork(void *stream, void *state, int32_t capacity_pages, int32_t pa
  * length, and it decodes one sequence per request.  The sizes that these
  * operators' workspace queries return are negative for shapes that the operator
  * refuses, by its status (-PKV_INVALID_ARGUMENT, -PKV_UNSUPPORTED).  Workspaces are
- * 16-byte aligned.
+ * 16-byte aligned.  Tokens are counted in 32 bits: block tables of at most 2^31 - 1024
+ * tokens, vocabularies of 2^31 - 2^15, rows of sums and budgets of 2^31 - 2^16.
  */
 
 /*
@@ -459,7 +460,9 @@ int pkv_evict_pages(void *stream, const pkv_layout *layout, void *const *pools, 
  * finite, or whose logits hold +inf, NaN or nothing but -inf, has none, and a
  * logit of -inf is none.  Where there are too few, the rest is -inf, at the lowest
  * pairs that are no candidates.  Candidates of different beams are compared in 64
- * bits, those of one beam by their logits.
+ * bits, by log-sum-exps joined in 64 bits from float32 exponentials and partial sums
+ * (off by up to 2^-21, and 2^-23 times the softmax's mean of max - x), those of one beam
+ * by their logits.
  *
  *  logits     : [groups][beams][vocab], kind 0 = bf16, 1 = f16, 2 = f32; strides in
  *               elements, each row's tokens adjacent

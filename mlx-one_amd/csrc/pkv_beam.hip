@@ -8,8 +8,11 @@
 // hold -inf and the lowest pairs that are no candidates.
 //
 // Which of two beams' tokens comes first hangs on the last digits of their
-// log-sum-exps, so those, and the comparison, are in 64 bits; within a beam the
-// logits themselves give the order.
+// log-sum-exps, so those are joined, and candidates compared, in 64 bits.  What they are
+// joined from is float32: hardware exponentials and each thread's sum of 32 or 64 of them,
+// which leaves a log-sum-exp off by up to 2^-21, and 2^-23 times the mean of max - x under
+// the softmax; closer beams come in the order of these sums.  Within a beam the logits
+// themselves give the order.
 //
 // One launch reads the logits, in chunks of a row held in registers: the chunk's
 // maximum and sum of exponentials, and its `count` best tokens.  Each wave finds
@@ -34,7 +37,7 @@ constexpr int kMergeList = 512;  // candidates of a group in LDS
 constexpr int kHeld = 16384;  // candidates of a group whose order is kept in LDS
 constexpr int kList = 256;  // candidates in LDS, per wave
 
-// Order of float32 as unsigned numbers; -inf and below (nothing) as 0.
+// Order of float32 as unsigned numbers (none is 0, which callers take for nothing).
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.0f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;

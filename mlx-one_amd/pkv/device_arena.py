@@ -208,7 +208,9 @@ class DevicePageArena:
         """Each slot becomes a copy of what its source held before the call, all at
         once, sharing its pages; pages that no slot holds any more are freed.  A
         beam step's bookkeeping: sources are the parents' slots, and may repeat
-        (``fork`` into slots that need not be empty)."""
+        (``fork`` into slots that need not be empty).  Lists update the host
+        length mirror; after device tensors ``sync_lengths`` does.  At most 4096
+        slots a call."""
         slots_d, host_slots = self._slots(slots)
         count = int(slots_d.numel())
         sources_d, host_sources = self._ints(sources, count)
@@ -238,7 +240,9 @@ class DevicePageArena:
         """Keep, from now on, the attention weight that every cached token draws
         (``mass [layers, slots, HK, tokens]`` float32, added to by each step's
         ``attend``): what ``evict`` goes by.  Call it before steps are captured.
-        The weight of a step that is rolled back stays counted."""
+        The weight of a step that is rolled back stays counted.  The sums take
+        4 bytes a layer, slot, KV head and token of ``max_tokens``, and a step up to
+        2 GiB of scratch for its scores; neither is part of a page budget."""
         if self.mass is None:
             self.mass = torch.zeros((len(self.pools), self.max_slots, self.fmt.num_kv_heads,
                                      self.max_pages * self.page_tokens), device=self.device)
@@ -273,7 +277,9 @@ class DevicePageArena:
         pages are taken before the old ones go; slots without room for them stay
         as they are and the arena records ``OUT_OF_PAGES``, which host lists of
         slots raise.  ``spare``: empty slots to work in, one at least (default:
-        free ones); the slots are cut as many at a time as there are."""
+        free ones); the slots are cut as many at a time as there are, and as the
+        kernels take (4096).  A call that is refused or fails leaves no spare
+        slot with pages."""
         if self.mass is None:
             raise ValueError("eviction goes by the attention weight: call track_mass() first")
         if sinks < 0 or recent < 0:
