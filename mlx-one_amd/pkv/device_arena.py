@@ -225,14 +225,17 @@ class DevicePageArena:
             for s, n in zip(host_slots, held):
                 self.lengths[s] = n
 
-    def _reorder_pages(self, slots_d, sources_d):
+    def _reorder_scratch(self, count):
+        return ops._scratch(nat.load().pkv_arena_reorder_workspace_bytes(count, self.max_pages),
+                            self.device, "arena reorder")
+
+    def _reorder_pages(self, slots_d, sources_d, workspace=None):
         count = int(slots_d.numel())
-        lib = nat.load()
-        workspace = ops._scratch(lib.pkv_arena_reorder_workspace_bytes(count, self.max_pages),
-                                 self.device, "arena reorder")
-        code = lib.pkv_arena_reorder(nat.stream_handle(self.device), nat.ptr(self.state),
-                                     *self._common(), nat.ptr(slots_d), nat.ptr(sources_d), count,
-                                     nat.ptr(workspace), workspace.numel())
+        if workspace is None:
+            workspace = self._reorder_scratch(count)
+        code = nat.load().pkv_arena_reorder(
+            nat.stream_handle(self.device), nat.ptr(self.state), *self._common(), nat.ptr(slots_d),
+            nat.ptr(sources_d), count, nat.ptr(workspace), workspace.numel())
         nat.check(code, "arena reorder")
 
     # -- eviction by attention weight -----------------------------------------------------
@@ -241,8 +244,8 @@ class DevicePageArena:
         (``mass [layers, slots, HK, tokens]`` float32, added to by each step's
         ``attend``): what ``evict`` goes by.  Call it before steps are captured.
         The weight of a step that is rolled back stays counted.  The sums take
-        4 bytes a layer, slot, KV head and token of ``max_tokens``, and a step up to
-        2 GiB of scratch for its scores; neither is part of a page budget."""
+        4 bytes a layer, slot, KV head and token of ``max_tokens``, and a decode step
+        up to 2 GiB of scratch for its scores; neither is part of a page budget."""
         if self.mass is None:
             self.mass = torch.zeros((len(self.pools), self.max_slots, self.fmt.num_kv_heads,
                                      self.max_pages * self.page_tokens), device=self.device)
@@ -356,11 +359,13 @@ class DevicePageArena:
             rows, sources = torch.where(cut, slots_d, -1), torch.where(cut, spare_d, slots_d)
             table, places = self.table[at], self._places(slots_d)
             evicted = self.evicted[places] + torch.where(cut, lens - kept_lens, 0)
+            workspace = self._reorder_scratch(int(slots_d.numel()))
+            # (once the sums move nothing is allocated any more)
             kept, n, _ = ops.evict_select(self.mass, lens, keep_d, max_keep=max_keep, sinks=sinks,
                                           recent=recent, rows=rows, new_mass=self.mass)
             ops.evict_pages(self.fmt, self.pools, kept, n, table, res.table)
             self.evicted[places] = evicted
-            self._reorder_pages(slots_d, sources)     # the sums have moved
+            self._reorder_pages(slots_d, sources, workspace)   # the sums have moved
         finally:
             # (whatever failed on the way: the spare slots are empty again)
             self.rollback(spare_d, none)

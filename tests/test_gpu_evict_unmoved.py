@@ -109,3 +109,21 @@ def test_a_failure_after_some_slots_were_cut(monkeypatch):
     assert arena.lengths[a] == 40 and arena.lengths[b] == 90
     assert arena.lengths == arena.lens.tolist() and arena.evicted[[a, b]].tolist() == [50, 0]
     model.check([a, b])
+
+
+@pytest.mark.parametrize("call", ["_scratch", "evict_select"])
+def test_no_memory_for_a_call_leaves_the_sums(call, monkeypatch):
+    """Memory is taken before the sums move: without any, nothing has."""
+    from pkv import ops
+
+    arena, a, b, model = _held()
+    free, mass = arena.status()[0], arena.mass.clone()
+
+    def fails(*_a, **_k):
+        raise MemoryError(call)
+
+    with monkeypatch.context() as patch:
+        patch.setattr(ops, call, fails)
+        with pytest.raises(MemoryError):
+            arena.evict([a, b], 40)
+    _unchanged(arena, a, b, model, free, mass)
