@@ -502,6 +502,44 @@ int pkv_arena_reorder(void *stream, void *state, int32_t capacity_pages, int32_t
                       int64_t workspace_bytes);
 int64_t pkv_arena_reorder_workspace_bytes(int32_t count, int32_t max_pages);
 
+/*
+ * ---- a serving step -----------------------------------------------------------------
+ *
+ * From the fused projection to the attention output, for rows packed over sequences
+ * and for sequences that share a prefix.
+ */
+
+/*
+ * Rotate the q and k heads of a fused projection and store k and v into the sequences'
+ * pages, in one pass.  A row of qkv holds num_heads + 2 * num_kv_heads heads (q, k, v) of
+ * head_dim elements; rows are row_stride elements apart.  Rows come packed: sequence b has
+ * rows row_starts[b] .. row_starts[b+1] - 1 (rising), or, with row_starts NULL, padded: rows
+ * b * tokens .. + widths[b] - 1 (widths NULL: tokens).  Rows of no sequence are neither read nor
+ * written.  Row i of a sequence is appended at start_pos[b] + i as pkv_append_quantize
+ * appends it (a position without a mapped page is dropped, its rotated rows still come out;
+ * a sequence whose start is negative has no rows).
+ *
+ * Pair i < num_freqs is (x[i], x[i + num_freqs]), turned by positions[axis[i]][row] * inv_freq[i]
+ * (an angle in 64 bits, cos and sin rounded once to 32); the head's elements from
+ * 2 * num_freqs on pass.  positions NULL: the cache position on the one axis.  The rotated
+ * values are rounded once to float_kind, and k is stored from that: the pages hold bit
+ * for bit what pkv_append_quantize makes of the k and v that come out.
+ * Replaces the rotation, split and append around PagedBatchCache.attend
+ * (src/mlx_one/models/shared/transformer.py:32-90, :146-184; engine/paged.py:103-154) for
+ * packed rows; several axes and packed rows have no counterpart in the reference.
+ *
+ *  positions : [num_axes][rows] int32 (num_axes 1..8), or NULL
+ *  axis      : [num_freqs] int32 in 0 .. num_axes - 1, or NULL for axis 0
+ *  q         : packed [rows][num_heads][head_dim]; padded [batch][num_heads][tokens][head_dim]
+ *  k, v      : the same with num_kv_heads, or both NULL
+ */
+int pkv_rope_append(void *stream, const pkv_layout *layout, void *pool, int64_t num_pages, const void *qkv,
+                    int64_t row_stride, int32_t rows, int32_t num_heads, int32_t batch, int32_t tokens,
+                    const int32_t *row_starts, const int32_t *widths, const int32_t *start_pos,
+                    const int32_t *positions, int32_t num_axes, const float *inv_freq, int32_t num_freqs,
+                    const int32_t *axis, const int32_t *block_table, int32_t max_pages, void *q, void *k,
+                    void *v);
+
 #ifdef __cplusplus
 }
 #endif

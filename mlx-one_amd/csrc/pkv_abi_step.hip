@@ -1,0 +1,93 @@
+// pkv_abi_step.hip -- extern "C" entry points of a serving step's operators (declared in
+// include/pkv.h): rotation with append, attention over packed prompts, attention over
+// shared prefixes.  Validation and errors as in pkv_abi.hip; no entry point lets an
+// exception out.
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "pkv.h"
+
+#include "pkv_error.h"
+#include "pkv_step.h"
+
+namespace {
+
+using pkv::check_launch;
+using pkv::fail;
+using pkv::geometry;
+
+// An entry point's body, with what it throws (no memory for an error text) as a
+// status, or as a size of -1.
+template <typename F>
+auto guarded(F body) noexcept -> decltype(body()) {
+  try {
+    return body();
+  } catch (...) {
+    return sizeof(body()) == sizeof(int64_t) ? -1 : PKV_LAUNCH_FAILED;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int pkv_rope_append(void *stream, const pkv_layout *layout, void *pool, int64_t num_pages, const void *qkv,
+                    int64_t row_stride, int32_t rows, int32_t num_heads, int32_t batch, int32_t tokens,
+                    const int32_t *row_starts, const int32_t *widths, const int32_t *start_pos,
+                    const int32_t *positions, int32_t num_axes, const float *inv_freq, int32_t num_freqs,
+                    const int32_t *axis, const int32_t *block_table, int32_t max_pages, void *q, void *k, void *v) {
+  return guarded([&]() -> int {
+    pkv_geometry g;
+    if (int rc = geometry(layout, &g)) return rc;
+    if (rows < 0 || batch < 0 || tokens < 0 || num_heads < 1 || num_pages < 0 || max_pages < 0)
+      return fail(PKV_INVALID_ARGUMENT, "invalid rotation and append shape");
+    if (num_freqs < 0 || 2 * (int64_t)num_freqs > g.dim)
+      return fail(PKV_INVALID_ARGUMENT, "at most head_dim / 2 frequencies");
+    if (num_axes < 1 || num_axes > 8) return fail(PKV_INVALID_ARGUMENT, "1 to 8 position axes");
+    if (axis && !positions) return fail(PKV_INVALID_ARGUMENT, "axes need positions");
+    if (row_starts && widths) return fail(PKV_INVALID_ARGUMENT, "packed rows take no widths");
+    if (!row_starts && (int64_t)batch * tokens != rows)
+      return fail(PKV_INVALID_ARGUMENT, "rows of a padded batch must be batch * tokens");
+    const int64_t all = (int64_t)num_heads + 2 * (int64_t)g.hk;
+    if (all > 65536) return fail(PKV_UNSUPPORTED, "at most 65536 heads of a row");
+    if (row_stride < all * g.dim) return fail(PKV_INVALID_ARGUMENT, "rows overlap: row_stride is below the row's elements");
+    if (row_stride > ((int64_t)1 << 40)) return fail(PKV_UNSUPPORTED, "row strides of at most 2^40 elements");
+    if (rows > (1 << 23) || batch > (1 << 20)) return fail(PKV_UNSUPPORTED, "at most 2^23 rows and 2^20 sequences");
+    if ((int64_t)rows * ((all + 3) / 4) > ((int64_t)1 << 23) * 256)
+      return fail(PKV_UNSUPPORTED, "at most 2^33 (row, head) pairs");
+    if ((int64_t)max_pages * g.page > INT32_MAX) return fail(PKV_INVALID_ARGUMENT, "block table too wide");
+    if (rows == 0 || batch == 0) return PKV_OK;
+    if (!qkv || !start_pos || !q || (num_freqs > 0 && !inv_freq) || (num_pages > 0 && !pool) ||
+        (max_pages > 0 && !block_table))
+      return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
+    if (!k != !v) return fail(PKV_INVALID_ARGUMENT, "k and v come out together");
+    pkv::RopeAppendArgs a;
+    a.g = pkv::to_geo(g);
+    a.pool = (uint8_t *)pool;
+    a.num_pages = num_pages;
+    a.qkv = (const uint16_t *)qkv;
+    a.row_stride = row_stride;
+    a.rows = rows;
+    a.heads = num_heads;
+    a.batch = batch;
+    a.tokens = tokens;
+    a.row_starts = row_starts;
+    a.widths = widths;
+    a.start_pos = start_pos;
+    a.positions = positions;
+    a.axis = axis;
+    a.axes = num_axes;
+    a.inv_freq = inv_freq;
+    a.half = num_freqs;
+    a.table = block_table;
+    a.max_pages = max_pages;
+    a.q = (uint16_t *)q;
+    a.k = (uint16_t *)k;
+    a.v = (uint16_t *)v;
+    return check_launch(pkv::launch_rope_append((hipStream_t)stream, a), "rotation and append launch");
+  });
+}
+
+}  // extern "C"

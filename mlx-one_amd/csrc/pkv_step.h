@@ -1,0 +1,29 @@
+// pkv_step.h -- argument structs and launchers of a serving step's operators: rotation
+// with append, attention over packed prompts, attention over shared prefixes.
+#pragma once
+#include "pkv_launch.h"
+
+namespace pkv {
+
+struct RopeAppendArgs {
+  Geo g;
+  uint8_t *pool;
+  int64_t num_pages;
+  const uint16_t *qkv;  // rows of heads + 2 * hk heads of dim elements, row_stride elements apart
+  int64_t row_stride;
+  int rows, heads, batch;
+  int tokens;  // row_starts NULL: sequence b has rows b * tokens ...
+  const int32_t *row_starts, *widths, *start_pos;
+  const int32_t *positions;  // [axes][rows], or NULL
+  const int32_t *axis;       // [half], or NULL for axis 0
+  int axes;
+  const float *inv_freq;  // [half]
+  int half;               // rotated pairs of a head
+  const int32_t *table;
+  int max_pages;
+  uint16_t *q, *k, *v;  // packed [rows][heads][dim], or by sequence [batch][heads][tokens][dim]; k, v may be NULL
+};
+
+hipError_t launch_rope_append(hipStream_t stream, const RopeAppendArgs &a);
+
+}  // namespace pkv

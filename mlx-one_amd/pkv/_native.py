@@ -81,6 +81,9 @@ SIGNATURES = {
     "pkv_arena_reorder": ([_c_p, _c_p, _i32, _i32, _c_p, _i32, _i32, _c_p, _c_p, _c_p, _i32,
                            _c_p, _i64], ctypes.c_int),
     "pkv_arena_reorder_workspace_bytes": ([_i32, _i32], _i64),
+    "pkv_rope_append": ([_c_p, _LP, _c_p, _i64, _c_p, _i64, _i32, _i32, _i32, _i32, _c_p, _c_p,
+                         _c_p, _c_p, _i32, _c_p, _i32, _c_p, _c_p, _i32, _c_p, _c_p, _c_p],
+                        ctypes.c_int),
 }
 
 

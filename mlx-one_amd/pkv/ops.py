@@ -740,3 +740,109 @@ def reorder_rows(state, targets, sources, *, dim=0):
     _launch(device, "reorder", nat.load().pkv_reorder_rows, state.data_ptr(), outer, num_rows,
             row_bytes, to.data_ptr(), source.data_ptr(), count)
     return state
+
+
+# ---- a serving step ------------------------------------------------------------------
+
+
+def rope_append(fmt: PageFormat, pool, qkv, block_table, start_pos, inv_freq, heads, *, row_starts=None,
+                widths=None, positions=None, axes=None, with_kv=False, out=None):
+    """Rotate the q and k heads of a fused projection and store k and v into the
+    sequences' pages, in one pass; returns the rotated q.
+
+    ``qkv`` holds ``heads`` query heads, then k and v of the format's KV heads, in rows of
+    ``(heads + 2 * HK) * D`` elements: packed ``[T, width]`` with ``row_starts [B + 1]`` (sequence
+    b has rows ``row_starts[b]`` to ``row_starts[b + 1] - 1``), or padded ``[B, N, width]`` with
+    ``widths [B]`` (default: N).  Row i of sequence b is appended at ``start_pos[b] + i``.
+
+    The first ``2 * len(inv_freq)`` elements of a head are rotated (rotate-half pairs), by the
+    cache position or by ``positions``, ``[T]`` (padded ``[B, N]``); positions on several axes,
+    ``[A, T]`` (``[A, B, N]``), go with ``axes [len(inv_freq)]``, the axis of each frequency.  Angles
+    are in 64 bits.  The pages equal ``append_quantize``'s of the k and v that come out, bit
+    for bit.
+
+    Returns q ``[T, heads, D]`` (padded ``[B, heads, N, D]``); ``with_kv`` also k and v, with HK
+    heads.  ``out``: a tensor, or with ``with_kv`` three, that take them; rows of no
+    sequence are left as they are there.
+    """
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() != (3 if row_starts is None else 2):
+        raise ValueError("qkv must be packed [T, width] with row_starts, or padded [B, N, width]")
+    _check_float(qkv, fmt, "qkv")
+    device = qkv.device
+    _check_dense(pool, torch.uint8, device, "pool", 2)
+    if pool.shape[1] != fmt.page_bytes:
+        raise ValueError("the pool's pages are not of this format")
+    kv_heads, dim = fmt.num_kv_heads, fmt.head_dim
+    width = qkv.shape[-1]
+    if heads < 1 or width != (heads + 2 * kv_heads) * dim:
+        raise ValueError("qkv width is not (heads + 2 * kv_heads) * head_dim")
+    if qkv.stride(-1) != 1 or qkv.stride(-2) < width or (
+            qkv.dim() == 3 and qkv.stride(0) != qkv.shape[1] * qkv.stride(1)):
+        qkv = qkv.contiguous()
+    starts = _i32(start_pos, device)
+    batch = starts.numel()
+    # (the tensors are named so that they live until the launch)
+    if row_starts is None:
+        if widths is not None:
+            widths, widths_at = _address(widths, device, batch, "widths")
+        else:
+            widths_at = None
+        batch_rows, tokens = qkv.shape[:2]
+        if batch_rows != batch:
+            raise ValueError("start_pos must hold a value per sequence")
+        rows, first_at, lead = batch * tokens, None, (batch, tokens)
+        shape = (lambda n: (batch, n, tokens, dim))
+    else:
+        if widths is not None:
+            raise ValueError("packed rows take no widths")
+        rows, tokens, widths_at = qkv.shape[0], 0, None
+        first, first_at = _address(row_starts, device, batch + 1, "row_starts")
+        lead = (rows,)
+        shape = (lambda n: (rows, n, dim))
+    table = _i32(block_table, device)
+    if table.dim() != 2 or table.shape[0] != batch:
+        raise ValueError("block table must be [batch, max_pages]")
+    _check_dense(inv_freq, torch.float32, device, "inv_freq", 1)
+    half = inv_freq.shape[0]
+    num_axes, positions_at, axis_at = 1, None, None
+    if positions is not None:
+        places = _i32(positions, device)
+        if axes is not None and places.dim() == len(lead) + 1:
+            num_axes = places.shape[0]
+        if tuple(places.shape) != ((num_axes,) if axes is not None else ()) + lead:
+            raise ValueError("positions must be one per row, or with axes one per axis and row")
+        positions_at = places.data_ptr()
+    if axes is not None:
+        if positions is None:
+            raise ValueError("axes need positions")
+        axis, axis_at = _address(axes, device, half, "axes")
+    outs = list(out) if with_kv and out is not None else [out]
+    counts = (heads, kv_heads, kv_heads) if with_kv else (heads,)
+    if out is None:
+        outs = [torch.empty(shape(n), dtype=qkv.dtype, device=device) for n in counts]
+    elif len(outs) != len(counts):
+        raise ValueError("out must hold q, k and v")
+    else:
+        for t, n in zip(outs, counts):
+            if not _dense(t, qkv.dtype, device, len(shape(n))) or tuple(t.shape) != shape(n):
+                raise ValueError(f"out must be contiguous {shape(n)} tensors of qkv's dtype and device")
+    addresses = [t.data_ptr() for t in outs] + [None] * (3 - len(outs))
+    _launch(device, "rotation and append", nat.load().pkv_rope_append, fmt.c_layout, pool.data_ptr(),
+            pool.shape[0], qkv.data_ptr(), qkv.stride(-2), rows, heads, batch, tokens, first_at, widths_at,
+            starts.data_ptr(), positions_at, num_axes, inv_freq.data_ptr(), half, axis_at,
+            table.data_ptr(), table.shape[1], *addresses)
+    return tuple(outs) if with_kv else outs[0]
+
+
+def rope_axes(sections, device="cuda", *, interleaved=False):
+    """The axis of each frequency for ``rope_append``: runs of ``sections[a]`` frequencies for axis
+    a, or, interleaved, the axes in turn, each as long as it has any of its ``sections[a]``
+    left."""
+    counts = [int(n) for n in sections]
+    if not counts or any(n < 0 for n in counts):
+        raise ValueError("sections must be counts of frequencies")
+    if interleaved:
+        order = [a for i in range(max(counts)) for a, n in enumerate(counts) if i < n]
+    else:
+        order = [a for a, n in enumerate(counts) for _ in range(n)]
+    return torch.tensor(order, dtype=torch.int32, device=device)

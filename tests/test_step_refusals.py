@@ -1,0 +1,51 @@
+"""CPU: what the operators of a serving step refuse, before any launch."""
+
+from __future__ import annotations
+
+import pytest
+
+from pkv import _native as nat
+
+torch = pytest.importorskip("torch")
+
+FAKE = 4096   # never dereferenced: the call fails or returns first
+
+
+def _layout(**kw):
+    base = dict(num_kv_heads=8, head_dim=128, page_tokens=16, bits=8, group_size=64, float_kind=0)
+    base.update(kw)
+    return nat.Layout(*base.values())
+
+
+def _rope(**kw):
+    a = dict(stream=None, layout=_layout(), pool=FAKE, num_pages=10, qkv=FAKE, stride=48 * 128, rows=6, heads=32,
+             batch=2, tokens=0, row_starts=FAKE, widths=None, start_pos=FAKE, positions=None, axes=1, inv_freq=FAKE,
+             freqs=64, axis=None, table=FAKE, max_pages=4, q=FAKE, k=None, v=None)
+    a.update(kw)
+    return nat.load().pkv_rope_append(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(layout=_layout(bits=5)), 2), (dict(heads=0), 1), (dict(rows=-1), 1), (dict(batch=-1), 1),
+    (dict(freqs=65), 1), (dict(freqs=-1), 1), (dict(axes=0), 1), (dict(axes=9), 1), (dict(axis=FAKE), 1),
+    (dict(widths=FAKE), 1), (dict(row_starts=None, tokens=2), 1), (dict(stride=48 * 128 - 1), 1),
+    (dict(stride=1 << 41), 2), (dict(rows=(1 << 23) + 1), 2), (dict(batch=(1 << 20) + 1), 2),
+    (dict(heads=1 << 17, stride=1 << 32), 2), (dict(max_pages=1 << 28), 1), (dict(qkv=None), 1), (dict(q=None), 1),
+    (dict(start_pos=None), 1), (dict(inv_freq=None), 1), (dict(pool=None), 1), (dict(table=None), 1),
+    (dict(k=FAKE), 1), (dict(v=FAKE), 1)])
+def test_rope_append(kw, code):
+    assert _rope(**kw) == code and nat.last_error()
+
+
+def test_calls_with_nothing_to_do_return():
+    assert _rope(rows=0) == 0 and _rope(batch=0) == 0 and _rope(rows=0, batch=0, qkv=None, q=None) == 0
+
+
+def test_sections():
+    from pkv import ops
+
+    assert ops.rope_axes((2, 3, 1), "cpu").tolist() == [0, 0, 1, 1, 1, 2]
+    assert ops.rope_axes((2, 3, 1), "cpu", interleaved=True).tolist() == [0, 1, 2, 0, 1, 1]
+    for bad in ((), (1, -1)):
+        with pytest.raises(ValueError):
+            ops.rope_axes(bad, "cpu")
