@@ -540,6 +540,27 @@ int pkv_rope_append(void *stream, const pkv_layout *layout, void *pool, int64_t 
                     const int32_t *axis, const int32_t *block_table, int32_t max_pages, void *q, void *k,
                     void *v);
 
+/*
+ * Causal attention within every sequence of packed rows: row i of sequence b (rows
+ * row_starts[b] .. row_starts[b+1] - 1, rising) attends rows row_starts[b] .. i of keys and
+ * values, query head h those of KV head h / (num_heads / num_kv_heads).  Rows of no sequence
+ * are neither read nor written.  Sums and softmax in float32; the weights are rounded
+ * once to float_kind, as operands.  What a later row holds, infinities and NaN among it,
+ * changes nothing for an earlier one.  Replaces the padded attention of a prompt's first
+ * pass (src/mlx_one/engine/paged_attention.py:127-206 over pages just written) for prompts
+ * whose keys and values are at hand.
+ *
+ *  queries        : rows of num_heads * head_dim elements, q_stride elements apart
+ *  keys, values   : rows of num_kv_heads * head_dim elements
+ *                   (strides multiples of 8, at most 2^23; tensors 16-byte aligned)
+ *  head_dim       : a multiple of 8, at most 256
+ *  out            : [rows][num_heads][head_dim]
+ */
+int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, const void *keys, int64_t k_stride,
+                         const void *values, int64_t v_stride, int32_t float_kind, int32_t rows, int32_t batch,
+                         const int32_t *row_starts, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                         float scale, void *out);
+
 #ifdef __cplusplus
 }
 #endif

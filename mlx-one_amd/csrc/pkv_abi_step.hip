@@ -90,4 +90,50 @@ int pkv_rope_append(void *stream, const pkv_layout *layout, void *pool, int64_t 
   });
 }
 
+int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, const void *keys, int64_t k_stride,
+                         const void *values, int64_t v_stride, int32_t float_kind, int32_t rows, int32_t batch,
+                         const int32_t *row_starts, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                         float scale, void *out) {
+  return guarded([&]() -> int {
+    if (float_kind != 0 && float_kind != 1) return fail(PKV_INVALID_ARGUMENT, "float_kind must be 0 or 1");
+    if (rows < 0 || batch < 0 || num_heads < 1 || num_kv_heads < 1 || head_dim < 1)
+      return fail(PKV_INVALID_ARGUMENT, "invalid prompt attention shape");
+    if (num_heads % num_kv_heads) return fail(PKV_INVALID_ARGUMENT, "num_heads must be a multiple of num_kv_heads");
+    if (head_dim > 256 || head_dim % 8)
+      return fail(PKV_UNSUPPORTED, "prompt attention supports head dimensions 8, 16, ... 256");
+    if (!std::isfinite(scale)) return fail(PKV_INVALID_ARGUMENT, "the softmax scale must be finite");
+    if (q_stride < (int64_t)num_heads * head_dim || k_stride < (int64_t)num_kv_heads * head_dim ||
+        v_stride < (int64_t)num_kv_heads * head_dim)
+      return fail(PKV_INVALID_ARGUMENT, "rows overlap: a stride is below its row's elements");
+    if ((q_stride | k_stride | v_stride) % 8) return fail(PKV_INVALID_ARGUMENT, "strides must be multiples of 8 elements");
+    if (std::max(q_stride, std::max(k_stride, v_stride)) > (1 << 23))
+      return fail(PKV_UNSUPPORTED, "strides of at most 2^23 elements");
+    if (rows > (1 << 24) || batch > (1 << 20)) return fail(PKV_UNSUPPORTED, "at most 2^24 rows and 2^20 sequences");
+    if (((int64_t)rows + 63 * (int64_t)std::min(rows, batch)) / 32 * num_heads > (1 << 23))
+      return fail(PKV_UNSUPPORTED, "at most 2^28 (row, head) pairs");
+    if (rows == 0 || batch == 0) return PKV_OK;
+    if (!queries || !keys || !values || !row_starts || !out) return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
+    if (((uintptr_t)queries | (uintptr_t)keys | (uintptr_t)values | (uintptr_t)out) % 16)
+      return fail(PKV_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+    pkv::PromptArgs a;
+    a.q = (const uint16_t *)queries;
+    a.k = (const uint16_t *)keys;
+    a.v = (const uint16_t *)values;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.float_kind = float_kind;
+    a.rows = rows;
+    a.batch = batch;
+    a.heads = num_heads;
+    a.kv_heads = num_kv_heads;
+    a.gqa = num_heads / num_kv_heads;
+    a.dim = head_dim;
+    a.row_starts = row_starts;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.out = (uint16_t *)out;
+    return check_launch(pkv::launch_prompt_attention((hipStream_t)stream, a), "prompt attention launch");
+  });
+}
+
 }  // extern "C"

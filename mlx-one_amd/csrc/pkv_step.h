@@ -26,4 +26,15 @@ struct RopeAppendArgs {
 
 hipError_t launch_rope_append(hipStream_t stream, const RopeAppendArgs &a);
 
+struct PromptArgs {
+  const uint16_t *q, *k, *v;  // rows, stride elements apart; head h at h * dim
+  int64_t q_stride, k_stride, v_stride;
+  int float_kind, rows, batch, heads, kv_heads, gqa, dim;
+  const int32_t *row_starts;
+  float scale_log2;
+  uint16_t *out;  // [rows][heads][dim]
+};
+
+hipError_t launch_prompt_attention(hipStream_t stream, const PromptArgs &a);
+
 }  // namespace pkv

@@ -84,6 +84,8 @@ SIGNATURES = {
     "pkv_rope_append": ([_c_p, _LP, _c_p, _i64, _c_p, _i64, _i32, _i32, _i32, _i32, _c_p, _c_p,
                          _c_p, _c_p, _i32, _c_p, _i32, _c_p, _c_p, _i32, _c_p, _c_p, _c_p],
                         ctypes.c_int),
+    "pkv_prompt_attention": ([_c_p, _c_p, _i64, _c_p, _i64, _c_p, _i64, _i32, _i32, _i32, _c_p,
+                              _i32, _i32, _i32, _f32, _c_p], ctypes.c_int),
 }
 
 

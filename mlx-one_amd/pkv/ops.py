@@ -846,3 +846,56 @@ def rope_axes(sections, device="cuda", *, interleaved=False):
     else:
         order = [a for a, n in enumerate(counts) for _ in range(n)]
     return torch.tensor(order, dtype=torch.int32, device=device)
+
+
+def _packed_rows(t, name):
+    """Packed heads ``[T, heads, D]`` as the kernels read them: heads side by side, rows any
+    multiple of 16 bytes apart (a copy where they are not), and the stride of rows."""
+    _, heads, dim = t.shape
+    if t.shape[0] > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim) or t.stride(0) < heads * dim
+                           or t.stride(0) % 8 or t.stride(0) > 1 << 23 or t.data_ptr() % 16):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, (t.stride(0) if t.shape[0] > 1 else heads * dim)
+
+
+def prompt_attention(q, k, v, row_starts, *, scale, out=None):
+    """Causal attention within every sequence of packed rows.
+
+    ``q [T, H, D]``, ``k`` and ``v [T, HK, D]`` (bfloat16 or float16; views of a fused projection
+    are read where they lie); sequence b is rows ``row_starts[b]`` to ``row_starts[b + 1] - 1``
+    (``row_starts [B + 1]``, rising).  Returns ``[T, H, D]``; rows of no sequence are left as they
+    are in ``out``.  Head dims up to 256; ones that are no multiple of 8 are padded by a copy.
+    """
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype not in FLOAT_KINDS or not t.is_cuda:
+            raise ValueError(f"{name} must be a [T, heads, D] f16/bf16 device tensor")
+    rows, heads, dim = q.shape
+    device = q.device
+    if k.shape != v.shape or k.shape[0] != rows or k.shape[2] != dim:
+        raise ValueError("k and v must be [T, HK, D] of q's rows and head dimension")
+    if any(t.dtype is not q.dtype or t.device != device for t in (k, v)):
+        raise ValueError("q, k and v must be of one dtype and device")
+    kv_heads = k.shape[1]
+    starts = _i32(row_starts, device)
+    if starts.dim() != 1 or starts.numel() < 1:
+        raise ValueError("row_starts must be [batch + 1]")
+    if out is not None and (not _dense(out, q.dtype, device, 3) or out.shape != q.shape):
+        raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
+    result = out
+    if dim % 8:
+        pad = 8 - dim % 8
+        q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
+        out = None
+    if out is None or out.data_ptr() % 16:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        if result is not None:
+            out[..., :dim] = result
+    (q, q_step), (k, k_step), (v, v_step) = (_packed_rows(t, name) for name, t in (("q", q), ("k", k), ("v", v)))
+    _launch(device, "prompt attention", nat.load().pkv_prompt_attention, q.data_ptr(), q_step, k.data_ptr(), k_step,
+            v.data_ptr(), v_step, FLOAT_KINDS[q.dtype], rows, starts.numel() - 1, starts.data_ptr(), heads, kv_heads,
+            q.shape[2], scale, out.data_ptr())
+    if result is None:
+        return out if out.shape[2] == dim else out[..., :dim].contiguous()
+    if result is not out:
+        result.copy_(out[..., :dim])
+    return result

@@ -37,7 +37,26 @@ def test_rope_append(kw, code):
     assert _rope(**kw) == code and nat.last_error()
 
 
+def _prompt(**kw):
+    a = dict(stream=None, q=FAKE, qs=32 * 128, k=FAKE, ks=8 * 128, v=FAKE, vs=8 * 128, kind=0, rows=6, batch=2,
+             row_starts=FAKE, heads=32, kv_heads=8, dim=128, scale=1.0, out=FAKE)
+    a.update(kw)
+    return nat.load().pkv_prompt_attention(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(kind=2), 1), (dict(rows=-1), 1), (dict(batch=-1), 1), (dict(heads=0), 1), (dict(kv_heads=0), 1),
+    (dict(heads=30), 1), (dict(dim=0), 1), (dict(dim=264), 2), (dict(dim=100), 2), (dict(scale=float("inf")), 1),
+    (dict(qs=32 * 128 - 8), 1), (dict(ks=8 * 127), 1), (dict(vs=1000), 1), (dict(ks=8 * 128 + 4), 1),
+    (dict(vs=(1 << 23) + 8), 2), (dict(rows=(1 << 24) + 1), 2), (dict(batch=(1 << 20) + 1), 2),
+    (dict(rows=1 << 24), 2), (dict(q=None), 1), (dict(k=None), 1), (dict(v=None), 1), (dict(out=None), 1),
+    (dict(row_starts=None), 1), (dict(q=FAKE + 8), 1), (dict(out=FAKE + 2), 1)])
+def test_prompt_attention(kw, code):
+    assert _prompt(**kw) == code and nat.last_error()
+
+
 def test_calls_with_nothing_to_do_return():
+    assert _prompt(rows=0) == 0 and _prompt(batch=0) == 0 and _prompt(rows=0, batch=0, q=None, out=None) == 0
     assert _rope(rows=0) == 0 and _rope(batch=0) == 0 and _rope(rows=0, batch=0, qkv=None, q=None) == 0
 
 
