@@ -561,6 +561,36 @@ int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, co
                          const int32_t *row_starts, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                          float scale, void *out);
 
+/*
+ * Attention of decode and verify queries where the sequences of a group hold the same first
+ * tokens (pages that a fork shares, or equal copies): the shared tokens are gone through
+ * once for the group's query rows together, the others once per sequence.  Results are
+ * pkv_paged_attention's, to the rounding of another split and of keys as 16-bit operands,
+ * for every sequence that a group names; the others' rows of out are left as they are.
+ * Group g is sequences members[group_starts[g]] .. members[group_starts[g+1] - 1] (distinct over
+ * the call) and shares its first prefix_lens[g] tokens, read through the first one's block
+ * table as far as that sequence goes; a group of one shares nothing.  At most 32 query rows
+ * per KV head of a sequence (num_queries x num_heads / num_kv_heads; 16 at head_dim >
+ * 128), 1024 members and groups.  The reference has no counterpart (every row of a
+ * batch reads all its pages, src/mlx_one/engine/paged_attention.py:160-206).
+ *
+ *  queries, block_table, seq_lens, q_pos, widths, scale, out: as pkv_paged_attention
+ *  members      : [num_members] int32 sequences (ids out of range are skipped)
+ *  group_starts : [num_groups + 1] int32, rising;  prefix_lens: [num_groups] int32 tokens
+ *  workspace    : pkv_shared_attention_workspace_bytes(...) bytes of device scratch, 16-byte
+ *                 aligned (calls that may overlap need one each); negative for shapes that
+ *                 are refused, by their status
+ */
+int pkv_shared_attention(void *stream, const pkv_layout *layout, const void *pool, int64_t num_pages,
+                         const void *queries, int32_t batch, int32_t num_heads, int32_t num_queries,
+                         const int32_t *block_table, int32_t max_pages, const int32_t *seq_lens,
+                         const int32_t *q_pos, const int32_t *widths, int32_t num_groups,
+                         const int32_t *members, int32_t num_members, const int32_t *group_starts,
+                         const int32_t *prefix_lens, float scale, void *workspace, int64_t workspace_bytes,
+                         void *out);
+int64_t pkv_shared_attention_workspace_bytes(const pkv_layout *layout, int32_t num_heads, int32_t num_queries,
+                                             int32_t num_members, int32_t num_groups);
+
 #ifdef __cplusplus
 }
 #endif

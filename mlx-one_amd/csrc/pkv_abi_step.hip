@@ -29,6 +29,23 @@ auto guarded(F body) noexcept -> decltype(body()) {
   }
 }
 
+int shared_shape(const pkv_layout *layout, int32_t num_heads, int32_t num_queries, int32_t num_members,
+                 int32_t num_groups, pkv_geometry *g) {
+  if (int rc = geometry(layout, g)) return rc;
+  if (num_heads < 1 || num_queries < 1 || num_members < 0 || num_groups < 0)
+    return fail(PKV_INVALID_ARGUMENT, "invalid shared attention shape");
+  if (num_heads % g->hk) return fail(PKV_INVALID_ARGUMENT, "num_heads must be a multiple of num_kv_heads");
+  const int64_t rows = (int64_t)num_queries * (num_heads / g->hk);
+  if (rows > pkv::shared_rows(g->dp))
+    return fail(PKV_UNSUPPORTED, "shared attention serves at most 32 query rows per KV head of a sequence (16 beyond "
+                                 "head dim 128)");
+  if (num_members > pkv::kMaxShared || num_groups > pkv::kMaxShared)
+    return fail(PKV_UNSUPPORTED, "shared attention serves at most 1024 sequences and groups");
+  if ((int64_t)num_members * g->hk > (1 << 16))
+    return fail(PKV_UNSUPPORTED, "at most 65536 (sequence, KV head) pairs");
+  return PKV_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -133,6 +150,64 @@ int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, co
     a.scale_log2 = scale * 1.4426950408889634f;
     a.out = (uint16_t *)out;
     return check_launch(pkv::launch_prompt_attention((hipStream_t)stream, a), "prompt attention launch");
+  });
+}
+
+int64_t pkv_shared_attention_workspace_bytes(const pkv_layout *layout, int32_t num_heads, int32_t num_queries,
+                                             int32_t num_members, int32_t num_groups) {
+  return guarded([&]() -> int64_t {
+    pkv_geometry g;
+    if (int rc = shared_shape(layout, num_heads, num_queries, num_members, num_groups, &g)) return -rc;
+    return pkv::shared_workspace(pkv::to_geo(g), num_members, num_queries * (num_heads / g.hk), num_groups);
+  });
+}
+
+int pkv_shared_attention(void *stream, const pkv_layout *layout, const void *pool, int64_t num_pages,
+                         const void *queries, int32_t batch, int32_t num_heads, int32_t num_queries,
+                         const int32_t *block_table, int32_t max_pages, const int32_t *seq_lens, const int32_t *q_pos,
+                         const int32_t *widths, int32_t num_groups, const int32_t *members, int32_t num_members,
+                         const int32_t *group_starts, const int32_t *prefix_lens, float scale, void *workspace,
+                         int64_t workspace_bytes, void *out) {
+  return guarded([&]() -> int {
+    pkv_geometry g;
+    if (int rc = shared_shape(layout, num_heads, num_queries, num_members, num_groups, &g)) return rc;
+    if (batch < 0 || num_pages < 0 || max_pages < 0) return fail(PKV_INVALID_ARGUMENT, "invalid shared attention shape");
+    if (batch > (1 << 20)) return fail(PKV_UNSUPPORTED, "at most 2^20 sequences");
+    if ((int64_t)max_pages * g.page > INT32_MAX) return fail(PKV_INVALID_ARGUMENT, "block table too wide");
+    if ((int64_t)max_pages * g.page > INT32_MAX - 4096) return fail(PKV_UNSUPPORTED, "block tables of at most 2^31 - 4097 tokens");
+    if (!std::isfinite(scale)) return fail(PKV_INVALID_ARGUMENT, "the softmax scale must be finite");
+    if (batch == 0 || num_members == 0 || num_groups == 0) return PKV_OK;
+    if (!pool || !queries || !block_table || !seq_lens || !members || !group_starts || !prefix_lens || !out)
+      return fail(PKV_INVALID_ARGUMENT, "NULL tensor");
+    if (num_pages < 1 || max_pages < 1) return fail(PKV_INVALID_ARGUMENT, "empty page pool or block table");
+    pkv::SharedArgs a;
+    a.g = pkv::to_geo(g);
+    a.gqa = num_heads / g.hk;
+    a.rows = num_queries * a.gqa;
+    const int64_t need = pkv::shared_workspace(a.g, num_members, a.rows, num_groups);
+    if (!workspace || workspace_bytes < need)
+      return fail(PKV_OUT_OF_MEMORY, "shared attention workspace too small: need " + std::to_string(need) + " bytes");
+    if ((uintptr_t)workspace % 16) return fail(PKV_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
+    a.pool = (const uint8_t *)pool;
+    a.num_pages = num_pages;
+    a.q = (const uint16_t *)queries;
+    a.batch = batch;
+    a.heads = num_heads;
+    a.nq = num_queries;
+    a.table = block_table;
+    a.max_pages = max_pages;
+    a.seq_lens = seq_lens;
+    a.q_pos = q_pos;
+    a.widths = widths;
+    a.scale = scale;
+    a.groups = num_groups;
+    a.count = num_members;
+    a.members = members;
+    a.group_starts = group_starts;
+    a.prefix_lens = prefix_lens;
+    a.workspace = workspace;
+    a.out = (uint16_t *)out;
+    return check_launch(pkv::launch_shared_attention((hipStream_t)stream, a), "shared attention launch");
   });
 }
 

@@ -37,4 +37,26 @@ struct PromptArgs {
 
 hipError_t launch_prompt_attention(hipStream_t stream, const PromptArgs &a);
 
+struct SharedArgs {
+  Geo g;
+  const uint8_t *pool;
+  int64_t num_pages;
+  const uint16_t *q;  // [B][H][nq][D]
+  int batch, heads, nq, gqa, rows;  // rows = nq * gqa per KV head: row r is query r / gqa of head r % gqa
+  const int32_t *table;
+  int max_pages;
+  const int32_t *seq_lens, *q_pos, *widths;
+  float scale;
+  int groups, count;  // members in all groups
+  const int32_t *members, *group_starts, *prefix_lens;
+  void *workspace;
+  uint16_t *out;  // as q
+};
+
+constexpr int kMaxShared = 1024;  // sequences, and groups
+// Query rows per block of the kernel, and the most a sequence may have per KV head.
+constexpr int shared_rows(int dp) { return dp > 128 ? 16 : 32; }
+int64_t shared_workspace(const Geo &g, int batch, int rows, int groups);
+hipError_t launch_shared_attention(hipStream_t stream, const SharedArgs &a);
+
 }  // namespace pkv

@@ -899,3 +899,54 @@ def prompt_attention(q, k, v, row_starts, *, scale, out=None):
     if result is not out:
         result.copy_(out[..., :dim])
     return result
+
+
+def shared_prefix_attention(fmt: PageFormat, pool, queries, block_table, seq_lens, members, group_starts,
+                            prefix_lens, *, scale, q_pos=None, widths=None, workspace=None, out=None):
+    """Attention of ``queries [B, H, Q, D]`` over the paged cache, where the sequences of a
+    group hold the same first tokens: these are gone through once for the group.
+
+    Group g is sequences ``members[group_starts[g]:group_starts[g + 1]]`` (distinct) and shares
+    its first ``prefix_lens[g]`` tokens -- pages that ``fork`` shares, or equal copies.  The other
+    operands and the result are ``paged_attention``'s (at most 32 query rows per KV head, 16
+    beyond head dim 128, 1024 sequences); rows of sequences that no group names are
+    left as they are in ``out``, or zero.
+    """
+    if queries.dim() != 4:
+        raise ValueError("queries must be [B, H, Q, D]")
+    batch, heads, nq, dim = queries.shape
+    if dim != fmt.head_dim:
+        raise ValueError("query head dimension differs from the page layout")
+    _check_float(queries, fmt, "queries")
+    device = queries.device
+    _check_dense(pool, torch.uint8, device, "pool", 2)
+    pages, page_bytes = pool.shape
+    if page_bytes != fmt.page_bytes:
+        raise ValueError("the pool's pages are not of this format")
+    table = _i32(block_table, device)
+    if table.dim() != 2 or table.shape[0] != batch:
+        raise ValueError("block table must be [batch, max_pages]")
+    lens = _per_row(seq_lens, device, batch, "seq_lens")
+    # (the tensors are named so that they live until the launch)
+    positions, positions_at = _address(q_pos, device, batch * nq, "q_pos")
+    live, live_at = _address(widths, device, batch, "widths")
+    _distinct(members, "members")
+    member = _i32(members, device)
+    count = member.numel()
+    starts, prefix = _i32(group_starts, device), _i32(prefix_lens, device)
+    groups = prefix.numel()
+    if starts.numel() != groups + 1:
+        raise ValueError("group_starts must hold a value per group and the end")
+    queries = queries.contiguous()
+    if out is None:
+        out = (torch.empty if count == batch else torch.zeros)(queries.shape, dtype=queries.dtype, device=device)
+    elif not _dense(out, queries.dtype, device, 4) or out.shape != queries.shape:
+        raise ValueError("out must be a contiguous tensor of the queries' shape, dtype and device")
+    lib, layout = nat.load(), fmt.c_layout
+    workspace = _scratch(lib.pkv_shared_attention_workspace_bytes(layout, heads, nq, count, groups), device,
+                         "shared attention", workspace)
+    _launch(device, "shared attention", lib.pkv_shared_attention, layout, pool.data_ptr(), pages, queries.data_ptr(),
+            batch, heads, nq, table.data_ptr(), table.shape[1], lens.data_ptr(), positions_at, live_at, groups,
+            member.data_ptr(), count, starts.data_ptr(), prefix.data_ptr(), scale, workspace.data_ptr(),
+            workspace.numel(), out.data_ptr())
+    return out

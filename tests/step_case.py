@@ -72,3 +72,56 @@ def attention_bound(want, weight, terms, scale, dtype, *, dim, tokens, operand, 
     h = half_step(dtype)
     inner = weight * rel
     return inner * (1 + h) + np.abs(want) * h + torch.finfo(dtype).smallest_normal * h
+
+
+def side64(fmt, pool, ids, values):
+    """K or V of pages ``ids`` as ``[HK, pages * page_tokens, D]`` float64."""
+    import torch
+
+    from cache_ops_case import _dequantized
+    from pkv import ops
+
+    ids = torch.as_tensor(ids, dtype=torch.int32, device="cuda")
+    parts = ops.gather_pages(fmt, pool, ids)
+    if fmt.quantized:
+        x, _ = _dequantized(*(parts[3:] if values else parts[:3]), fmt.bits, fmt.group_size, fmt.head_dim)
+    else:
+        x = parts[int(values)].double().cpu().numpy()
+    return x.transpose(1, 0, 2, 3).reshape(fmt.num_kv_heads, -1, fmt.head_dim)
+
+
+def paged64(fmt, pool, table, lens, queries, scale, *, q_pos=None, widths=None):
+    """``(out, bound)`` ``[B, H, Q, D]``: paged attention in 64 bits over the pages' values, and
+    the error of a kernel whose keys, values and weights of quantized pages are rounded to
+    float16 operands (of float pages: the keys and values as they are, bfloat16 weights to
+    twice their bits)."""
+    import torch
+
+    q = queries.double().cpu().numpy()
+    table = table.cpu().numpy()
+    batch, heads, nq, dim = q.shape
+    gqa = heads // fmt.num_kv_heads
+    half = half_step(torch.float16)
+    key = half if fmt.quantized else 0.0
+    operand = half if fmt.quantized or fmt.dtype is torch.float16 else half_step(torch.bfloat16) ** 2
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(batch):
+        length = min(int(lens[b]), table.shape[1] * fmt.page_tokens)
+        pages = -(-max(length, 0) // fmt.page_tokens)
+        mapped = (table[b, :pages] >= 0) & (table[b, :pages] < pool.shape[0])
+        if length <= 0 or not mapped.any():
+            continue
+        ids = np.where(mapped, table[b, :pages], 0)
+        there = np.repeat(mapped, fmt.page_tokens)[:length]
+        k, v = (side64(fmt, pool, ids, s)[:, :length][:, there] for s in (False, True))
+        w = nq if widths is None else int(widths[b])
+        for i in range(min(w, nq)):
+            pos = int(lens[b]) - w + i if q_pos is None else int(q_pos[b][i])
+            sees = int(there[:max(min(pos + 1, length), 0)].sum())
+            for h in range(heads):
+                with np.errstate(invalid="ignore", over="ignore"):
+                    o, weight, terms = attention64(q[b, h, i:i + 1], k[h // gqa], v[h // gqa], np.array([sees]), scale)
+                out[b, h, i] = o[0]
+                bound[b, h, i] = attention_bound(o, weight, terms, scale, fmt.dtype, dim=dim, tokens=length,
+                                                 operand=operand, key=key)[0]
+    return out, bound

@@ -55,7 +55,34 @@ def test_prompt_attention(kw, code):
     assert _prompt(**kw) == code and nat.last_error()
 
 
+def _shared(**kw):
+    a = dict(stream=None, layout=_layout(), pool=FAKE, num_pages=10, queries=FAKE, batch=2, heads=32, nq=1,
+             table=FAKE, max_pages=4, lens=FAKE, q_pos=None, widths=None, groups=1, members=FAKE, count=2,
+             starts=FAKE, prefix=FAKE, scale=1.0, ws=FAKE, ws_bytes=1 << 40, out=FAKE)
+    a.update(kw)
+    return nat.load().pkv_shared_attention(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(layout=_layout(bits=5)), 2), (dict(heads=30), 1), (dict(heads=0), 1), (dict(nq=0), 1), (dict(nq=9), 2),
+    (dict(nq=5, layout=_layout(head_dim=256)), 2), (dict(batch=-1), 1), (dict(groups=-1), 1), (dict(count=-1), 1),
+    (dict(groups=1025), 2), (dict(count=1025), 2), (dict(batch=(1 << 20) + 1), 2), (dict(max_pages=1 << 28), 1),
+    (dict(scale=float("nan")), 1), (dict(pool=None), 1), (dict(queries=None), 1), (dict(table=None), 1),
+    (dict(lens=None), 1), (dict(members=None), 1), (dict(starts=None), 1), (dict(prefix=None), 1), (dict(out=None), 1),
+    (dict(num_pages=0), 1), (dict(max_pages=0), 1), (dict(ws=None), 3), (dict(ws_bytes=100), 3), (dict(ws=FAKE + 8), 1),
+    (dict(heads=512, layout=_layout(num_kv_heads=512), count=1024), 2)])
+def test_shared_attention(kw, code):
+    assert _shared(**kw) == code and nat.last_error()
+
+
+def test_shared_workspace():
+    size = nat.load().pkv_shared_attention_workspace_bytes
+    assert size(_layout(), 32, 1, 32, 1) > 0 and size(_layout(), 32, 1, 0, 0) > 0
+    assert size(_layout(), 30, 1, 32, 1) == -1 and size(_layout(), 32, 9, 32, 1) == -2
+
+
 def test_calls_with_nothing_to_do_return():
+    assert _shared(batch=0) == 0 and _shared(count=0) == 0 and _shared(groups=0) == 0
     assert _prompt(rows=0) == 0 and _prompt(batch=0) == 0 and _prompt(rows=0, batch=0, q=None, out=None) == 0
     assert _rope(rows=0) == 0 and _rope(batch=0) == 0 and _rope(rows=0, batch=0, qkv=None, q=None) == 0
 
