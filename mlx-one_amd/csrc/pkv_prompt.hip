@@ -5,8 +5,8 @@
 // A chunk is 32 consecutive queries of one head; the chunks of a (sequence, KV head) are
 // ordered by position, then head, and a workgroup of four waves takes 4 * QB consecutive
 // ones, a wave QB: with a few heads per KV head a workgroup's chunks end at nearly the same
-// key.  Keys come in stages of 64, K and V copied straight to LDS in rows (global_load_lds),
-// NBUF - 1 stages ahead.
+// key.  Keys come in stages of 64 (32 beyond head dim 128), K and V copied straight to LDS
+// in rows (global_load_lds), a stage ahead.
 //
 //   S^T = K.Q^T       v_mfma_f32_32x32x16, 32 keys x 32 queries: a lane has one query
 //   O^T += V^T.P^T    the same; V^T comes out of V's rows by transposing LDS reads
@@ -19,6 +19,8 @@
 //
 // Only the last tiles of a wave, on the diagonal, are masked.  There a masked key's V may be
 // anything: where it is not finite those elements are taken apart (a rare branch).
+#include <type_traits>
+
 #include "pkv_mfma.h"
 #include "pkv_step.h"
 
@@ -28,7 +30,8 @@ namespace {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-constexpr int kStage = 64;  // keys
+
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
 template <int FK>
 struct Wide;
@@ -39,6 +42,10 @@ struct Wide<0> {
   static __device__ __forceinline__ f16v mma(b8 a, b8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
+  // sum + the pair's two values
+  static __device__ __forceinline__ float add(__bf16 x, __bf16 y, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(b2{x, y}, b2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+  }
   static constexpr uint16_t kInf = 0x7F80;
 };
 template <>
@@ -48,15 +55,22 @@ struct Wide<1> {
   static __device__ __forceinline__ f16v mma(h8 a, h8 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float add(_Float16 x, _Float16 y, float sum) {
+    return __builtin_amdgcn_fdot2(h2{x, y}, h2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+  }
   static constexpr uint16_t kInf = 0x7C00;
 };
 
 template <int DP>
 struct PromptShape {
-  static constexpr int UNITS = DP / 8;                 // 16-byte units per row
-  static constexpr int SIDE = kStage * DP * 2;         // bytes of a stage's K (or V)
-  static constexpr int NBUF = DP > 128 ? 2 : 3;
-  static constexpr int COPIES = kStage * UNITS / 256;  // 16-byte units per thread and side
+  static constexpr int UNITS = DP / 8;                // 16-byte units per row
+  static constexpr int TILES = DP > 128 ? 1 : 2;      // 32-key tiles per stage
+  static constexpr int KEYS = 32 * TILES;
+  static constexpr int SIDE = KEYS * DP * 2;          // bytes of a stage's K (or V)
+  static constexpr int COPIES = KEYS * UNITS / 256;   // 16-byte units per thread and side
+  // a tile's product with V runs beside the next tile's scores: V stays a stage longer
+  static constexpr int KBUF = 2, VBUF = 3;
+  static constexpr int BYTES = (KBUF + VBUF) * SIDE;
 };
 
 // Where unit u of row m of a stage's K sits, so that the operand reads (one unit of 32 rows)
@@ -145,7 +159,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
   using E = typename W::E;
   using S = PromptShape<DP>;
   constexpr int KS = DP / 16, NB = DP / 32, PER = 4 * QB;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[S::NBUF * 2 * S::SIDE];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int kh = blockIdx.x % a.kv_heads;
@@ -166,7 +180,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
     head[i] = kh * a.gqa + c % a.gqa;
   }
   const int last = (min(chunks, (blk + 1) * PER) - 1) / a.gqa;  // 32-key tile of the block's last chunk
-  const int stages = last / 2 + 1;
+  const int stages = last / S::TILES + 1;
   // the wave's last tile, and its first with a mask (a wave without chunks has no tile)
   const int top = max(place[0], place[QB - 1]), clear = place[0];
 
@@ -175,24 +189,25 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
   const uint8_t *vbase = (const uint8_t *)(a.v + (int64_t)first * a.v_stride + kh * a.dim);
   const int live_units = a.dim / 8;
   auto copy = [&](int s) __attribute__((always_inline)) {
-    uint8_t *dst = lds + (s % S::NBUF) * (2 * S::SIDE) + wave * 1024;
+    uint8_t *kdst = lds + s % S::KBUF * S::SIDE + wave * 1024;
+    uint8_t *vdst = lds + (S::KBUF + s % S::VBUF) * S::SIDE + wave * 1024;
 #pragma unroll
     for (int i = 0; i < S::COPIES; ++i) {
       const int at = tid + 256 * i, m = at / S::UNITS;
       const int ku = k_unit<DP>(m, at % S::UNITS), vu = v_unit<DP>(m, at % S::UNITS);
-      const int64_t row = min(s * kStage + m, n - 1);
+      const int64_t row = min(s * S::KEYS + m, n - 1);
       if (ku < live_units)
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) uint32_t *)(kbase + row * a.k_stride * 2 + ku * 16),
-            (__attribute__((address_space(3))) uint32_t *)(dst + i * 4096), 16, 0, 0);
+            (__attribute__((address_space(3))) uint32_t *)(kdst + i * 4096), 16, 0, 0);
       if (vu < live_units)
         __builtin_amdgcn_global_load_lds(
             (const __attribute__((address_space(1))) uint32_t *)(vbase + row * a.v_stride * 2 + vu * 16),
-            (__attribute__((address_space(3))) uint32_t *)(dst + S::SIDE + i * 4096), 16, 0, 0);
+            (__attribute__((address_space(3))) uint32_t *)(vdst + i * 4096), 16, 0, 0);
     }
   };
   if (a.dim < DP) {  // the units past the head dim hold zeros
-    for (int i = tid; i < S::NBUF * 2 * S::SIDE / 16; i += 256) *((u4 *)lds + i) = u4{0, 0, 0, 0};
+    for (int i = tid; i < S::BYTES / 16; i += 256) *((u4 *)lds + i) = u4{0, 0, 0, 0};
     barrier();
   }
 
@@ -208,6 +223,9 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
       u4 x = {0, 0, 0, 0};
       if (d < a.dim && place[i] >= 0) x = *(const u4 *)(src + d);
       q[i][ks] = __builtin_bit_cast(T, x);
+      // (accumulation registers: the MFMAs take them from there as operands, and the vector
+      // registers are left to O and the scores)
+      asm("" : "+a"(q[i][ks]));
     }
   }
 
@@ -222,13 +240,6 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) O[i][j][e] = 0.0f;
   }
-  // (in registers: an inline constant 0 as an MFMA's accumulator has given wrong results
-  // where its destination partly overlaps an operand)
-  f16v zero;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
-  asm volatile("" : "+v"(zero));
-
   int koff[KS], voff[NB];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) koff[ks] = (col * S::UNITS + k_unit<DP>(col, 2 * ks + half)) * 16;
@@ -239,36 +250,26 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
       voff[nb] = (r * S::UNITS + v_unit<DP>(r, 4 * nb + 2 * j + (i & 3) / 2)) * 16 + 8 * (i & 1);
   }
 
-  for (int s = 0; s < S::NBUF - 1; ++s)
-    if (s < stages) copy(s);
-  for (int at = 0; at < 2 * stages; ++at) {
-    const int s = at >> 1;
-    if ((at & 1) == 0) {
-      // this wave's copies of stage s are done, then everyone's
-      if (s + 1 < stages && S::NBUF > 2) __builtin_amdgcn_s_waitcnt(0x0F70 | (2 * S::COPIES));  // the next stage's may fly
-      else __builtin_amdgcn_s_waitcnt(0x0F70);
-      barrier();
-      if (s + S::NBUF - 1 < stages) copy(s + S::NBUF - 1);
-    }
-    if (at > top) continue;
-    const uint8_t *ktile = lds + (s % S::NBUF) * (2 * S::SIDE) + (at & 1) * 32 * DP * 2, *vtile = ktile + S::SIDE;
-
-    f16v x[QB];
-#pragma unroll
-    for (int i = 0; i < QB; ++i) x[i] = zero;
+  // S^T = K.Q^T of a tile.  (From zeros in registers: an MFMA with an inline constant 0 as
+  // its accumulator has given wrong results where its destination partly overlaps an operand.)
+  f16v zero = {0};
+  asm volatile("" : "+v"(zero));
+  auto scores = [&](const uint8_t *ktile, f16v (&x)[QB]) __attribute__((always_inline)) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const T k = __builtin_bit_cast(T, *(const u4 *)(ktile + koff[ks]));
 #pragma unroll
-      for (int i = 0; i < QB; ++i) x[i] = W::mma(k, q[i][ks], x[i]);
+      for (int i = 0; i < QB; ++i) x[i] = W::mma(k, q[i][ks], ks == 0 ? zero : x[i]);
     }
+  };
+  // the exponents, less the running maximum: it moves when a score passes it by kTau
+  auto settle = [&](auto masks, f16v (&x)[QB], int at) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < QB; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[i][e] = __builtin_fmaf(x[i][e], a.scale_log2, -m[i]);
     // key 8g + 4 half + r of the tile is seen by the queries from it on
-    const bool masked = at >= clear;
-    if (masked) {
+    if constexpr (decltype(masks)::value) {
 #pragma unroll
       for (int i = 0; i < QB; ++i) {
         const int sees = (place[i] - at) * 32 + col - 4 * half;
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
       for (int e = 1; e < 16; ++e) mx[i] = __builtin_elementwise_maximum(mx[i], x[i][e]);
       need |= mx[i] > thr[i];
     }
-    if (__any(need)) {
+    if (__builtin_expect(__any(need), 0)) {
 #pragma unroll
       for (int i = 0; i < QB; ++i) {
         const float up = xor32_max(mx[i]);
@@ -301,35 +302,95 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
         for (int j = 0; j < NB; ++j) O[i][j] *= alpha;
       }
     }
-    T p[QB][2];
+  };
+  // the weights as operands, and their sums
+  auto weights = [&](const f16v (&x)[QB], T (&p)[QB][2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < QB; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const E r = (E)__builtin_amdgcn_exp2f(x[i][e]);
-        p[i][e / 8][e % 8] = r;
-        l[i] += (float)r;
+      for (int e = 0; e < 16; e += 2) {
+        const E r0 = (E)__builtin_amdgcn_exp2f(x[i][e]), r1 = (E)__builtin_amdgcn_exp2f(x[i][e + 1]);
+        p[i][e / 8][e % 8] = r0;
+        p[i][e / 8][e % 8 + 1] = r1;
+        l[i] = W::add(r0, r1, l[i]);
       }
-    bool odd = false;
-    if (masked) {  // infinities or NaN among the tile's values?
+  };
+  auto product = [&](const uint8_t *vtile, const T (&p)[QB][2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const u4 w = __builtin_bit_cast(u4, v_operand<DP, T>(vtile + kk * 16 * DP * 2 + voff[nb]));
+      for (int nb = 0; nb < NB; ++nb) {
+        const T v = v_operand<DP, T>(vtile + kk * 16 * DP * 2 + voff[nb]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7FFFu) >= W::kInf || (w[e] >> 16 & 0x7FFFu) >= W::kInf;
-        }
+        for (int i = 0; i < QB; ++i) O[i][nb] = W::mma(v, p[i][kk], O[i][nb]);
+      }
+  };
+  auto ktile = [&](int at) __attribute__((always_inline)) {
+    return lds + at / S::TILES % S::KBUF * S::SIDE + at % S::TILES * 32 * DP * 2;
+  };
+  auto vtile = [&](int at) __attribute__((always_inline)) {
+    return lds + (S::KBUF + at / S::TILES % S::VBUF) * S::SIDE + at % S::TILES * 32 * DP * 2;
+  };
+  // stage s is here; everyone is done with the scores of stage s - 1 and the products of
+  // stage s - 2, whose places the next stage takes
+  auto turn = [&](int s) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    barrier();
+    if (s + 1 < stages) copy(s + 1);
+  };
+
+  copy(0);
+  // ---- tiles that the wave's queries see whole, two at a time: a tile's weights and
+  // product go beside the next one's scores
+  const int whole = max(clear, 0) & ~1;
+  if (whole > 0) {
+    f16v x[QB];
+    turn(0);
+    scores(ktile(0), x);
+    settle(std::false_type{}, x, 0);
+    f16v y[QB];
+    T p[QB][2];
+    int at = 1;
+    for (; at + 1 < whole; at += 2) {
+      if (S::TILES == 1) turn(at);
+      scores(ktile(at), y);
+      weights(x, p);
+      product(vtile(at - 1), p);
+      settle(std::false_type{}, y, at);
+      turn((at + 1) / S::TILES);
+      scores(ktile(at + 1), x);
+      weights(y, p);
+      product(vtile(at), p);
+      settle(std::false_type{}, x, at + 1);
     }
-    if (!__any(odd)) {
+    if (S::TILES == 1) turn(at);
+    scores(ktile(at), y);
+    weights(x, p);
+    product(vtile(at - 1), p);
+    settle(std::false_type{}, y, at);
+    weights(y, p);
+    product(vtile(at), p);
+  }
+  // ---- and the rest
+  for (int at = whole; at < stages * S::TILES; ++at) {
+    if (at % S::TILES == 0) turn(at / S::TILES);
+    if (at > top) continue;
+    f16v x[QB];
+    T p[QB][2];
+    scores(ktile(at), x);
+    settle(std::true_type{}, x, at);
+    weights(x, p);
+    bool odd = false;  // infinities or NaN among the tile's values?
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const T v = v_operand<DP, T>(vtile + kk * 16 * DP * 2 + voff[nb]);
+      for (int nb = 0; nb < NB; ++nb) {
+        const u4 w = __builtin_bit_cast(u4, v_operand<DP, T>(vtile(at) + kk * 16 * DP * 2 + voff[nb]));
 #pragma unroll
-          for (int i = 0; i < QB; ++i) O[i][nb] = W::mma(v, p[i][kk], O[i][nb]);
-        }
+        for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7FFFu) >= W::kInf || (w[e] >> 16 & 0x7FFFu) >= W::kInf;
+      }
+    if (__builtin_expect(!__any(odd), 1)) {
+      product(vtile(at), p);
     } else {
       // their products with the masked keys' zero weights must not be NaN: the finite
       // values go through the product; of the others, kind by kind, the keys that a
@@ -344,7 +405,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
           for (int e = 0; e < 8; ++e) seen[e] = 8 * (2 * kk + e / 4) + e % 4 <= sees ? (E)1.0f : (E)0.0f;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
-            const T v = v_operand<DP, T>(vtile + kk * 16 * DP * 2 + voff[nb]);
+            const T v = v_operand<DP, T>(vtile(at) + kk * 16 * DP * 2 + voff[nb]);
             uint16_t w[8];
             __builtin_memcpy(w, &v, 16);
             T part = v;
