@@ -107,7 +107,8 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, int rank, int pe
     const int mine = lane < a.batch ? prompt_blocks(prompt_rows(a, lane, first), a.gqa, per) : 0;
     if (rank >= wave_sum(mine)) return false;
     // the largest level of which more than `rank` blocks are at or above
-    int lo = 0, hi = 1 << 24;
+    int lo = 0, hi = 1;
+    while (__ballot(mine >= hi)) hi <<= 1;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (wave_sum(max(0, mine - mid)) > rank) lo = mid;
@@ -187,29 +188,49 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
   // ---- K and V rows to LDS: thread tid copies unit tid + 256 i of a stage
   const uint8_t *kbase = (const uint8_t *)(a.k + (int64_t)first * a.k_stride + kh * a.dim);
   const uint8_t *vbase = (const uint8_t *)(a.v + (int64_t)first * a.v_stride + kh * a.dim);
-  const int live_units = a.dim / 8;
+  uint32_t krow[S::COPIES], kat[S::COPIES], vat[S::COPIES];  // row; byte offsets from the stage's first row
+  uint32_t live = 0;                                         // units within the head dim
+#pragma unroll
+  for (int i = 0; i < S::COPIES; ++i) {
+    const int at = tid + 256 * i, m = at / S::UNITS;
+    const int ku = k_unit<DP>(m, at % S::UNITS), vu = v_unit<DP>(m, at % S::UNITS);
+    krow[i] = m;
+    kat[i] = m * (uint32_t)a.k_stride * 2 + ku * 16;
+    vat[i] = m * (uint32_t)a.v_stride * 2 + vu * 16;
+    live |= (ku < a.dim / 8 ? 1u : 0u) << (2 * i) | (vu < a.dim / 8 ? 2u : 0u) << (2 * i);
+  }
   auto copy = [&](int s) __attribute__((always_inline)) {
     uint8_t *kdst = lds + s % S::KBUF * S::SIDE + wave * 1024;
     uint8_t *vdst = lds + (S::KBUF + s % S::VBUF) * S::SIDE + wave * 1024;
+    const uint8_t *ksrc = kbase + (int64_t)s * S::KEYS * a.k_stride * 2;
+    const uint8_t *vsrc = vbase + (int64_t)s * S::KEYS * a.v_stride * 2;
+    auto unit = [](const uint8_t *from, uint8_t *to) __attribute__((always_inline)) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)from,
+                                       (__attribute__((address_space(3))) uint32_t *)to, 16, 0, 0);
+    };
+    if (a.dim == DP && (s + 1) * S::KEYS <= n) {  // whole rows, all of them there
+#pragma unroll
+      for (int i = 0; i < S::COPIES; ++i) {
+        unit(ksrc + kat[i], kdst + i * 4096);
+        unit(vsrc + vat[i], vdst + i * 4096);
+      }
+      return;
+    }
+    // rows past the last one read it again (their keys are masked)
+    const int rows = n - s * S::KEYS;
 #pragma unroll
     for (int i = 0; i < S::COPIES; ++i) {
-      const int at = tid + 256 * i, m = at / S::UNITS;
-      const int ku = k_unit<DP>(m, at % S::UNITS), vu = v_unit<DP>(m, at % S::UNITS);
-      const int64_t row = min(s * S::KEYS + m, n - 1);
-      if (ku < live_units)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) uint32_t *)(kbase + row * a.k_stride * 2 + ku * 16),
-            (__attribute__((address_space(3))) uint32_t *)(kdst + i * 4096), 16, 0, 0);
-      if (vu < live_units)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) uint32_t *)(vbase + row * a.v_stride * 2 + vu * 16),
-            (__attribute__((address_space(3))) uint32_t *)(vdst + i * 4096), 16, 0, 0);
+      const int64_t past = max((int)krow[i] - (rows - 1), 0);
+      if (live >> (2 * i) & 1) unit(ksrc + kat[i] - past * a.k_stride * 2, kdst + i * 4096);
+      if (live >> (2 * i) & 2) unit(vsrc + vat[i] - past * a.v_stride * 2, vdst + i * 4096);
     }
   };
   if (a.dim < DP) {  // the units past the head dim hold zeros
     for (int i = tid; i < S::BYTES / 16; i += 256) *((u4 *)lds + i) = u4{0, 0, 0, 0};
     barrier();
   }
+
+  copy(0);
 
   // ---- queries: lane (col, half) holds elements 16 ks + 8 half + e of query col
   T q[QB][KS];
@@ -339,7 +360,6 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
     if (s + 1 < stages) copy(s + 1);
   };
 
-  copy(0);
   // ---- tiles that the wave's queries see whole, two at a time: a tile's weights and
   // product go beside the next one's scores
   const int whole = max(clear, 0) & ~1;
