@@ -3,9 +3,8 @@
 //   o_i = sum_{j <= i} softmax_j(scale * q_i . k_j) v_j     per sequence and head
 //
 // A chunk is 32 consecutive queries of one head; the chunks of a (sequence, KV head) are
-// ordered by position, then head, and a workgroup of four waves takes 4 * QB consecutive
-// ones, a wave QB: with a few heads per KV head a workgroup's chunks end at nearly the same
-// key.  Keys come in stages of 64 (32 beyond head dim 128), K and V copied straight to LDS
+// ordered by position, then head, and the four waves of a workgroup take consecutive ones:
+// with a few heads per KV head they end at nearly the same key.  Keys come in stages of 64 (32 beyond head dim 128), K and V copied straight to LDS
 // in rows (global_load_lds), a stage ahead.
 //
 //   S^T = K.Q^T       v_mfma_f32_32x32x16, 32 keys x 32 queries: a lane has one query
@@ -95,16 +94,17 @@ __device__ __forceinline__ int prompt_rows(const PromptArgs &a, int b, int &firs
 }
 
 // Workgroups of a sequence of n rows, per KV head.
-__device__ __forceinline__ int prompt_blocks(int n, int gqa, int per) {
-  return n <= 0 ? 0 : ((n + 31) / 32 * gqa + per - 1) / per;
+constexpr int kChunks = 4;
+__device__ __forceinline__ int prompt_blocks(int n, int gqa) {
+  return n <= 0 ? 0 : ((n + 31) / 32 * gqa + kChunks - 1) / kChunks;
 }
 
 // The workgroup's (sequence, block): longest blocks first where the batch fits a wave's
 // lanes, else sequence by sequence.  The whole wave calls.
-__device__ __forceinline__ bool find_block(const PromptArgs &a, int rank, int per, int lane, int &b, int &blk) {
+__device__ __forceinline__ bool find_block(const PromptArgs &a, int rank, int lane, int &b, int &blk) {
   if (a.batch <= 64) {
     int first;
-    const int mine = lane < a.batch ? prompt_blocks(prompt_rows(a, lane, first), a.gqa, per) : 0;
+    const int mine = lane < a.batch ? prompt_blocks(prompt_rows(a, lane, first), a.gqa) : 0;
     if (rank >= wave_sum(mine)) return false;
     // the largest level of which more than `rank` blocks are at or above
     int lo = 0, hi = 1;
@@ -124,7 +124,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, int rank, int pe
   int carry = 0;
   for (int c = 0; c < a.batch; c += 64) {
     int first;
-    const int mine = c + lane < a.batch ? prompt_blocks(prompt_rows(a, c + lane, first), a.gqa, per) : 0;
+    const int mine = c + lane < a.batch ? prompt_blocks(prompt_rows(a, c + lane, first), a.gqa) : 0;
     const int incl = wave_scan_incl(mine, lane) + carry;
     const unsigned long long hit = __ballot(incl > rank);
     if (hit) {
@@ -143,9 +143,11 @@ __device__ __forceinline__ void barrier() {
   asm volatile("s_barrier" ::: "memory");
 }
 
+typedef __attribute__((address_space(3))) uint8_t ldsbyte;
+
 // A lane's V^T operand (dim 32 nb + col, 16 keys) out of V's rows in LDS.
 template <int DP, typename T>
-__device__ __forceinline__ T v_operand(const uint8_t *src) {
+__device__ __forceinline__ T v_operand(const ldsbyte *src) {
   typedef short s4v __attribute__((ext_vector_type(4)));
   struct { s4v lo, hi; } v;
   v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v *)src);
@@ -153,52 +155,45 @@ __device__ __forceinline__ T v_operand(const uint8_t *src) {
   return __builtin_bit_cast(T, v);
 }
 
-template <int DP, int FK, int QB>
-__global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
+template <int DP, int FK>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const PromptArgs a) {
   using W = Wide<FK>;
   using T = typename W::T;
   using E = typename W::E;
   using S = PromptShape<DP>;
-  constexpr int KS = DP / 16, NB = DP / 32, PER = 4 * QB;
+  constexpr int KS = DP / 16, NB = DP / 32;
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int kh = blockIdx.x % a.kv_heads;
   int b, blk;
-  if (!find_block(a, blockIdx.x / a.kv_heads, PER, lane, b, blk)) return;
+  if (!find_block(a, blockIdx.x / a.kv_heads, lane, b, blk)) return;
   b = __builtin_amdgcn_readfirstlane(b);
   blk = __builtin_amdgcn_readfirstlane(blk);
   int first;
   const int n = prompt_rows(a, b, first);
   const int chunks = (n + 31) / 32 * a.gqa;
 
-  // the wave's chunks, rising; -1: none
-  int place[QB], head[QB];
-#pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int c = blk * PER + wave * QB + i;
-    place[i] = c < chunks ? c / a.gqa : -1;
-    head[i] = kh * a.gqa + c % a.gqa;
-  }
-  const int last = (min(chunks, (blk + 1) * PER) - 1) / a.gqa;  // 32-key tile of the block's last chunk
+  // the wave's chunk: 32 queries from 32 * place on, of one head (place -1: none)
+  const int chunk = blk * kChunks + wave;
+  const int place = chunk < chunks ? chunk / a.gqa : -1, head = kh * a.gqa + chunk % a.gqa;
+  const int last = (min(chunks, (blk + 1) * kChunks) - 1) / a.gqa;  // 32-key tile of the block's last chunk
   const int stages = last / S::TILES + 1;
-  // the wave's last tile, and its first with a mask (a wave without chunks has no tile)
-  const int top = max(place[0], place[QB - 1]), clear = place[0];
 
   // ---- K and V rows to LDS: thread tid copies unit tid + 256 i of a stage
   const uint8_t *kbase = (const uint8_t *)(a.k + (int64_t)first * a.k_stride + kh * a.dim);
   const uint8_t *vbase = (const uint8_t *)(a.v + (int64_t)first * a.v_stride + kh * a.dim);
-  uint32_t krow[S::COPIES], kat[S::COPIES], vat[S::COPIES];  // row; byte offsets from the stage's first row
-  uint32_t live = 0;                                         // units within the head dim
+  // Copies i are STEP rows apart: V's units keep their places, K's are moved by bit 4 of
+  // the row alone.
+  constexpr int STEP = 256 / S::UNITS;
+  const int crow = tid / S::UNITS, vu = v_unit<DP>(crow, tid % S::UNITS);
+  int ku[2];
 #pragma unroll
-  for (int i = 0; i < S::COPIES; ++i) {
-    const int at = tid + 256 * i, m = at / S::UNITS;
-    const int ku = k_unit<DP>(m, at % S::UNITS), vu = v_unit<DP>(m, at % S::UNITS);
-    krow[i] = m;
-    kat[i] = m * (uint32_t)a.k_stride * 2 + ku * 16;
-    vat[i] = m * (uint32_t)a.v_stride * 2 + vu * 16;
-    live |= (ku < a.dim / 8 ? 1u : 0u) << (2 * i) | (vu < a.dim / 8 ? 2u : 0u) << (2 * i);
-  }
+  for (int f = 0; f < 2; ++f) ku[f] = k_unit<DP>((crow & ~16) | (((crow >> 4) ^ f) & 1) << 4, tid % S::UNITS);
+  const uint32_t vat = crow * (uint32_t)a.v_stride * 2 + vu * 16;
+  uint32_t kat[2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f) kat[f] = crow * (uint32_t)a.k_stride * 2 + ku[f] * 16;
   auto copy = [&](int s) __attribute__((always_inline)) {
     uint8_t *kdst = lds + s % S::KBUF * S::SIDE + wave * 1024;
     uint8_t *vdst = lds + (S::KBUF + s % S::VBUF) * S::SIDE + wave * 1024;
@@ -211,8 +206,8 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
     if (a.dim == DP && (s + 1) * S::KEYS <= n) {  // whole rows, all of them there
 #pragma unroll
       for (int i = 0; i < S::COPIES; ++i) {
-        unit(ksrc + kat[i], kdst + i * 4096);
-        unit(vsrc + vat[i], vdst + i * 4096);
+        unit(ksrc + (int64_t)i * STEP * a.k_stride * 2 + kat[i * STEP / 16 % 2], kdst + i * 4096);
+        unit(vsrc + (int64_t)i * STEP * a.v_stride * 2 + vat, vdst + i * 4096);
       }
       return;
     }
@@ -220,9 +215,10 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
     const int rows = n - s * S::KEYS;
 #pragma unroll
     for (int i = 0; i < S::COPIES; ++i) {
-      const int64_t past = max((int)krow[i] - (rows - 1), 0);
-      if (live >> (2 * i) & 1) unit(ksrc + kat[i] - past * a.k_stride * 2, kdst + i * 4096);
-      if (live >> (2 * i) & 2) unit(vsrc + vat[i] - past * a.v_stride * 2, vdst + i * 4096);
+      const int f = i * STEP / 16 % 2;
+      const int64_t back = i * STEP - max(crow + i * STEP - (rows - 1), 0);
+      if (ku[f] < a.dim / 8) unit(ksrc + back * a.k_stride * 2 + kat[f], kdst + i * 4096);
+      if (vu < a.dim / 8) unit(vsrc + back * a.v_stride * 2 + vat, vdst + i * 4096);
     }
   };
   if (a.dim < DP) {  // the units past the head dim hold zeros
@@ -233,35 +229,27 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
   copy(0);
 
   // ---- queries: lane (col, half) holds elements 16 ks + 8 half + e of query col
-  T q[QB][KS];
-#pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int64_t row = first + min(max(place[i], 0) * 32 + col, n - 1);
-    const uint16_t *src = a.q + row * a.q_stride + (int64_t)head[i] * a.dim;
+  T q[KS];
+  {
+    const int64_t row = first + min(max(place, 0) * 32 + col, n - 1);
+    const uint16_t *src = a.q + row * a.q_stride + (int64_t)head * a.dim;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int d = 16 * ks + 8 * half;
       u4 x = {0, 0, 0, 0};
-      if (d < a.dim && place[i] >= 0) x = *(const u4 *)(src + d);
-      q[i][ks] = __builtin_bit_cast(T, x);
-      // (accumulation registers: the MFMAs take them from there as operands, and the vector
-      // registers are left to O and the scores)
-      asm("" : "+a"(q[i][ks]));
+      if (d < a.dim && place >= 0) x = *(const u4 *)(src + d);
+      q[ks] = __builtin_bit_cast(T, x);
     }
   }
 
-  float m[QB], thr[QB], l[QB];
-  f16v O[QB][NB];
+  float m = 0.0f, thr = -INFINITY, l = 0.0f;
+  f16v O[NB];
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    m[i] = l[i] = 0.0f;
-    thr[i] = -INFINITY;
+  for (int j = 0; j < NB; ++j)
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) O[i][j][e] = 0.0f;
-  }
-  int koff[KS], voff[NB];
+    for (int e = 0; e < 16; ++e) O[j][e] = 0.0f;
+
+  uint32_t koff[KS], voff[NB];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) koff[ks] = (col * S::UNITS + k_unit<DP>(col, 2 * ks + half)) * 16;
   {
@@ -275,82 +263,65 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
   // its accumulator has given wrong results where its destination partly overlaps an operand.)
   f16v zero = {0};
   asm volatile("" : "+v"(zero));
-  auto scores = [&](const uint8_t *ktile, f16v (&x)[QB]) __attribute__((always_inline)) {
+  ldsbyte *const base = (ldsbyte *)lds;
+  auto scores = [&](uint32_t ktile, f16v &x) __attribute__((always_inline)) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const T k = __builtin_bit_cast(T, *(const u4 *)(ktile + koff[ks]));
-#pragma unroll
-      for (int i = 0; i < QB; ++i) x[i] = W::mma(k, q[i][ks], ks == 0 ? zero : x[i]);
+      const u4 k = *(const __attribute__((address_space(3))) u4 *)(base + (koff[ks] + ktile));
+      x = W::mma(__builtin_bit_cast(T, k), q[ks], ks == 0 ? zero : x);
     }
   };
   // the exponents, less the running maximum: it moves when a score passes it by kTau
-  auto settle = [&](auto masks, f16v (&x)[QB], int at) __attribute__((always_inline)) {
+  auto settle = [&](auto masks, f16v &x, int at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < QB; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) x[i][e] = __builtin_fmaf(x[i][e], a.scale_log2, -m[i]);
+    for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(x[e], a.scale_log2, -m);
     // key 8g + 4 half + r of the tile is seen by the queries from it on
     if constexpr (decltype(masks)::value) {
+      const int sees = (place - at) * 32 + col - 4 * half;
 #pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        const int sees = (place[i] - at) * 32 + col - 4 * half;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[i][e] = 8 * (e / 4) + e % 4 <= sees ? x[i][e] : -INFINITY;
-      }
+      for (int e = 0; e < 16; ++e) x[e] = 8 * (e / 4) + e % 4 <= sees ? x[e] : -INFINITY;
     }
-    float mx[QB];
-    bool need = false;
+    float mx = x[0];
 #pragma unroll
-    for (int i = 0; i < QB; ++i) {
-      mx[i] = x[i][0];
+    for (int e = 1; e < 16; ++e) mx = __builtin_elementwise_maximum(mx, x[e]);
+    if (__builtin_expect(__any(mx > thr), 0)) {
+      const float up = xor32_max(mx);
+      const bool moves = up > thr;
+      const float by = moves ? up : 0.0f;
+      const float alpha = !moves ? 1.0f : thr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
+      m += by;
+      thr = moves ? kTau : thr;
+      l *= alpha;
 #pragma unroll
-      for (int e = 1; e < 16; ++e) mx[i] = __builtin_elementwise_maximum(mx[i], x[i][e]);
-      need |= mx[i] > thr[i];
-    }
-    if (__builtin_expect(__any(need), 0)) {
+      for (int e = 0; e < 16; ++e) x[e] -= by;
 #pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        const float up = xor32_max(mx[i]);
-        const bool moves = up > thr[i];
-        const float by = moves ? up : 0.0f;
-        const float alpha = !moves ? 1.0f : thr[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
-        m[i] += by;
-        thr[i] = moves ? kTau : thr[i];
-        l[i] *= alpha;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[i][e] -= by;
-#pragma unroll
-        for (int j = 0; j < NB; ++j) O[i][j] *= alpha;
-      }
+      for (int j = 0; j < NB; ++j) O[j] *= alpha;
     }
   };
-  // the weights as operands, and their sums
-  auto weights = [&](const f16v (&x)[QB], T (&p)[QB][2]) __attribute__((always_inline)) {
+  // the weights as operands, and their sum
+  auto weights = [&](const f16v &x, T (&p)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < QB; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const E r0 = (E)__builtin_amdgcn_exp2f(x[i][e]), r1 = (E)__builtin_amdgcn_exp2f(x[i][e + 1]);
-        p[i][e / 8][e % 8] = r0;
-        p[i][e / 8][e % 8 + 1] = r1;
-        l[i] = W::add(r0, r1, l[i]);
-      }
+    for (int e = 0; e < 16; e += 2) {
+      const E r0 = (E)__builtin_amdgcn_exp2f(x[e]), r1 = (E)__builtin_amdgcn_exp2f(x[e + 1]);
+      p[e / 8][e % 8] = r0;
+      p[e / 8][e % 8 + 1] = r1;
+      l = W::add(r0, r1, l);
+    }
   };
-  auto product = [&](const uint8_t *vtile, const T (&p)[QB][2]) __attribute__((always_inline)) {
+  auto product = [&](uint32_t vtile, const T (&p)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const T v = v_operand<DP, T>(vtile + kk * 16 * DP * 2 + voff[nb]);
-#pragma unroll
-        for (int i = 0; i < QB; ++i) O[i][nb] = W::mma(v, p[i][kk], O[i][nb]);
-      }
+      for (int nb = 0; nb < NB; ++nb)
+        O[nb] = W::mma(v_operand<DP, T>(base + (voff[nb] + vtile) + kk * 16 * DP * 2), p[kk], O[nb]);
   };
+  // where tile `at` lies: uniform offsets (of a stage, then of its second tile)
   auto ktile = [&](int at) __attribute__((always_inline)) {
-    return lds + at / S::TILES % S::KBUF * S::SIDE + at % S::TILES * 32 * DP * 2;
+    return (uint32_t)__builtin_amdgcn_readfirstlane(at / S::TILES % S::KBUF * S::SIDE + at % S::TILES * (32 * DP * 2));
   };
   auto vtile = [&](int at) __attribute__((always_inline)) {
-    return lds + (S::KBUF + at / S::TILES % S::VBUF) * S::SIDE + at % S::TILES * 32 * DP * 2;
+    return (uint32_t)__builtin_amdgcn_readfirstlane((S::KBUF + at / S::TILES % S::VBUF) * S::SIDE +
+                                                    at % S::TILES * (32 * DP * 2));
   };
   // stage s is here; everyone is done with the scores of stage s - 1 and the products of
   // stage s - 2, whose places the next stage takes
@@ -362,14 +333,13 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
 
   // ---- tiles that the wave's queries see whole, two at a time: a tile's weights and
   // product go beside the next one's scores
-  const int whole = max(clear, 0) & ~1;
+  const int whole = max(place, 0) & ~1;
   if (whole > 0) {
-    f16v x[QB];
+    f16v x, y;
+    T p[2];
     turn(0);
     scores(ktile(0), x);
     settle(std::false_type{}, x, 0);
-    f16v y[QB];
-    T p[QB][2];
     int at = 1;
     for (; at + 1 < whole; at += 2) {
       if (S::TILES == 1) turn(at);
@@ -394,9 +364,9 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
   // ---- and the rest
   for (int at = whole; at < stages * S::TILES; ++at) {
     if (at % S::TILES == 0) turn(at / S::TILES);
-    if (at > top) continue;
-    f16v x[QB];
-    T p[QB][2];
+    if (at > place) continue;
+    f16v x;
+    T p[2];
     scores(ktile(at), x);
     settle(std::true_type{}, x, at);
     weights(x, p);
@@ -405,7 +375,7 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        const u4 w = __builtin_bit_cast(u4, v_operand<DP, T>(vtile(at) + kk * 16 * DP * 2 + voff[nb]));
+        const u4 w = __builtin_bit_cast(u4, v_operand<DP, T>(base + (voff[nb] + vtile(at)) + kk * 16 * DP * 2));
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7FFFu) >= W::kInf || (w[e] >> 16 & 0x7FFFu) >= W::kInf;
       }
@@ -415,76 +385,55 @@ __global__ __launch_bounds__(256, 1) void prompt_kernel(const PromptArgs a) {
       // their products with the masked keys' zero weights must not be NaN: the finite
       // values go through the product; of the others, kind by kind, the keys that a
       // query sees are counted by one
+      const int sees = (place - at) * 32 + col - 4 * half;
 #pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        const int sees = (place[i] - at) * 32 + col - 4 * half;
+      for (int kk = 0; kk < 2; ++kk) {
+        T seen;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-          T seen;
+        for (int e = 0; e < 8; ++e) seen[e] = 8 * (2 * kk + e / 4) + e % 4 <= sees ? (E)1.0f : (E)0.0f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) seen[e] = 8 * (2 * kk + e / 4) + e % 4 <= sees ? (E)1.0f : (E)0.0f;
+        for (int nb = 0; nb < NB; ++nb) {
+          const T v = v_operand<DP, T>(base + (voff[nb] + vtile(at)) + kk * 16 * DP * 2);
+          uint16_t w[8];
+          __builtin_memcpy(w, &v, 16);
+          T part = v;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const T v = v_operand<DP, T>(vtile(at) + kk * 16 * DP * 2 + voff[nb]);
-            uint16_t w[8];
-            __builtin_memcpy(w, &v, 16);
-            T part = v;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) part[e] = (w[e] & 0x7FFF) >= W::kInf ? (E)0.0f : part[e];
-            O[i][nb] = W::mma(part, p[i][kk], O[i][nb]);
+          for (int e = 0; e < 8; ++e) part[e] = (w[e] & 0x7FFF) >= W::kInf ? (E)0.0f : part[e];
+          O[nb] = W::mma(part, p[kk], O[nb]);
 #pragma unroll 1
-            for (int kind = 0; kind < 3; ++kind) {
+          for (int kind = 0; kind < 3; ++kind) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const bool hit = kind == 2 ? (w[e] & 0x7FFF) > W::kInf : w[e] == (W::kInf | (kind << 15));
-                part[e] = hit ? (E)1.0f : (E)0.0f;
-              }
-              const f16v count = W::mma(part, seen, zero);
-              const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
-#pragma unroll
-              for (int e = 0; e < 16; ++e) O[i][nb][e] += count[e] > 0.0f ? what : 0.0f;
+            for (int e = 0; e < 8; ++e) {
+              const bool hit = kind == 2 ? (w[e] & 0x7FFF) > W::kInf : w[e] == (W::kInf | (kind << 15));
+              part[e] = hit ? (E)1.0f : (E)0.0f;
             }
+            const f16v count = W::mma(part, seen, zero);
+            const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+            for (int e = 0; e < 16; ++e) O[nb][e] += count[e] > 0.0f ? what : 0.0f;
           }
         }
       }
     }
   }
 
+  const int row = place * 32 + col;
+  const float inv = 1.0f / xor32_add(l);
+  if (place < 0 || row >= n) return;
+  uint16_t *dst = a.out + ((int64_t)(first + row) * a.heads + head) * a.dim;
 #pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int row = place[i] * 32 + col;
-    const float inv = 1.0f / xor32_add(l[i]);
-    if (place[i] < 0 || row >= n) continue;
-    uint16_t *dst = a.out + ((int64_t)(first + row) * a.heads + head[i]) * a.dim;
+  for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * nb + 8 * g + 4 * half;
+      if (d >= a.dim) continue;
+      E r[4];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = 32 * nb + 8 * g + 4 * half;
-        if (d >= a.dim) continue;
-        E r[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = (E)(O[i][nb][4 * g + e] * inv);
-        u2 w;
-        __builtin_memcpy(&w, r, 8);
-        *(u2 *)(dst + d) = w;
-      }
-  }
-}
-
-template <int QB>
-hipError_t launch(hipStream_t stream, const PromptArgs &a, int64_t blocks) {
-  const dim3 grid((unsigned)blocks), block(256);
-#define PKV_PROMPT(DP_, FK_, QB_)                                                            \
-  if (a.dim <= DP_ && a.float_kind == FK_) {                                                 \
-    hipLaunchKernelGGL((prompt_kernel<DP_, FK_, QB_>), grid, block, 0, stream, a);           \
-    return hipGetLastError();                                                                \
-  }
-  PKV_PROMPT(64, 0, QB) PKV_PROMPT(64, 1, QB)
-  PKV_PROMPT(128, 0, QB) PKV_PROMPT(128, 1, QB)
-  PKV_PROMPT(256, 0, 1) PKV_PROMPT(256, 1, 1)
-#undef PKV_PROMPT
-  return hipErrorInvalidValue;
+      for (int e = 0; e < 4; ++e) r[e] = (E)(O[nb][4 * g + e] * inv);
+      u2 w;
+      __builtin_memcpy(&w, r, 8);
+      *(u2 *)(dst + d) = w;
+    }
 }
 
 }  // namespace
@@ -492,13 +441,19 @@ hipError_t launch(hipStream_t stream, const PromptArgs &a, int64_t blocks) {
 hipError_t launch_prompt_attention(hipStream_t stream, const PromptArgs &a) {
   if (a.rows == 0 || a.batch == 0) return hipSuccess;
   // workgroups, at most: every sequence's last one may be short
-  auto blocks = [&](int per) {
-    const int64_t seqs = a.batch < a.rows ? a.batch : a.rows;
-    return (((int64_t)a.rows + 31 * seqs) / 32 * a.gqa / per + seqs) * a.kv_heads;
-  };
-  const bool wide = a.dim <= 128 && blocks(8) >= 512;
-  if (wide) return launch<2>(stream, a, blocks(8));
-  return launch<1>(stream, a, blocks(4));
+  const int64_t seqs = a.batch < a.rows ? a.batch : a.rows;
+  const int64_t blocks = (((int64_t)a.rows + 31 * seqs) / 32 * a.gqa / kChunks + seqs) * a.kv_heads;
+  const dim3 grid((unsigned)blocks), block(256);
+#define PKV_PROMPT(DP_, FK_)                                                     \
+  if (a.dim <= DP_ && a.float_kind == FK_) {                                     \
+    hipLaunchKernelGGL((prompt_kernel<DP_, FK_>), grid, block, 0, stream, a);    \
+    return hipGetLastError();                                                    \
+  }
+  PKV_PROMPT(64, 0) PKV_PROMPT(64, 1)
+  PKV_PROMPT(128, 0) PKV_PROMPT(128, 1)
+  PKV_PROMPT(256, 0) PKV_PROMPT(256, 1)
+#undef PKV_PROMPT
+  return hipErrorInvalidValue;
 }
 
 }  // namespace pkv
