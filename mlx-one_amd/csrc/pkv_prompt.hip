@@ -16,7 +16,7 @@
 // (2^-9 relative for bfloat16, beside the output's own rounding of the same size), and summed as
 // rounded, so that weights still add up to one.
 //
-// Only the last tiles of a wave, on the diagonal, are masked.  There a masked key's V may be
+// Only the last tile of a wave, on the diagonal, is masked.  There a masked key's V may be
 // anything: where it is not finite those elements are taken apart (a rare branch).
 #include <type_traits>
 
@@ -100,40 +100,41 @@ __device__ __forceinline__ int prompt_blocks(int n, int gqa) {
 }
 
 // The workgroup's (sequence, block): longest blocks first where the batch fits a wave's
-// lanes, else sequence by sequence.  The whole wave calls.
-__device__ __forceinline__ bool find_block(const PromptArgs &a, int rank, int lane, int &b, int &blk) {
-  if (a.batch <= 64) {
-    int first;
-    const int mine = lane < a.batch ? prompt_blocks(prompt_rows(a, lane, first), a.gqa) : 0;
-    if (rank >= wave_sum(mine)) return false;
-    // the largest level of which more than `rank` blocks are at or above
-    int lo = 0, hi = 1;
-    while (__ballot(mine >= hi)) hi <<= 1;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (wave_sum(max(0, mine - mid)) > rank) lo = mid;
-      else hi = mid;
-    }
-    const int above = wave_sum(max(0, mine - lo - 1));
-    unsigned long long at = __ballot(mine > lo);
-    for (int i = rank - above; i > 0; --i) at &= at - 1;
-    b = __ffsll((long long)at) - 1;
-    blk = lo;
-    return true;
-  }
+// lanes, else sequence by sequence; and the sequence's rows.  The whole wave calls.
+__device__ __forceinline__ bool find_block(const PromptArgs &a, int rank, int lane, int &b, int &blk, int &first,
+                                           int &n) {
   int carry = 0;
   for (int c = 0; c < a.batch; c += 64) {
-    int first;
-    const int mine = c + lane < a.batch ? prompt_blocks(prompt_rows(a, c + lane, first), a.gqa) : 0;
-    const int incl = wave_scan_incl(mine, lane) + carry;
-    const unsigned long long hit = __ballot(incl > rank);
-    if (hit) {
-      const int f = __ffsll((long long)hit) - 1;
-      b = c + f;
+    int start = 0;
+    const int rows = c + lane < a.batch ? prompt_rows(a, c + lane, start) : 0;
+    const int mine = prompt_blocks(rows, a.gqa);
+    int f;
+    if (a.batch <= 64) {
+      if (rank >= wave_sum(mine)) return false;
+      // the largest level of which more than `rank` blocks are at or above
+      int lo = 0, hi = 1;
+      while (__ballot(mine >= hi)) hi <<= 1;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (wave_sum(max(0, mine - mid)) > rank) lo = mid;
+        else hi = mid;
+      }
+      unsigned long long at = __ballot(mine > lo);
+      for (int i = rank - wave_sum(max(0, mine - lo - 1)); i > 0; --i) at &= at - 1;
+      f = __ffsll((long long)at) - 1;
+      blk = lo;
+    } else {
+      const int incl = wave_scan_incl(mine, lane) + carry;
+      const unsigned long long hit = __ballot(incl > rank);
+      carry = __builtin_amdgcn_readlane(incl, 63);
+      if (!hit) continue;
+      f = __ffsll((long long)hit) - 1;
       blk = __builtin_amdgcn_readlane(incl, f) - 1 - rank;
-      return true;
     }
-    carry = __builtin_amdgcn_readlane(incl, 63);
+    b = c + f;
+    first = __builtin_amdgcn_readlane(start, f);
+    n = __builtin_amdgcn_readlane(rows, f);
+    return true;
   }
   return false;
 }
@@ -166,12 +167,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int kh = blockIdx.x % a.kv_heads;
-  int b, blk;
-  if (!find_block(a, blockIdx.x / a.kv_heads, lane, b, blk)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  blk = __builtin_amdgcn_readfirstlane(blk);
-  int first;
-  const int n = prompt_rows(a, b, first);
+  int b, blk, first, n;
+  if (!find_block(a, blockIdx.x / a.kv_heads, lane, b, blk, first, n)) return;
   const int chunks = (n + 31) / 32 * a.gqa;
 
   // the wave's chunk: 32 queries from 32 * place on, of one head (place -1: none)
@@ -249,13 +246,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
 #pragma unroll
     for (int e = 0; e < 16; ++e) O[j][e] = 0.0f;
 
-  uint32_t koff[KS], voff[NB];
+  // (a swizzle moves a unit within 16: beyond head dim 128 the second half lies 256 bytes on)
+  constexpr int KO = KS < 8 ? KS : 8, VO = NB < 4 ? NB : 4;
+  uint32_t koff[KO], voff[VO];
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) koff[ks] = (col * S::UNITS + k_unit<DP>(col, 2 * ks + half)) * 16;
+  for (int ks = 0; ks < KO; ++ks) koff[ks] = (col * S::UNITS + k_unit<DP>(col, 2 * ks + half)) * 16;
   {
     const int i = lane & 15, j = (lane >> 4) & 1, r = 4 * half + i / 4;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int nb = 0; nb < VO; ++nb)
       voff[nb] = (r * S::UNITS + v_unit<DP>(r, 4 * nb + 2 * j + (i & 3) / 2)) * 16 + 8 * (i & 1);
   }
 
@@ -267,17 +266,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
   auto scores = [&](uint32_t ktile, f16v &x) __attribute__((always_inline)) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const u4 k = *(const __attribute__((address_space(3))) u4 *)(base + (koff[ks] + ktile));
+      const u4 k = *(const __attribute__((address_space(3))) u4 *)(base + (koff[ks % KO] + ktile) + ks / KO * 256);
       x = W::mma(__builtin_bit_cast(T, k), q[ks], ks == 0 ? zero : x);
     }
   };
   // the exponents, less the running maximum: it moves when a score passes it by kTau
-  auto settle = [&](auto masks, f16v &x, int at) __attribute__((always_inline)) {
+  auto settle = [&](auto masks, f16v &x) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(x[e], a.scale_log2, -m);
-    // key 8g + 4 half + r of the tile is seen by the queries from it on
+    // on the diagonal, key 8g + 4 half + r is seen by the queries from it on
     if constexpr (decltype(masks)::value) {
-      const int sees = (place - at) * 32 + col - 4 * half;
+      const int sees = col - 4 * half;
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] = 8 * (e / 4) + e % 4 <= sees ? x[e] : -INFINITY;
     }
@@ -313,7 +312,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
-        O[nb] = W::mma(v_operand<DP, T>(base + (voff[nb] + vtile) + kk * 16 * DP * 2), p[kk], O[nb]);
+        O[nb] = W::mma(v_operand<DP, T>(base + (voff[nb % VO] + vtile) + kk * 16 * DP * 2 + nb / VO * 256), p[kk], O[nb]);
   };
   // where tile `at` lies: uniform offsets (of a stage, then of its second tile)
   auto ktile = [&](int at) __attribute__((always_inline)) {
@@ -331,61 +330,63 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
     if (s + 1 < stages) copy(s + 1);
   };
 
-  // ---- tiles that the wave's queries see whole, two at a time: a tile's weights and
-  // product go beside the next one's scores
-  const int whole = max(place, 0) & ~1;
-  if (whole > 0) {
+  // ---- the wave's tiles: a tile's weights and product go beside the next one's scores;
+  // the last one, on the diagonal, is masked
+  if (place >= 0) {
     f16v x, y;
     T p[2];
     turn(0);
     scores(ktile(0), x);
-    settle(std::false_type{}, x, 0);
-    int at = 1;
-    for (; at + 1 < whole; at += 2) {
-      if (S::TILES == 1) turn(at);
-      scores(ktile(at), y);
+    if (place == 0) {
+      settle(std::true_type{}, x);
+    } else {
+      settle(std::false_type{}, x);
+      int at = 1;
+      for (; at + 1 < place; at += 2) {
+        if (S::TILES == 1) turn(at);
+        scores(ktile(at), y);
+        weights(x, p);
+        product(vtile(at - 1), p);
+        settle(std::false_type{}, y);
+        turn((at + 1) / S::TILES);
+        scores(ktile(at + 1), x);
+        weights(y, p);
+        product(vtile(at), p);
+        settle(std::false_type{}, x);
+      }
+      if (at < place) {
+        if (S::TILES == 1) turn(at);
+        scores(ktile(at), y);
+        weights(x, p);
+        product(vtile(at - 1), p);
+        settle(std::false_type{}, y);
+        x = y;
+      }
+      if (place % S::TILES == 0) turn(place / S::TILES);
+      scores(ktile(place), y);
       weights(x, p);
-      product(vtile(at - 1), p);
-      settle(std::false_type{}, y, at);
-      turn((at + 1) / S::TILES);
-      scores(ktile(at + 1), x);
-      weights(y, p);
-      product(vtile(at), p);
-      settle(std::false_type{}, x, at + 1);
+      product(vtile(place - 1), p);
+      settle(std::true_type{}, y);
+      x = y;
     }
-    if (S::TILES == 1) turn(at);
-    scores(ktile(at), y);
     weights(x, p);
-    product(vtile(at - 1), p);
-    settle(std::false_type{}, y, at);
-    weights(y, p);
-    product(vtile(at), p);
-  }
-  // ---- and the rest
-  for (int at = whole; at < stages * S::TILES; ++at) {
-    if (at % S::TILES == 0) turn(at / S::TILES);
-    if (at > place) continue;
-    f16v x;
-    T p[2];
-    scores(ktile(at), x);
-    settle(std::true_type{}, x, at);
-    weights(x, p);
+    const uint32_t vlast = vtile(place);
     bool odd = false;  // infinities or NaN among the tile's values?
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        const u4 w = __builtin_bit_cast(u4, v_operand<DP, T>(base + (voff[nb] + vtile(at)) + kk * 16 * DP * 2));
+        const u4 w = __builtin_bit_cast(u4, v_operand<DP, T>(base + (voff[nb % VO] + vlast) + kk * 16 * DP * 2 + nb / VO * 256));
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7FFFu) >= W::kInf || (w[e] >> 16 & 0x7FFFu) >= W::kInf;
       }
     if (__builtin_expect(!__any(odd), 1)) {
-      product(vtile(at), p);
+      product(vlast, p);
     } else {
       // their products with the masked keys' zero weights must not be NaN: the finite
       // values go through the product; of the others, kind by kind, the keys that a
       // query sees are counted by one
-      const int sees = (place - at) * 32 + col - 4 * half;
+      const int sees = col - 4 * half;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
         T seen;
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
         for (int e = 0; e < 8; ++e) seen[e] = 8 * (2 * kk + e / 4) + e % 4 <= sees ? (E)1.0f : (E)0.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const T v = v_operand<DP, T>(base + (voff[nb] + vtile(at)) + kk * 16 * DP * 2);
+          const T v = v_operand<DP, T>(base + (voff[nb % VO] + vlast) + kk * 16 * DP * 2 + nb / VO * 256);
           uint16_t w[8];
           __builtin_memcpy(w, &v, 16);
           T part = v;
@@ -416,6 +417,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
       }
     }
   }
+
+  // the block's other waves may go further
+  for (int st = place < 0 ? 0 : place / S::TILES + 1; st < stages; ++st) turn(st);
 
   const int row = place * 32 + col;
   const float inv = 1.0f / xor32_add(l);
