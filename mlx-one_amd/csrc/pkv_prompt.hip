@@ -144,8 +144,6 @@ __device__ __forceinline__ void barrier() {
   asm volatile("s_barrier" ::: "memory");
 }
 
-typedef __attribute__((address_space(3))) uint8_t ldsbyte;
-
 // A lane's V^T operand (dim 32 nb + col, 16 keys) out of V's rows in LDS.
 template <int DP, typename T>
 __device__ __forceinline__ T v_operand(const ldsbyte *src) {
@@ -196,15 +194,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
     uint8_t *vdst = lds + (S::KBUF + s % S::VBUF) * S::SIDE + wave * 1024;
     const uint8_t *ksrc = kbase + (int64_t)s * S::KEYS * a.k_stride * 2;
     const uint8_t *vsrc = vbase + (int64_t)s * S::KEYS * a.v_stride * 2;
-    auto unit = [](const uint8_t *from, uint8_t *to) __attribute__((always_inline)) {
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)from,
-                                       (__attribute__((address_space(3))) uint32_t *)to, 16, 0, 0);
-    };
     if (a.dim == DP && (s + 1) * S::KEYS <= n) {  // whole rows, all of them there
 #pragma unroll
       for (int i = 0; i < S::COPIES; ++i) {
-        unit(ksrc + (int64_t)i * STEP * a.k_stride * 2 + kat[i * STEP / 16 % 2], kdst + i * 4096);
-        unit(vsrc + (int64_t)i * STEP * a.v_stride * 2 + vat, vdst + i * 4096);
+        copy_to_lds(ksrc + (int64_t)i * STEP * a.k_stride * 2, kat[i * STEP / 16 % 2], kdst + i * 4096);
+        copy_to_lds(vsrc + (int64_t)i * STEP * a.v_stride * 2, vat, vdst + i * 4096);
       }
       return;
     }
@@ -214,8 +208,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
     for (int i = 0; i < S::COPIES; ++i) {
       const int f = i * STEP / 16 % 2;
       const int64_t back = i * STEP - max(crow + i * STEP - (rows - 1), 0);
-      if (ku[f] < a.dim / 8) unit(ksrc + back * a.k_stride * 2 + kat[f], kdst + i * 4096);
-      if (vu < a.dim / 8) unit(vsrc + back * a.v_stride * 2 + vat, vdst + i * 4096);
+      if (ku[f] < a.dim / 8) copy_to_lds(ksrc + back * a.k_stride * 2 + kat[f], kdst + i * 4096);
+      if (vu < a.dim / 8) copy_to_lds(vsrc + back * a.v_stride * 2 + vat, vdst + i * 4096);
     }
   };
   if (a.dim < DP) {  // the units past the head dim hold zeros
@@ -384,8 +378,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
       product(vlast, p);
     } else {
       // their products with the masked keys' zero weights must not be NaN: the finite
-      // values go through the product; of the others, kind by kind, the keys that a
-      // query sees are counted by one
+      // values go through the product; the others are counted over the keys that a query
+      // sees, kind by kind in digits of 64
       const int sees = col - 4 * half;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) {
@@ -394,25 +388,19 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
         for (int e = 0; e < 8; ++e) seen[e] = 8 * (2 * kk + e / 4) + e % 4 <= sees ? (E)1.0f : (E)0.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          const T v = v_operand<DP, T>(base + (voff[nb % VO] + vlast) + kk * 16 * DP * 2 + nb / VO * 256);
+          T v = v_operand<DP, T>(base + (voff[nb % VO] + vlast) + kk * 16 * DP * 2 + nb / VO * 256), kind;
           uint16_t w[8];
           __builtin_memcpy(w, &v, 16);
-          T part = v;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) part[e] = (w[e] & 0x7FFF) >= W::kInf ? (E)0.0f : part[e];
-          O[nb] = W::mma(part, p[kk], O[nb]);
-#pragma unroll 1
-          for (int kind = 0; kind < 3; ++kind) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const bool hit = kind == 2 ? (w[e] & 0x7FFF) > W::kInf : w[e] == (W::kInf | (kind << 15));
-              part[e] = hit ? (E)1.0f : (E)0.0f;
-            }
-            const f16v count = W::mma(part, seen, zero);
-            const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
-#pragma unroll
-            for (int e = 0; e < 16; ++e) O[nb][e] += count[e] > 0.0f ? what : 0.0f;
+          for (int e = 0; e < 8; ++e) {
+            const bool bad = (w[e] & 0x7FFF) >= W::kInf;
+            kind[e] = !bad ? (E)0.0f : w[e] == W::kInf ? (E)1.0f : w[e] == (W::kInf | 0x8000) ? (E)64.0f : (E)4096.0f;
+            v[e] = bad ? (E)0.0f : v[e];
           }
+          O[nb] = W::mma(v, p[kk], O[nb]);
+          const f16v count = W::mma(kind, seen, zero);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) O[nb][e] += seen_kinds(count[e]);
         }
       }
     }

@@ -5,6 +5,29 @@
 
 namespace pkv {
 
+// What values that are not finite add to a sum: `count` holds how many are +inf, -inf and
+// NaN, in digits of 64.
+__device__ __forceinline__ float seen_kinds(float count) {
+  const int n = (int)count;
+  const bool plus = n & 63, minus = n >> 6 & 63, nan = n >> 12;
+  return nan || (plus && minus) ? __builtin_nanf("") : plus ? INFINITY : minus ? -INFINITY : 0.0f;
+}
+
+// Sixteen bytes of each active lane from memory to LDS at `to` + 16 lane (`to` alike for the
+// wave).  Written as an instruction, which has no result register: for the builtin the compiler
+// waits for every copy under way before any read of LDS.  The caller waits (vmcnt) before it
+// reads what was copied.  The second form reads at base + offset, base alike for the wave.
+typedef __attribute__((address_space(3))) uint8_t ldsbyte;
+__device__ __forceinline__ void copy_to_lds(const uint8_t *from, uint8_t *to) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ldsbyte *)to);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory", "m0");
+}
+__device__ __forceinline__ void copy_to_lds(const uint8_t *base, uint32_t offset, uint8_t *to) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(ldsbyte *)to);
+  // (a request reads scalars that a vector instruction wrote five wait states later at the soonest)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(at) : "memory", "m0");
+}
+
 struct RopeAppendArgs {
   Geo g;
   uint8_t *pool;
