@@ -13,11 +13,13 @@
 // runs as workgroups.  Its four waves take pairs of a run's tiles in turn:
 //   S^T = K.Q^T      v_mfma_f32_16x16x32, one tile: lane (row, jj) holds tokens 4jj + r
 //   O^T += V^T.P^T   v_mfma_f32_16x16x32, the pair's 32 tokens
-// K and V go from the pages straight to operand registers, codes as float16 (one rounding of
-// 2^-11 where scale and bias are applied, as the output's, or better), queries of quantized
-// pages as float16 scaled by a power of two per row, which is exact for what their scores
-// keep.  Scores, maxima, sums and parts are float32.  Weights are rounded to the operand type
-// (bfloat16 pages: as the sum of two), and summed as they enter the product.
+// K and V go from the pages straight to operand registers.  Quantized K enters as its codes
+// (1024 + c, exact in float16; queries as float16, each row scaled by a power of two, which
+// is exact for what its scores keep), group scales and biases are applied to the float32
+// scores:  s = sum_g scale_g (q_g . c'_g) + (bias_g - 1024 scale_g) sum(q_g).  Quantized V is
+// rounded once to float16 (2^-11).  Weights are rounded to the operand type, or, where that
+// would show in the result (bfloat16 pages, float16 results of quantized ones), enter as the
+// sum of two; they are summed as they enter.  Scores, maxima, sums and parts are float32.
 //
 // A token past a sequence's end or on an unmapped page is absent; one that a row may not see
 // yet changes nothing for it, not even where it is not finite.
@@ -32,7 +34,9 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTarget = 512;  // runs to aim at beyond one per segment: two for each of 256 CUs
+// Runs to aim at beyond one per segment: two workgroups for each of 256 CUs.  A tile of a
+// sequence's own comes from memory, a shared one mostly from a cache.
+constexpr int kTarget = 512, kSharedCost = 5, kOwnCost = 3;
 
 // Workspace: [member][8] descriptors, then per run its rows' (m, l) and sums of V.
 struct SharedParts {
@@ -61,7 +65,9 @@ struct SharedPlan {
   int group_tiles[kMaxShared];      // shared tiles
   int group_run[kMaxShared + 1];    // first run
   int own_run[kMaxShared + 1];      // a member's first run, counted behind the groups'
-  int reduce[2 * kWaves];
+  int sequence[kMaxShared];         // a member's sequence, -1 for none
+  int length[kMaxShared];           // its tokens
+  int reduce[3 * kWaves];
   int long_run, own_long;           // tiles per run
 };
 
@@ -70,19 +76,29 @@ __device__ __forceinline__ int seq_length(const SharedArgs &a, int b) {
 }
 __device__ __forceinline__ int tiles_of(int tokens) { return (tokens + PKV_TILE - 1) / PKV_TILE; }
 
-__device__ __forceinline__ int64_t block_sum(SharedPlan &p, int64_t v, int tid) {
-  // (two halves: every sum is below 2^46)
-  const int lo = wave_sum((int)(v & 0x7FFFFF)), hi = wave_sum((int)(v >> 23));
+// Runs of a segment, of about `most` tiles each.
+__device__ __forceinline__ int runs_of(int tiles, int most) { return (tiles + most - 1) / most; }
+// Tiles of each of n runs: whole turns of the waves' pairs.
+__device__ __forceinline__ int run_length(int tiles, int n) {
+  constexpr int turn = 2 * kWaves;
+  return ((tiles + n - 1) / n + turn - 1) / turn * turn;
+}
+
+// Sums over the workgroup.
+__device__ __forceinline__ void block_sum(SharedPlan &p, int64_t &v, int &x, int tid) {
+  // (v in two halves: it is below 2^46)
+  const int part[3] = {wave_sum((int)(v & 0x7FFFFF)), wave_sum((int)(v >> 23)), wave_sum(x)};
   __syncthreads();
-  if ((tid & 63) == 63) {
-    p.reduce[2 * (tid >> 6)] = lo;
-    p.reduce[2 * (tid >> 6) + 1] = hi;
-  }
+  if ((tid & 63) == 63)
+    for (int k = 0; k < 3; ++k) p.reduce[3 * (tid >> 6) + k] = part[k];
   __syncthreads();
-  int64_t s = 0;
+  v = 0;
+  x = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) s += (int64_t)p.reduce[2 * w] + ((int64_t)p.reduce[2 * w + 1] << 23);
-  return s;
+  for (int w = 0; w < kWaves; ++w) {
+    v += (int64_t)p.reduce[3 * w] + ((int64_t)p.reduce[3 * w + 1] << 23);
+    x += p.reduce[3 * w + 2];
+  }
 }
 
 // In-place exclusive sums of v[0..n), v[n] = the total.
@@ -107,7 +123,7 @@ __device__ __forceinline__ void block_scan(SharedPlan &p, int *v, int n, int tid
   __syncthreads();
 }
 
-// The last i with v[i] <= x, 0 <= i < n (v[0] <= x).
+// The last i with v[i] <= x, 0 <= i < n (v[0] <= x; v does not fall).
 __device__ __forceinline__ int last_at_most(const int *v, int n, int x) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
@@ -117,6 +133,12 @@ __device__ __forceinline__ int last_at_most(const int *v, int n, int x) {
   }
   return lo;
 }
+// The same, x alike for the wave.
+__device__ __forceinline__ int last_at_most_uniform(const int *v, int n, int x, int lane) {
+  int i = 0;
+  while (i + 64 < n && __builtin_amdgcn_readfirstlane(v[i + 64]) <= x) i += 64;
+  return i + __popcll(__ballot(i + lane < n && v[min(i + lane, n - 1)] <= x)) - 1;
+}
 
 __device__ __forceinline__ int row_blocks(const SharedArgs &a, const SharedPlan &p, int g, int per) {
   return (max(0, p.group_first[g + 1] - p.group_first[g]) * a.rows + per - 1) / per;
@@ -124,40 +146,55 @@ __device__ __forceinline__ int row_blocks(const SharedArgs &a, const SharedPlan 
 
 __device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p, int per, int tid) {
   for (int g = tid; g <= a.groups; g += kThreads) p.group_first[g] = min(max(a.group_starts[g], 0), a.count);
+  for (int g = tid; g < a.groups; g += kThreads) p.group_tiles[g] = a.prefix_lens[g];
+  for (int j = tid; j < a.count; j += kThreads) {
+    const int b = a.members[j];
+    const bool known = b >= 0 && b < a.batch;
+    p.sequence[j] = known ? b : -1;
+    p.length[j] = p.own_run[j] = known ? seq_length(a, b) : 0;
+  }
   __syncthreads();
-  int64_t shared = 0, own = 0;
+  int64_t cost = 0;
   for (int g = tid; g < a.groups; g += kThreads) {
     const int first = p.group_first[g], n = p.group_first[g + 1] - first;
-    int tiles = 0;
-    if (n > 1) {  // (one sequence shares nothing)
-      const int b = a.members[first];
-      if (b >= 0 && b < a.batch) tiles = max(0, min(a.prefix_lens[g], seq_length(a, b))) / PKV_TILE;
-    }
+    // (one sequence shares nothing)
+    const int tiles = n > 1 ? max(0, min(p.group_tiles[g], p.own_run[first])) / PKV_TILE : 0;
     p.group_tiles[g] = tiles;
-    shared += (int64_t)tiles * row_blocks(a, p, g, per) * a.g.hk;
+    cost += kSharedCost * (int64_t)tiles * row_blocks(a, p, g, per) * a.g.hk;
   }
   __syncthreads();
   const int last = p.group_first[a.groups];
   for (int j = tid; j < a.count; j += kThreads) {
-    int tiles = 0;
-    if (j >= p.group_first[0] && j < last) {
-      const int b = a.members[j];
-      if (b >= 0 && b < a.batch)
-        tiles = max(0, tiles_of(seq_length(a, b)) - p.group_tiles[last_at_most(p.group_first, a.groups, j)]);
-    }
-    p.own_run[j] = tiles;
-    own += (int64_t)tiles * a.g.hk;
+    const bool in = j >= p.group_first[0] && j < last;
+    const int tiles = in ? tiles_of(p.own_run[j]) - p.group_tiles[last_at_most(p.group_first, a.groups, j)] : 0;
+    p.own_run[j] = max(0, tiles);
+    cost += kOwnCost * (int64_t)p.own_run[j] * a.g.hk;
   }
-  shared = block_sum(p, shared, tid);
-  own = block_sum(p, own, tid);
-  // a shared tile's rows are many: it counts twice
-  const int64_t cost = (2 * shared + own + kTarget - 1) / kTarget;
-  const int step = 2 * kWaves;
-  const int long_run = (int)((cost / 2 + step) / step * step), own_long = (int)((cost + step) / step * step);
+  // Long enough runs that all of them are in flight together, as short as that allows: a
+  // segment's length is rounded up to whole runs, so each wave tries another allowance.
+  int segs = 0;
+  for (int g = tid; g < a.groups; g += kThreads) segs += p.group_tiles[g] > 0 ? row_blocks(a, p, g, per) * a.g.hk : 0;
+  for (int j = tid; j < a.count; j += kThreads) segs += p.own_run[j] > 0 ? a.g.hk : 0;
+  block_sum(p, cost, segs, tid);
+  auto lengths = [&](int k, int &long_run, int &own_long) {
+    const float each = (float)cost / (float)max(kTarget - (int)((int64_t)segs * (k + 1) / kWaves), kTarget / 4);
+    long_run = (int)fminf(each * (1.0f / kSharedCost), 1e9f) + 1;
+    own_long = (int)fminf(each * (1.0f / kOwnCost), 1e9f) + 1;
+  };
+  int long_run, own_long, count = 0;
+  lengths(tid >> 6, long_run, own_long);
+  for (int g = tid & 63; g < a.groups; g += 64) count += row_blocks(a, p, g, per) * runs_of(p.group_tiles[g], long_run);
+  for (int j = tid & 63; j < a.count; j += 64) count += runs_of(p.own_run[j], own_long);
+  count = wave_sum(count);
   __syncthreads();
+  if ((tid & 63) == 63) p.reduce[tid >> 6] = count;
+  __syncthreads();
+  int k = 0;
+  while (k < kWaves - 1 && (int64_t)p.reduce[k] * a.g.hk > kTarget) ++k;
+  lengths(k, long_run, own_long);
   for (int g = tid; g < a.groups; g += kThreads)
-    p.group_run[g] = row_blocks(a, p, g, per) * a.g.hk * ((p.group_tiles[g] + long_run - 1) / long_run);
-  for (int j = tid; j < a.count; j += kThreads) p.own_run[j] = a.g.hk * ((p.own_run[j] + own_long - 1) / own_long);
+    p.group_run[g] = row_blocks(a, p, g, per) * a.g.hk * runs_of(p.group_tiles[g], long_run);
+  for (int j = tid; j < a.count; j += kThreads) p.own_run[j] = a.g.hk * runs_of(p.own_run[j], own_long);
   if (tid == 0) {
     p.long_run = long_run;
     p.own_long = own_long;
@@ -188,6 +225,23 @@ struct SharedCfg : Cfg<BITS, DP, G, 1, FK, 1> {
   static constexpr int PAGE_BITS = BITS, GROUP = G;
 };
 
+// Bytes of one side of a pair of tiles: payloads and metadata.
+template <typename C>
+constexpr int side_bytes() { return 2 * 256 * C::LW + (C::QUANT ? 2 * 64 * C::NG : 0); }
+
+// Until at most N of the wave's requests to memory are under way; until LDS has been read.
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The lane, made anew: kept over the loop it goes to scratch memory, and reading it back there
+// waits for the requests before.
+__device__ __forceinline__ int lane_again() {
+  uint32_t l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(l));
+  return (int)l;
+}
+
 // One run of a segment: its tiles, rows and where they come from.
 struct Run {
   int kh, t0, t1;      // tiles [t0, t1)
@@ -198,72 +252,204 @@ struct Run {
   int slot;
 };
 
-// A pair of tiles in flight.
+struct __attribute__((aligned(16))) TilePlace {
+  int64_t head;
+  int tip;
+};
+
+// A pair of tiles in flight: payloads, and the metadata of a lane's four tokens.
 template <typename C>
 struct Pair {
   uint32_t k[2][C::LW], v[2][C::LW];
-  uint32_t km[2][C::NG], vm[2][C::QUANT ? 4 * C::NG : 1];
+  uint32_t km[2][C::MW], vm[2][C::MW];
 };
 
 template <typename C, int RB>
-__device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork &w, const Run &run, int lane, int wave,
-                                          float *s_acc, float (*s_ml)[shared_rows(64)][2]) {
+__device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork &w, const SharedPlan &plan, const Run &run,
+                                          int lane, int wave, TilePlace *where, uint8_t *lds, float (*s_ml)[shared_rows(64)][2]) {
   using T = typename C::T;
   using E = typename C::E;
   constexpr int KB = C::KB, NB = C::NB, NG = C::NG, DP = 32 * KB;
+  constexpr int GB = C::QUANT ? C::GROUP / 32 : KB;  // 32-element blocks per accumulator
   const Geo &g = a.g;
   const int col = lane & 15, jj = lane >> 4;
   const int tpp = g.page / PKV_TILE;
 
+  // ---- the wave's pairs: tiles t0 + 2 (wave + 4 i), + 1.  LDS keeps where 32 pairs' tiles
+  // are: the tile in its page, -1 for none, and the page's head.
+  constexpr int kTileBytes = 256 * C::LW;
+  const int pairs = (run.t1 - run.t0 + 1) / 2;
+  auto window = [&](int i0) __attribute__((always_inline)) {
+    const int t = run.t0 + 2 * (wave + kWaves * (i0 + lane / 2)) + (lane & 1), page = t / tpp;
+    int id = -1;
+    if (t < run.t1) id = a.table[(int64_t)run.b * a.max_pages + page];
+    const bool there = id >= 0 && id < a.num_pages;
+    where[lane].head = (int64_t)(there ? id : 0) * g.page_bytes + (int64_t)run.kh * g.head_bytes;
+    where[lane].tip = there ? t - page * tpp : -1;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  // A pair's K and V are requested a pair ahead: into registers of their own for one block of
+  // rows; for two, whose accumulators take that room, into LDS, each side as soon as the pair
+  // before has been read from there.
+  constexpr bool STAGED = RB > 1;
+  Pair<C> p, next;
+  int next_there = 0;
+  const uint8_t *heads[2];  // the requested pair's tiles
+  int tips[2];
+  auto locate = [&](int i) __attribute__((always_inline)) {
+    next_there = 0;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const TilePlace at = where[2 * (i & 31) + s];
+      const int tip = __builtin_amdgcn_readfirstlane(at.tip);
+      const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)at.head);
+      const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(at.head >> 32));
+      if (tip >= 0) next_there |= 1 << s;
+      tips[s] = max(tip, 0);
+      heads[s] = a.pool + (int64_t)((uint64_t)hi << 32 | lo);
+    }
+  };
+  auto fetch = [&](Pair<C> &to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      load_payload<C, true>(to.k[s], heads[s] + tips[s] * kTileBytes, lane);
+      load_payload<C, true>(to.v[s], heads[s] + g.v_offset + tips[s] * kTileBytes, lane);
+      if constexpr (C::QUANT) {
+        load_meta<C, true>(to.km[s], heads[s] + g.kmeta_offset + tips[s] * (PKV_TILE * NG * 4) + 16 * NG * jj);
+        load_meta<C, true>(to.vm[s], heads[s] + g.vmeta_offset + tips[s] * (PKV_TILE * NG * 4) + 16 * NG * jj);
+      }
+    }
+  };
+  // One side of a pair: two tiles' payloads, then two tiles' metadata.
+  constexpr int kSide = side_bytes<C>(), kCopies = C::LW / 2 + (C::QUANT ? 1 : 0);
+  uint8_t *const ring = lds + wave * 2 * kSide;
+  auto stage = [&](int64_t payload, int64_t meta, uint8_t *to) __attribute__((always_inline)) {
+    const int lane = lane_again();
+#pragma unroll
+    for (int c = 0; c < C::LW / 2; ++c) {
+      if constexpr (kTileBytes >= 1024) {
+        const int s = c * 1024 / kTileBytes;
+        copy_to_lds(heads[s] + (payload + tips[s] * kTileBytes + c * 1024 % kTileBytes), lane * 16, to + c * 1024);
+      } else {
+        copy_to_lds(lane < 32 ? heads[0] + (payload + tips[0] * kTileBytes) + lane * 16
+                              : heads[1] + (payload + tips[1] * kTileBytes) + (lane - 32) * 16, to + c * 1024);
+      }
+    }
+    if constexpr (C::QUANT) {
+      constexpr int per = 4 * NG;  // lanes for a tile's
+      const uint8_t *from = lane < per ? heads[0] + (meta + tips[0] * (16 * per)) + lane * 16
+                                       : heads[1] + (meta + tips[1] * (16 * per)) + (lane - per) * 16;
+      if (lane < 2 * per) copy_to_lds(from, to + 2 * kTileBytes);
+    }
+  };
+  auto stage_k = [&]() __attribute__((always_inline)) { stage(0, g.kmeta_offset, ring); };
+  auto stage_v = [&]() __attribute__((always_inline)) { stage(g.v_offset, g.vmeta_offset, ring + kSide); };
+  auto take = [&](const uint8_t *from, uint32_t (&words)[2][C::LW], uint32_t (&meta)[2][C::MW]) __attribute__((always_inline)) {
+    const int lane = lane_again(), jj = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      load_payload<C, false>(words[s], from + s * kTileBytes, lane);
+      if constexpr (C::QUANT) load_meta<C, false>(meta[s], from + 2 * kTileBytes + (s * 4 + jj) * (16 * NG));
+    }
+  };
+  if (wave < pairs) window(0);
+
   // ---- rows: operands, how far each sees
-  T q[RB][KB];
-  float mult[RB];
+  T q[RB][KB];  // (two blocks of rows: kept in LDS)
+  float mult[RB], qs[RB][NG];
   int lim[RB];
+  uint16_t raw[RB][KB][8];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     const int r = run.row0 + rb * 16 + col;
     const bool there = rb * 16 + col < run.rows;
-    const int member = run.member + (there ? r / a.rows : 0), in = there ? r % a.rows : 0;
-    int b = a.members[member];
-    const bool known = there && b >= 0 && b < a.batch;
-    b = known ? b : 0;
-    const int qi = in / a.gqa, h = run.kh * a.gqa + in % a.gqa;
-    const int L = seq_length(a, b), width = a.widths ? a.widths[b] : a.nq;
-    const int pos = a.q_pos ? a.q_pos[(int64_t)b * a.nq + qi] : a.seq_lens[b] - width + qi;
-    lim[rb] = known && qi < width ? min(pos, L - 1) : -1;
-    const uint16_t *src = a.q + (((int64_t)b * a.heads + h) * a.nq + qi) * g.dim;
-    uint16_t raw[KB][8];
+    const int member = there ? r / a.rows : 0, in = there ? r - member * a.rows : 0;
+    const int b = plan.sequence[run.member + member];
+    const int qi = in / a.gqa, h = run.kh * a.gqa + in - qi * a.gqa, at = max(b, 0);
+    const int L = plan.length[run.member + member];
+    const int width = a.widths ? a.widths[at] : a.nq;
+    const int pos = a.q_pos ? a.q_pos[(int64_t)at * a.nq + qi] : a.seq_lens[at] - width + qi;
+    lim[rb] = there && b >= 0 && qi < width ? min(pos, L - 1) : -1;
+    const uint16_t *src = a.q + (((int64_t)at * a.heads + h) * a.nq + qi) * g.dim;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       const int d0 = 32 * kb + 8 * jj;
       if ((g.dim & 7) == 0 && ((uintptr_t)a.q & 15) == 0) {
         u4 x = {0, 0, 0, 0};
-        if (lim[rb] >= 0 && d0 < g.dim) x = *(const u4 *)(src + d0);
-        __builtin_memcpy(raw[kb], &x, 16);
+        if (there && d0 < g.dim) x = *(const u4 *)(src + d0);
+        __builtin_memcpy(raw[rb][kb], &x, 16);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) raw[kb][e] = lim[rb] >= 0 && d0 + e < g.dim ? src[d0 + e] : (uint16_t)0;
+        for (int e = 0; e < 8; ++e) raw[rb][kb][e] = there && d0 + e < g.dim ? src[d0 + e] : (uint16_t)0;
       }
     }
+  }
+  if constexpr (STAGED) __syncthreads();  // (the plan's memory is taken)
+  if (wave < pairs) {
+    locate(0);
+    if constexpr (STAGED) {
+      stage_k();
+      stage_v();
+    } else {
+      fetch(next);
+    }
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
     mult[rb] = a.scale * kLog2e;
     if constexpr (!C::QUANT) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) __builtin_memcpy(&q[rb][kb], raw[kb], 16);
+      for (int kb = 0; kb < KB; ++kb) __builtin_memcpy(&q[rb][kb], raw[rb][kb], 16);
+      qs[rb][0] = 0.0f;
     } else {
-      // float16 operands: a row's largest element to [2^7, 2^8)
-      float most = 0.0f;
+      if (g.float_kind == 1) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) __builtin_memcpy(&q[rb][kb], raw[rb][kb], 16);
+      } else {
+        // bfloat16 to float16: a row's largest element to [2^7, 2^8)
+        typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+        us2 tops = {0, 0};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2)
+            tops = __builtin_elementwise_max(tops, us2{raw[rb][kb][e], raw[rb][kb][e + 1]} & (uint16_t)0x7FFF);
+        const float most = xor32_max(xor16_max(bits_to_float(max(tops.x, tops.y), 0)));
+        const int shift = most > 0.0f && most < INFINITY ? min(8 - __builtin_amdgcn_frexp_expf(most), 126) : 0;
+        mult[rb] = ldexpf(mult[rb], -shift);
+        const float by = __int_as_float((127 + shift) << 23);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            // (exact down to float16's smallest step, 2^-31 of the row's largest)
+            const auto two = __builtin_amdgcn_cvt_pkrtz(bits_to_float(raw[rb][kb][e], 0) * by,
+                                                        bits_to_float(raw[rb][kb][e + 1], 0) * by);
+            q[rb][kb][e] = (_Float16)two[0];
+            q[rb][kb][e + 1] = (_Float16)two[1];
+          }
+      }
+#pragma unroll
+      for (int x = 0; x < NG; ++x) qs[rb][x] = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(bits_to_float(raw[kb][e], g.float_kind)));
-      most = xor32_max(xor16_max(most));
-      const int shift = most > 0.0f && most < INFINITY ? 8 - __builtin_amdgcn_frexp_expf(most) : 0;
-      mult[rb] = ldexpf(mult[rb], -shift);
+        for (int e = 0; e < 8; e += 2)
+          qs[rb][kb / GB] = __builtin_amdgcn_fdot2(h2{q[rb][kb][e], q[rb][kb][e + 1]}, h2{(_Float16)1.0f, (_Float16)1.0f}, qs[rb][kb / GB], false);
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q[rb][kb][e] = (_Float16)ldexpf(bits_to_float(raw[kb][e], g.float_kind), shift);
+      for (int x = 0; x < NG; ++x) qs[rb][x] = xor32_add(xor16_add(qs[rb][x]));
     }
+  }
+  const uint32_t q_at = (uint32_t)lane * 8;  // operand (rb, kb): kept[(rb * KB + kb) * 512 + q_at]
+  uint16_t *kept = (uint16_t *)(lds + kWaves * 2 * kSide);
+  if constexpr (RB > 1) {
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      if (wave == rb)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) *(T *)(kept + (rb * KB + kb) * 512 + q_at) = q[rb][kb];
+    __syncthreads();
   }
   int least = 0x7FFFFFFF;  // every live row sees the tokens up to it
 #pragma unroll
@@ -273,129 +459,93 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
   least = __builtin_amdgcn_readfirstlane(least);
 
   float m[RB], thr[RB];
-  f4 O[RB][NB], sum[RB];
+  f4 O[RB][NB];
+  float sum[RB];  // the lane's tokens'
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     m[rb] = 0.0f;
     thr[rb] = -INFINITY;
-    sum[rb] = f4{0, 0, 0, 0};
+    sum[rb] = 0.0f;
 #pragma unroll
     for (int n = 0; n < NB; ++n) O[rb][n] = f4{0, 0, 0, 0};
   }
   const f4 zero = register_zero();
-  T ones;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) ones[e] = (E)1.0f;
+  // whether weights enter as the sum of two operands
+  const bool split = C::QUANT ? g.float_kind == 1 : !C::F16;
 
-  // ---- the wave's pairs: tiles t0 + 2 (wave + 4 i), + 1.  Lane l keeps the page of its
-  // tile l (of pair l / 2) among 32 pairs.
-  const int pairs = (run.t1 - run.t0 + 1) / 2;
-  int pages = -1;
-  auto window = [&](int i0) __attribute__((always_inline)) {
-    const int t = run.t0 + 2 * (wave + kWaves * (i0 + lane / 2)) + (lane & 1);
-    pages = t < run.t1 ? a.table[(int64_t)run.b * a.max_pages + t / tpp] : -1;
-    if (pages >= a.num_pages) pages = -1;
-  };
-  Pair<C> next;
-  int next_there = 0;
-  auto fetch = [&](int i) __attribute__((always_inline)) {
-    next_there = 0;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int id = __builtin_amdgcn_readlane(pages, 2 * (i & 31) + s);
-      if (id >= 0) next_there |= 1 << s;
-      const int t = run.t0 + 2 * (wave + kWaves * i) + s;
-      const uint8_t *head = a.pool + (int64_t)max(id, 0) * g.page_bytes + (int64_t)run.kh * g.head_bytes;
-      const int tip = t % tpp;
-      load_payload<C>(next.k[s], head + tip * g.tile_bytes, lane);
-      load_payload<C>(next.v[s], head + g.v_offset + tip * g.tile_bytes, lane);
-      if constexpr (C::QUANT) {
-        const uint32_t *km = (const uint32_t *)(head + g.kmeta_offset) + (tip * PKV_TILE + col) * NG;
-#pragma unroll
-        for (int x = 0; x < NG; ++x) next.km[s][x] = km[x];
-        const u4 *vm = (const u4 *)(head + g.vmeta_offset + (tip * PKV_TILE + 4 * jj) * NG * 4);
-#pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          const u4 y = vm[x];
-          next.vm[s][4 * x] = y.x; next.vm[s][4 * x + 1] = y.y; next.vm[s][4 * x + 2] = y.z; next.vm[s][4 * x + 3] = y.w;
-        }
-      }
-    }
-  };
-  if (wave < pairs) {
-    window(0);
-    fetch(0);
-  }
-  for (int i = 0; wave + kWaves * i < pairs; ++i) {
-    Pair<C> p = next;
+  // One pair.  CAREFUL: tokens of it are absent, or hidden from some row.
+  auto pair = [&](int i, auto careful) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    const bool more = wave + kWaves * (i + 1) < pairs;
     const int there = next_there;
-    if (wave + kWaves * (i + 1) < pairs) {
-      if (((i + 1) & 31) == 0) window(i + 1);
-      fetch(i + 1);
+    if constexpr (!STAGED) {
+      p = next;
+      if (more) {
+        if (((i + 1) & 31) == 0) window(i + 1);
+        locate(i + 1);
+        fetch(next);
+      }
+    } else {
+      wait_loads<kCopies>();
+      take(ring, p.k, p.km);
     }
     const int tok0 = (run.t0 + 2 * (wave + kWaves * i)) * PKV_TILE;  // the pair's first token
-    const bool masked = there != 3 || tok0 + 2 * PKV_TILE - 1 > least;
-    if (masked) {
-      // absent tokens hold zeros
+
+    // S^T = K.Q^T, and the scores from it
+    const uint32_t q_at = RB > 1 ? lane_again() * 8 : 0;  // (read again for each pair)
+    auto query = [&](int rb, int kb) __attribute__((always_inline)) {
+      if constexpr (RB > 1) return *(const T *)(kept + (rb * KB + kb) * 512 + q_at);
+      else return q[rb][kb];
+    };
+    float x[RB][8];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const bool here = there >> s & 1;
-        const int t = tok0 + s * PKV_TILE;
+    for (int s = 0; s < 2; ++s) {
+      f4 S[RB][NG];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        T k;
+        if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (C::QUANT) k = Conv<C::PAGE_BITS>::kop(p.k[s], kb);  // 1024 + code
+        else k = __builtin_bit_cast(T, u4{p.k[s][4 * kb], p.k[s][4 * kb + 1], p.k[s][4 * kb + 2], p.k[s][4 * kb + 3]});
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          S[rb][kb / GB] = mma(k, query(rb, kb), kb % GB == 0 ? zero : S[rb][kb / GB]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
         if constexpr (C::QUANT) {
-          const bool kt = here && t + col < run.L;
 #pragma unroll
-          for (int x = 0; x < NG; ++x) p.km[s][x] = kt ? p.km[s][x] : 0u;
+          for (int x_ = 0; x_ < NG; ++x_) {
+            const h2 sb = __builtin_bit_cast(h2, p.km[s][e * NG + x_]);
+            const float sc = (float)sb.x, off = __builtin_fmaf(-1024.0f, sc, (float)sb.y);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int x = 0; x < NG; ++x) p.vm[s][e * NG + x] = here && t + 4 * jj + e < run.L ? p.vm[s][e * NG + x] : 0u;
-        } else {
-          const uint32_t kmask = here && t + col < run.L ? 0xFFFFFFFFu : 0u;
-          uint32_t vmask[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            vmask[e] = (here && t + 4 * jj + 2 * e < run.L ? 0xFFFFu : 0u) |
-                       (here && t + 4 * jj + 2 * e + 1 < run.L ? 0xFFFF0000u : 0u);
-#pragma unroll
-          for (int x = 0; x < C::LW; ++x) {
-            p.k[s][x] &= kmask;
-            p.v[s][x] &= vmask[x & 1];
+            for (int rb = 0; rb < RB; ++rb)
+              x[rb][4 * s + e] = __builtin_fmaf(S[rb][x_][e], sc, x_ == 0 ? off * qs[rb][x_] : __builtin_fmaf(off, qs[rb][x_], x[rb][4 * s + e]));
           }
+        } else {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) x[rb][4 * s + e] = S[rb][0][e];
         }
       }
     }
 
-    // S^T = K.Q^T
-    f4 S[2][RB];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) S[s][rb] = zero;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        T k;
-        if constexpr (C::QUANT) {
-          const h2 sb = __builtin_bit_cast(h2, p.km[s][32 * kb / C::GROUP]);
-          const h8 c = Conv<C::PAGE_BITS>::kop(p.k[s], kb) - (h8)(_Float16)1024.0f;
-          k = __builtin_elementwise_fma(c, (h8)sb.x, (h8)sb.y);
-        } else {
-          k = __builtin_bit_cast(T, u4{p.k[s][4 * kb], p.k[s][4 * kb + 1], p.k[s][4 * kb + 2], p.k[s][4 * kb + 3]});
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) S[s][rb] = mma(k, q[rb][kb], S[s][rb]);
+    if constexpr (STAGED) {
+      if (more) {
+        if (((i + 1) & 31) == 0) window(i + 1);
+        locate(i + 1);
+        wait_lds();
+        stage_k();
       }
+    }
 
     // softmax: a lane's 8 tokens of its row
-    float x[RB][8];
     float mx[RB];
     bool need = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[rb][e] = __builtin_fmaf(S[e >> 2][rb][e & 3], mult[rb], -m[rb]);
-      if (masked) {
+      for (int e = 0; e < 8; ++e) x[rb][e] = __builtin_fmaf(x[rb][e], mult[rb], -m[rb]);
+      if constexpr (CAREFUL) {
         const int sees = lim[rb] - tok0 - 4 * jj;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -408,7 +558,7 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
       for (int e = 1; e < 8; ++e) mx[rb] = __builtin_elementwise_maximum(mx[rb], x[rb][e]);
       need |= mx[rb] > thr[rb];
     }
-    if (__any(need)) {
+    if (__builtin_expect(__any(need), 0)) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         const float up = xor32_max(xor16_max(mx[rb]));
@@ -424,24 +574,37 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
         for (int n = 0; n < NB; ++n) O[rb][n] *= alpha;
       }
     }
-    constexpr bool SPLIT = !C::F16;  // bfloat16 weights as the sum of two
-    T P[RB], low[SPLIT ? RB : 1];
+    // (the sum is that of the weights as they enter the product)
+    T P[RB], low[RB];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = __builtin_amdgcn_exp2f(x[rb][e]);
-        P[rb][e] = (E)y;
-        if constexpr (SPLIT) low[rb][e] = (E)(y - (float)P[rb][e]);
+        x[rb][e] = __builtin_amdgcn_exp2f(x[rb][e]);
+        P[rb][e] = (E)x[rb][e];
       }
-      sum[rb] = mma(ones, P[rb], sum[rb]);
-      if constexpr (SPLIT) sum[rb] = mma(ones, low[rb], sum[rb]);
+    if (split) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          low[rb][e] = (E)(x[rb][e] - (float)P[rb][e]);
+          sum[rb] += x[rb][e];
+        }
+    } else {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[rb] += (float)P[rb][e];
     }
 
-    // O^T += V^T.P^T
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      T v;
+    if constexpr (STAGED) {
+      if (more) wait_loads<kCopies>();
+      else wait_loads<0>();
+      take(ring + kSide, p.v, p.vm);
+    }
+    // V's operand of dims 16n ..
+    auto value = [&](int n) __attribute__((always_inline)) {
       if constexpr (C::QUANT) {
         constexpr int per = C::GROUP / 16;
         h4 half[2];
@@ -456,66 +619,112 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
           }
           half[s] = __builtin_elementwise_fma(Conv<C::PAGE_BITS>::vop(p.v[s], n) - (h4)(_Float16)1024.0f, sc, bi);
         }
-        v = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        return (T)__builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
       } else {
-        v = __builtin_bit_cast(T, u4{p.v[0][2 * n], p.v[0][2 * n + 1], p.v[1][2 * n], p.v[1][2 * n + 1]});
+        return __builtin_bit_cast(T, u4{p.v[0][2 * n], p.v[0][2 * n + 1], p.v[1][2 * n], p.v[1][2 * n + 1]});
       }
-      bool odd = false;
-      if (masked) {
-        const u4 bits = __builtin_bit_cast(u4, v);
+    };
+    [[maybe_unused]] bool odd = false;
+    if constexpr (CAREFUL) {
+      // absent tokens hold zeros; are there infinities or NaN among the others?
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int t = (there >> s & 1) ? run.L - tok0 - s * PKV_TILE - 4 * jj : 0;  // the lane's tokens there
+        if constexpr (C::QUANT) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int x_ = 0; x_ < NG; ++x_) p.vm[s][e * NG + x_] = e < t ? p.vm[s][e * NG + x_] : 0u;
+        } else {
+#pragma unroll
+          for (int x_ = 0; x_ < C::LW; ++x_)
+            p.v[s][x_] &= (2 * (x_ & 1) < t ? 0xFFFFu : 0u) | (2 * (x_ & 1) + 1 < t ? 0xFFFF0000u : 0u);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const u4 bits = __builtin_bit_cast(u4, value(n));
 #pragma unroll
         for (int e = 0; e < 4; ++e) odd |= (bits[e] & 0x7FFFu) >= C::INF || (bits[e] >> 16 & 0x7FFFu) >= C::INF;
       }
-      if (!__any(odd)) {
+    }
+
+    // O^T += V^T.P^T
+    if (CAREFUL && __builtin_expect(__any(odd), 0)) {
+      // infinities and NaN: their products with a hidden token's zero weight must not be
+      // NaN.  The finite values go through the product; the others are counted over the
+      // tokens that a row sees, kind by kind in digits of 64 (there are 32 tokens).
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          O[rb][n] = mma(v, P[rb], O[rb][n]);
-          if constexpr (SPLIT) O[rb][n] = mma(v, low[rb], O[rb][n]);
-        }
-      } else {
-        // infinities and NaN: their products with a hidden token's zero weight must not be
-        // NaN.  The finite values go through the product; of the others, kind by kind,
-        // the tokens that a row sees are counted by one.
+      for (int n = 0; n < NB; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        T v = value(n), kind;
         uint16_t bits[8];
         __builtin_memcpy(bits, &v, 16);
 #pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool bad = (bits[e] & 0x7FFF) >= C::INF;
+          kind[e] = !bad ? (E)0.0f : bits[e] == C::INF ? (E)1.0f : bits[e] == (C::INF | 0x8000) ? (E)64.0f : (E)4096.0f;
+          v[e] = bad ? (E)0.0f : v[e];
+        }
+#pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           const int sees = lim[rb] - tok0 - 4 * jj;
-          T part, seen;
+          T seen;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            part[e] = (bits[e] & 0x7FFF) >= C::INF ? (E)0.0f : v[e];
-            seen[e] = PKV_TILE * (e >> 2) + (e & 3) <= sees ? (E)1.0f : (E)0.0f;
-          }
-          O[rb][n] = mma(part, P[rb], O[rb][n]);
-          if constexpr (SPLIT) O[rb][n] = mma(part, low[rb], O[rb][n]);
-#pragma unroll 1
-          for (int kind = 0; kind < 3; ++kind) {
+          for (int e = 0; e < 8; ++e) seen[e] = PKV_TILE * (e >> 2) + (e & 3) <= sees ? (E)1.0f : (E)0.0f;
+          O[rb][n] = mma(v, P[rb], O[rb][n]);
+          if (split) O[rb][n] = mma(v, low[rb], O[rb][n]);
+          const f4 count = mma(kind, seen, zero);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const bool hit = kind == 2 ? (bits[e] & 0x7FFF) > C::INF : bits[e] == (C::INF | (kind << 15));
-              part[e] = hit ? (E)1.0f : (E)0.0f;
-            }
-            const f4 count = mma(part, seen, zero);
-            const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
-#pragma unroll
-            for (int e = 0; e < 4; ++e) O[rb][n][e] += count[e] > 0.0f ? what : 0.0f;
-          }
+          for (int e = 0; e < 4; ++e) O[rb][n][e] += seen_kinds(count[e]);
         }
       }
+    } else if (split) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);
+        const T v = value(n);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) O[rb][n] = mma(v, low[rb], mma(v, P[rb], O[rb][n]));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);
+        const T v = value(n);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) O[rb][n] = mma(v, P[rb], O[rb][n]);
+      }
     }
+    if constexpr (STAGED) {
+      if (more) {
+        wait_lds();
+        stage_v();
+      }
+    }
+  };
+  // (the pairs that need care are a run's last, but for missing pages)
+  int i = 0;
+  for (; wave + kWaves * i < pairs; ++i) {
+    const int last_token = (run.t0 + 2 * (wave + kWaves * i)) * PKV_TILE + 2 * PKV_TILE - 1;
+    if (__builtin_expect(next_there != 3 || last_token > least, 0)) break;
+    pair(i, std::false_type());
   }
+  for (; wave + kWaves * i < pairs; ++i) pair(i, std::true_type());
 
   // ---- the four waves' parts joined, 16 rows at a time, and written
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
+  for (int rb = 0; rb < RB; ++rb) {
+    sum[rb] = xor32_add(xor16_add(sum[rb]));
     if (jj == 0) {
       // (a row that sees nothing has none, whatever went through its lanes)
       s_ml[wave][rb * 16 + col][0] = thr[rb] == -INFINITY || lim[rb] < 0 ? -INFINITY : m[rb];
-      s_ml[wave][rb * 16 + col][1] = sum[rb][0];
+      s_ml[wave][rb * 16 + col][1] = sum[rb];
     }
+  }
   __syncthreads();
   constexpr int ROW = DP + 4;
+  float *s_acc = (float *)lds;
   const int tid = wave * 64 + lane;
   float *acc = w.acc + (int64_t)run.slot * shared_rows(DP) * DP;
   float *ml = w.ml + (int64_t)run.slot * shared_rows(DP) * 2;
@@ -559,12 +768,17 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
 }
 
 template <int BITS, int DP, int G, int FK>
-__global__ __launch_bounds__(kThreads, 1) void shared_kernel(const SharedArgs a, const SharedWork w) {
+__global__ __launch_bounds__(kThreads, 2) void shared_kernel(const SharedArgs a, const SharedWork w) {
   using C = SharedCfg<BITS, DP, G, FK>;
   constexpr int PER = shared_rows(DP);
-  __shared__ SharedPlan plan;
-  __shared__ __attribute__((aligned(16))) float s_acc[kWaves * 16 * (DP + 4)];
+  // the plan; behind it the copies and the rows of two blocks; behind those the sums
+  constexpr int kRing = PER > 16 ? kWaves * 2 * side_bytes<C>() + 2 * C::KB * 1024 : 0;
+  constexpr int kSums = kWaves * 16 * (DP + 4) * 4;
+  constexpr int kLds = std::max({(int)sizeof(SharedPlan), kRing, kSums});
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+  SharedPlan &plan = *(SharedPlan *)lds;
   __shared__ float s_ml[kWaves][shared_rows(64)][2];
+  __shared__ TilePlace s_place[kWaves][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   lay_out(a, w, plan, PER, tid);
   const int shared_runs = plan.group_run[a.groups], runs = shared_runs + plan.own_run[a.count];
@@ -576,86 +790,122 @@ __global__ __launch_bounds__(kThreads, 1) void shared_kernel(const SharedArgs a,
       const int g = in ? last_at_most(plan.group_first, a.groups, j) : 0;
       int32_t *d = w.desc + 8 * j;
       d[0] = plan.group_run[g];
-      d[1] = in ? (plan.group_tiles[g] + plan.long_run - 1) / plan.long_run : 0;
+      d[1] = in ? runs_of(plan.group_tiles[g], plan.long_run) : 0;
       d[2] = (j - plan.group_first[g]) * a.rows;
       d[3] = shared_runs + plan.own_run[j];
       d[4] = (plan.own_run[j + 1] - plan.own_run[j]) / a.g.hk;
       d[5] = in;
     }
   }
-  for (int u = blockIdx.x; u < runs && u < w.most; u += gridDim.x) {
+  const int u = blockIdx.x;
+  if (u < runs && u < w.most) {
     Run run;
     run.slot = u;
     if (u < shared_runs) {
-      const int g = last_at_most(plan.group_run, a.groups, u);
-      const int n = (plan.group_tiles[g] + plan.long_run - 1) / plan.long_run, at = u - plan.group_run[g];
-      const int seg = at / n, c = at - seg * n, blk = seg / a.g.hk;
+      const int g = last_at_most_uniform(plan.group_run, a.groups, u, lane);
+      const int tiles = plan.group_tiles[g], n = runs_of(tiles, plan.long_run), at = u - plan.group_run[g];
+      const int seg = at / n, blk = seg / a.g.hk, len = run_length(tiles, n);
       run.kh = seg - blk * a.g.hk;
-      run.t0 = c * plan.long_run;
-      run.t1 = min(plan.group_tiles[g], run.t0 + plan.long_run);
+      run.t0 = min((at - seg * n) * len, tiles);
+      run.t1 = min(tiles, run.t0 + len);
       run.member = plan.group_first[g];
       run.row0 = blk * PER;
       run.rows = min(PER, (plan.group_first[g + 1] - run.member) * a.rows - run.row0);
     } else {
-      const int j = last_at_most(plan.own_run, a.count, u - shared_runs);
+      const int j = last_at_most_uniform(plan.own_run, a.count, u - shared_runs, lane);
       const int n = (plan.own_run[j + 1] - plan.own_run[j]) / a.g.hk, at = u - shared_runs - plan.own_run[j];
-      const int g = last_at_most(plan.group_first, a.groups, j);
+      const int g = last_at_most_uniform(plan.group_first, a.groups, j, lane);
       run.kh = at / n;
-      const int c = at - run.kh * n;
-      run.t0 = plan.group_tiles[g] + c * plan.own_long;
-      run.t1 = min(tiles_of(seq_length(a, a.members[j])), run.t0 + plan.own_long);
+      const int first = plan.group_tiles[g], end = tiles_of(plan.length[j]), len = run_length(end - first, n);
+      run.t0 = min(first + (at - run.kh * n) * len, end);
+      run.t1 = min(end, run.t0 + len);
       run.member = j;
       run.row0 = 0;
       run.rows = a.rows;
     }
-    run.b = __builtin_amdgcn_readfirstlane(a.members[run.member]);
-    run.L = __builtin_amdgcn_readfirstlane(seq_length(a, run.b));
+    // (a member that is no sequence has no tokens; the first of a group with a prefix is one)
+    run.b = max(0, __builtin_amdgcn_readfirstlane(plan.sequence[run.member]));
+    run.L = __builtin_amdgcn_readfirstlane(plan.length[run.member]);
     run.kh = __builtin_amdgcn_readfirstlane(run.kh);
     run.t0 = __builtin_amdgcn_readfirstlane(run.t0);
     run.t1 = __builtin_amdgcn_readfirstlane(run.t1);
     run.member = __builtin_amdgcn_readfirstlane(run.member);
     run.row0 = __builtin_amdgcn_readfirstlane(run.row0);
     run.rows = __builtin_amdgcn_readfirstlane(run.rows);
-    if (run.rows <= 16) run_tiles<C, 1>(a, w, run, lane, wave, s_acc, s_ml);
-    else if constexpr (PER > 16) run_tiles<C, 2>(a, w, run, lane, wave, s_acc, s_ml);
+    if (run.rows <= 16) run_tiles<C, 1>(a, w, plan, run, lane, wave, s_place[wave], lds, s_ml);
+    else if constexpr (PER > 16) run_tiles<C, 2>(a, w, plan, run, lane, wave, s_place[wave], lds, s_ml);
   }
 }
 
-// One wave per (member, KV head, row): the row's parts joined.
+// One wave per (member, KV head, row): the row's parts joined.  Lane l weighs part l (of 64 at
+// a time); the parts' rows are read eight at a time.
 template <int DP>
 __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedArgs a, const SharedWork w) {
-  constexpr int PER = shared_rows(DP), EPL = DP / 64;
+  constexpr int PER = shared_rows(DP), EPL = DP / 64, KEPT = 8;
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
+  const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
   const int per_member = a.g.hk * a.rows;
-  if (unit >= (int64_t)a.count * per_member) return;
-  const int j = (int)(unit / per_member), in = (int)(unit % per_member), kh = in / a.rows, r = in % a.rows;
+  if (unit >= a.count * per_member) return;
+  const int j = unit / per_member, in = unit - j * per_member, kh = in / a.rows, r = in - kh * a.rows;
   const int b = a.members[j];
   const int32_t *d = w.desc + 8 * j;
   if (b < 0 || b >= a.batch || !d[5]) return;
   const int row = d[2] + r, shared = d[1], own = d[4];
-  const int first = d[0] + (row / PER * a.g.hk + kh) * shared, own_first = d[3] + kh * own;
+  // the first parts' rows among all runs' rows
+  const int64_t first = (int64_t)(d[0] + (row / PER * a.g.hk + kh) * shared) * PER + row % PER;
+  const int64_t own_first = (int64_t)(d[3] + kh * own) * PER + r;
   const int n = shared + own;
-  auto at = [&](int i) {  // the part's row among all runs' rows
-    return i < shared ? (int64_t)(first + i) * PER + row % PER : (int64_t)(own_first + i - shared) * PER + r;
+  auto at = [&](int i) { return i < shared ? first + (int64_t)i * PER : own_first + (int64_t)(i - shared) * PER; };
+  float x[KEPT][EPL];
+  auto request = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < KEPT; ++i) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) x[i][e] = 0.0f;
+      if (i0 + i < n) __builtin_memcpy(x[i], w.acc + at(i0 + i) * DP + lane * EPL, 4 * EPL);
+    }
   };
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 64) top = __builtin_elementwise_maximum(top, w.ml[2 * at(i)]);
+  request(0);
+  float top = -INFINITY, m = -INFINITY, l = 0.0f;  // m and l: lane's part of the first 64
+  for (int i = lane; i < n; i += 64) {
+    float2 ml;
+    __builtin_memcpy(&ml, w.ml + 2 * at(i), 8);
+    if (i == lane) {
+      m = ml.x;
+      l = ml.y;
+    }
+    top = __builtin_elementwise_maximum(top, ml.x);
+  }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) top = __builtin_elementwise_maximum(top, __shfl_xor(top, o, 64));
-  float l = 0.0f, acc[EPL];
+  float total = 0.0f, acc[EPL];
 #pragma unroll
   for (int e = 0; e < EPL; ++e) acc[e] = 0.0f;
-  for (int i = 0; i < n; ++i) {
-    const int64_t p = at(i);
-    const float m = w.ml[2 * p];
-    if (m == -INFINITY) continue;
-    const float scale = __builtin_amdgcn_exp2f(m - top);
-    l += w.ml[2 * p + 1] * scale;
+  for (int c = 0; c < n; c += 64) {
+    if (c > 0) {
+      m = -INFINITY;
+      l = 0.0f;
+      if (c + lane < n) {
+        m = w.ml[2 * at(c + lane)];
+        l = w.ml[2 * at(c + lane) + 1];
+      }
+    }
+    // (a part without a visible token has weight 0, whatever the maximum)
+    const float weight = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    total += l * weight;
+    for (int i = c; i < n && i < c + 64; i += KEPT) {
+      if (i > 0) request(i);
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) acc[e] += w.acc[p * DP + lane * EPL + e] * scale;
+      for (int y = 0; y < KEPT; ++y) {
+        const float wy = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(weight), i - c + y));
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) acc[e] = wy == 0.0f ? acc[e] : __builtin_fmaf(x[y][e], wy, acc[e]);
+      }
+    }
   }
-  const float inv = top == -INFINITY ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
+  const float inv = top == -INFINITY ? 0.0f : 1.0f / total;
   const int qi = r / a.gqa, h = kh * a.gqa + r % a.gqa;
   uint16_t *o = a.out + (((int64_t)b * a.heads + h) * a.nq + qi) * a.g.dim;
 #pragma unroll
