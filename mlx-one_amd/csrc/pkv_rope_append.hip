@@ -14,6 +14,8 @@
 //  * rows kernel: a wave per (row, q head) or (row, KV head).  Any dims and strides.
 //  * tiles kernel: a workgroup per 16-token tile of the cache and run of heads; 16-byte
 //    loads and stores, K and V tiles stored in whole payload chunks.
+#include <algorithm>
+
 #include "pkv_step.h"
 #include "pkv_tile_store.h"
 
@@ -225,6 +227,10 @@ __device__ __forceinline__ bool find_tile(const RopeAppendArgs &a, int tile, int
   return false;
 }
 
+// u / d for u < 2^11 by one product: inv = ceil(2^20 / d) is off by less than d <= 2^7 of 2^-20.
+__device__ __forceinline__ uint32_t inverse(int d) { return d > 0 ? ((1u << 20) + d - 1) / d : 0; }
+__device__ __forceinline__ int over(int u, uint32_t inv) { return (int)((uint32_t)u * inv >> 20); }
+
 template <int DP, int G, int BITS>
 __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppendArgs a, int per_wave) {
   constexpr int KB = DP / 32;
@@ -241,14 +247,16 @@ __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppend
   const int pos0 = (start / PKV_TILE + nth) * PKV_TILE;
   const int rel = pos0 - start;  // the tile's token t is the sequence's new token rel + t
   const int page = pos0 / g.page < a.max_pages ? a.table[(int64_t)b * a.max_pages + pos0 / g.page] : -1;
+  const uint32_t by_half = inverse(a.half);
   for (int u = threadIdx.x; u < PKV_TILE * a.half; u += 256) {
-    const int t = u / a.half, j = u - t * a.half;
+    const int t = over(u, by_half), j = u - t * a.half;
     if (rel + t < 0 || rel + t >= n) continue;
     cos_sin((double)pair_position(a, first + rel + t, pos0 + t, j) * (double)a.inv_freq[j], s_cos[t][j], s_sin[t][j]);
   }
   __syncthreads();
   const int lo = max(0, -rel), hi = min(PKV_TILE, n - rel);  // the tile's new tokens
   const int pairs = a.half / 8, plain = (g.dim - 2 * a.half) / 8;  // 16-byte units per token
+  const uint32_t by_pairs = inverse(pairs), by_plain = inverse(plain);
   const int all = a.heads + 2 * g.hk;
   for (int i = 0; i < per_wave; ++i) {
     const int h = (blockIdx.y * per_wave + i) * 4 + wave;
@@ -280,7 +288,7 @@ __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppend
       uint16_t *rows = (uint16_t *)s_buf[wave];
       if (!is_q) wave_lds_sync();  // (the last head's reads of the buffer are done)
       for (int u = lane; u < PKV_TILE * pairs; u += 64) {
-        const int t = u / pairs, c = u - t * pairs;
+        const int t = over(u, by_pairs), c = u - t * pairs;
         if (t < lo || t >= hi) continue;
         const uint16_t *src = src0 + (int64_t)t * a.row_stride + 8 * c;
         const u4 w0 = *(const u4 *)src, w1 = *(const u4 *)(src + a.half);
@@ -309,7 +317,7 @@ __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppend
         }
       }
       for (int u = lane; u < PKV_TILE * plain; u += 64) {
-        const int t = u / plain, d = 2 * a.half + 8 * (u - t * plain);
+        const int t = over(u, by_plain), d = 2 * a.half + 8 * (u - t * plain);
         if (t < lo || t >= hi) continue;
         const u4 w = *(const u4 *)(src0 + (int64_t)t * a.row_stride + d);
         if (out) *(u4 *)(out + out_at(a, out_heads, b, first + rel + t, rel + t, out_head) + d) = w;
@@ -332,6 +340,11 @@ __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppend
 
 }  // namespace
 
+// Workgroups to leave of a tile kernel's launch.  10K rows of 20 heads (670 tiles): 30 us at two
+// workgroups to a tile, 31 at three, 36 at five; 24K rows of 48 heads (1524): 168 at one, 162 at
+// two, 166 at three.
+constexpr int kLeast = 1536;
+
 hipError_t launch_rope_append(hipStream_t stream, const RopeAppendArgs &a) {
   if (a.rows == 0 || a.batch == 0) return hipSuccess;
   const dim3 block(256);
@@ -341,8 +354,10 @@ hipError_t launch_rope_append(hipStream_t stream, const RopeAppendArgs &a) {
   if (vec && (int64_t)a.rows >= 8 * (int64_t)a.batch) {
     const int tiles = (a.rows + PKV_TILE - 1) / PKV_TILE + 2 * (a.batch < a.rows ? a.batch : a.rows);
     const int all = a.heads + 2 * a.g.hk;
+    // A workgroup computes its tile's angles for all its heads: as many heads as leave
+    // kLeast workgroups, so that six may be on each CU.
     int per_wave = 1;
-    while (per_wave < 4 && (int64_t)tiles * (all / (8 * per_wave)) >= 2048) per_wave *= 2;
+    while (4 * per_wave < all && (int64_t)tiles * ((all + 4 * per_wave + 3) / (4 * per_wave + 4)) >= kLeast) ++per_wave;
     const dim3 grid(tiles, (all + 4 * per_wave - 1) / (4 * per_wave));
 #define PKV_TILES(DP_, G_, BITS_)                                                                    \
   if (a.g.dp == DP_ && a.g.bits == BITS_ && (BITS_ == 16 || a.g.group == G_)) {                      \

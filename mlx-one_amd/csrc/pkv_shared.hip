@@ -9,11 +9,17 @@
 //
 // Every workgroup first lays out the call's work from the lengths on the device: the
 // prefix of a (group, KV head, block of rows) and the own tokens of a (sequence, KV
-// head) are segments of 16-token tiles, cut into runs so that there are about as many
-// runs as workgroups.  Its four waves take pairs of a run's tiles in turn:
+// head) are segments of 16-token tiles, cut into runs so that all are in flight together.  Its
+// four waves take pairs of a run's tiles in turn:
 //   S^T = K.Q^T      v_mfma_f32_16x16x32, one tile: lane (row, jj) holds tokens 4jj + r
 //   O^T += V^T.P^T   v_mfma_f32_16x16x32, the pair's 32 tokens
-// K and V go from the pages straight to operand registers.  Quantized K enters as its codes
+// What bounds it are the instructions that turn codes into operands (a pair takes about 400, and
+// 560 for two blocks of 16 rows), then the way from the lengths to the first tile, about 8 us.
+// So two waves share a SIMD: one block of rows keeps the next pair in registers; two, which
+// need those for sums, copy it to LDS.  (In registers at one wave per SIMD: 69 us for 32
+// sequences behind 4096 tokens int8, 87 us for eight answers to each of four 24000-token documents
+// int4, 47 us for five queries each of 16 sequences; now 34, 56 and 33 us, with the merge.)
+// Quantized K enters as its codes
 // (1024 + c, exact in float16; queries as float16, each row scaled by a power of two, which
 // is exact for what its scores keep), group scales and biases are applied to the float32
 // scores:  s = sum_g scale_g (q_g . c'_g) + (bias_g - 1024 scale_g) sum(q_g).  Quantized V is
@@ -34,9 +40,10 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f;
-// Runs to aim at beyond one per segment: two workgroups for each of 256 CUs.  A tile of a
-// sequence's own comes from memory, a shared one mostly from a cache.
-constexpr int kTarget = 512, kSharedCost = 5, kOwnCost = 3;
+// Runs to aim at: two workgroups for each of 256 CUs.  A shared tile serves 32 rows, one of a
+// sequence's own a few: costs of 3 and 2 (32 sequences behind 4096 tokens: 34 us; 5 and 3: 38; 2
+// and 1: 40).
+constexpr int kTarget = 512, kSharedCost = 3, kOwnCost = 2;
 
 // Workspace: [member][8] descriptors, then per run its rows' (m, l) and sums of V.
 struct SharedParts {
