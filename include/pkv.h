@@ -566,12 +566,13 @@ int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, co
  * tokens (pages that a fork shares, or equal copies): the shared tokens are gone through
  * once for the group's query rows together, the others once per sequence.  Results are
  * pkv_paged_attention's, to the rounding of another split and of keys as 16-bit operands,
- * for every sequence that a group names; the others' rows of out are left as they are.
+ * for every sequence that a group names; the others' rows of out are left as they are, or
+ * with zero_others (and a group and a member at least) become zeros.
  * Group g is sequences members[group_starts[g]] .. members[group_starts[g+1] - 1] (distinct over
  * the call) and shares its first prefix_lens[g] tokens, read through the first one's block
  * table as far as that sequence goes; a group of one shares nothing.  At most 32 query rows
  * per KV head of a sequence (num_queries x num_heads / num_kv_heads; 16 at head_dim >
- * 128), 1024 members and groups.  The reference has no counterpart (every row of a
+ * 128), 1024 members and groups, 2^25 query rows.  The reference has no counterpart (every row of a
  * batch reads all its pages, src/mlx_one/engine/paged_attention.py:160-206).
  *
  *  queries, block_table, seq_lens, q_pos, widths, scale, out: as pkv_paged_attention
@@ -587,7 +588,7 @@ int pkv_shared_attention(void *stream, const pkv_layout *layout, const void *poo
                          const int32_t *q_pos, const int32_t *widths, int32_t num_groups,
                          const int32_t *members, int32_t num_members, const int32_t *group_starts,
                          const int32_t *prefix_lens, float scale, void *workspace, int64_t workspace_bytes,
-                         void *out);
+                         void *out, int32_t zero_others);
 int64_t pkv_shared_attention_workspace_bytes(const pkv_layout *layout, int32_t num_heads, int32_t num_queries,
                                              int32_t num_members, int32_t num_groups);
 

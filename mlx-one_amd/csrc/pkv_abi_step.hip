@@ -167,12 +167,13 @@ int pkv_shared_attention(void *stream, const pkv_layout *layout, const void *poo
                          const int32_t *block_table, int32_t max_pages, const int32_t *seq_lens, const int32_t *q_pos,
                          const int32_t *widths, int32_t num_groups, const int32_t *members, int32_t num_members,
                          const int32_t *group_starts, const int32_t *prefix_lens, float scale, void *workspace,
-                         int64_t workspace_bytes, void *out) {
+                         int64_t workspace_bytes, void *out, int32_t zero_others) {
   return guarded([&]() -> int {
     pkv_geometry g;
     if (int rc = shared_shape(layout, num_heads, num_queries, num_members, num_groups, &g)) return rc;
     if (batch < 0 || num_pages < 0 || max_pages < 0) return fail(PKV_INVALID_ARGUMENT, "invalid shared attention shape");
     if (batch > (1 << 20)) return fail(PKV_UNSUPPORTED, "at most 2^20 sequences");
+    if ((int64_t)batch * num_heads * num_queries > (1 << 25)) return fail(PKV_UNSUPPORTED, "at most 2^25 query rows");
     if ((int64_t)max_pages * g.page > INT32_MAX) return fail(PKV_INVALID_ARGUMENT, "block table too wide");
     if ((int64_t)max_pages * g.page > INT32_MAX - 4096) return fail(PKV_UNSUPPORTED, "block tables of at most 2^31 - 4097 tokens");
     if (!std::isfinite(scale)) return fail(PKV_INVALID_ARGUMENT, "the softmax scale must be finite");
@@ -207,6 +208,7 @@ int pkv_shared_attention(void *stream, const pkv_layout *layout, const void *poo
     a.prefix_lens = prefix_lens;
     a.workspace = workspace;
     a.out = (uint16_t *)out;
+    a.zero_others = zero_others;
     return check_launch(pkv::launch_shared_attention((hipStream_t)stream, a), "shared attention launch");
   });
 }

@@ -844,19 +844,30 @@ __global__ __launch_bounds__(kThreads, 2) void shared_kernel(const SharedArgs a,
   }
 }
 
-// One wave per (member, KV head, row): the row's parts joined.  Lane l weighs part l (of 64 at
+// One wave per (sequence, KV head, row): the row's parts joined.  Lane l weighs part l (of 64 at
 // a time); the parts' rows are read eight at a time.
 template <int DP>
 __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedArgs a, const SharedWork w) {
   constexpr int PER = shared_rows(DP), EPL = DP / 64, KEPT = 8;
   const int lane = threadIdx.x & 63;
   const int unit = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + (threadIdx.x >> 6));
-  const int per_member = a.g.hk * a.rows;
-  if (unit >= a.count * per_member) return;
-  const int j = unit / per_member, in = unit - j * per_member, kh = in / a.rows, r = in - kh * a.rows;
-  const int b = a.members[j];
-  const int32_t *d = w.desc + 8 * j;
-  if (b < 0 || b >= a.batch || !d[5]) return;
+  const int per_row = a.g.hk * a.rows;
+  const int b = unit / per_row, in = unit - b * per_row, kh = in / a.rows, r = in - kh * a.rows;
+  if (b >= a.batch) return;
+  // the sequence's member
+  int j = -1;
+  for (int c = 0; c < a.count && j < 0; c += 64) {
+    const unsigned long long hit = __ballot(c + lane < a.count && a.members[c + lane] == b);
+    if (hit) j = c + __ffsll((long long)hit) - 1;
+  }
+  const int32_t *d = w.desc + 8 * max(j, 0);
+  const int qi = r / a.gqa, h = kh * a.gqa + r % a.gqa;
+  uint16_t *o = a.out + (((int64_t)b * a.heads + h) * a.nq + qi) * a.g.dim;
+  if (j < 0 || !d[5]) {
+    if (a.zero_others)
+      for (int e = lane; e < a.g.dim; e += 64) o[e] = 0;
+    return;
+  }
   const int row = d[2] + r, shared = d[1], own = d[4];
   // the first parts' rows among all runs' rows
   const int64_t first = (int64_t)(d[0] + (row / PER * a.g.hk + kh) * shared) * PER + row % PER;
@@ -913,8 +924,6 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedArgs
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
   const float inv = top == -INFINITY ? 0.0f : 1.0f / total;
-  const int qi = r / a.gqa, h = kh * a.gqa + r % a.gqa;
-  uint16_t *o = a.out + (((int64_t)b * a.heads + h) * a.nq + qi) * a.g.dim;
 #pragma unroll
   for (int e = 0; e < EPL; ++e)
     if (lane * EPL + e < a.g.dim) o[lane * EPL + e] = float_to_bits(acc[e] * inv, a.g.float_kind);
@@ -951,7 +960,7 @@ hipError_t launch_shared_attention(hipStream_t stream, const SharedArgs &a) {
 #undef PKV_SHARED_Q
 #undef PKV_SHARED
   if (e != hipSuccess) return e;
-  const dim3 rows((unsigned)(((int64_t)a.count * a.g.hk * a.rows + kWaves - 1) / kWaves));
+  const dim3 rows((unsigned)(((int64_t)a.batch * a.g.hk * a.rows + kWaves - 1) / kWaves));
   if (a.g.dp == 64) hipLaunchKernelGGL((shared_merge_kernel<64>), rows, block, 0, stream, a, w);
   else if (a.g.dp == 128) hipLaunchKernelGGL((shared_merge_kernel<128>), rows, block, 0, stream, a, w);
   else hipLaunchKernelGGL((shared_merge_kernel<256>), rows, block, 0, stream, a, w);

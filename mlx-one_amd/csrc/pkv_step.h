@@ -74,6 +74,7 @@ struct SharedArgs {
   const int32_t *members, *group_starts, *prefix_lens;
   void *workspace;
   uint16_t *out;  // as q
+  int zero_others;  // the rows of sequences that no group names become zeros
 };
 
 constexpr int kMaxShared = 1024;  // sequences, and groups

@@ -85,7 +85,7 @@ SIGNATURES = {
                          _c_p, _c_p, _i32, _c_p, _i32, _c_p, _c_p, _i32, _c_p, _c_p, _c_p],
                         ctypes.c_int),
     "pkv_shared_attention": ([_c_p, _LP, _c_p, _i64, _c_p, _i32, _i32, _i32, _c_p, _i32, _c_p, _c_p,
-                              _c_p, _i32, _c_p, _i32, _c_p, _c_p, _f32, _c_p, _i64, _c_p],
+                              _c_p, _i32, _c_p, _i32, _c_p, _c_p, _f32, _c_p, _i64, _c_p, _i32],
                              ctypes.c_int),
     "pkv_shared_attention_workspace_bytes": ([_LP, _i32, _i32, _i32, _i32], _i64),
     "pkv_prompt_attention": ([_c_p, _c_p, _i64, _c_p, _i64, _c_p, _i64, _i32, _i32, _i32, _c_p,

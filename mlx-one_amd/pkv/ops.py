@@ -938,8 +938,9 @@ def shared_prefix_attention(fmt: PageFormat, pool, queries, block_table, seq_len
     if starts.numel() != groups + 1:
         raise ValueError("group_starts must hold a value per group and the end")
     queries = queries.contiguous()
-    if out is None:
-        out = (torch.empty if count == batch else torch.zeros)(queries.shape, dtype=queries.dtype, device=device)
+    fresh = out is None
+    if fresh:
+        out = (torch.empty if count and groups else torch.zeros)(queries.shape, dtype=queries.dtype, device=device)
     elif not _dense(out, queries.dtype, device, 4) or out.shape != queries.shape:
         raise ValueError("out must be a contiguous tensor of the queries' shape, dtype and device")
     lib, layout = nat.load(), fmt.c_layout
@@ -948,5 +949,5 @@ def shared_prefix_attention(fmt: PageFormat, pool, queries, block_table, seq_len
     _launch(device, "shared attention", lib.pkv_shared_attention, layout, pool.data_ptr(), pages, queries.data_ptr(),
             batch, heads, nq, table.data_ptr(), table.shape[1], lens.data_ptr(), positions_at, live_at, groups,
             member.data_ptr(), count, starts.data_ptr(), prefix.data_ptr(), scale, workspace.data_ptr(),
-            workspace.numel(), out.data_ptr())
+            workspace.numel(), out.data_ptr(), fresh)
     return out

@@ -237,6 +237,24 @@ def test_later_tokens_that_are_not_finite(bits, dtype):
         assert np.all(seen == np.isfinite(held)[:, None])
 
 
+def test_others_of_a_whole_batch_are_zeros():
+    """As many members as sequences, one of them out of range: the rows of the sequence that
+    none names are zeros, whatever the memory of the result held."""
+    from pkv import ops
+
+    fmt = _format(8, 64, 64)
+    pool, table, lens, members, starts, prefix = _cache(fmt, [(50, [10, 20, 30])])
+    q = _queries(fmt, 3, 4, 1)
+    for ids, at, left in ((members[:2] + [-1], [0, 3], members[2]), (members, [1, 3], members[0])):
+        ids = torch.tensor(ids, dtype=torch.int32, device="cuda")
+        torch.full_like(q, 9.0)  # (memory that the call's result may take)
+        got = ops.shared_prefix_attention(fmt, pool, q, table, lens, ids, at, prefix, scale=0.1)
+        assert bool((got[left] == 0).all()) and bool((got != 9.0).all())
+    for count in (0, 3):
+        got = ops.shared_prefix_attention(fmt, pool, q, table, lens, members[:count], [0], [], scale=0.1)
+        assert bool((got == 0).all())
+
+
 def test_repeats_and_workspaces():
     """The same bits each time, in a workspace that held anything."""
     from pkv import ops

@@ -58,7 +58,7 @@ def test_prompt_attention(kw, code):
 def _shared(**kw):
     a = dict(stream=None, layout=_layout(), pool=FAKE, num_pages=10, queries=FAKE, batch=2, heads=32, nq=1,
              table=FAKE, max_pages=4, lens=FAKE, q_pos=None, widths=None, groups=1, members=FAKE, count=2,
-             starts=FAKE, prefix=FAKE, scale=1.0, ws=FAKE, ws_bytes=1 << 40, out=FAKE)
+             starts=FAKE, prefix=FAKE, scale=1.0, ws=FAKE, ws_bytes=1 << 40, out=FAKE, zero_others=0)
     a.update(kw)
     return nat.load().pkv_shared_attention(*a.values())
 
@@ -70,7 +70,7 @@ def _shared(**kw):
     (dict(scale=float("nan")), 1), (dict(pool=None), 1), (dict(queries=None), 1), (dict(table=None), 1),
     (dict(lens=None), 1), (dict(members=None), 1), (dict(starts=None), 1), (dict(prefix=None), 1), (dict(out=None), 1),
     (dict(num_pages=0), 1), (dict(max_pages=0), 1), (dict(ws=None), 3), (dict(ws_bytes=100), 3), (dict(ws=FAKE + 8), 1),
-    (dict(heads=512, layout=_layout(num_kv_heads=512), count=1024), 2)])
+    (dict(heads=512, layout=_layout(num_kv_heads=512), count=1024), 2), (dict(batch=1 << 20, nq=2), 2)])
 def test_shared_attention(kw, code):
     assert _shared(**kw) == code and nat.last_error()
 
