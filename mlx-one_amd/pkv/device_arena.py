@@ -30,6 +30,7 @@ import torch
 from pkv import _native as nat
 from pkv import ops
 from pkv.cache_errors import CacheCapacityError, CacheCorruptionError
+from pkv.modes import ModelCapabilityUnsupported
 
 OUT_OF_PAGES, TABLE_FULL, BAD_ARGUMENT, CORRUPT = 1, 2, 4, 8
 HEADER_WORDS = 16
@@ -425,6 +426,34 @@ class DevicePageArena:
         free = int(self.state[0].item())
         return self.state[HEADER_WORDS:HEADER_WORDS + free].cpu()
 
+    def prefix_groups(self, slots, *, least=1):
+        """The sequences among ``slots`` that share their first pages (``fork``, an adopted
+        prefix), as ``ops.shared_prefix_attention`` takes them: ``(members, group_starts,
+        prefix_lens)`` device tensors, members as places in ``slots``, every sequence in one
+        group.  Sequences with the same first page are a group, which shares the whole pages
+        that all of them hold alike, up to the shortest one's length; fewer than ``least``
+        tokens count as none.  Reads the table on the host: call it when the batch changes,
+        not every step (a group stays right as its sequences grow)."""
+        slots = [int(s) for s in slots]
+        rows = self.table[torch.tensor(slots, dtype=torch.int64, device=self.device)].cpu()
+        lens = self.lens.cpu()[slots].tolist() if slots else []
+        by_first = {}
+        for place in range(len(slots)):
+            held = lens[place] // self.page_tokens
+            key = int(rows[place, 0]) if held else None
+            by_first.setdefault((place,) if key is None else key, []).append(place)
+        members, starts, prefixes = [], [0], []
+        for group in by_first.values():
+            held = min(lens[p] for p in group) // self.page_tokens
+            same = (rows[group, :held] == rows[group[0], :held]).all(0)
+            alike = held if bool(same.all()) else int(same.int().argmin())
+            tokens = alike * self.page_tokens if len(group) > 1 else 0
+            members += group
+            starts.append(len(members))
+            prefixes.append(tokens if tokens >= least else 0)
+        return tuple(torch.tensor(x, dtype=torch.int32, device=self.device)
+                     for x in (members, starts, prefixes))
+
     def pages(self, slot):
         n = -(-int(self.lens[slot].item()) // self.page_tokens)
         return self.table[slot, :n].cpu().tolist()
@@ -435,8 +464,11 @@ class DeviceBatchCache:
     layer's pool and runs paged attention, with every operand already on the
     device (``PagedBatchCache.attend``, ``engine/paged.py:245-267``)."""
 
-    def __init__(self, arena, layer, reservation, *, workspace=None, waves=0):
+    def __init__(self, arena, layer, reservation, *, workspace=None, waves=0, shared=None):
         self.arena, self.layer, self.res = arena, layer, reservation
+        # (members, group_starts, prefix_lens): attention goes through shared prefixes once
+        self.shared = shared
+        self.takes_projection = shared is not None
         # a captured step brings its own workspace (and the waves it was sized
         # for): the shared per-device one may be replaced by a later eager call
         self.workspace, self.waves = workspace, waves
@@ -472,6 +504,40 @@ class DeviceBatchCache:
                                    waves=waves, workspace=self.workspace)
 
 
+    def attend_projection(self, qkv, inv_freq, heads, *, scale, position_ids=None):
+        """A step over shared prefixes: ``qkv [B, T, width]`` (q|k|v heads) rotated at
+        ``position_ids [B, T]`` and appended in one pass, then attention that reads each
+        group's prefix once; ``[B, T, heads * D]``."""
+        fmt, pool, res = self.arena.fmt, self.arena.pools[self.layer], self.res
+        q = ops.rope_append(fmt, pool, qkv.to(fmt.dtype), res.table, res.starts, inv_freq, heads,
+                            widths=res.widths, positions=position_ids)
+        out = ops.shared_prefix_attention(fmt, pool, q, res.table, res.lens, *self.shared, scale=scale,
+                                          widths=res.widths, workspace=self.workspace)
+        if self.arena.mass is not None:
+            ops.attention_mass(fmt, pool, q, res.table, res.lens, scale=scale, widths=res.widths,
+                               mass=self.arena.mass[self.layer], counted=res.starts, rows=res.slots)
+        return out.transpose(1, 2).reshape(*qkv.shape[:2], -1).to(qkv.dtype)
+
+
+class DevicePromptCache:
+    """One layer of a batch of packed prompts, all of them in slots that were empty: the rows
+    of sequence b are ``row_starts[b]`` to ``row_starts[b + 1] - 1``."""
+
+    takes_projection = True
+
+    def __init__(self, arena, layer, reservation, row_starts):
+        self.arena, self.layer, self.res, self.row_starts = arena, layer, reservation, row_starts
+
+    def attend_projection(self, qkv, inv_freq, heads, *, scale, position_ids=None):
+        """``qkv [T, width]`` rotated and appended in one pass, then attention within each
+        prompt over k and v as they are (not as the pages hold them); ``[T, heads * D]``."""
+        fmt, res = self.arena.fmt, self.res
+        q, k, v = ops.rope_append(fmt, self.arena.pools[self.layer], qkv.to(fmt.dtype), res.table,
+                                  res.starts, inv_freq, heads, row_starts=self.row_starts,
+                                  positions=position_ids, with_kv=True)
+        return ops.prompt_attention(q, k, v, self.row_starts, scale=scale).flatten(1).to(qkv.dtype)
+
+
 class DeviceRunner:
     """Batch steps of a model over device-arena slots: ``PagedRunner.execute``
     (``engine/paged.py:308-417``) with the page bookkeeping on the device.  One
@@ -483,30 +549,26 @@ class DeviceRunner:
             raise ValueError("the arena needs one pool per model layer")
         self.model, self.arena = model, arena
 
-    def _forward(self, hidden, res, workspace=None, waves=0):
+    def _forward(self, hidden, res, workspace=None, waves=0, shared=None):
         batch, width, _ = hidden.shape
         positions = self.arena.positions(res).view(batch, 1)
         if width > 1:
             positions = positions + torch.arange(width, dtype=torch.int32, device=hidden.device)
-        caches = tuple(DeviceBatchCache(self.arena, layer, res, workspace=workspace, waves=waves)
+        caches = tuple(DeviceBatchCache(self.arena, layer, res, workspace=workspace, waves=waves,
+                                        shared=shared)
                        for layer in range(len(self.arena.pools)))
         return self.model.forward(hidden, cache=caches, position_ids=positions)
 
-    def execute(self, slots, hidden, widths=None):
-        """``hidden [B, T, hidden]`` for ``slots`` (row b's columns past
-        ``widths[b]`` are padding); returns the model's ``[B, T, hidden]``."""
-        batch, width, _ = hidden.shape
-        slots = [int(s) for s in slots]
-        widths = [width] * batch if widths is None else [int(w) for w in widths]
-        if len(slots) != batch or len(widths) != batch or any(w < 1 or w > width for w in widths):
-            raise ValueError("one slot and a width in 1..T per row")
+    def _step(self, slots, widths, forward):
+        """Reserve ``widths`` tokens in ``slots`` and run ``forward(reservation)``; a step that
+        raises leaves the slots as they were."""
         before = [self.arena.lengths[s] for s in slots]
         res = self.arena.reserve(slots, widths)
         # the reserve kernel's error bits, read after the forward is enqueued:
         # by then the reserve has long run, so the check costs no stall
         probe = self.arena.error_probe()
         try:
-            out = self._forward(hidden, res)
+            out = forward(res)
         except BaseException:
             self.arena.rollback(slots, before)
             raise
@@ -519,7 +581,43 @@ class DeviceRunner:
             self.arena._raise(err)
         return out
 
-    def capture_decode(self, slots, hidden, *, warm=True):
+    def prefill(self, slots, hidden, widths):
+        """Whole prompts, packed: ``hidden [sum(widths), hidden]`` holds the rows of ``slots``
+        (which must be empty) one after the other, without padding; returns the model's
+        rows.  Attention reads k and v as the projection made them; ``execute`` reads them
+        back from the pages, as later steps do."""
+        slots, widths = [int(s) for s in slots], [int(w) for w in widths]
+        if len(widths) != len(slots) or any(w < 1 for w in widths) or hidden.dim() != 2 \
+                or hidden.shape[0] != sum(widths):
+            raise ValueError("one slot and a width of at least 1 per prompt, a row per token")
+        if any(self.arena.lengths[s] for s in slots):
+            raise ValueError("packed prompts go into empty slots")
+        if self.arena.mass is not None:
+            raise ModelCapabilityUnsupported("packed prompts do not keep attention sums: use execute")
+        starts = [0]
+        for w in widths:
+            starts.append(starts[-1] + w)
+        row_starts = torch.tensor(starts, dtype=torch.int32, device=hidden.device)
+
+        def forward(res):
+            caches = tuple(DevicePromptCache(self.arena, layer, res, row_starts)
+                           for layer in range(len(self.arena.pools)))
+            return self.model.forward(hidden, cache=caches, position_ids=None)
+
+        return self._step(slots, widths, forward)
+
+    def execute(self, slots, hidden, widths=None, *, shared=None):
+        """``hidden [B, T, hidden]`` for ``slots`` (row b's columns past
+        ``widths[b]`` are padding); returns the model's ``[B, T, hidden]``.  ``shared``: the
+        arena's ``prefix_groups(slots)``, whose prefixes attention then reads once."""
+        batch, width, _ = hidden.shape
+        slots = [int(s) for s in slots]
+        widths = [width] * batch if widths is None else [int(w) for w in widths]
+        if len(slots) != batch or len(widths) != batch or any(w < 1 or w > width for w in widths):
+            raise ValueError("one slot and a width in 1..T per row")
+        return self._step(slots, widths, lambda res: self._forward(hidden, res, shared=shared))
+
+    def capture_decode(self, slots, hidden, *, warm=True, shared=None):
         """Graphs of one decode step (one token per slot) reading the static
         buffer ``hidden [B, 1, hidden]``: returns a ``CapturedStep`` whose
         ``replay()`` appends a token to every slot and leaves the step's output
@@ -528,7 +626,8 @@ class DeviceRunner:
         them.  ``warm`` runs one step eagerly first (it sizes the buffers and
         warms the libraries; without it the caller must have run a step of
         this shape).  Replays do not advance the host length mirror:
-        ``arena.sync_lengths()`` reads the device's."""
+        ``arena.sync_lengths()`` reads the device's.  ``shared`` as in ``execute``; its
+        tensors are the graph's and are kept."""
         arena = self.arena
         device = arena.device
         slots_d = torch.tensor([int(s) for s in slots], dtype=torch.int32, device=device)
@@ -539,12 +638,15 @@ class DeviceRunner:
         # capture, and held by the CapturedStep
         spec = self.model.spec
         waves = ops.default_waves(arena.fmt, spec.query_heads, 1, count)
-        workspace = torch.empty(max(256, ops.call_workspace_bytes(arena.fmt, spec.query_heads, 1,
-                                                                  count, waves)),
-                                dtype=torch.uint8, device=device)
+        if shared is None:
+            nbytes = ops.call_workspace_bytes(arena.fmt, spec.query_heads, 1, count, waves)
+        else:
+            nbytes = ops.shared_workspace_bytes(arena.fmt, spec.query_heads, 1, shared[0].numel(),
+                                                shared[2].numel())
+        workspace = torch.empty(max(256, nbytes), dtype=torch.uint8, device=device)
         if warm:
             res = arena.reserve(slots_d, widths_d)
-            self._forward(hidden, res, workspace, waves)
+            self._forward(hidden, res, workspace, waves, shared)
         else:
             res = Reservation(slots_d, widths_d,
                               torch.empty((count, arena.max_pages), dtype=torch.int32,
@@ -559,11 +661,11 @@ class DeviceRunner:
             with torch.cuda.graph(reserve_graph, stream=stream):
                 arena.reserve(slots_d, widths_d, out=res)
             with torch.cuda.graph(graph, stream=stream):
-                out = self._forward(hidden, res, workspace, waves)
+                out = self._forward(hidden, res, workspace, waves, shared)
         torch.cuda.current_stream(device).wait_stream(stream)
         if warm:
             arena.sync_lengths()
-        return CapturedStep(graph, out, hidden, res, (slots_d, widths_d), workspace, waves,
+        return CapturedStep(graph, out, hidden, res, (slots_d, widths_d, shared), workspace, waves,
                             reserve_graph)
 
 
@@ -576,7 +678,7 @@ class CapturedStep:
     out: torch.Tensor               # the step's output, rewritten by each replay
     hidden: torch.Tensor            # the static input buffer
     reservation: Reservation        # the batch operands the reserve kernel rewrites
-    operands: tuple                 # slot ids and widths read by the reserve kernel
+    operands: tuple                 # slot ids, widths and prefix groups that the kernels read
     workspace: torch.Tensor = None  # the attention's split-K partials (every layer's launch)
     waves: int = 0                  # the attention waves the workspace is sized for
     reserve_graph: torch.cuda.CUDAGraph = None   # the page reservation, replayed first

@@ -144,7 +144,14 @@ class AttentionLayer:
     def __call__(self, x, cache, position_ids):
         """One layer through ``cache.attend`` (``transformer.py:202-209``).  Host
         ``position_ids`` stay on the host for the cache's position check (no
-        device sync); RoPE reads a device copy."""
+        device sync); RoPE reads a device copy.  A cache that takes the fused
+        projection as it is (``attend_projection``: packed prompts, steps over shared
+        prefixes) rotates and appends by itself; ``x`` is then as it expects it,
+        ``[T, hidden]`` or ``[B, T, hidden]``."""
+        if getattr(cache, "takes_projection", False):
+            out = cache.attend_projection(x @ self.wqkv, self.inv_freq, self.spec.query_heads,
+                                          scale=self.scale, position_ids=position_ids)
+            return out @ self.wo
         q, k, v = self.project(x, position_ids.to(x.device, non_blocking=True))
         out = cache.attend(q, k, v, scale=self.scale, position_ids=position_ids)
         batch, _, width, _ = out.shape

@@ -901,6 +901,15 @@ def prompt_attention(q, k, v, row_starts, *, scale, out=None):
     return result
 
 
+def shared_workspace_bytes(fmt: PageFormat, heads, queries, members, groups):
+    """Workspace of ``shared_prefix_attention`` for as many members and groups, whatever their
+    lengths."""
+    need = int(nat.load().pkv_shared_attention_workspace_bytes(fmt.c_layout, heads, queries, members, groups))
+    if need < 0:
+        nat.check(-need, "shared attention")
+    return need
+
+
 def shared_prefix_attention(fmt: PageFormat, pool, queries, block_table, seq_lens, members, group_starts,
                             prefix_lens, *, scale, q_pos=None, widths=None, workspace=None, out=None):
     """Attention of ``queries [B, H, Q, D]`` over the paged cache, where the sequences of a
@@ -944,8 +953,7 @@ def shared_prefix_attention(fmt: PageFormat, pool, queries, block_table, seq_len
     elif not _dense(out, queries.dtype, device, 4) or out.shape != queries.shape:
         raise ValueError("out must be a contiguous tensor of the queries' shape, dtype and device")
     lib, layout = nat.load(), fmt.c_layout
-    workspace = _scratch(lib.pkv_shared_attention_workspace_bytes(layout, heads, nq, count, groups), device,
-                         "shared attention", workspace)
+    workspace = _scratch(shared_workspace_bytes(fmt, heads, nq, count, groups), device, "shared attention", workspace)
     _launch(device, "shared attention", lib.pkv_shared_attention, layout, pool.data_ptr(), pages, queries.data_ptr(),
             batch, heads, nq, table.data_ptr(), table.shape[1], lens.data_ptr(), positions_at, live_at, groups,
             member.data_ptr(), count, starts.data_ptr(), prefix.data_ptr(), scale, workspace.data_ptr(),
