@@ -773,12 +773,13 @@ def rope_append(fmt: PageFormat, pool, qkv, block_table, start_pos, inv_freq, he
     if pool.shape[1] != fmt.page_bytes:
         raise ValueError("the pool's pages are not of this format")
     kv_heads, dim = fmt.num_kv_heads, fmt.head_dim
-    width = qkv.shape[-1]
+    *lead, width = qkv.shape
     if heads < 1 or width != (heads + 2 * kv_heads) * dim:
         raise ValueError("qkv width is not (heads + 2 * kv_heads) * head_dim")
-    if qkv.stride(-1) != 1 or qkv.stride(-2) < width or (
-            qkv.dim() == 3 and qkv.stride(0) != qkv.shape[1] * qkv.stride(1)):
+    steps = qkv.stride()
+    if steps[-1] != 1 or steps[-2] < width or (len(lead) == 2 and steps[0] != lead[1] * steps[1]):
         qkv = qkv.contiguous()
+        steps = qkv.stride()
     starts = _i32(start_pos, device)
     batch = starts.numel()
     # (the tensors are named so that they live until the launch)
@@ -787,18 +788,15 @@ def rope_append(fmt: PageFormat, pool, qkv, block_table, start_pos, inv_freq, he
             widths, widths_at = _address(widths, device, batch, "widths")
         else:
             widths_at = None
-        batch_rows, tokens = qkv.shape[:2]
-        if batch_rows != batch:
+        if lead[0] != batch:
             raise ValueError("start_pos must hold a value per sequence")
-        rows, first_at, lead = batch * tokens, None, (batch, tokens)
-        shape = (lambda n: (batch, n, tokens, dim))
+        tokens, first_at = lead[1], None
+        rows = batch * tokens
     else:
         if widths is not None:
             raise ValueError("packed rows take no widths")
-        rows, tokens, widths_at = qkv.shape[0], 0, None
+        rows, tokens, widths_at = lead[0], 0, None
         first, first_at = _address(row_starts, device, batch + 1, "row_starts")
-        lead = (rows,)
-        shape = (lambda n: (rows, n, dim))
     table = _i32(block_table, device)
     if table.dim() != 2 or table.shape[0] != batch:
         raise ValueError("block table must be [batch, max_pages]")
@@ -809,26 +807,27 @@ def rope_append(fmt: PageFormat, pool, qkv, block_table, start_pos, inv_freq, he
         places = _i32(positions, device)
         if axes is not None and places.dim() == len(lead) + 1:
             num_axes = places.shape[0]
-        if tuple(places.shape) != ((num_axes,) if axes is not None else ()) + lead:
+        if [*places.shape] != [num_axes] * (axes is not None) + lead:
             raise ValueError("positions must be one per row, or with axes one per axis and row")
         positions_at = places.data_ptr()
     if axes is not None:
         if positions is None:
             raise ValueError("axes need positions")
         axis, axis_at = _address(axes, device, half, "axes")
-    outs = list(out) if with_kv and out is not None else [out]
-    counts = (heads, kv_heads, kv_heads) if with_kv else (heads,)
+    shapes = [(rows, n, dim) if row_starts is not None else (batch, n, tokens, dim)
+              for n in ((heads, kv_heads, kv_heads) if with_kv else (heads,))]
     if out is None:
-        outs = [torch.empty(shape(n), dtype=qkv.dtype, device=device) for n in counts]
-    elif len(outs) != len(counts):
-        raise ValueError("out must hold q, k and v")
+        outs = [torch.empty(shape, dtype=qkv.dtype, device=device) for shape in shapes]
     else:
-        for t, n in zip(outs, counts):
-            if not _dense(t, qkv.dtype, device, len(shape(n))) or tuple(t.shape) != shape(n):
-                raise ValueError(f"out must be contiguous {shape(n)} tensors of qkv's dtype and device")
-    addresses = [t.data_ptr() for t in outs] + [None] * (3 - len(outs))
+        outs = list(out) if with_kv else [out]
+        if len(outs) != len(shapes):
+            raise ValueError("out must hold q, k and v")
+        for t, shape in zip(outs, shapes):
+            if not _dense(t, qkv.dtype, device, len(shape)) or t.shape != shape:
+                raise ValueError(f"out must be contiguous {shape} tensors of qkv's dtype and device")
+    addresses = [t.data_ptr() for t in outs] if with_kv else (outs[0].data_ptr(), None, None)
     _launch(device, "rotation and append", nat.load().pkv_rope_append, fmt.c_layout, pool.data_ptr(),
-            pool.shape[0], qkv.data_ptr(), qkv.stride(-2), rows, heads, batch, tokens, first_at, widths_at,
+            pool.shape[0], qkv.data_ptr(), steps[-2], rows, heads, batch, tokens, first_at, widths_at,
             starts.data_ptr(), positions_at, num_axes, inv_freq.data_ptr(), half, axis_at,
             table.data_ptr(), table.shape[1], *addresses)
     return tuple(outs) if with_kv else outs[0]
@@ -848,14 +847,17 @@ def rope_axes(sections, device="cuda", *, interleaved=False):
     return torch.tensor(order, dtype=torch.int32, device=device)
 
 
-def _packed_rows(t, name):
+def _packed_rows(t, rows, heads, dim):
     """Packed heads ``[T, heads, D]`` as the kernels read them: heads side by side, rows any
-    multiple of 16 bytes apart (a copy where they are not), and the stride of rows."""
-    _, heads, dim = t.shape
-    if t.shape[0] > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim) or t.stride(0) < heads * dim
-                           or t.stride(0) % 8 or t.stride(0) > 1 << 23 or t.data_ptr() % 16):
+    multiple of 16 bytes apart (a copy where they are not).  ``(tensor, address, stride of
+    rows)``."""
+    step, head_step, one = t.stride()
+    at = t.data_ptr()
+    if rows > 0 and (one != 1 or (head_step != dim and heads > 1) or step < heads * dim or step % 8
+                     or step > 1 << 23 or at % 16):
         t = t.clone(memory_format=torch.contiguous_format)
-    return t, (t.stride(0) if t.shape[0] > 1 else heads * dim)
+        at, step = t.data_ptr(), heads * dim
+    return t, at, (step if rows > 1 else heads * dim)
 
 
 def prompt_attention(q, k, v, row_starts, *, scale, out=None):
@@ -866,36 +868,39 @@ def prompt_attention(q, k, v, row_starts, *, scale, out=None):
     (``row_starts [B + 1]``, rising).  Returns ``[T, H, D]``; rows of no sequence are left as they
     are in ``out``.  Head dims up to 256; ones that are no multiple of 8 are padded by a copy.
     """
-    for name, t in (("q", q), ("k", k), ("v", v)):
+    for t in (q, k, v):
         if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype not in FLOAT_KINDS or not t.is_cuda:
-            raise ValueError(f"{name} must be a [T, heads, D] f16/bf16 device tensor")
+            raise ValueError("q, k and v must be [T, heads, D] f16/bf16 device tensors")
     rows, heads, dim = q.shape
-    device = q.device
-    if k.shape != v.shape or k.shape[0] != rows or k.shape[2] != dim:
+    device, dtype = q.device, q.dtype
+    key_rows, kv_heads, key_dim = k.shape
+    if k.shape != v.shape or key_rows != rows or key_dim != dim:
         raise ValueError("k and v must be [T, HK, D] of q's rows and head dimension")
-    if any(t.dtype is not q.dtype or t.device != device for t in (k, v)):
+    if k.dtype is not dtype or v.dtype is not dtype or k.device != device or v.device != device:
         raise ValueError("q, k and v must be of one dtype and device")
-    kv_heads = k.shape[1]
     starts = _i32(row_starts, device)
     if starts.dim() != 1 or starts.numel() < 1:
         raise ValueError("row_starts must be [batch + 1]")
-    if out is not None and (not _dense(out, q.dtype, device, 3) or out.shape != q.shape):
+    if out is not None and (not _dense(out, dtype, device, 3) or out.shape != q.shape):
         raise ValueError("out must be a contiguous tensor of q's shape, dtype and device")
-    result = out
+    result, width = out, dim
     if dim % 8:
-        pad = 8 - dim % 8
-        q, k, v = (torch.nn.functional.pad(t, (0, pad)) for t in (q, k, v))
+        width = dim + 8 - dim % 8
+        q, k, v = (torch.nn.functional.pad(t, (0, width - dim)) for t in (q, k, v))
         out = None
     if out is None or out.data_ptr() % 16:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        out = torch.empty((rows, heads, width), dtype=dtype, device=device)
         if result is not None:
             out[..., :dim] = result
-    (q, q_step), (k, k_step), (v, v_step) = (_packed_rows(t, name) for name, t in (("q", q), ("k", k), ("v", v)))
-    _launch(device, "prompt attention", nat.load().pkv_prompt_attention, q.data_ptr(), q_step, k.data_ptr(), k_step,
-            v.data_ptr(), v_step, FLOAT_KINDS[q.dtype], rows, starts.numel() - 1, starts.data_ptr(), heads, kv_heads,
-            q.shape[2], scale, out.data_ptr())
+    # (the tensors are named so that they live until the launch)
+    q, q_at, q_step = _packed_rows(q, rows, heads, width)
+    k, k_at, k_step = _packed_rows(k, rows, kv_heads, width)
+    v, v_at, v_step = _packed_rows(v, rows, kv_heads, width)
+    _launch(device, "prompt attention", nat.load().pkv_prompt_attention, q_at, q_step, k_at, k_step, v_at, v_step,
+            FLOAT_KINDS[dtype], rows, starts.numel() - 1, starts.data_ptr(), heads, kv_heads, width, scale,
+            out.data_ptr())
     if result is None:
-        return out if out.shape[2] == dim else out[..., :dim].contiguous()
+        return out if width == dim else out[..., :dim].contiguous()
     if result is not out:
         result.copy_(out[..., :dim])
     return result
