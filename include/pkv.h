@@ -577,7 +577,7 @@ int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, co
  *
  *  queries, block_table, seq_lens, q_pos, widths, scale, out: as pkv_paged_attention
  *  members      : [num_members] int32 sequences (ids out of range are skipped)
- *  group_starts : [num_groups + 1] int32, rising;  prefix_lens: [num_groups] int32 tokens
+ *  group_starts : [num_groups + 1] int32, rising (if they fall, no sequence is named);  prefix_lens: [num_groups] int32 tokens
  *  workspace    : pkv_shared_attention_workspace_bytes(...) bytes of device scratch, 16-byte
  *                 aligned (calls that may overlap need one each); negative for shapes that
  *                 are refused, by their status

@@ -162,14 +162,21 @@ __device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p,
   }
   __syncthreads();
   int64_t cost = 0;
+  bool falls = false;
   for (int g = tid; g < a.groups; g += kThreads) {
     const int first = p.group_first[g], n = p.group_first[g + 1] - first;
+    falls |= n < 0;
     // (one sequence shares nothing)
     const int tiles = n > 1 ? max(0, min(p.group_tiles[g], p.own_run[first])) / PKV_TILE : 0;
     p.group_tiles[g] = tiles;
     cost += kSharedCost * (int64_t)tiles * row_blocks(a, p, g, per) * a.g.hk;
   }
-  __syncthreads();
+  if (__syncthreads_or(falls)) {  // groups that would overlap: none
+    cost = 0;
+    for (int g = tid; g <= a.groups; g += kThreads) p.group_first[g] = 0;
+    for (int g = tid; g < a.groups; g += kThreads) p.group_tiles[g] = 0;
+    __syncthreads();
+  }
   const int last = p.group_first[a.groups];
   for (int j = tid; j < a.count; j += kThreads) {
     const bool in = j >= p.group_first[0] && j < last;
@@ -563,13 +570,13 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
       mx[rb] = x[rb][0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx[rb] = __builtin_elementwise_maximum(mx[rb], x[rb][e]);
-      need |= mx[rb] > thr[rb];
+      need |= !(mx[rb] <= thr[rb]);  // (also where they are NaN: a row of NaN is one, not none)
     }
     if (__builtin_expect(__any(need), 0)) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         const float up = xor32_max(xor16_max(mx[rb]));
-        const bool moves = up > thr[rb];
+        const bool moves = !(up <= thr[rb]);
         const float by = moves ? up : 0.0f;
         const float alpha = !moves ? 1.0f : thr[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
         m[rb] += by;
@@ -760,7 +767,7 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
       if (tid < 16 && rb * 16 + tid < run.rows) {
         float l = 0.0f, best = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < kWaves; ++x) best = fmaxf(best, s_ml[x][rb * 16 + tid][0]);
+        for (int x = 0; x < kWaves; ++x) best = __builtin_elementwise_maximum(best, s_ml[x][rb * 16 + tid][0]);
 #pragma unroll
         for (int x = 0; x < kWaves; ++x) {
           const float mx = s_ml[x][rb * 16 + tid][0];

@@ -139,6 +139,25 @@ def test_later_rows_that_are_not_finite(dim, dtype):
             assert not bool(torch.isfinite(got[first:end, :4, at[1]]).any())
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_queries_that_are_not_numbers(dim):
+    """A query with a NaN has a NaN result, in its row and head alone."""
+    from pkv import ops
+
+    gen = torch.Generator().manual_seed(dim)
+    q, k, v = (torch.randn((300, h, dim), generator=gen).cuda().bfloat16() for h in (4, 2, 2))
+    starts = [0, 100, 300]
+    want = ops.prompt_attention(q, k, v, starts, scale=0.1)
+    rows = [(0, 1), (50, 0), (99, 3), (100, 2), (231, 1)]
+    for at in rows:
+        q[at][5] = float("nan")
+    got = ops.prompt_attention(q, k, v, starts, scale=0.1)
+    for at in rows:
+        assert bool(got[at].isnan().all())
+        got[at] = want[at]
+    assert torch.equal(got, want)
+
+
 def test_an_infinite_value_among_finite_ones():
     """A visible infinity gives itself, both signs NaN, with finite scores."""
     from pkv import ops

@@ -237,6 +237,41 @@ def test_later_tokens_that_are_not_finite(bits, dtype):
         assert np.all(seen == np.isfinite(held)[:, None])
 
 
+@pytest.mark.parametrize("bits", [4, 8, 16])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_queries_that_are_not_numbers(bits, dtype):
+    """A query with a NaN has a NaN result, in its row alone."""
+    from pkv import ops
+
+    fmt = _format(bits, 128, 64, dtype=getattr(torch, dtype))
+    pool, table, lens, members, starts, prefix = _cache(fmt, [(300, [30, 400, 8]), (0, [50])])
+    q = _queries(fmt, 4, 4, 2)
+    call = lambda: ops.shared_prefix_attention(fmt, pool, q, table, lens, members, starts, prefix, scale=0.1)
+    want = call()
+    rows = [(0, 0, 1), (1, 5, 0), (3, 7, 1), (2, 3, 0)]
+    for at in rows:
+        q[at][9] = float("nan")
+    got = call()
+    for at in rows:
+        assert bool(got[at].isnan().all())
+        got[at] = want[at]
+    assert torch.equal(got, want)
+
+
+def test_starts_that_fall():
+    """Groups that would overlap name no sequence."""
+    from pkv import ops
+
+    fmt = _format(8, 64, 64)
+    pool, table, lens, members, starts, prefix = _cache(fmt, [(50, [10, 20, 30])])
+    q = _queries(fmt, 3, 4, 1)
+    ids = torch.tensor(members, dtype=torch.int32, device="cuda")
+    for at in ([0, 3, 1, 3], [2, 0, 3, 3], [0, 2, 3, -5]):
+        out = torch.full_like(q, 9.0)
+        ops.shared_prefix_attention(fmt, pool, q, table, lens, ids, at, [48, 48, 48], scale=0.1, out=out)
+        assert bool((out == 9.0).all())
+
+
 def test_others_of_a_whole_batch_are_zeros():
     """As many members as sequences, one of them out of range: the rows of the sequence that
     none names are zeros, whatever the memory of the result held."""
