@@ -161,6 +161,7 @@ __device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p,
     p.length[j] = p.own_run[j] = known ? seq_length(a, b) : 0;
   }
   __syncthreads();
+  const int own_cost = a.rows > 16 ? kSharedCost : kOwnCost;  // (two blocks of rows)
   int64_t cost = 0;
   bool falls = false;
   for (int g = tid; g < a.groups; g += kThreads) {
@@ -182,7 +183,7 @@ __device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p,
     const bool in = j >= p.group_first[0] && j < last;
     const int tiles = in ? tiles_of(p.own_run[j]) - p.group_tiles[last_at_most(p.group_first, a.groups, j)] : 0;
     p.own_run[j] = max(0, tiles);
-    cost += kOwnCost * (int64_t)p.own_run[j] * a.g.hk;
+    cost += own_cost * (int64_t)p.own_run[j] * a.g.hk;
   }
   // Long enough runs that all of them are in flight together, as short as that allows: a
   // segment's length is rounded up to whole runs, so each wave tries another allowance.
@@ -193,7 +194,7 @@ __device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p,
   auto lengths = [&](int k, int &long_run, int &own_long) {
     const float each = (float)cost / (float)max(kTarget - (int)((int64_t)segs * (k + 1) / kWaves), kTarget / 4);
     long_run = (int)fminf(each * (1.0f / kSharedCost), 1e9f) + 1;
-    own_long = (int)fminf(each * (1.0f / kOwnCost), 1e9f) + 1;
+    own_long = (int)fminf(each / (float)own_cost, 1e9f) + 1;
   };
   int long_run, own_long, count = 0;
   lengths(tid >> 6, long_run, own_long);
