@@ -19,16 +19,17 @@
 // need those for sums, copy it to LDS.  (In registers at one wave per SIMD: 69 us for 32
 // sequences behind 4096 tokens int8, 87 us for eight answers to each of four 24000-token documents
 // int4, 47 us for five queries each of 16 sequences; now 34, 56 and 33 us, with the merge.)
-// Quantized K enters as its codes
-// (1024 + c, exact in float16; queries as float16, each row scaled by a power of two, which
-// is exact for what its scores keep), group scales and biases are applied to the float32
+//
+// Quantized K enters as its codes (1024 + c, exact in float16; queries as float16, bfloat16 ones
+// with each row scaled by a power of two), group scales and biases are applied to the float32
 // scores:  s = sum_g scale_g (q_g . c'_g) + (bias_g - 1024 scale_g) sum(q_g).  Quantized V is
 // rounded once to float16 (2^-11).  Weights are rounded to the operand type, or, where that
 // would show in the result (bfloat16 pages, float16 results of quantized ones), enter as the
 // sum of two; they are summed as they enter.  Scores, maxima, sums and parts are float32.
 //
 // A token past a sequence's end or on an unmapped page is absent; one that a row may not see
-// yet changes nothing for it, not even where it is not finite.
+// yet changes nothing for it, not even where it is not finite.  (An infinity that it sees may
+// come out as NaN where weights are two operands.)
 #include <algorithm>
 
 #include "pkv_mfma.h"
