@@ -232,15 +232,18 @@ __device__ __forceinline__ bool find_tile(const RopeAppendArgs &a, int tile, int
 __device__ __forceinline__ uint32_t inverse(int d) { return d > 0 ? ((1u << 20) + d - 1) / d : 0; }
 __device__ __forceinline__ int over(int u, uint32_t inv) { return (int)((uint32_t)u * inv >> 20); }
 
-template <int DP, int G, int BITS>
+template <int DP, int G, int BITS, int FK>
 __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppendArgs a, int per_wave) {
   constexpr int KB = DP / 32;
   constexpr int ROW = DP + 8;  // rows of a K tile in LDS, 16 bytes apart
   constexpr int VW = tile_row_words<DP, BITS>();
-  __shared__ float s_cos[PKV_TILE][DP / 2], s_sin[PKV_TILE][DP / 2];
+  // a token's angles: the first four of every eight, then the last four, so that units are 16
+  // bytes apart; rows a quarter of the banks further on
+  __shared__ __attribute__((aligned(16))) float s_cos[PKV_TILE][DP / 2 + 16], s_sin[PKV_TILE][DP / 2 + 16];
   __shared__ __attribute__((aligned(16))) uint32_t s_buf[4][16 * (ROW / 2 > VW ? ROW / 2 : VW)];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Geo &g = a.g;
+  Geo g = a.g;
+  g.float_kind = FK;
   int b, nth;
   if (!find_tile(a, blockIdx.x, lane, b, nth)) return;
   int first, start;
@@ -252,7 +255,8 @@ __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppend
   for (int u = threadIdx.x; u < PKV_TILE * a.half; u += 256) {
     const int t = over(u, by_half), j = u - t * a.half;
     if (rel + t < 0 || rel + t >= n) continue;
-    cos_sin((double)pair_position(a, first + rel + t, pos0 + t, j) * (double)a.inv_freq[j], s_cos[t][j], s_sin[t][j]);
+    const int at = (j & 4 ? a.half / 2 : 0) + (j >> 3) * 4 + (j & 3);
+    cos_sin((double)pair_position(a, first + rel + t, pos0 + t, j) * (double)a.inv_freq[j], s_cos[t][at], s_sin[t][at]);
   }
   __syncthreads();
   const int lo = max(0, -rel), hi = min(PKV_TILE, n - rel);  // the tile's new tokens
@@ -296,13 +300,18 @@ __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppend
         uint16_t x0[8], x1[8], y0[8], y1[8];
         __builtin_memcpy(x0, &w0, 16);
         __builtin_memcpy(x1, &w1, 16);
+        f4 cs[2], sn[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          cs[i] = *(const f4 *)&s_cos[t][i * (a.half / 2) + 4 * c];
+          sn[i] = *(const f4 *)&s_sin[t][i * (a.half / 2) + 4 * c];
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float f0, f1;
-          turn(bits_to_float(x0[e], g.float_kind), bits_to_float(x1[e], g.float_kind), s_cos[t][8 * c + e],
-               s_sin[t][8 * c + e], f0, f1);
-          y0[e] = float_to_bits(f0, g.float_kind);
-          y1[e] = float_to_bits(f1, g.float_kind);
+          turn(bits_to_float(x0[e], FK), bits_to_float(x1[e], FK), cs[e / 4][e % 4], sn[e / 4][e % 4], f0, f1);
+          y0[e] = float_to_bits(f0, FK);
+          y1[e] = float_to_bits(f1, FK);
         }
         u4 o0, o1;
         __builtin_memcpy(&o0, y0, 16);
@@ -362,7 +371,10 @@ hipError_t launch_rope_append(hipStream_t stream, const RopeAppendArgs &a) {
     const dim3 grid(tiles, (all + 4 * per_wave - 1) / (4 * per_wave));
 #define PKV_TILES(DP_, G_, BITS_)                                                                    \
   if (a.g.dp == DP_ && a.g.bits == BITS_ && (BITS_ == 16 || a.g.group == G_)) {                      \
-    hipLaunchKernelGGL((rope_append_tiles_kernel<DP_, G_, BITS_>), grid, block, 0, stream, a, per_wave); \
+    if (a.g.float_kind == 1)                                                                         \
+      hipLaunchKernelGGL((rope_append_tiles_kernel<DP_, G_, BITS_, 1>), grid, block, 0, stream, a, per_wave); \
+    else                                                                                             \
+      hipLaunchKernelGGL((rope_append_tiles_kernel<DP_, G_, BITS_, 0>), grid, block, 0, stream, a, per_wave); \
     return hipGetLastError();                                                                        \
   }
 #define PKV_TILES_Q(DP_, G_) PKV_TILES(DP_, G_, 4) PKV_TILES(DP_, G_, 8)
