@@ -292,38 +292,53 @@ __global__ __launch_bounds__(256) void rope_append_tiles_kernel(const RopeAppend
     } else {
       uint16_t *rows = (uint16_t *)s_buf[wave];
       if (!is_q) wave_lds_sync();  // (the last head's reads of the buffer are done)
-      for (int u = lane; u < PKV_TILE * pairs; u += 64) {
-        const int t = over(u, by_pairs), c = u - t * pairs;
-        if (t < lo || t >= hi) continue;
-        const uint16_t *src = src0 + (int64_t)t * a.row_stride + 8 * c;
-        const u4 w0 = *(const u4 *)src, w1 = *(const u4 *)(src + a.half);
-        uint16_t x0[8], x1[8], y0[8], y1[8];
-        __builtin_memcpy(x0, &w0, 16);
-        __builtin_memcpy(x1, &w1, 16);
-        f4 cs[2], sn[2];
+      // (two units' loads under way at a time)
+      for (int u0 = lane; u0 < PKV_TILE * pairs; u0 += 128) {
+        int t[2], c[2];
+        bool mine[2];
+        u4 w[2][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          cs[i] = *(const f4 *)&s_cos[t][i * (a.half / 2) + 4 * c];
-          sn[i] = *(const f4 *)&s_sin[t][i * (a.half / 2) + 4 * c];
+        for (int k = 0; k < 2; ++k) {
+          const int u = u0 + 64 * k;
+          t[k] = over(u, by_pairs);
+          c[k] = u - t[k] * pairs;
+          mine[k] = t[k] >= lo && t[k] < hi;
+          if (!mine[k]) continue;
+          const uint16_t *src = src0 + (int64_t)t[k] * a.row_stride + 8 * c[k];
+          w[k][0] = *(const u4 *)src;
+          w[k][1] = *(const u4 *)(src + a.half);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float f0, f1;
-          turn(bits_to_float(x0[e], FK), bits_to_float(x1[e], FK), cs[e / 4][e % 4], sn[e / 4][e % 4], f0, f1);
-          y0[e] = float_to_bits(f0, FK);
-          y1[e] = float_to_bits(f1, FK);
-        }
-        u4 o0, o1;
-        __builtin_memcpy(&o0, y0, 16);
-        __builtin_memcpy(&o1, y1, 16);
-        if (out) {
-          uint16_t *dst = out + out_at(a, out_heads, b, first + rel + t, rel + t, out_head) + 8 * c;
-          *(u4 *)dst = o0;
-          *(u4 *)(dst + a.half) = o1;
-        }
-        if (!is_q) {
-          *(u4 *)(rows + t * ROW + 8 * c) = o0;
-          *(u4 *)(rows + t * ROW + a.half + 8 * c) = o1;
+        for (int k = 0; k < 2; ++k) {
+          if (!mine[k]) continue;
+          uint16_t x0[8], x1[8], y0[8], y1[8];
+          __builtin_memcpy(x0, &w[k][0], 16);
+          __builtin_memcpy(x1, &w[k][1], 16);
+          f4 cs[2], sn[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            cs[i] = *(const f4 *)&s_cos[t[k]][i * (a.half / 2) + 4 * c[k]];
+            sn[i] = *(const f4 *)&s_sin[t[k]][i * (a.half / 2) + 4 * c[k]];
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float f0, f1;
+            turn(bits_to_float(x0[e], FK), bits_to_float(x1[e], FK), cs[e / 4][e % 4], sn[e / 4][e % 4], f0, f1);
+            y0[e] = float_to_bits(f0, FK);
+            y1[e] = float_to_bits(f1, FK);
+          }
+          u4 o0, o1;
+          __builtin_memcpy(&o0, y0, 16);
+          __builtin_memcpy(&o1, y1, 16);
+          if (out) {
+            uint16_t *dst = out + out_at(a, out_heads, b, first + rel + t[k], rel + t[k], out_head) + 8 * c[k];
+            *(u4 *)dst = o0;
+            *(u4 *)(dst + a.half) = o1;
+          }
+          if (!is_q) {
+            *(u4 *)(rows + t[k] * ROW + 8 * c[k]) = o0;
+            *(u4 *)(rows + t[k] * ROW + a.half + 8 * c[k]) = o1;
+          }
         }
       }
       for (int u = lane; u < PKV_TILE * plain; u += 64) {
