@@ -7,18 +7,18 @@
 // so a prefix is read once per 32 of the group's query rows per KV head (16 beyond head dim
 // 128) instead of once per sequence.
 //
-// Every workgroup first lays out the call's work from the lengths on the device: the
-// prefix of a (group, KV head, block of rows) and the own tokens of a (sequence, KV
-// head) are segments of 16-token tiles, cut into runs so that all are in flight together.  Its
+// Every workgroup (up to 64 sequences every wave) first lays out the call's work from the
+// lengths on the device: the prefix of a (group, KV head, block of rows) and the own tokens of
+// a (sequence, KV head) are segments of 16-token tiles, cut into runs so that all are in flight together.  Its
 // four waves take pairs of a run's tiles in turn:
 //   S^T = K.Q^T      v_mfma_f32_16x16x32, one tile: lane (row, jj) holds tokens 4jj + r
 //   O^T += V^T.P^T   v_mfma_f32_16x16x32, the pair's 32 tokens
 // What bounds it are the instructions that turn codes into operands (a pair takes about 400, and
-// 560 for two blocks of 16 rows), then the way from the lengths to the first tile, about 8 us.
+// 560 for two blocks of 16 rows), then the way from the lengths to the first tile, about 6 us.
 // So two waves share a SIMD: one block of rows keeps the next pair in registers; two, which
 // need those for sums, copy it to LDS.  (In registers at one wave per SIMD: 69 us for 32
 // sequences behind 4096 tokens int8, 87 us for eight answers to each of four 24000-token documents
-// int4, 47 us for five queries each of 16 sequences; now 34, 56 and 33 us, with the merge.)
+// int4, 47 us for five queries each of 16 sequences; now 32, 55 and 31 us, with the merge.)
 //
 // Quantized K enters as its codes (1024 + c, exact in float16; queries as float16, bfloat16 ones
 // with each row scaled by a power of two), group scales and biases are applied to the float32
@@ -152,7 +152,14 @@ __device__ __forceinline__ int row_blocks(const SharedArgs &a, const SharedPlan 
   return (max(0, p.group_first[g + 1] - p.group_first[g]) * a.rows + per - 1) / per;
 }
 
-__device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p, int per, int tid) {
+// The lengths of runs by the k-th allowance for the segments' ends.
+__device__ __forceinline__ void run_lengths(int64_t cost, int segs, int own_cost, int k, int &long_run, int &own_long) {
+  const float each = (float)cost / (float)max(kTarget - (int)((int64_t)segs * (k + 1) / kWaves), kTarget / 4);
+  long_run = (int)fminf(each * (1.0f / kSharedCost), 1e9f) + 1;
+  own_long = (int)fminf(each / (float)own_cost, 1e9f) + 1;
+}
+
+__device__ __forceinline__ void lay_out(const SharedArgs &a, SharedPlan &p, int per, int tid) {
   for (int g = tid; g <= a.groups; g += kThreads) p.group_first[g] = min(max(a.group_starts[g], 0), a.count);
   for (int g = tid; g < a.groups; g += kThreads) p.group_tiles[g] = a.prefix_lens[g];
   for (int j = tid; j < a.count; j += kThreads) {
@@ -192,13 +199,8 @@ __device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p,
   for (int g = tid; g < a.groups; g += kThreads) segs += p.group_tiles[g] > 0 ? row_blocks(a, p, g, per) * a.g.hk : 0;
   for (int j = tid; j < a.count; j += kThreads) segs += p.own_run[j] > 0 ? a.g.hk : 0;
   block_sum(p, cost, segs, tid);
-  auto lengths = [&](int k, int &long_run, int &own_long) {
-    const float each = (float)cost / (float)max(kTarget - (int)((int64_t)segs * (k + 1) / kWaves), kTarget / 4);
-    long_run = (int)fminf(each * (1.0f / kSharedCost), 1e9f) + 1;
-    own_long = (int)fminf(each / (float)own_cost, 1e9f) + 1;
-  };
   int long_run, own_long, count = 0;
-  lengths(tid >> 6, long_run, own_long);
+  run_lengths(cost, segs, own_cost, tid >> 6, long_run, own_long);
   for (int g = tid & 63; g < a.groups; g += 64) count += row_blocks(a, p, g, per) * runs_of(p.group_tiles[g], long_run);
   for (int j = tid & 63; j < a.count; j += 64) count += runs_of(p.own_run[j], own_long);
   count = wave_sum(count);
@@ -207,7 +209,7 @@ __device__ void lay_out(const SharedArgs &a, const SharedWork &w, SharedPlan &p,
   __syncthreads();
   int k = 0;
   while (k < kWaves - 1 && (int64_t)p.reduce[k] * a.g.hk > kTarget) ++k;
-  lengths(k, long_run, own_long);
+  run_lengths(cost, segs, own_cost, k, long_run, own_long);
   for (int g = tid; g < a.groups; g += kThreads)
     p.group_run[g] = row_blocks(a, p, g, per) * a.g.hk * runs_of(p.group_tiles[g], long_run);
   for (int j = tid; j < a.count; j += kThreads) p.own_run[j] = a.g.hk * runs_of(p.own_run[j], own_long);
@@ -281,7 +283,7 @@ struct Pair {
 };
 
 template <typename C, int RB>
-__device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork &w, const SharedPlan &plan, const Run &run,
+__device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork &w, const int *sequence, const int *length, const Run &run,
                                           int lane, int wave, TilePlace *where, uint8_t *lds, float (*s_ml)[shared_rows(64)][2]) {
   using T = typename C::T;
   using E = typename C::E;
@@ -381,9 +383,9 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
     const int r = run.row0 + rb * 16 + col;
     const bool there = rb * 16 + col < run.rows;
     const int member = there ? r / a.rows : 0, in = there ? r - member * a.rows : 0;
-    const int b = plan.sequence[run.member + member];
+    const int b = sequence[run.member + member];
     const int qi = in / a.gqa, h = run.kh * a.gqa + in - qi * a.gqa, at = max(b, 0);
-    const int L = plan.length[run.member + member];
+    const int L = length[run.member + member];
     const int width = a.widths ? a.widths[at] : a.nq;
     const int pos = a.q_pos ? a.q_pos[(int64_t)at * a.nq + qi] : a.seq_lens[at] - width + qi;
     lim[rb] = there && b >= 0 && qi < width ? min(pos, L - 1) : -1;
@@ -401,7 +403,7 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
       }
     }
   }
-  if constexpr (STAGED) __syncthreads();  // (the plan's memory is taken)
+  if constexpr (STAGED) __syncthreads();  // (a plan's memory is taken)
   if (wave < pairs) {
     locate(0);
     if constexpr (STAGED) {
@@ -783,20 +785,10 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
   }
 }
 
-template <int BITS, int DP, int G, int FK>
-__global__ __launch_bounds__(kThreads, 2) void shared_kernel(const SharedArgs a, const SharedWork w) {
-  using C = SharedCfg<BITS, DP, G, FK>;
-  constexpr int PER = shared_rows(DP);
-  // the plan; behind it the copies and the rows of two blocks; behind those the sums
-  constexpr int kRing = PER > 16 ? kWaves * 2 * side_bytes<C>() + 2 * C::KB * 1024 : 0;
-  constexpr int kSums = kWaves * 16 * (DP + 4) * 4;
-  constexpr int kLds = std::max({(int)sizeof(SharedPlan), kRing, kSums});
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-  SharedPlan &plan = *(SharedPlan *)lds;
-  __shared__ float s_ml[kWaves][shared_rows(64)][2];
-  __shared__ TilePlace s_place[kWaves][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  lay_out(a, w, plan, PER, tid);
+// Run u of the call and, in the first workgroup, what the merge needs: by a plan in LDS.
+__device__ __forceinline__ bool planned_run(const SharedArgs &a, const SharedWork &w, SharedPlan &plan, int per, int u, int tid, Run &run) {
+  const int lane = tid & 63;
+  lay_out(a, plan, per, tid);
   const int shared_runs = plan.group_run[a.groups], runs = shared_runs + plan.own_run[a.count];
   if (blockIdx.x == 0) {
     // where a member's parts are, for the merge: its group's first run and runs per
@@ -813,43 +805,155 @@ __global__ __launch_bounds__(kThreads, 2) void shared_kernel(const SharedArgs a,
       d[5] = in;
     }
   }
-  const int u = blockIdx.x;
-  if (u < runs && u < w.most) {
-    Run run;
-    run.slot = u;
-    if (u < shared_runs) {
-      const int g = last_at_most_uniform(plan.group_run, a.groups, u, lane);
-      const int tiles = plan.group_tiles[g], n = runs_of(tiles, plan.long_run), at = u - plan.group_run[g];
-      const int seg = at / n, blk = seg / a.g.hk, len = run_length(tiles, n);
-      run.kh = seg - blk * a.g.hk;
-      run.t0 = min((at - seg * n) * len, tiles);
-      run.t1 = min(tiles, run.t0 + len);
-      run.member = plan.group_first[g];
-      run.row0 = blk * PER;
-      run.rows = min(PER, (plan.group_first[g + 1] - run.member) * a.rows - run.row0);
-    } else {
-      const int j = last_at_most_uniform(plan.own_run, a.count, u - shared_runs, lane);
-      const int n = (plan.own_run[j + 1] - plan.own_run[j]) / a.g.hk, at = u - shared_runs - plan.own_run[j];
-      const int g = last_at_most_uniform(plan.group_first, a.groups, j, lane);
-      run.kh = at / n;
-      const int first = plan.group_tiles[g], end = tiles_of(plan.length[j]), len = run_length(end - first, n);
-      run.t0 = min(first + (at - run.kh * n) * len, end);
-      run.t1 = min(end, run.t0 + len);
-      run.member = j;
-      run.row0 = 0;
-      run.rows = a.rows;
+  if (u >= runs) return false;
+  run.slot = u;
+  if (u < shared_runs) {
+    const int g = last_at_most_uniform(plan.group_run, a.groups, u, lane);
+    const int tiles = plan.group_tiles[g], n = runs_of(tiles, plan.long_run), at = u - plan.group_run[g];
+    const int seg = at / n, blk = seg / a.g.hk, len = run_length(tiles, n);
+    run.kh = seg - blk * a.g.hk;
+    run.t0 = min((at - seg * n) * len, tiles);
+    run.t1 = min(tiles, run.t0 + len);
+    run.member = plan.group_first[g];
+    run.row0 = blk * per;
+    run.rows = min(per, (plan.group_first[g + 1] - run.member) * a.rows - run.row0);
+  } else {
+    const int j = last_at_most_uniform(plan.own_run, a.count, u - shared_runs, lane);
+    const int n = (plan.own_run[j + 1] - plan.own_run[j]) / a.g.hk, at = u - shared_runs - plan.own_run[j];
+    const int g = last_at_most_uniform(plan.group_first, a.groups, j, lane);
+    run.kh = at / n;
+    const int first = plan.group_tiles[g], end = tiles_of(plan.length[j]), len = run_length(end - first, n);
+    run.t0 = min(first + (at - run.kh * n) * len, end);
+    run.t1 = min(end, run.t0 + len);
+    run.member = j;
+    run.row0 = 0;
+    run.rows = a.rows;
+  }
+  return true;
+}
+
+// The same for at most 64 members and 63 groups, by each wave for itself: lane l has member l and
+// group l.  (No barrier: 2.9 us until the run is known instead of 4.8, for 16 sequences in four
+// groups.)
+__device__ __forceinline__ bool small_run(const SharedArgs &a, const SharedWork &w, int per, int u, int wave, int lane, int *sequence,
+                          int *length, Run &run) {
+  const int hk = a.g.hk;
+  int first = min(max(a.group_starts[min(lane, a.groups)], 0), a.count);
+  int tiles = lane < a.groups ? a.prefix_lens[lane] : 0;
+  const int b = lane < a.count ? a.members[lane] : -1;
+  const bool known = b >= 0 && b < a.batch;
+  const int len = known ? seq_length(a, b) : 0;
+  sequence[lane] = known ? b : -1;
+  length[lane] = len;
+  const int next = __shfl(first, min(lane + 1, 63), 64);
+  int n = lane < a.groups ? next - first : 0;
+  if (__any(n < 0)) first = n = tiles = 0;  // groups that would overlap: none
+  const int held = __shfl(len, min(first, 63), 64);
+  tiles = n > 1 ? max(0, min(tiles, held)) / PKV_TILE : 0;  // (one sequence shares nothing)
+  const int blocks = (n * a.rows + per - 1) / per;
+  const int last = __builtin_amdgcn_readlane(first, a.groups);
+  int g = -1;  // the member's group
+  for (int k = 0; k < a.groups; ++k) g += lane >= __builtin_amdgcn_readlane(first, k);
+  const bool in = g >= 0 && lane < last;
+  g = max(g, 0);
+  const int skipped = __shfl(tiles, g, 64);
+  const int own = in ? max(0, tiles_of(len) - skipped) : 0;
+  const int own_cost = a.rows > 16 ? kSharedCost : kOwnCost;
+  const int64_t mine = ((int64_t)kSharedCost * tiles * blocks + (int64_t)own_cost * own) * hk;
+  const int lo = wave_sum((int)(mine & 0x7FFFFF));
+  const int hi = wave_sum((int)(mine >> 23));
+  const int64_t cost = lo + ((int64_t)hi << 23);
+  const int segs = wave_sum((tiles > 0 ? blocks : 0) + (own > 0 ? 1 : 0)) * hk;
+  int long_run = 0, own_long = 0, shared_n = 0, own_n = 0;  // a segment's runs
+  for (int k = 0; k < kWaves; ++k) {
+    run_lengths(cost, segs, own_cost, k, long_run, own_long);
+    shared_n = runs_of(tiles, long_run);
+    own_n = runs_of(own, own_long);
+    if ((int64_t)wave_sum(blocks * shared_n + own_n) * hk <= kTarget) break;
+  }
+  const int group_runs = blocks * hk * shared_n, own_runs = hk * own_n;
+  const int group_end = wave_scan_incl(group_runs, lane), own_end = wave_scan_incl(own_runs, lane);
+  const int group_run = group_end - group_runs, own_run = own_end - own_runs;
+  const int shared_runs = __builtin_amdgcn_readlane(group_end, 63);
+  const int runs = shared_runs + __builtin_amdgcn_readlane(own_end, 63);
+  if (blockIdx.x == 0) {
+    const int d0 = __shfl(group_run, g, 64), d1 = __shfl(shared_n, g, 64), at = __shfl(first, g, 64);
+    if (wave == 0 && lane < a.count) {
+      int32_t *d = w.desc + 8 * lane;
+      d[0] = d0;
+      d[1] = in ? d1 : 0;
+      d[2] = (lane - at) * a.rows;
+      d[3] = shared_runs + own_run;
+      d[4] = own_n;
+      d[5] = in;
     }
+  }
+  if (u >= runs) return false;
+  run.slot = u;
+  if (u < shared_runs) {
+    const int k = __popcll(__ballot(lane < a.groups && group_run <= u)) - 1;
+    const int total = __builtin_amdgcn_readlane(tiles, k), c = __builtin_amdgcn_readlane(shared_n, k);
+    const int at = u - __builtin_amdgcn_readlane(group_run, k), seg = at / c, blk = seg / hk, size = run_length(total, c);
+    run.kh = seg - blk * hk;
+    run.t0 = min((at - seg * c) * size, total);
+    run.t1 = min(total, run.t0 + size);
+    run.member = __builtin_amdgcn_readlane(first, k);
+    run.row0 = blk * per;
+    run.rows = min(per, __builtin_amdgcn_readlane(n, k) * a.rows - run.row0);
+  } else {
+    const int k = __popcll(__ballot(lane < a.count && own_run <= u - shared_runs)) - 1;
+    const int c = __builtin_amdgcn_readlane(own_n, k), at = u - shared_runs - __builtin_amdgcn_readlane(own_run, k);
+    const int from = __builtin_amdgcn_readlane(skipped, k), end = tiles_of(__builtin_amdgcn_readlane(len, k));
+    const int size = run_length(end - from, c);
+    run.kh = at / c;
+    run.t0 = min(from + (at - run.kh * c) * size, end);
+    run.t1 = min(end, run.t0 + size);
+    run.member = k;
+    run.row0 = 0;
+    run.rows = a.rows;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return true;
+}
+
+template <int BITS, int DP, int G, int FK>
+__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void shared_kernel(const SharedArgs a, const SharedWork w) {
+  using C = SharedCfg<BITS, DP, G, FK>;
+  constexpr int PER = shared_rows(DP);
+  // the plan; behind it the copies and the rows of two blocks; behind those the sums
+  constexpr int kRing = PER > 16 ? kWaves * 2 * side_bytes<C>() + 2 * C::KB * 1024 : 0;
+  constexpr int kSums = kWaves * 16 * (DP + 4) * 4;
+  constexpr int kLds = std::max({(int)sizeof(SharedPlan), kRing, kSums});
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+  SharedPlan &plan = *(SharedPlan *)lds;
+  __shared__ float s_ml[kWaves][shared_rows(64)][2];
+  __shared__ TilePlace s_place[kWaves][64];
+  __shared__ int s_members[kWaves][2][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int u = blockIdx.x;
+  Run run;
+  const int *sequence = plan.sequence, *length = plan.length;
+  bool found;
+  if (a.count <= 64 && a.groups < 64) {
+    found = small_run(a, w, PER, u, wave, lane, s_members[wave][0], s_members[wave][1], run);
+    sequence = s_members[wave][0];
+    length = s_members[wave][1];
+  } else {
+    found = planned_run(a, w, plan, PER, u, tid, run);
+  }
+  if (found && u < w.most) {
     // (a member that is no sequence has no tokens; the first of a group with a prefix is one)
-    run.b = max(0, __builtin_amdgcn_readfirstlane(plan.sequence[run.member]));
-    run.L = __builtin_amdgcn_readfirstlane(plan.length[run.member]);
+    run.b = max(0, __builtin_amdgcn_readfirstlane(sequence[run.member]));
+    run.L = __builtin_amdgcn_readfirstlane(length[run.member]);
     run.kh = __builtin_amdgcn_readfirstlane(run.kh);
     run.t0 = __builtin_amdgcn_readfirstlane(run.t0);
     run.t1 = __builtin_amdgcn_readfirstlane(run.t1);
     run.member = __builtin_amdgcn_readfirstlane(run.member);
     run.row0 = __builtin_amdgcn_readfirstlane(run.row0);
     run.rows = __builtin_amdgcn_readfirstlane(run.rows);
-    if (run.rows <= 16) run_tiles<C, 1>(a, w, plan, run, lane, wave, s_place[wave], lds, s_ml);
-    else if constexpr (PER > 16) run_tiles<C, 2>(a, w, plan, run, lane, wave, s_place[wave], lds, s_ml);
+    if (run.rows <= 16) run_tiles<C, 1>(a, w, sequence, length, run, lane, wave, s_place[wave], lds, s_ml);
+    else if constexpr (PER > 16) run_tiles<C, 2>(a, w, sequence, length, run, lane, wave, s_place[wave], lds, s_ml);
   }
 }
 

@@ -148,6 +148,17 @@ def test_sharp_and_flat_weights(bits, gain, k_scale):
     _check(_format(bits, 128, 64, dtype=torch.float16), [(200, [40, 300, 7])], 4, 2, gain=min(gain, 100.0), k_scale=k_scale)
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("groups", [
+    [(100, [1 + 7 * i % 40 for i in range(64)])], [(100, [1 + 7 * i % 40 for i in range(65)])],
+    [(40, [3, 20])] * 31 + [(0, [9])], [(40, [3, 20])] * 31 + [(0, [9]), (0, [2])], [(0, [5])] * 63, [(0, [5])] * 64,
+    [(48, [2, 30, 17])] * 33, [(16, [1 + i % 3, 20]) for i in range(70)], [(3000, [10] * 8)] * 12],
+    ids=lambda g: f"{len(g)}-{sum(len(own) for _, own in g)}")
+def test_many_members_and_groups(bits, groups):
+    """Up to 64 members in 63 groups each wave lays the call out by itself, beyond by a plan."""
+    _check(_format(bits, 64, 32, 16, 1), groups, 4, 1)
+
+
 def test_long_prefixes():
     """Runs of many pairs, more than a wave's page window."""
     _check(_format(8, 64, 64, 16, 1), [(20000, [100, 3000, 1])], 2, 1)
