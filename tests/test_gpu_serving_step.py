@@ -240,3 +240,88 @@ def test_another_stream():
         got = run()
     torch.cuda.current_stream().wait_stream(stream)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("bits", [4, 8, 16])
+def test_pages_past_32_bits(bits):
+    """Pages that lie beyond 4 GiB in their pool hold and give what pages of a small pool do."""
+    from pkv import ops
+
+    fmt = ops.PageFormat(8, 128, 128, bits, 64, torch.bfloat16)
+    count = (9 << 29) // fmt.page_bytes + 8
+    far, near = torch.empty((count, fmt.page_bytes), dtype=torch.uint8, device="cuda"), ops.allocate_pool(fmt, 8)
+    far[-8:] = 0
+    lens = torch.tensor([200, 330, 140], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[0, 1, -1], [0, 2, 3], [0, 4, -1]], dtype=torch.int32, device="cuda")
+    zero, inv = torch.zeros_like(lens), _frequencies(64)
+    qkv = _projection(670, 16, fmt, 1)
+    qkv[200:328] = qkv[:128]    # the first page is one for all three
+    qkv[530:658] = qkv[:128]
+    last = _projection(1, 16, fmt, 2, (3,))
+    got = []
+    for pool, at in ((near, table), (far, torch.where(table < 0, table, table + count - 8))):
+        q = ops.rope_append(fmt, pool, qkv, at, zero, inv, 16, row_starts=[0, 200, 530, 670])
+        step = ops.rope_append(fmt, pool, last, at, lens, inv, 16)
+        out = ops.shared_prefix_attention(fmt, pool, step, at, lens + 1, [0, 1, 2], [0, 3], [128], scale=0.1)
+        got.append((q, step, out, pool[-8:][:5].clone()))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert bool((got[0][2] != 0).any(-1).all())
+
+
+def test_rows_past_32_bits():
+    """Packed rows whose elements are numbered past 2^31: the last prompts as by themselves."""
+    from pkv import ops
+
+    rows, heads, dim = 540_000, 32, 128
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.empty((rows, heads, dim), dtype=torch.bfloat16, device="cuda")
+    q[-9:] = torch.randn((9, heads, dim), generator=gen, device="cuda")
+    q[:-9] = q[-1]
+    k, v = (torch.randn((rows, 2, dim), generator=gen, device="cuda").bfloat16() for _ in range(2))
+    starts = list(range(0, rows - 9, 30)) + [rows - 9, rows - 4, rows]
+    out = ops.prompt_attention(q, k, v, starts, scale=0.1)
+    want = ops.prompt_attention(*(t[-9:].contiguous() for t in (q, k, v)), [0, 5, 9], scale=0.1)
+    assert torch.equal(out[-9:], want)
+    some = slice(30 * 9000, 30 * 9001)
+    assert torch.equal(out[some], ops.prompt_attention(*(t[some].contiguous() for t in (q, k, v)), [0, 30], scale=0.1))
+
+
+def test_captured_prompts():
+    """Rotation with append and prompt attention in a graph, replayed for other rows and other
+    lengths with eager calls between, each replay against the eager calls."""
+    from pkv import ops
+
+    arena = _arena(8)
+    fmt, inv, scale = arena.fmt, _frequencies(32), 0.125
+    slots = [arena.open_slot() for _ in range(3)]
+    res = arena.reserve(slots, [300, 300, 300])
+    cuts = [[0, 100, 130, 300], [0, 1, 2, 300], [0, 0, 290, 300], [0, 64, 128, 256]]
+    starts = torch.tensor(cuts[0], dtype=torch.int32, device="cuda")
+    qkv = _projection(300, 8, fmt, 1)
+
+    def run(pool):
+        q, k, v = ops.rope_append(fmt, pool, qkv, res.table, res.starts, inv, 8, row_starts=starts, with_kv=True, out=held[0])
+        return ops.prompt_attention(q, k, v, starts, scale=scale, out=held[1])
+
+    shapes = [(300, 8, 64), (300, 2, 64), (300, 2, 64)]
+    held = ([torch.zeros(s, dtype=fmt.dtype, device="cuda") for s in shapes], torch.zeros(shapes[0], dtype=fmt.dtype, device="cuda"))
+    mine, pool = held, arena.pools[0]
+    run(pool)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        with torch.cuda.graph(graph, stream=stream):
+            run(pool)
+    torch.cuda.current_stream().wait_stream(stream)
+    for turn in range(8):
+        starts.copy_(torch.tensor(cuts[turn % 4], dtype=torch.int32))
+        qkv.copy_(_projection(300, 8, fmt, 50 + turn))
+        held = ([t.clone() for t in mine[0]], mine[1].clone())
+        other = pool.clone()
+        want = run(other)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(mine[1], want) and torch.equal(pool, other)
+        assert all(torch.equal(a, b) for a, b in zip(mine[0], held[0]))
