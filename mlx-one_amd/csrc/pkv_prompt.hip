@@ -21,8 +21,8 @@
 //
 // Bound by the issue of matrix and vector instructions: a tile's weights and product are
 // issued beside the next tile's scores, and two waves share a SIMD (one beyond head dim 128,
-// where two would spill: 355 us against 144 for 16 heads of 256).  16,000 rows of 32 heads of 128: 1.93
-// ms, 1.09 PFLOP/s (86% of an 8192^3 product); 16 prompts of 100 to 2,000 rows 0.25 ms.
+// where two would spill: 355 us against 144 then for 16 heads of 256).  16,000 rows of 32 heads of 128: 1.93
+// ms, 1.09 PFLOP/s (86% of an 8192^3 product); 16 prompts of 100 to 2,000 rows 0.23 ms.
 #include <type_traits>
 
 #include "pkv_mfma.h"
@@ -414,20 +414,27 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
 
   const int row = place * 32 + col;
   const float inv = 1.0f / xor32_add(l);
-  if (place < 0 || row >= n) return;
+  if (place < 0) return;
+  const bool there = row < n;
   uint16_t *dst = a.out + ((int64_t)(first + row) * a.heads + head) * a.dim;
+  // (a lane's four dims beside the other half's: 16 bytes a store, g even from half 0 and g + 1
+  // from half 1)
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = 32 * nb + 8 * g + 4 * half;
-      if (d >= a.dim) continue;
-      E r[4];
+    for (int g = 0; g < 4; g += 2) {
+      u2 w[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = (E)(O[nb][4 * g + e] * inv);
-      u2 w;
-      __builtin_memcpy(&w, r, 8);
-      *(u2 *)(dst + d) = w;
+      for (int i = 0; i < 2; ++i) {
+        E r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = (E)(O[nb][4 * (g + i) + e] * inv);
+        __builtin_memcpy(&w[i], r, 8);
+      }
+      const auto x = __builtin_amdgcn_permlane32_swap(w[0].x, w[1].x, false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(w[0].y, w[1].y, false, false);
+      const int d = 32 * nb + 8 * (g + half);
+      if (there && d < a.dim) *(u4 *)(dst + d) = u4{x[0], y[0], x[1], y[1]};
     }
 }
 
