@@ -571,6 +571,7 @@ class DeviceRunner:
             out = forward(res)
         except BaseException:
             self.arena.rollback(slots, before)
+            self.arena.probe_failed(probe)    # (what a failed reserve recorded goes with its step)
             raise
         err = self.arena.probe_failed(probe)
         if err:
@@ -615,7 +616,15 @@ class DeviceRunner:
         widths = [width] * batch if widths is None else [int(w) for w in widths]
         if len(slots) != batch or len(widths) != batch or any(w < 1 or w > width for w in widths):
             raise ValueError("one slot and a width in 1..T per row")
+        self._check_groups(shared, batch)
         return self._step(slots, widths, lambda res: self._forward(hidden, res, shared=shared))
+
+    @staticmethod
+    def _check_groups(shared, batch):
+        """Groups of another batch would leave rows without attention."""
+        if shared is not None and (len(shared) != 3 or shared[0].numel() != batch
+                                   or shared[1].numel() != shared[2].numel() + 1):
+            raise ValueError("shared must be the prefix_groups of the batch's slots")
 
     def capture_decode(self, slots, hidden, *, warm=True, shared=None):
         """Graphs of one decode step (one token per slot) reading the static
@@ -633,6 +642,7 @@ class DeviceRunner:
         slots_d = torch.tensor([int(s) for s in slots], dtype=torch.int32, device=device)
         widths_d = torch.ones_like(slots_d)
         count = int(slots_d.numel())
+        self._check_groups(shared, count)
         # the graph's split-K partials live in a workspace of its own, sized as an
         # eager call's (so both run the same split) for the waves fixed at
         # capture, and held by the CapturedStep

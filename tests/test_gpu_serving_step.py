@@ -168,6 +168,10 @@ def test_runner(bits):
     assert one.lengths == two.lengths
     with pytest.raises(ValueError):
         shared.prefill(slots, packed, lens)
+    with pytest.raises(ValueError):
+        shared.execute(batch[:6], _hidden(1, 30, (6,)), shared=groups)
+    with pytest.raises(ValueError):
+        shared.capture_decode(batch[:6], _hidden(1, 30, (6,)), shared=groups)
     fresh = one.open_slot()
     with pytest.raises(ValueError):
         shared.prefill([fresh], packed, [5])
@@ -325,3 +329,33 @@ def test_captured_prompts():
         torch.cuda.synchronize()
         assert torch.equal(mine[1], want) and torch.equal(pool, other)
         assert all(torch.equal(a, b) for a, b in zip(mine[0], held[0]))
+
+
+def test_steps_that_run_out_of_pages():
+    """A prefill or a shared step without pages raises and changes neither lengths nor the
+    tokens that the pages hold."""
+    from pkv import ops
+    from pkv.cache_errors import CacheCapacityError
+    from pkv.device_arena import DevicePageArena, DeviceRunner
+    from pkv.modes import ModelCapabilityUnsupported
+
+    fmt = ops.PageFormat(2, 64, 16, 8, 32, torch.bfloat16)
+    arena = DevicePageArena(fmt, 7, num_layers=2, max_slots=8, max_tokens=512)
+    runner = DeviceRunner(_model(2), arena)
+    a, b, c = (arena.open_slot() for _ in range(3))
+    runner.prefill([a], _hidden(96, 1), [96])
+    arena.fork([a], [b])
+    held = [p[arena.pages(a)].clone() for p in arena.pools]
+    with pytest.raises(CacheCapacityError):
+        runner.prefill([c], _hidden(100, 2), [100])
+    groups = arena.prefix_groups([a, b])
+    assert groups[2].tolist() == [96]
+    with pytest.raises(CacheCapacityError):
+        runner.execute([a, b], _hidden(8, 3, (2,)), shared=groups)
+    with pytest.raises(ModelCapabilityUnsupported):    # (more query rows than a shared step takes)
+        runner.execute([a, b], _hidden(9, 3, (2,)), shared=groups)
+    assert arena.lengths[:3] == [96, 96, 0] and arena.lens.tolist()[:3] == [96, 96, 0]
+    assert all(torch.equal(p[arena.pages(a)], h) for p, h in zip(arena.pools, held))
+    out = runner.execute([a], _hidden(2, 4, (1,)), shared=arena.prefix_groups([a]))
+    assert bool(torch.isfinite(out).all()) and arena.lengths[:2] == [98, 96]
+    arena.check()
