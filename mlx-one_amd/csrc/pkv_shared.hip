@@ -283,8 +283,9 @@ struct Pair {
 };
 
 template <typename C, int RB>
-__device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork &w, const int *sequence, const int *length, const Run &run,
-                                          int lane, int wave, TilePlace *where, uint8_t *lds, float (*s_ml)[shared_rows(64)][2]) {
+__device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork &w, const int *sequence,
+                                          const int *length, const Run &run, int lane, int wave, TilePlace *where,
+                                          uint8_t *lds, float (*s_ml)[shared_rows(64)][2]) {
   using T = typename C::T;
   using E = typename C::E;
   constexpr int KB = C::KB, NB = C::NB, NG = C::NG, DP = 32 * KB;
@@ -363,7 +364,8 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
   };
   auto stage_k = [&]() __attribute__((always_inline)) { stage(0, g.kmeta_offset, ring); };
   auto stage_v = [&]() __attribute__((always_inline)) { stage(g.v_offset, g.vmeta_offset, ring + kSide); };
-  auto take = [&](const uint8_t *from, uint32_t (&words)[2][C::LW], uint32_t (&meta)[2][C::MW]) __attribute__((always_inline)) {
+  auto take = [&](const uint8_t *from, uint32_t (&words)[2][C::LW], uint32_t (&meta)[2][C::MW])
+      __attribute__((always_inline)) {
     const int lane = lane_again(), jj = lane >> 4;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -454,7 +456,8 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 8; e += 2)
-          qs[rb][kb / GB] = __builtin_amdgcn_fdot2(h2{q[rb][kb][e], q[rb][kb][e + 1]}, h2{(_Float16)1.0f, (_Float16)1.0f}, qs[rb][kb / GB], false);
+          qs[rb][kb / GB] = __builtin_amdgcn_fdot2(h2{q[rb][kb][e], q[rb][kb][e + 1]},
+                                                   h2{(_Float16)1.0f, (_Float16)1.0f}, qs[rb][kb / GB], false);
 #pragma unroll
       for (int x = 0; x < NG; ++x) qs[rb][x] = xor32_add(xor16_add(qs[rb][x]));
     }
@@ -538,7 +541,8 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
             const float sc = (float)sb.x, off = __builtin_fmaf(-1024.0f, sc, (float)sb.y);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
-              x[rb][4 * s + e] = __builtin_fmaf(S[rb][x_][e], sc, x_ == 0 ? off * qs[rb][x_] : __builtin_fmaf(off, qs[rb][x_], x[rb][4 * s + e]));
+              x[rb][4 * s + e] = __builtin_fmaf(S[rb][x_][e], sc, x_ == 0 ? off * qs[rb][x_]
+                                                                          : __builtin_fmaf(off, qs[rb][x_], x[rb][4 * s + e]));
           }
         } else {
 #pragma unroll
@@ -786,7 +790,8 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
 }
 
 // Run u of the call and, in the first workgroup, what the merge needs: by a plan in LDS.
-__device__ __forceinline__ bool planned_run(const SharedArgs &a, const SharedWork &w, SharedPlan &plan, int per, int u, int tid, Run &run) {
+__device__ __forceinline__ bool planned_run(const SharedArgs &a, const SharedWork &w, SharedPlan &plan, int per, int u,
+                                            int tid, Run &run) {
   const int lane = tid & 63;
   lay_out(a, plan, per, tid);
   const int shared_runs = plan.group_run[a.groups], runs = shared_runs + plan.own_run[a.count];
@@ -835,8 +840,8 @@ __device__ __forceinline__ bool planned_run(const SharedArgs &a, const SharedWor
 // The same for at most 64 members and 63 groups, by each wave for itself: lane l has member l and
 // group l.  (No barrier: 2.9 us until the run is known instead of 4.8, for 16 sequences in four
 // groups.)
-__device__ __forceinline__ bool small_run(const SharedArgs &a, const SharedWork &w, int per, int u, int wave, int lane, int *sequence,
-                          int *length, Run &run) {
+__device__ __forceinline__ bool small_run(const SharedArgs &a, const SharedWork &w, int per, int u, int wave, int lane,
+                                          int *sequence, int *length, Run &run) {
   const int hk = a.g.hk;
   int first = min(max(a.group_starts[min(lane, a.groups)], 0), a.count);
   int tiles = lane < a.groups ? a.prefix_lens[lane] : 0;

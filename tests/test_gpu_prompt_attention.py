@@ -86,6 +86,16 @@ def test_large(heads, kv_heads, dim, lens):
     _check(lens, heads, kv_heads, dim, rows=rows)
 
 
+@pytest.mark.parametrize("batch", [2, 3, 4, 7, 12, 13, 64, 70])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (6, 2)])
+def test_orders(batch, heads, kv_heads):
+    """Sequences of unlike lengths, empty ones among them, as blocks are found in each order."""
+    rng = np.random.default_rng(batch)
+    lens = [int(n) for n in rng.integers(0, 200, batch)]
+    lens[0], lens[-1], lens[batch // 2] = 300, 33, 0
+    _check(lens, heads, kv_heads, behind=3)
+
+
 def test_many_sequences():
     rng = np.random.default_rng(0)
     _check([int(n) for n in rng.integers(0, 40, 150)], 2, 1, 64)

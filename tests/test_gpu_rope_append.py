@@ -131,14 +131,14 @@ def test_pages_and_starts(bits, page, lens, cached):
 
 
 @pytest.mark.parametrize("bits", [4, 8, 16])
-@pytest.mark.parametrize("lens", [(1, 3, 2), (30, 0, 17)])
+@pytest.mark.parametrize("lens", [(1, 3, 2), (30, 0, 17), (70, 0, 47)])
 def test_padded(bits, lens):
     _check(bits, 128, 64, lens=lens, padded=True)
     _check(bits, 64, 32, lens=lens, padded=True, axes=3, dtype=torch.float16)
 
 
 @pytest.mark.parametrize("dim,half", [(128, 32), (128, 0), (128, 20), (80, 16), (256, 128), (64, 24)])
-@pytest.mark.parametrize("lens", [(1, 2), (50, 20)])
+@pytest.mark.parametrize("lens", [(1, 2), (50, 20), (110, 45)])
 def test_part_of_a_head_and_axes(dim, half, lens):
     _check(8, dim, 32, lens=lens, half=half)
     _check(16, dim, 32, lens=lens, half=half, axes=3)
@@ -146,19 +146,19 @@ def test_part_of_a_head_and_axes(dim, half, lens):
 
 
 @pytest.mark.parametrize("spare,offset", [(8, 0), (24, 8), (3, 0), (0, 1), (8, 4)])
-@pytest.mark.parametrize("lens", [(1, 1), (33, 50)])
+@pytest.mark.parametrize("lens", [(1, 1), (33, 50), (77, 90)])
 def test_strided_rows(spare, offset, lens):
     _check(8, 128, 64, lens=lens, spare=spare, offset=offset)
 
 
 @pytest.mark.parametrize("bits", [4, 16])
-@pytest.mark.parametrize("lens", [(2, 1, 3), (70, 20, 33)])
+@pytest.mark.parametrize("lens", [(2, 1, 3), (70, 20, 33), (70, 50, 33)])
 def test_places_without_a_page(bits, lens):
     """Unmapped pages, a sequence that is not one, rows behind the last sequence."""
     _check(bits, 128, 64, lens=lens, cached=[30, 0, 14], unmap=[(0, 1), (1, 0)], behind=5)
 
 
-@pytest.mark.parametrize("lens", [(1, 1, 2), (64, 9, 40)])
+@pytest.mark.parametrize("lens", [(1, 1, 2), (64, 9, 40), (90, 9, 70)])
 def test_far_positions(lens):
     """Angles whose 32-bit product would have no digit left, and frequencies above one."""
     n = sum(lens)
@@ -170,7 +170,7 @@ def test_far_positions(lens):
 
 
 @pytest.mark.parametrize("bits", [4, 8, 16])
-@pytest.mark.parametrize("lens", [(1, 2, 1), (40, 17, 3)])
+@pytest.mark.parametrize("lens", [(1, 2, 1), (40, 17, 3), (98, 47, 3)])
 def test_values_that_are_not_finite(bits, lens):
     def edit(qkv):
         qkv[0, 5], qkv[1, -3], qkv[2, 700], qkv[3, -130] = float("inf"), float("nan"), -float("inf"), 60000.0
@@ -184,7 +184,7 @@ def test_negative_start():
     """A sequence that starts before its cache has no rows."""
     from pkv import ops
 
-    for n in (1, 20):
+    for n in (1, 20, 64):
         fmt = ops.PageFormat(2, 64, 16, 8, 32, torch.bfloat16)
         pool = ops.allocate_pool(fmt, 8)
         qkv = torch.randn((2 * n, 6 * 64), device="cuda").bfloat16()
