@@ -567,7 +567,9 @@ int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, co
  * once for the group's query rows together, the others once per sequence.  Results are
  * pkv_paged_attention's, to the rounding of another split and of keys as 16-bit operands,
  * for every sequence that a group names; the others' rows of out are left as they are, or
- * with zero_others (and a group and a member at least) become zeros.
+ * with zero_others (and a group and a member at least) become zeros.  A token that a row may
+ * not see changes nothing for it, whatever it holds; an infinity in V that it sees may come
+ * out as NaN.
  * Group g is sequences members[group_starts[g]] .. members[group_starts[g+1] - 1] (distinct over
  * the call) and shares its first prefix_lens[g] tokens, read through the first one's block
  * table as far as that sequence goes; a group of one shares nothing.  At most 32 query rows

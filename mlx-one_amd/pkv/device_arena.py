@@ -433,7 +433,8 @@ class DevicePageArena:
         group.  Sequences with the same first page are a group, which shares the whole pages
         that all of them hold alike, up to the shortest one's length; fewer than ``least``
         tokens count as none.  Reads the table on the host: call it when the batch changes,
-        not every step (a group stays right as its sequences grow)."""
+        not every step (a group stays right as its sequences grow; not past a ``truncate``,
+        ``evict`` or ``reorder`` that takes shared pages from a member)."""
         slots = [int(s) for s in slots]
         rows = self.table[torch.tensor(slots, dtype=torch.int64, device=self.device)].cpu()
         lens = self.lens.cpu()[slots].tolist() if slots else []
