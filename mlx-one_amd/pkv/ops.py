@@ -776,10 +776,7 @@ def rope_append(fmt: PageFormat, pool, qkv, block_table, start_pos, inv_freq, he
     *lead, width = qkv.shape
     if heads < 1 or width != (heads + 2 * kv_heads) * dim:
         raise ValueError("qkv width is not (heads + 2 * kv_heads) * head_dim")
-    steps = qkv.stride()
-    if steps[-1] != 1 or steps[-2] < width or (len(lead) == 2 and steps[0] != lead[1] * steps[1]):
-        qkv = qkv.contiguous()
-        steps = qkv.stride()
+    qkv, step = _projection_rows(qkv)
     starts = _i32(start_pos, device)
     batch = starts.numel()
     # (the tensors are named so that they live until the launch)
@@ -827,10 +824,22 @@ def rope_append(fmt: PageFormat, pool, qkv, block_table, start_pos, inv_freq, he
                 raise ValueError(f"out must be contiguous {shape} tensors of qkv's dtype and device")
     addresses = [t.data_ptr() for t in outs] if with_kv else (outs[0].data_ptr(), None, None)
     _launch(device, "rotation and append", nat.load().pkv_rope_append, fmt.c_layout, pool.data_ptr(),
-            pool.shape[0], qkv.data_ptr(), steps[-2], rows, heads, batch, tokens, first_at, widths_at,
+            pool.shape[0], qkv.data_ptr(), step, rows, heads, batch, tokens, first_at, widths_at,
             starts.data_ptr(), positions_at, num_axes, inv_freq.data_ptr(), half, axis_at,
             table.data_ptr(), table.shape[1], *addresses)
     return tuple(outs) if with_kv else outs[0]
+
+
+def _projection_rows(qkv):
+    """A projection ``[rows, width]`` or ``[B, N, width]`` as the kernels read it, its rows one
+    after the other (a copy where they are not): ``(tensor, elements between rows)``.  A
+    dimension of one element has any stride, which says nothing."""
+    *lead, width = qkv.shape
+    steps = [(n, step) for n, step in zip(lead, qkv.stride()) if n != 1]
+    step = steps[-1][1] if steps else width
+    if qkv.stride(-1) != 1 or step < width or (len(steps) == 2 and steps[0][1] != steps[1][0] * step):
+        return qkv.clone(memory_format=torch.contiguous_format), width
+    return qkv, step
 
 
 def rope_axes(sections, device="cuda", *, interleaved=False):
