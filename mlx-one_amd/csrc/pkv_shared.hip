@@ -23,7 +23,8 @@
 // Quantized K enters as its codes (1024 + c, exact in float16; queries as float16, bfloat16 ones
 // with each row scaled by a power of two), group scales and biases are applied to the float32
 // scores:  s = sum_g scale_g (q_g . c'_g) + (bias_g - 1024 scale_g) sum(q_g).  Quantized V is
-// rounded once to float16 (2^-11).  Weights are rounded to the operand type, or, where that
+// rounded once to float16 (2^-11); a row that sees a value past float16's range, which pages can
+// hold, is computed anew by the kernel that joins the parts (65,504 and more in V: rare, and slow).  Weights are rounded to the operand type, or, where that
 // would show in the result (bfloat16 pages, float16 results of quantized ones), enter as the
 // sum of two; they are summed as they enter.  Scores, maxima, sums and parts are float32.
 //
@@ -34,6 +35,7 @@
 
 #include "pkv_mfma.h"
 #include "pkv_step.h"
+#include "pkv_token.h"
 
 namespace pkv {
 
@@ -797,7 +799,8 @@ __device__ __forceinline__ bool planned_run(const SharedArgs &a, const SharedWor
   const int shared_runs = plan.group_run[a.groups], runs = shared_runs + plan.own_run[a.count];
   if (blockIdx.x == 0) {
     // where a member's parts are, for the merge: its group's first run and runs per
-    // segment, its first row in the group; its own first run and runs per KV head
+    // segment, its first row in the group; its own first run and runs per KV head; whose
+    // table the group's tiles are read through, and how many there are
     for (int j = tid; j < a.count; j += kThreads) {
       const bool in = j >= plan.group_first[0] && j < plan.group_first[a.groups];
       const int g = in ? last_at_most(plan.group_first, a.groups, j) : 0;
@@ -808,6 +811,8 @@ __device__ __forceinline__ bool planned_run(const SharedArgs &a, const SharedWor
       d[3] = shared_runs + plan.own_run[j];
       d[4] = (plan.own_run[j + 1] - plan.own_run[j]) / a.g.hk;
       d[5] = in;
+      d[6] = in ? plan.sequence[plan.group_first[g]] : -1;
+      d[7] = plan.group_tiles[g];
     }
   }
   if (u >= runs) return false;
@@ -883,6 +888,7 @@ __device__ __forceinline__ bool small_run(const SharedArgs &a, const SharedWork 
   const int runs = shared_runs + __builtin_amdgcn_readlane(own_end, 63);
   if (blockIdx.x == 0) {
     const int d0 = __shfl(group_run, g, 64), d1 = __shfl(shared_n, g, 64), at = __shfl(first, g, 64);
+    const int leader = __shfl(known ? b : -1, min(at, 63), 64);
     if (wave == 0 && lane < a.count) {
       int32_t *d = w.desc + 8 * lane;
       d[0] = d0;
@@ -891,6 +897,8 @@ __device__ __forceinline__ bool small_run(const SharedArgs &a, const SharedWork 
       d[3] = shared_runs + own_run;
       d[4] = own_n;
       d[5] = in;
+      d[6] = leader;
+      d[7] = skipped;
     }
   }
   if (u >= runs) return false;
@@ -960,6 +968,56 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void shared_kernel(cons
     if (run.rows <= 16) run_tiles<C, 1>(a, w, sequence, length, run, lane, wave, s_place[wave], lds, s_ml);
     else if constexpr (PER > 16) run_tiles<C, 2>(a, w, sequence, length, run, lane, wave, s_place[wave], lds, s_ml);
   }
+}
+
+// Row r of (sequence b, KV head kh) by itself, a tile at a time in 32 bits: the sums of
+// p_t v_t (the lane's dims) and of p_t = 2^(s_t - top).  The first `shared` tiles are read through
+// `leader`'s table.  q: the row's queries as float32, in LDS.  The whole wave calls.
+template <int DP>
+__device__ __forceinline__ float row_alone(const SharedArgs &a, int b, int leader, int shared, int kh, int qi,
+                                           const float *q, float top, int lane, float (&acc)[DP / 64]) {
+  constexpr int EPL = DP / 64;
+  const Geo &g = a.g;
+  const int t = lane & 15, jj = lane >> 4, tpp = g.page / PKV_TILE;
+  const int width = a.widths ? a.widths[b] : a.nq;
+  const int pos = a.q_pos ? a.q_pos[(int64_t)b * a.nq + qi] : a.seq_lens[b] - width + qi;
+  const int last = qi < width ? min(pos, seq_length(a, b) - 1) : -1;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) acc[e] = 0.0f;
+  float total = 0.0f;
+  for (int tile = 0; tile * PKV_TILE <= last; ++tile) {
+    const int page = a.table[(int64_t)(tile < shared ? leader : b) * a.max_pages + tile / tpp];
+    if (page < 0 || page >= a.num_pages) continue;
+    const uint8_t *head = a.pool + (int64_t)page * g.page_bytes + (int64_t)kh * g.head_bytes;
+    const uint8_t *k = head + (int64_t)(tile % tpp) * g.tile_bytes, *v = k + g.v_offset;
+    auto word = [&](int64_t meta, int tt, int d) __attribute__((always_inline)) {
+      return *(const uint32_t *)(head + meta + ((int64_t)(tile % tpp * PKV_TILE + tt) * g.ng + d / g.group) * 4);
+    };
+    float s = 0.0f;
+    for (int d0 = 8 * jj; d0 < DP; d0 += 32) {  // (a group holds whole eights)
+      const uint32_t m = word(g.kmeta_offset, t, d0);
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_fmaf((float)read_code(k, 0, g.bits, t, d0 + e, g.chunk), f16_bits_to_f32(m),
+                                       f16_bits_to_f32(m >> 16));
+        s = __builtin_fmaf(x, q[d0 + e], s);
+      }
+    }
+    s = xor32_add(xor16_add(s));
+    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, a.scale * kLog2e, -top));
+    for (int tt = 0; tt < PKV_TILE && tile * PKV_TILE + tt <= last; ++tt) {
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), tt));
+      total += w;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        const int d = lane * EPL + e;
+        const uint32_t m = word(g.vmeta_offset, tt, d);
+        const float x = __builtin_fmaf((float)read_code(v, 1, g.bits, tt, d, g.chunk), f16_bits_to_f32(m),
+                                       f16_bits_to_f32(m >> 16));
+        acc[e] = __builtin_fmaf(x, w, acc[e]);
+      }
+    }
+  }
+  return total;
 }
 
 // One wave per (sequence, KV head, row): the row's parts joined.  Lane l weighs part l (of 64 at
@@ -1041,6 +1099,23 @@ __global__ __launch_bounds__(kThreads) void shared_merge_kernel(const SharedArgs
   }
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o, 64);
+  // Values of quantized pages go up to 2^24, past float16's range: an operand that has become an
+  // infinity leaves sums that are not finite, and the row is computed by itself.
+  bool lost = false;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) lost |= !(fabsf(acc[e]) < INFINITY);
+  if (__builtin_expect(a.g.bits != 16 && fabsf(top) < INFINITY && __any(lost), 0)) {
+    __shared__ float s_q[kWaves][DP];
+    float *q = s_q[threadIdx.x >> 6];
+    const uint16_t *src = a.q + (((int64_t)b * a.heads + h) * a.nq + qi) * a.g.dim;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      const int i = lane + 64 * e;
+      q[i] = i < a.g.dim ? bits_to_float(src[i], a.g.float_kind) : 0.0f;
+    }
+    wave_lds_sync();
+    total = row_alone<DP>(a, b, max(d[6], 0), d[6] < 0 ? 0 : d[7], kh, qi, q, top, lane, acc);
+  }
   const float inv = top == -INFINITY ? 0.0f : 1.0f / total;
 #pragma unroll
   for (int e = 0; e < EPL; ++e)
