@@ -13,8 +13,9 @@
 // The contraction over keys takes a lane's scores as they lie (keys 8g + 4h + r in slot
 // 8h + 4(g & 1) + r), so P never crosses lanes.  Softmax in the exp2 domain with float32
 // maximum and sum; P is rounded once to the activation type, as the operand of its product
-// (2^-8 relative for bfloat16, beside the output's own rounding of the same size), and summed as
-// rounded, so that weights still add up to one.
+// (2^-8 relative for bfloat16, beside the output's own rounding of the same size; 2^-11 for float16,
+// and from 2^-21 of the largest weight down half of a fixed step, 2^-32 of that weight), and summed
+// as rounded, so that weights still add up to one.
 //
 // Only the last tile of a wave, on the diagonal, is masked.  There a masked key's V may be
 // anything: where it is not finite those elements are taken apart (a rare branch).
@@ -49,6 +50,7 @@ struct Wide<0> {
     return __builtin_amdgcn_fdot2_f32_bf16(b2{x, y}, b2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
   }
   static constexpr uint16_t kInf = 0x7F80;
+  static constexpr float kLift = 0.0f;
 };
 template <>
 struct Wide<1> {
@@ -61,6 +63,9 @@ struct Wide<1> {
     return __builtin_amdgcn_fdot2(h2{x, y}, h2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
   }
   static constexpr uint16_t kInf = 0x7C00;
+  // weights as 2^kLift of themselves, the largest 2^(kTau + kLift) then: those of less than
+  // 2^-14 have fewer bits
+  static constexpr float kLift = 7.0f;
 };
 
 template <int DP>
@@ -271,7 +276,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
       x = W::mma(__builtin_bit_cast(T, k), q[ks], ks == 0 ? zero : x);
     }
   };
-  // the exponents, less the running maximum: it moves when a score passes it by kTau
+  // the exponents, less the running maximum and plus kLift: it moves when a score passes it by
+  // kTau
   auto settle = [&](auto masks, f16v &x) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[e] = __builtin_fmaf(x[e], a.scale_log2, -m);
@@ -287,10 +293,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_kernel(const Pro
     if (__builtin_expect(__any(mx > thr), 0)) {
       const float up = xor32_max(mx);
       const bool moves = up > thr;
-      const float by = moves ? up : 0.0f;
-      const float alpha = !moves ? 1.0f : thr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
+      const float by = moves ? up - W::kLift : 0.0f;
+      const float alpha = !moves ? 1.0f : thr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by);
       m += by;
-      thr = moves ? kTau : thr;
+      thr = moves ? kTau + W::kLift : thr;
       l *= alpha;
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] -= by;
