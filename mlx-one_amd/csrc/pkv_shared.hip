@@ -26,7 +26,8 @@
 // rounded once to float16 (2^-11); a row that sees a value past float16's range, which pages can
 // hold, is computed anew by the kernel that joins the parts (65,504 and more in V: rare, and slow).  Weights are rounded to the operand type, or, where that
 // would show in the result (bfloat16 pages, float16 results of quantized ones), enter as the
-// sum of two; they are summed as they enter.  Scores, maxima, sums and parts are float32.
+// sum of two; they are summed as they enter.  (In float16 a weight has a fixed step of 2^-31 of the
+// largest, or less.)  Scores, maxima, sums and parts are float32.
 //
 // A token past a sequence's end or on an unmapped page is absent; one that a row may not see
 // yet changes nothing for it, not even where it is not finite.  (An infinity that it sees may
@@ -242,6 +243,9 @@ struct SharedCfg : Cfg<BITS, DP, G, 1, FK, 1> {
   using T = typename std::conditional<F16, h8, b8>::type;
   using E = typename std::conditional<F16, _Float16, __bf16>::type;
   static constexpr uint16_t INF = F16 ? 0x7C00 : 0x7F80;
+  // weights as 2^LIFT of themselves, the largest 2^(kTau + LIFT) then: float16's have fewer bits
+  // below 2^-14
+  static constexpr float LIFT = F16 ? 7.0f : 0.0f;
   static constexpr int PAGE_BITS = BITS, GROUP = G;
 };
 
@@ -587,10 +591,10 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
       for (int rb = 0; rb < RB; ++rb) {
         const float up = xor32_max(xor16_max(mx[rb]));
         const bool moves = !(up <= thr[rb]);
-        const float by = moves ? up : 0.0f;
-        const float alpha = !moves ? 1.0f : thr[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
+        const float by = moves ? up - C::LIFT : 0.0f;
+        const float alpha = !moves ? 1.0f : thr[rb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by);
         m[rb] += by;
-        thr[rb] = moves ? kTau : thr[rb];
+        thr[rb] = moves ? kTau + C::LIFT : thr[rb];
         sum[rb] *= alpha;
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[rb][e] -= by;
@@ -613,7 +617,7 @@ __device__ __forceinline__ void run_tiles(const SharedArgs &a, const SharedWork 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           low[rb][e] = (E)(x[rb][e] - (float)P[rb][e]);
-          sum[rb] += x[rb][e];
+          sum[rb] += (float)P[rb][e] + (float)low[rb][e];
         }
     } else {
 #pragma unroll
