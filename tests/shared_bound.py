@@ -22,14 +22,14 @@ def _sizes(fmt, pool, ids):
     return size.transpose(1, 0, 2, 3).reshape(fmt.num_kv_heads, -1, size.shape[-1])
 
 
-def shared64(fmt, pool, table, lens, queries, scale, *, q_pos=None, widths=None):
+def shared64(fmt, pool, table, lens, queries, scale, *, q_pos=None, widths=None, values=None, products=None):
     """``(out, bound)`` ``[B, H, Q, D]`` over the pages' values.
 
-    Scores of quantized pages: exact keys, so D + 8 roundings of 2^-24 of the terms as they
-    enter (``_sizes``), and a bfloat16 query's conversion to float16, 2^-31 of the row's largest
+    Scores: as many roundings of 2^-24 as there are ``products`` that are not zero (default D), and
+    8; of quantized pages, whose keys are exact, of the terms as they enter (``_sizes``), and a bfloat16 query's conversion to float16, 2^-31 of the row's largest
     element.  Weights: float16 operands (2^-11), or two operands where results are float16
     (quantized pages) or pages bfloat16; a fixed step of 2^-31 of the largest weight in
-    float16, half of it an error.  Quantized values: 2^-11."""
+    float16, half of it an error.  Quantized values: 2^-11 (or ``values``)."""
     import torch
 
     q = queries.double().cpu().numpy()
@@ -42,8 +42,8 @@ def shared64(fmt, pool, table, lens, queries, scale, *, q_pos=None, widths=None)
         operand = half if fmt.dtype is torch.bfloat16 else half ** 2
     else:
         operand = half if f16 else half_step(torch.bfloat16) ** 2
-    value = half if fmt.quantized else 0.0
-    group = fmt.group_size
+    value = values if values is not None else half if fmt.quantized else 0.0
+    group, products = fmt.group_size, dim if products is None else products
     out, bound = np.zeros(q.shape), np.zeros(q.shape)
     for b in range(batch):
         length = int(lens[b])
@@ -64,12 +64,12 @@ def shared64(fmt, pool, table, lens, queries, scale, *, q_pos=None, widths=None)
                 extra = 0.0
                 if fmt.quantized:
                     by_group = np.add.reduceat(np.abs(row), np.arange(0, dim, group))
-                    extra = (dim + 8) * 2.0 ** -24 * float((sizes[kh, :sees] @ by_group).max())
+                    extra = (products + 8) * 2.0 ** -24 * float((sizes[kh, :sees] @ by_group).max())
                     if fmt.dtype is torch.bfloat16:
                         extra += dim * 2.0 ** -31 * float(np.abs(row).max() * np.abs(k[kh, :sees]).max())
                 # (as ``key``, relative to the terms, and without what that adds for the values)
                 key = extra / max(float(terms[0]), 1e-300)
-                wide = attention_bound(o, weight, terms, scale, fmt.dtype, dim=dim, tokens=length, operand=operand, key=key)
+                wide = attention_bound(o, weight, terms, scale, fmt.dtype, dim=products, tokens=length, operand=operand, key=key)
                 h_out = half_step(fmt.dtype)
                 wide += weight * (value - key) * (1 + h_out)
                 if f16:
