@@ -419,6 +419,14 @@ class DevicePageArena:
             self.state[1:2].zero_()
         return err
 
+    def recorded(self):
+        """The error bits as the stream stands now, on the device."""
+        return self.state[1:2].clone()
+
+    def keep_recorded(self, recorded):
+        """Drop the error bits that were not among ``recorded``'s."""
+        self.state[1:2].bitwise_and_(recorded)
+
     def refcounts(self):
         return self.state[HEADER_WORDS + self.capacity:HEADER_WORDS + 2 * self.capacity].cpu()
 
@@ -564,6 +572,7 @@ class DeviceRunner:
         """Reserve ``widths`` tokens in ``slots`` and run ``forward(reservation)``; a step that
         raises leaves the slots as they were."""
         before = [self.arena.lengths[s] for s in slots]
+        recorded = self.arena.recorded()
         res = self.arena.reserve(slots, widths)
         # the reserve kernel's error bits, read after the forward is enqueued:
         # by then the reserve has long run, so the check costs no stall
@@ -572,7 +581,8 @@ class DeviceRunner:
             out = forward(res)
         except BaseException:
             self.arena.rollback(slots, before)
-            self.arena.probe_failed(probe)    # (what a failed reserve recorded goes with its step)
+            # (what a failed reserve recorded goes with its step; what was there before stays)
+            self.arena.keep_recorded(recorded)
             raise
         err = self.arena.probe_failed(probe)
         if err:
