@@ -580,18 +580,22 @@ class DeviceRunner:
         try:
             out = forward(res)
         except BaseException:
-            self.arena.rollback(slots, before)
+            self._take_back(slots, before, res)
             # (what a failed reserve recorded goes with its step; what was there before stays)
             self.arena.keep_recorded(recorded)
             raise
         err = self.arena.probe_failed(probe)
         if err:
-            # a failed reserve grew no slot (its append wrote nothing): only
-            # the host length mirror moved
-            for s, n in zip(slots, before):
-                self.arena.lengths[s] = n
+            self._take_back(slots, before, res)
             self.arena._raise(err)
         return out
+
+    def _take_back(self, slots, before, res):
+        """Cut a step's slots back to the lengths that its reserve found on the device (the
+        host's may be behind, after replays), and the host's to what they were."""
+        self.arena.rollback(res.slots, res.starts)
+        for s, n in zip(slots, before):
+            self.arena.lengths[s] = n
 
     def prefill(self, slots, hidden, widths):
         """Whole prompts, packed: ``hidden [sum(widths), hidden]`` holds the rows of ``slots``
