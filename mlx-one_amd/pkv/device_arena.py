@@ -23,6 +23,7 @@ its slots unchanged.
 from __future__ import annotations
 
 import ctypes
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -45,6 +46,29 @@ class Reservation:
     table: torch.Tensor        # [B, max_pages] int32 page ids (entries past a slot's pages unset)
     starts: torch.Tensor       # [B] int32 length before the step (= the first new position)
     lens: torch.Tensor         # [B] int32 length after the step
+
+
+class PrefixGroups:
+    """What ``DevicePageArena.prefix_groups`` found: ``(members, group_starts, prefix_lens)`` device
+    tensors, to be unpacked, and the slots that they are of.  ``holds(slots)`` until a member
+    is cut below what its group shares."""
+
+    def __init__(self, slots, tensors, shared):
+        self.slots, self.tensors = tuple(slots), tensors
+        self.shared = shared        # {slot: (its group, tokens that the group shares)}
+        self.cut = False
+
+    def __iter__(self):
+        return iter(self.tensors)
+
+    def __getitem__(self, i):
+        return self.tensors[i]
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def holds(self, slots):
+        return self.slots == tuple(slots) and not self.cut
 
 
 class DevicePageArena:
@@ -81,6 +105,7 @@ class DevicePageArena:
         # the attention weight each cached token has drawn, and the tokens evicted
         # from each slot (one more entry than slots): kept once track_mass() asks
         self.mass = self.evicted = None
+        self._groups = weakref.WeakSet()    # prefix groups that are still in use
         nat.check(lib.pkv_arena_init(nat.stream_handle(self.device), nat.ptr(self.state),
                                      self.capacity), "arena init")
 
@@ -169,7 +194,13 @@ class DevicePageArena:
         if host_slots is not None and host_keep is not None:
             for s, k in zip(host_slots, host_keep):
                 self.lengths[s] = k
+                self._cut_groups(s, k)
         return slots_d, keep_d
+
+    def _cut_groups(self, slot, keep):
+        """Slot ``slot`` holds only its first ``keep`` tokens as before."""
+        for groups in self._groups:
+            groups.cut |= groups.shared.get(slot, (0, 0))[1] > keep
 
     def release(self, slots):
         """Drop every page of the slots and return them to the free slot list."""
@@ -225,6 +256,9 @@ class DevicePageArena:
             held = [self.lengths[s] for s in host_sources]
             for s, n in zip(host_slots, held):
                 self.lengths[s] = n
+            for groups in self._groups:    # (members of one group share what they share)
+                of = groups.shared.get
+                groups.cut |= any(of(s, (0, 0))[1] and of(s) != of(p) for s, p in zip(host_slots, host_sources))
 
     def _reorder_scratch(self, count):
         return ops._scratch(nat.load().pkv_arena_reorder_workspace_bytes(count, self.max_pages),
@@ -312,7 +346,7 @@ class DevicePageArena:
             raise ValueError("one budget per slot")
         if count == 0:
             return
-        opened = []
+        opened, held = [], {s: self.lengths[s] for s in host_slots or ()}
         if spare is None:
             if not self._free_slots:
                 raise CacheCapacityError("eviction needs a free sequence slot", retryable=True)
@@ -335,6 +369,7 @@ class DevicePageArena:
         except BaseException:
             if host_slots is not None:           # (slots before this one may have been cut)
                 self.sync_lengths()
+                self._cut_shorter(held)
             raise
         finally:
             self._free_slots.extend(reversed(opened))
@@ -343,9 +378,17 @@ class DevicePageArena:
             if err or host_keep is None:
                 self.sync_lengths()
             if err:
+                self._cut_shorter(held)
                 self._raise(err)
             for s, k in zip(host_slots, host_keep or ()):
                 self.lengths[s] = min(self.lengths[s], k)
+            self._cut_shorter(held)
+
+    def _cut_shorter(self, held):
+        """The slots that are shorter than they were have their tokens on pages of their own."""
+        for s, n in held.items():
+            if self.lengths[s] < n:
+                self._cut_groups(s, 0)
 
     def _evict(self, slots_d, keep_d, spare_d, sinks, recent, max_keep):
         valid = (slots_d >= 0) & (slots_d < self.max_slots)
@@ -437,13 +480,16 @@ class DevicePageArena:
     def prefix_groups(self, slots, *, least=1):
         """The sequences among ``slots`` that share their first pages (``fork``, an adopted
         prefix), as ``ops.shared_prefix_attention`` takes them: ``(members, group_starts,
-        prefix_lens)`` device tensors, members as places in ``slots``, every sequence in one
-        group.  Sequences with the same first page are a group, which shares the whole pages
+        prefix_lens)`` device tensors (a ``PrefixGroups``), members as places in ``slots``, every
+        sequence in one group.  Sequences with the same first page are a group, which shares the whole pages
         that all of them hold alike, up to the shortest one's length; fewer than ``least``
         tokens count as none.  Reads the table on the host: call it when the batch changes,
         not every step (a group stays right as its sequences grow; not past a ``truncate``,
-        ``evict`` or ``reorder`` that takes shared pages from a member)."""
+        ``evict`` or ``reorder`` that takes shared pages from a member: lists of slots that do
+        are noticed, device tensors are the caller's to know)."""
         slots = [int(s) for s in slots]
+        if any(s < 0 or s >= self.max_slots for s in slots):
+            raise ValueError("slots must be valid slot ids")
         rows = self.table[torch.tensor(slots, dtype=torch.int64, device=self.device)].cpu()
         lens = self.lens.cpu()[slots].tolist() if slots else []
         by_first = {}
@@ -451,7 +497,7 @@ class DevicePageArena:
             held = lens[place] // self.page_tokens
             key = int(rows[place, 0]) if held else None
             by_first.setdefault((place,) if key is None else key, []).append(place)
-        members, starts, prefixes = [], [0], []
+        members, starts, prefixes, shared = [], [0], [], {}
         for group in by_first.values():
             held = min(lens[p] for p in group) // self.page_tokens
             same = (rows[group, :held] == rows[group[0], :held]).all(0)
@@ -460,8 +506,11 @@ class DevicePageArena:
             members += group
             starts.append(len(members))
             prefixes.append(tokens if tokens >= least else 0)
-        return tuple(torch.tensor(x, dtype=torch.int32, device=self.device)
-                     for x in (members, starts, prefixes))
+            shared.update((slots[p], (len(prefixes), prefixes[-1])) for p in group)
+        groups = PrefixGroups(slots, tuple(torch.tensor(x, dtype=torch.int32, device=self.device)
+                                           for x in (members, starts, prefixes)), shared)
+        self._groups.add(groups)
+        return groups
 
     def pages(self, slot):
         n = -(-int(self.lens[slot].item()) // self.page_tokens)
@@ -593,7 +642,7 @@ class DeviceRunner:
     def _take_back(self, slots, before, res):
         """Cut a step's slots back to the lengths that its reserve found on the device (the
         host's may be behind, after replays), and the host's to what they were."""
-        self.arena.rollback(res.slots, res.starts)
+        self.arena.rollback(res.slots, res.starts)    # (groups hold: they were made before the step)
         for s, n in zip(slots, before):
             self.arena.lengths[s] = n
 
@@ -625,21 +674,28 @@ class DeviceRunner:
     def execute(self, slots, hidden, widths=None, *, shared=None):
         """``hidden [B, T, hidden]`` for ``slots`` (row b's columns past
         ``widths[b]`` are padding); returns the model's ``[B, T, hidden]``.  ``shared``: the
-        arena's ``prefix_groups(slots)``, whose prefixes attention then reads once."""
+        arena's ``prefix_groups(slots)``, whose prefixes attention then reads once; those of
+        other slots or another order, or with a member cut below its prefix, are refused.
+        (A tuple of the three tensors, or the groups of another arena that holds the same, are
+        taken at their word.)"""
         batch, width, _ = hidden.shape
         slots = [int(s) for s in slots]
         widths = [width] * batch if widths is None else [int(w) for w in widths]
         if len(slots) != batch or len(widths) != batch or any(w < 1 or w > width for w in widths):
             raise ValueError("one slot and a width in 1..T per row")
-        self._check_groups(shared, batch)
+        self._check_groups(shared, slots)
         return self._step(slots, widths, lambda res: self._forward(hidden, res, shared=shared))
 
-    @staticmethod
-    def _check_groups(shared, batch):
-        """Groups of another batch would leave rows without attention."""
-        if shared is not None and (len(shared) != 3 or shared[0].numel() != batch
-                                   or shared[1].numel() != shared[2].numel() + 1):
-            raise ValueError("shared must be the prefix_groups of the batch's slots")
+    def _check_groups(self, shared, slots):
+        """Groups of another batch would leave rows without attention, or with another
+        sequence's prefix."""
+        if isinstance(shared, PrefixGroups):
+            good = shared.holds(slots)
+        else:
+            good = shared is None or (len(shared) == 3 and shared[0].numel() == len(slots)
+                                      and shared[1].numel() == shared[2].numel() + 1)
+        if not good:
+            raise ValueError("shared must be the prefix_groups of the batch's slots, as they are now")
 
     def capture_decode(self, slots, hidden, *, warm=True, shared=None):
         """Graphs of one decode step (one token per slot) reading the static
@@ -654,10 +710,11 @@ class DeviceRunner:
         tensors are the graph's and are kept."""
         arena = self.arena
         device = arena.device
-        slots_d = torch.tensor([int(s) for s in slots], dtype=torch.int32, device=device)
+        slots = [int(s) for s in slots]
+        self._check_groups(shared, slots)
+        slots_d = torch.tensor(slots, dtype=torch.int32, device=device)
         widths_d = torch.ones_like(slots_d)
-        count = int(slots_d.numel())
-        self._check_groups(shared, count)
+        count = len(slots)
         # the graph's split-K partials live in a workspace of its own, sized as an
         # eager call's (so both run the same split) for the waves fixed at
         # capture, and held by the CapturedStep
@@ -709,6 +766,8 @@ class CapturedStep:
     reserve_graph: torch.cuda.CUDAGraph = None   # the page reservation, replayed first
 
     def replay(self):
+        if isinstance(self.operands[-1], PrefixGroups) and self.operands[-1].cut:
+            raise ValueError("a sequence of the captured step was cut below its shared prefix")
         if self.reserve_graph is not None:
             self.reserve_graph.replay()
         self.graph.replay()
