@@ -158,6 +158,20 @@ __global__ __launch_bounds__(256) void append_tiles_kernel(const AppendArgs a, i
 
 // ---- gather to the reference format ---------------------------------------
 
+
+__device__ __forceinline__ int read_code(const uint8_t *tile, int side, int bits, int tt, int d,
+                                         int chunk) {
+  if (side == 0) {
+    const int kb = d / 32, jj = (d % 32) / 8, e = d % 8, lane = tt + 16 * jj;
+    if (bits == 8) return tile[payload_offset(lane, 8 * kb + e, chunk)];
+    const int nib = k4_nibble(e);
+    return (tile[payload_offset(lane, 4 * kb + nib / 2, chunk)] >> (4 * (nib & 1))) & 15;
+  }
+  const int n = d / 16, col = d % 16, jj = tt / 4, r = tt % 4, lane = col + 16 * jj;
+  if (bits == 8) return tile[payload_offset(lane, 4 * n + r, chunk)];
+  return (tile[payload_offset(lane, 4 * (n / 2) + v4_byte(r), chunk)] >> (4 * (n % 2))) & 15;
+}
+
 // One thread per (page, head, token, output byte); grid-stride.
 __global__ __launch_bounds__(256) void gather_kernel(const GatherArgs a) {
   const Geo &g = a.g;

@@ -160,18 +160,4 @@ __device__ __forceinline__ void store_token(const Geo &g, uint8_t *head, int slo
   }
 }
 
-// The code of element d of token tt in a quantized tile's payload (side 0: K, 1: V).
-__device__ __forceinline__ int read_code(const uint8_t *tile, int side, int bits, int tt, int d,
-                                         int chunk) {
-  if (side == 0) {
-    const int kb = d / 32, jj = (d % 32) / 8, e = d % 8, lane = tt + 16 * jj;
-    if (bits == 8) return tile[payload_offset(lane, 8 * kb + e, chunk)];
-    const int nib = k4_nibble(e);
-    return (tile[payload_offset(lane, 4 * kb + nib / 2, chunk)] >> (4 * (nib & 1))) & 15;
-  }
-  const int n = d / 16, col = d % 16, jj = tt / 4, r = tt % 4, lane = col + 16 * jj;
-  if (bits == 8) return tile[payload_offset(lane, 4 * n + r, chunk)];
-  return (tile[payload_offset(lane, 4 * (n / 2) + v4_byte(r), chunk)] >> (4 * (n % 2))) & 15;
-}
-
 }  // namespace pkv
