@@ -514,8 +514,8 @@ int64_t pkv_arena_reorder_workspace_bytes(int32_t count, int32_t max_pages);
  * pages, in one pass.  A row of qkv holds num_heads + 2 * num_kv_heads heads (q, k, v) of
  * head_dim elements; rows are row_stride elements apart.  Rows come packed: sequence b has
  * rows row_starts[b] .. row_starts[b+1] - 1 (rising), or, with row_starts NULL, padded: rows
- * b * tokens .. + widths[b] - 1 (widths NULL: tokens).  Rows of no sequence are neither read nor
- * written.  Row i of a sequence is appended at start_pos[b] + i as pkv_append_quantize
+ * b * tokens .. + widths[b] - 1 (widths NULL: tokens).  Rows of no sequence change nothing, and
+ * their places in q, k and v are not written.  Row i of a sequence is appended at start_pos[b] + i as pkv_append_quantize
  * appends it (a position without a mapped page is dropped, its rotated rows still come out;
  * a sequence whose start is negative has no rows).
  *
@@ -545,8 +545,10 @@ int pkv_rope_append(void *stream, const pkv_layout *layout, void *pool, int64_t 
  * row_starts[b] .. row_starts[b+1] - 1, rising) attends rows row_starts[b] .. i of keys and
  * values, query head h those of KV head h / (num_heads / num_kv_heads).  Rows of no sequence
  * are neither read nor written.  Sums and softmax in float32; the weights are rounded
- * once to float_kind, as operands.  What a later row holds, infinities and NaN among it,
- * changes nothing for an earlier one.  Replaces the padded attention of a prompt's first
+ * once to float_kind, as operands (bfloat16 ones too, which pkv_paged_attention takes as the
+ * sum of two over bfloat16 pages), and summed as they are rounded.  What a later row holds,
+ * infinities and NaN among it, changes nothing for an earlier one; an infinity in V comes out
+ * as NaN for a row that gives it a weight too small for its type.  Replaces the padded attention of a prompt's first
  * pass (src/mlx_one/engine/paged_attention.py:127-206 over pages just written) for prompts
  * whose keys and values are at hand.
  *
@@ -569,7 +571,8 @@ int pkv_prompt_attention(void *stream, const void *queries, int64_t q_stride, co
  * for every sequence that a group names; the others' rows of out are left as they are, or
  * with zero_others (and a group and a member at least) become zeros.  A token that a row may
  * not see changes nothing for it, whatever it holds; an infinity in V that it sees may come
- * out as NaN.
+ * out as NaN.  A row that sees values past 65504 in quantized V is computed in float32 by
+ * itself, which takes longer.
  * Group g is sequences members[group_starts[g]] .. members[group_starts[g+1] - 1] (distinct over
  * the call) and shares its first prefix_lens[g] tokens, read through the first one's block
  * table as far as that sequence goes; a group of one shares nothing.  At most 32 query rows

@@ -649,8 +649,9 @@ class DeviceRunner:
     def prefill(self, slots, hidden, widths):
         """Whole prompts, packed: ``hidden [sum(widths), hidden]`` holds the rows of ``slots``
         (which must be empty) one after the other, without padding; returns the model's
-        rows.  Attention reads k and v as the projection made them; ``execute`` reads them
-        back from the pages, as later steps do."""
+        rows.  Attention reads k and v as the projection made them, with weights of one operand
+        (``ops.prompt_attention``); ``execute`` reads them back from the pages, as later steps
+        do."""
         slots, widths = [int(s) for s in slots], [int(w) for w in widths]
         if len(widths) != len(slots) or any(w < 1 for w in widths) or hidden.dim() != 2 \
                 or hidden.shape[0] != sum(widths):

@@ -876,6 +876,8 @@ def prompt_attention(q, k, v, row_starts, *, scale, out=None):
     are read where they lie); sequence b is rows ``row_starts[b]`` to ``row_starts[b + 1] - 1``
     (``row_starts [B + 1]``, rising).  Returns ``[T, H, D]``; rows of no sequence are left as they
     are in ``out``.  Head dims up to 256; ones that are no multiple of 8 are padded by a copy.
+    Weights are rounded to the inputs' type, where ``paged_attention`` over bfloat16 pages keeps
+    them as the sum of two.
     """
     for t in (q, k, v):
         if not isinstance(t, torch.Tensor) or t.dim() != 3 or t.dtype not in FLOAT_KINDS or not t.is_cuda:
